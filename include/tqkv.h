@@ -307,6 +307,123 @@ size_t tqkv_sparse_workspace_size(int32_t B, int32_t H, int32_t H_kv, int32_t D,
                                   int64_t total_tokens, int32_t keep);
 
 /*
+ * Paged cache: rows of many sequences in one pool of pages (no counterpart in
+ * the reference, whose caches are one block a sequence; the row formats and
+ * the attention are tqkv_affine_quantize's and tqkv_decode_attend_affine's).
+ *
+ * The pool's buffers are [num_pages, kv_heads, page_rows, .]: K and V (bf16
+ * rows [dim]) for TQKV_CACHE_BF16, or the six affine buffers (K packed,
+ * scales, biases, V packed, scales, biases) for TQKV_CACHE_AFFINE. Row t of
+ * sequence b of every KV head lies in page table[b * table_stride +
+ * t / page_rows] at row t % page_rows; lens[b] rows are held. Sequences may
+ * share pages (a common prompt) wherever a call only reads them. table and
+ * lens are device arrays that the kernels read when they run, so a captured
+ * call follows their later contents. A page index outside [0, num_pages)
+ * holds no rows: it is neither read nor written, and its rows get no
+ * attention. lens below 0 counts as 0, and above table_stride * page_rows as
+ * that.
+ *
+ * weights (optional, NULL for none): f32 [batch, kv_heads, table_stride *
+ * page_rows], the attention weight that row t of sequence b has gathered so
+ * far: tqkv_paged_append clears the rows it writes, tqkv_paged_decode_attend
+ * adds to them and tqkv_paged_evict ranks by them. They belong to the sequence and not to
+ * the page, so sequences that share pages gather their own.
+ *
+ * dim in {64, 128, 256, 512}; page_rows in {16, 32, 64, 128, 256}; batch at
+ * most 1024; affine: bits_k and bits_v 4 or 8 each, group_size in {32, 64,
+ * 128} dividing dim (bf16 ignores the three). TQKV_EUNSUPPORTED otherwise.
+ * slot pointers are 16-byte aligned, and the pool, table, lens and weights
+ * belong to the calling thread's current device.
+ */
+typedef struct tqkv_paged_kv {
+  int32_t kind; /* TQKV_CACHE_BF16 or TQKV_CACHE_AFFINE */
+  int32_t batch;
+  int32_t kv_heads;
+  int32_t dim;
+  int32_t page_rows;
+  int32_t group_size;
+  int32_t bits_k;
+  int32_t bits_v;
+  int64_t num_pages;
+  int64_t table_stride; /* entries of a sequence's row of the table */
+  void* slot[6];
+  const int32_t* table; /* device [batch, table_stride] */
+  const int32_t* lens;  /* device [batch] */
+  float* weights;       /* device [batch, kv_heads, table_stride * page_rows] or NULL */
+} tqkv_paged_kv;
+
+/*
+ * Writes new tokens' keys and values into their pages: bf16 rows as they are,
+ * affine rows quantized bit for bit as tqkv_affine_quantize does. Tokens of
+ * all sequences lie one behind the other: starts (device int32 [batch + 1],
+ * ascending) gives each sequence's first token, and sequence b's count =
+ * starts[b + 1] - starts[b] tokens become its rows [lens[b] - count, lens[b]):
+ * lens counts the new rows already. starts = NULL: one token a sequence
+ * (tokens == batch). Head h of token i is at k + i * token_stride + h *
+ * head_stride (bf16 elements; v alike), so a fused projection's output is
+ * read in place; k and v are 16-byte aligned and the strides multiples of 8.
+ * Tokens outside [starts[0], starts[batch]), rows below 0 or past the table
+ * and rows of invalid pages are not written. Two tokens must not share a row
+ * (so a page that is written belongs to one sequence). One launch.
+ */
+int32_t tqkv_paged_append(const tqkv_paged_kv* kv, const uint16_t* k, const uint16_t* v,
+                          const int32_t* starts, int64_t tokens, int64_t token_stride,
+                          int64_t head_stride, tqkv_stream stream);
+
+/*
+ * Attention of one new token a sequence over its pages, softmax(scale * q.K^T)
+ * . V: tqkv_decode_attend_affine with a length and pages for each sequence.
+ * q: bf16, head h of sequence b at q + b * q_stride + h * dim (16-byte
+ * aligned, q_stride a multiple of 8); out: bf16 [batch, H, dim]. H / kv_heads
+ * from 1 to 32. window > 0: the last `window` rows only; otherwise all.
+ * max_rows: the host's bound on lens (at most table_stride * page_rows); it
+ * sizes the grid and the workspace, and a sequence that holds more attends
+ * its first max_rows rows as if it held no more. A sequence without rows gets
+ * zeros. The work is divided over the whole batch's rows, long and short
+ * sequences alike, by lens as they are on the device; results depend on lens
+ * and max_rows and not on the run. With kv->weights, each attended row's
+ * softmax weights, summed over the query heads of its KV head, are added to
+ * it (f32, in a fixed order).
+ * workspace: tqkv_paged_decode_workspace_size() bytes, 16-byte aligned, or
+ * NULL for the library's scratch; calls that share one must not overlap in
+ * time. Two launches, no other allocation.
+ */
+int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint16_t* q, int64_t q_stride,
+                                 int32_t H, float scale, int64_t window, int64_t max_rows,
+                                 uint16_t* out, void* workspace, size_t workspace_bytes,
+                                 tqkv_stream stream);
+/* Its workspace: split partials, and f32 scores [batch, H, max_rows] where
+ * kv->weights is set. Host arithmetic only; 0 for arguments that the call
+ * refuses. */
+size_t tqkv_paged_decode_workspace_size(const tqkv_paged_kv* kv, int32_t H, int64_t max_rows);
+
+/*
+ * Cuts every sequence back to `budget` rows by the weights it has gathered
+ * (kv->weights, required), each KV head for itself: the first `sinks` and the
+ * last `recent` rows stay, and between them the rows of the largest weight
+ * (ties: the lower row; a NaN counts as -inf). The kept rows move, in their
+ * order, to rows 0, 1, ... of the pages that dst_table (device int32 [batch,
+ * dst_stride]) names in the same pool, their weights to dst_weights (f32
+ * [batch, kv_heads, dst_stride * page_rows], NULL for none), and dst_lens[b]
+ * (device) becomes min(lens[b], budget); a sequence of at most `budget` rows
+ * moves whole. kept (int32 [batch, kv_heads, budget], or NULL) receives the
+ * rows' old positions, -1 behind the last. Other rows of the new pages, and
+ * dst_weights behind the last row, stay as they were. The destination pages
+ * must not be among the pages of kv->table nor twice in dst_table, and
+ * dst_weights must not overlap kv->weights; dst_lens may be kv->lens. Rows
+ * whose old or new page is invalid are not moved (their weights are).
+ * budget >= 1, sinks + recent <= budget <= dst_stride * page_rows.
+ * workspace: tqkv_paged_evict_workspace_size() bytes (the kept positions) or
+ * NULL for the library's scratch; neither is used where kept is given. Two
+ * launches.
+ */
+int32_t tqkv_paged_evict(const tqkv_paged_kv* kv, int64_t budget, int64_t sinks, int64_t recent,
+                         const int32_t* dst_table, int64_t dst_stride, int32_t* dst_lens,
+                         float* dst_weights, int32_t* kept, void* workspace,
+                         size_t workspace_bytes, tqkv_stream stream);
+size_t tqkv_paged_evict_workspace_size(const tqkv_paged_kv* kv, int64_t budget);
+
+/*
  * Which decode kernel tqkv_decode_attend_affine runs for a layout: "mfma"
  * (scores on the matrix cores; group_size 32, 64 or 128, D in {64, 128, 256},
  * heads a launch in {1, 2, 4, 8} with heads * D / group_size <= 16), "tiles"

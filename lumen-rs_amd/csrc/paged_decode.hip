@@ -1,0 +1,241 @@
+// Paged decode attention: the join of the segments, the gathered weights, and
+// the host side. The attention kernel is in paged_decode.hpp.
+#include "paged_decode.hpp"
+
+namespace tqkv {
+namespace paged {
+
+extern template void launch_affine<64>(const DecodeArgs&, int, int, int, dim3, hipStream_t);
+extern template void launch_affine<128>(const DecodeArgs&, int, int, int, dim3, hipStream_t);
+extern template void launch_affine<256>(const DecodeArgs&, int, int, int, dim3, hipStream_t);
+extern template void launch_affine<512>(const DecodeArgs&, int, int, int, dim3, hipStream_t);
+
+namespace {
+
+constexpr int kJoinThreads = 256;
+constexpr int kWeightRows = 1024;  // rows whose weights a workgroup adds
+
+// Where sequence b's segments lie: its first tile of all, and the totals.
+__device__ __forceinline__ void place(const DecodeArgs& a, int b, int64_t* red, int* first,
+                                      int* total) {
+  int64_t mine = 0;  // tiles before b in the high half, all in the low
+  for (int i = threadIdx.x; i < a.pool.batch; i += kJoinThreads) {
+    const int64_t t = span_of(a, i).tiles;
+    mine += t + (i < b ? t << 32 : 0);
+  }
+  for (int off = 32; off > 0; off >>= 1) mine += __shfl_xor(mine, off, 64);
+  __syncthreads();
+  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = mine;
+  __syncthreads();
+  mine = 0;
+  for (int w = 0; w < kJoinThreads / 64; ++w) mine += red[w];
+  *first = int(mine >> 32);
+  *total = int(mine & 0xffffffff);
+}
+
+// Maximum and sum over the segments [w0, w1] of one (sequence, head), by a
+// wavefront: each lane its segments in order, then a butterfly.
+__device__ __forceinline__ void head_sum(const DecodeArgs& a, int b, int h, int w0, int w1,
+                                         float* top, float* sum) {
+  const int lane = threadIdx.x % 64;
+  float m = -INFINITY;
+  for (int w = w0 + lane; w <= w1; w += 64) m = fmaxf(m, a.part_m[int64_t(w + b) * a.H + h]);
+  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+  float l = 0.0f;
+  for (int w = w0 + lane; w <= w1; w += 64) {
+    const float pm = a.part_m[int64_t(w + b) * a.H + h], pl = a.part_l[int64_t(w + b) * a.H + h];
+    l += pm == -INFINITY ? 0.0f * pl : pl * exp2f(pm - m);
+  }
+  for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
+  *top = m;
+  *sum = l;
+}
+
+// Workgroups [0, batch x H): the output of one (sequence, head) from its
+// segments, in their order. The others: kWeightRows rows of one (sequence, KV
+// head): weights[row] += sum over the group's heads of 2^(s - m) / l.
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeArgs a, int D,
+                                                                  int row_blocks) {
+  __shared__ int64_t red[kJoinThreads / 64];
+  __shared__ float head_m[32], head_r[32];
+  const int tid = threadIdx.x, outs = a.pool.batch * a.H;
+  const bool joins = int(blockIdx.x) < outs;
+  int b, h = 0, kvh = 0, block = 0;
+  if (joins) {
+    b = blockIdx.x / a.H;
+    h = blockIdx.x % a.H;
+  } else {
+    const int i = blockIdx.x - outs;
+    block = i % row_blocks;
+    kvh = i / row_blocks % a.pool.Hkv;
+    b = i / row_blocks / a.pool.Hkv;
+  }
+  const Span span = span_of(a, b);
+  if (joins && span.n == 0) {
+    for (int d = tid; d < D; d += kJoinThreads) a.out[int64_t(blockIdx.x) * D + d] = 0;
+    return;
+  }
+  const int row0 = span.lo / kTile * kTile + block * kWeightRows;
+  if (!joins && row0 >= span.n) return;
+  int first, total;
+  place(a, b, red, &first, &total);
+  const int per = tiles_per_wg(total, a.W);
+  const int w0 = first / per, w1 = (first + span.tiles - 1) / per;
+  if (joins) {
+    if (w0 == w1) return;  // written by the attention kernel
+    float m, l;
+    head_sum(a, b, h, w0, w1, &m, &l);
+    for (int d = tid; d < D; d += kJoinThreads) {
+      float o = 0.0f;
+      for (int w = w0; w <= w1; ++w) {
+        const float pm = a.part_m[int64_t(w + b) * a.H + h];
+        const float s = pm == -INFINITY ? 0.0f : exp2f(pm - m);
+        o = fmaf(s, a.part_o[(int64_t(w + b) * a.H + h) * D + d], o);
+      }
+      a.out[int64_t(blockIdx.x) * D + d] = f32_to_bf16(l == 0.0f ? 0.0f : o / l);
+    }
+    return;
+  }
+  for (int i = tid / 64; i < a.G; i += kJoinThreads / 64) {
+    float m, l;
+    head_sum(a, b, kvh * a.G + i, w0, w1, &m, &l);
+    if (tid % 64 == 0) {
+      head_m[i] = m == -INFINITY ? 0.0f : m + kDown;
+      head_r[i] = l == 0.0f ? 0.0f : 1.0f / l;
+    }
+  }
+  __syncthreads();
+  float* weights = a.pool.weights + (int64_t(b) * a.pool.Hkv + kvh) * a.pool.wstride;
+  const float* scores = a.scores + (int64_t(b) * a.H + kvh * a.G) * a.srows;
+  for (int row = row0 + tid; row < row0 + kWeightRows && row < span.n; row += kJoinThreads) {
+    if (row < span.lo) continue;
+    float sum = 0.0f;
+    for (int i = 0; i < a.G; ++i)
+      sum += __builtin_amdgcn_exp2f(scores[i * a.srows + row] - head_m[i]) * head_r[i];
+    weights[row] += sum;
+  }
+}
+
+// Workgroups wanted over all KV heads: enough that every CU has several.
+constexpr int kTargetWgs = 1024;
+
+struct Plan {
+  int groups16, W;
+  int64_t srows;
+  size_t slots, bytes;
+};
+
+// Host plan of a call that check() accepted. False where H or max_rows is out
+// of range.
+bool plan_of(const tqkv_paged_kv* kv, int32_t H, int64_t max_rows, Plan* out) {
+  if (H < 1 || H % kv->kv_heads != 0 || H / kv->kv_heads > 32 || max_rows < 1 ||
+      max_rows > kv->table_stride * kv->page_rows)
+    return false;
+  Plan p;
+  p.groups16 = (H / kv->kv_heads + 15) / 16;
+  p.srows = (max_rows + kTile - 1) / kTile * kTile;
+  const int64_t units = int64_t(kv->kv_heads) * p.groups16;
+  int64_t W = (kTargetWgs + units - 1) / units;
+  // No more than the longest possible batch fills.
+  const int64_t most = (int64_t(kv->batch) * (p.srows / kTile) + kMinTiles - 1) / kMinTiles;
+  if (W > most) W = most;
+  p.W = int(W);
+  p.slots = size_t(p.W) + kv->batch;
+  size_t floats = p.slots * H * (size_t(kv->dim) + 2);
+  floats = (floats + 3) / 4 * 4;
+  if (kv->weights) floats += size_t(kv->batch) * H * size_t(p.srows);
+  p.bytes = floats * sizeof(float);
+  *out = p;
+  return true;
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace tqkv
+
+extern "C" size_t tqkv_paged_decode_workspace_size(const tqkv_paged_kv* kv, int32_t H,
+                                                   int64_t max_rows) {
+  tqkv::paged::Pool pool;
+  tqkv::paged::Plan plan;
+  if (tqkv::paged::check(kv, &pool) != TQKV_OK || !tqkv::paged::plan_of(kv, H, max_rows, &plan))
+    return 0;
+  return plan.bytes;
+}
+
+extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint16_t* q,
+                                            int64_t q_stride, int32_t H, float scale,
+                                            int64_t window, int64_t max_rows, uint16_t* out,
+                                            void* workspace, size_t workspace_bytes,
+                                            tqkv_stream stream) {
+  using namespace tqkv;
+  using namespace tqkv::paged;
+  DecodeArgs a{};
+  if (int32_t rc = check(kv, &a.pool)) return rc;
+  if (!q || !out) return fail(TQKV_EINVAL_ARG, "null pointer");
+  if (!aligned(q, 16) || !aligned(out, 2) || q_stride % 8 != 0)
+    return fail(TQKV_EINVAL_ARG, "q is 16-byte aligned and q_stride (%lld) a multiple of 8",
+                (long long)q_stride);
+  Plan plan;
+  if (H >= 1 && H % kv->kv_heads == 0 && H / kv->kv_heads > 32)
+    return fail(TQKV_EUNSUPPORTED, "%d query heads a KV head", H / kv->kv_heads);
+  if (!plan_of(kv, H, max_rows, &plan))
+    return fail(TQKV_EINVAL_SHAPE, "H=%d kv_heads=%d max_rows=%lld", H, kv->kv_heads,
+                (long long)max_rows);
+  a.window = window > 0 && window < max_rows ? int(window) : 0;
+  const int64_t seen = a.window > 0 ? a.window + kTile : plan.srows;
+  const int row_blocks = kv->weights ? int((seen + kWeightRows - 1) / kWeightRows) : 0;
+  const int64_t blocks = int64_t(kv->batch) * H + int64_t(kv->batch) * kv->kv_heads * row_blocks;
+  // Tile numbers over the whole batch are 32-bit in the kernels, and a grid
+  // holds below 2^32 threads.
+  if (int64_t(kv->batch) * (plan.srows / kTile + 1) > 0x7fffffffLL ||
+      blocks > 0xffffffffLL / kJoinThreads)
+    return fail(TQKV_EUNSUPPORTED, "batch=%d max_rows=%lld", kv->batch, (long long)max_rows);
+  if (!workspace) {
+    if (int32_t rc = scratch_for_current_device(plan.bytes, &workspace)) return rc;
+  } else if (workspace_bytes < plan.bytes || !aligned(workspace, 16)) {
+    return fail(TQKV_EINVAL_ARG, "workspace of %zu bytes (16-byte aligned), need %zu",
+                workspace_bytes, plan.bytes);
+  }
+  const int D = kv->dim;
+  for (int i = 0; i < 6; ++i) a.slot[i] = kv->slot[i];
+  a.q = q;
+  a.qstride = q_stride;
+  a.out = out;
+  a.H = H;
+  a.G = H / kv->kv_heads;
+  a.groups16 = plan.groups16;
+  a.max_rows = int(max_rows);
+  a.W = plan.W;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_m = a.part_o + plan.slots * H * D;
+  a.part_l = a.part_m + plan.slots * H;
+  a.srows = plan.srows;
+  if (kv->weights)
+    a.scores = static_cast<float*>(workspace) + (plan.slots * H * (size_t(D) + 2) + 3) / 4 * 4;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid(unsigned(a.W), unsigned(kv->kv_heads * a.groups16));
+  if (kv->kind == TQKV_CACHE_BF16) {
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, st, a);
+    };
+    switch (D) {
+      case 64: go(paged_decode_kernel<Bf16Rows<64>>); break;
+      case 128: go(paged_decode_kernel<Bf16Rows<128>>); break;
+      case 256: go(paged_decode_kernel<Bf16Rows<256>>); break;
+      default: go(paged_decode_kernel<Bf16Rows<512>>); break;
+    }
+  } else {
+    switch (D) {
+      case 64: launch_affine<64>(a, kv->bits_k, kv->bits_v, kv->group_size, grid, st); break;
+      case 128: launch_affine<128>(a, kv->bits_k, kv->bits_v, kv->group_size, grid, st); break;
+      case 256: launch_affine<256>(a, kv->bits_k, kv->bits_v, kv->group_size, grid, st); break;
+      default: launch_affine<512>(a, kv->bits_k, kv->bits_v, kv->group_size, grid, st); break;
+    }
+  }
+  TQKV_LAUNCHED();
+  hipLaunchKernelGGL(paged_join_kernel, dim3(unsigned(blocks)), dim3(kJoinThreads), 0, st, a, D,
+                     row_blocks);
+  TQKV_LAUNCHED();
+  return ok();
+}

@@ -1,0 +1,8 @@
+// Paged decode attention, affine layouts of head dim 64.
+#include "paged_decode.hpp"
+
+namespace tqkv {
+namespace paged {
+template void launch_affine<64>(const DecodeArgs&, int, int, int, dim3, hipStream_t);
+}  // namespace paged
+}  // namespace tqkv

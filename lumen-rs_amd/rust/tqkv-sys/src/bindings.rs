@@ -47,6 +47,25 @@ pub struct tqkv_affine_seg {
 
 #[repr(C)]
 #[derive(Debug, Copy, Clone)]
+pub struct tqkv_paged_kv {
+    pub kind: i32,
+    pub batch: i32,
+    pub kv_heads: i32,
+    pub dim: i32,
+    pub page_rows: i32,
+    pub group_size: i32,
+    pub bits_k: i32,
+    pub bits_v: i32,
+    pub num_pages: i64,
+    pub table_stride: i64,
+    pub slot: [*mut c_void; 6],
+    pub table: *const i32,
+    pub lens: *const i32,
+    pub weights: *mut f32,
+}
+
+#[repr(C)]
+#[derive(Debug, Copy, Clone)]
 pub struct tqkv_cache_config {
     pub kind: i32,
     pub batch: i32,
@@ -132,6 +151,11 @@ extern "C" {
     pub fn tqkv_decode_attend_affine_pages(q: *const u16, B: i32, H: i32, H_kv: i32, D: i32, group_size: i32, bits_k: i32, bits_v: i32, scale: f32, seg: *const tqkv_affine_seg, chosen: *const i32, keep: i32, pages: i64, out: *mut u16, workspace: *mut c_void, workspace_bytes: usize, stream: tqkv_stream) -> i32;
     pub fn tqkv_decode_attend_affine_sparse(q: *const u16, B: i32, H: i32, H_kv: i32, D: i32, group_size: i32, bits_k: i32, bits_v: i32, scale: f32, seg: *const tqkv_affine_seg, key_min: *const u16, key_max: *const u16, max_pages: i64, pages: i64, keep: i32, out: *mut u16, chosen_out: *mut i32, workspace: *mut c_void, workspace_bytes: usize, stream: tqkv_stream) -> i32;
     pub fn tqkv_sparse_workspace_size(B: i32, H: i32, H_kv: i32, D: i32, total_tokens: i64, keep: i32) -> usize;
+    pub fn tqkv_paged_append(kv: *const tqkv_paged_kv, k: *const u16, v: *const u16, starts: *const i32, tokens: i64, token_stride: i64, head_stride: i64, stream: tqkv_stream) -> i32;
+    pub fn tqkv_paged_decode_attend(kv: *const tqkv_paged_kv, q: *const u16, q_stride: i64, H: i32, scale: f32, window: i64, max_rows: i64, out: *mut u16, workspace: *mut c_void, workspace_bytes: usize, stream: tqkv_stream) -> i32;
+    pub fn tqkv_paged_decode_workspace_size(kv: *const tqkv_paged_kv, H: i32, max_rows: i64) -> usize;
+    pub fn tqkv_paged_evict(kv: *const tqkv_paged_kv, budget: i64, sinks: i64, recent: i64, dst_table: *const i32, dst_stride: i64, dst_lens: *mut i32, dst_weights: *mut f32, kept: *mut i32, workspace: *mut c_void, workspace_bytes: usize, stream: tqkv_stream) -> i32;
+    pub fn tqkv_paged_evict_workspace_size(kv: *const tqkv_paged_kv, budget: i64) -> usize;
     pub fn tqkv_decode_kernel_name(H: i32, H_kv: i32, D: i32, group_size: i32, bits_k: i32, bits_v: i32) -> *const c_char;
     pub fn tqkv_decode_kernel_for_rows(H: i32, H_kv: i32, D: i32, group_size: i32, bits_k: i32, bits_v: i32, max_rows: i64) -> *const c_char;
     pub fn tqkv_decode_attend_codebook(q: *const u16, B: i32, H: i32, H_kv: i32, D: i32, scale: f32, rotation: *const f32, centroids_k: *const f32, bits_k: i32, centroids_v: *const f32, bits_v: i32, k_codes: *const u8, k_sigma: *const f32, v_codes: *const u8, v_sigma: *const f32, cap: i64, n: i64, out: *mut u16, workspace: *mut c_void, workspace_bytes: usize, stream: tqkv_stream) -> i32;

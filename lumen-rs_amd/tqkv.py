@@ -69,6 +69,13 @@ class CacheState(ctypes.Structure):
 CACHE_BF16, CACHE_AFFINE, CACHE_CODEBOOK = 0, 1, 2
 
 
+class PagedKv(ctypes.Structure):
+    _fields_ = [("kind", I32), ("batch", I32), ("kv_heads", I32), ("dim", I32),
+                ("page_rows", I32), ("group_size", I32), ("bits_k", I32), ("bits_v", I32),
+                ("num_pages", I64), ("table_stride", I64), ("slot", P * 6), ("table", P),
+                ("lens", P), ("weights", P)]
+
+
 class TqConfig(ctypes.Structure):
     _fields_ = [("head_dim", I32), ("bits", I32), ("qjl_m", I32), ("lloyd_max_iter", I32),
                 ("seed", ctypes.c_uint64)]
@@ -116,6 +123,13 @@ _SIGS = {
     "tqkv_decode_attend_affine_sparse": (I32, [P, I32, I32, I32, I32, I32, I32, I32, F32, P, P,
                                                P, I64, I64, I32, P, P, P, SZ, P]),
     "tqkv_sparse_workspace_size": (SZ, [I32, I32, I32, I32, I64, I32]),
+    "tqkv_paged_append": (I32, [ctypes.POINTER(PagedKv), P, P, P, I64, I64, I64, P]),
+    "tqkv_paged_decode_attend": (I32, [ctypes.POINTER(PagedKv), P, I64, I32, F32, I64, I64, P, P,
+                                       SZ, P]),
+    "tqkv_paged_decode_workspace_size": (SZ, [ctypes.POINTER(PagedKv), I32, I64]),
+    "tqkv_paged_evict": (I32, [ctypes.POINTER(PagedKv), I64, I64, I64, P, I64, P, P, P, P, SZ,
+                               P]),
+    "tqkv_paged_evict_workspace_size": (SZ, [ctypes.POINTER(PagedKv), I64]),
     "tqkv_synth_bf16": (I32, [P, I64, I32, ctypes.c_uint64, F32, F32, P]),
     "tqkv_lloyd_max": (I32, [ctypes.c_uint32, SZ, P, P]),
     "tqkv_rotation_matrix": (I32, [I32, ctypes.c_uint64, P]),
@@ -501,6 +515,40 @@ def decode_attend_affine_sparse(q, B, H, H_kv, D, gs, bits_k, bits_v, scale, seg
 
 def sparse_workspace_size(B, H, H_kv, D, total, keep):
     return lib().tqkv_sparse_workspace_size(B, H, H_kv, D, total, keep)
+
+
+def paged_kv(kind, batch, kv_heads, dim, page_rows, num_pages, slots, table, table_stride, lens,
+             weights=None, group_size=0, bits_k=0, bits_v=0):
+    """A pool of pages and its sequences (tqkv_paged_kv). slots: the pool's
+    device pointers (K, V; or the six affine buffers)."""
+    return PagedKv(kind, batch, kv_heads, dim, page_rows, group_size, bits_k, bits_v, num_pages,
+                   table_stride, (P * 6)(*slots), table, lens, weights)
+
+
+def paged_append(kv, k, v, starts, tokens, token_stride, head_stride, stream=None):
+    """starts None: one token a sequence."""
+    check(lib().tqkv_paged_append(ctypes.byref(kv), k, v, starts, tokens, token_stride,
+                                  head_stride, stream))
+
+
+def paged_decode_attend(kv, q, q_stride, H, scale, max_rows, out, window=-1, workspace=None,
+                        workspace_bytes=0, stream=None):
+    check(lib().tqkv_paged_decode_attend(ctypes.byref(kv), q, q_stride, H, scale, window,
+                                         max_rows, out, workspace, workspace_bytes, stream))
+
+
+def paged_decode_workspace_size(kv, H, max_rows):
+    return lib().tqkv_paged_decode_workspace_size(ctypes.byref(kv), H, max_rows)
+
+
+def paged_evict(kv, budget, sinks, recent, dst_table, dst_stride, dst_lens, dst_weights=None,
+                kept=None, workspace=None, workspace_bytes=0, stream=None):
+    check(lib().tqkv_paged_evict(ctypes.byref(kv), budget, sinks, recent, dst_table, dst_stride,
+                                 dst_lens, dst_weights, kept, workspace, workspace_bytes, stream))
+
+
+def paged_evict_workspace_size(kv, budget):
+    return lib().tqkv_paged_evict_workspace_size(ctypes.byref(kv), budget)
 
 
 def tq_rotate_query(rotation, q, dim, rq, stream=None):
