@@ -14,6 +14,7 @@ namespace {
 
 constexpr int kJoinThreads = 256;
 constexpr int kWeightRows = 1024;  // rows whose weights a workgroup adds
+constexpr int kMaxSegments = 1024;  // of one sequence: the workgroups of a KV head
 
 // Where sequence b's segments lie: its first tile of all, and the totals.
 __device__ __forceinline__ void place(const DecodeArgs& a, int b, int64_t* red, int* first,
@@ -33,31 +34,54 @@ __device__ __forceinline__ void place(const DecodeArgs& a, int b, int64_t* red, 
   *total = int(mine & 0xffffffff);
 }
 
-// Maximum and sum over the segments [w0, w1] of one (sequence, head), by a
-// wavefront: each lane its segments in order, then a butterfly.
-__device__ __forceinline__ void head_sum(const DecodeArgs& a, int b, int h, int w0, int w1,
-                                         float* top, float* sum) {
-  const int lane = threadIdx.x % 64;
-  float m = -INFINITY;
-  for (int w = w0 + lane; w <= w1; w += 64) m = fmaxf(m, a.part_m[int64_t(w + b) * a.H + h]);
+// 2^(m_s - m) of every segment s of one (sequence, head) into LDS, and the sum
+// of the segments' sums by those. All threads call it.
+__device__ __forceinline__ float segment_weights(const DecodeArgs& a, int64_t slot0, int n, int h,
+                                                 float* weight, float* red, float* top) {
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  float pm[kMaxSegments / kJoinThreads], pl[kMaxSegments / kJoinThreads], m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kMaxSegments / kJoinThreads; ++i) {
+    const int s = tid + i * kJoinThreads;
+    pm[i] = s < n ? a.part_m[(slot0 + s) * a.H + h] : -INFINITY;
+    pl[i] = s < n ? a.part_l[(slot0 + s) * a.H + h] : 0.0f;
+    m = fmaxf(m, pm[i]);
+  }
   for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+  __syncthreads();
+  if (lane == 0) red[wave] = m;
+  __syncthreads();
+  for (int w = 0; w < kJoinThreads / 64; ++w) m = fmaxf(m, red[w]);
   float l = 0.0f;
-  for (int w = w0 + lane; w <= w1; w += 64) {
-    const float pm = a.part_m[int64_t(w + b) * a.H + h], pl = a.part_l[int64_t(w + b) * a.H + h];
-    l += pm == -INFINITY ? 0.0f * pl : pl * exp2f(pm - m);
+#pragma unroll
+  for (int i = 0; i < kMaxSegments / kJoinThreads; ++i) {
+    const int s = tid + i * kJoinThreads;
+    const float w = pm[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[i] - m);
+    if (s < n) weight[s] = w;
+    l += w * pl[i];  // a NaN sum stays one
   }
   for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
+  __syncthreads();
+  if (lane == 0) red[wave] = l;
+  __syncthreads();
+  l = 0.0f;
+  for (int w = 0; w < kJoinThreads / 64; ++w) l += red[w];
   *top = m;
-  *sum = l;
+  return l;
 }
 
 // Workgroups [0, batch x H): the output of one (sequence, head) from its
-// segments, in their order. The others: kWeightRows rows of one (sequence, KV
-// head): weights[row] += sum over the group's heads of 2^(s - m) / l.
-__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeArgs a, int D,
+// segments: a quad of channels a thread, the segments dealt over the rows of
+// threads, then the rows in order. The others: kWeightRows rows of one
+// (sequence, KV head), weights[row] += sum over the group's heads of
+// 2^(s - m) / l.
+template <int D>
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeArgs a,
                                                                   int row_blocks) {
-  __shared__ int64_t red[kJoinThreads / 64];
-  __shared__ float head_m[32], head_r[32];
+  constexpr int kQuads = D / 4, kDeal = kJoinThreads / kQuads;
+  __shared__ int64_t red64[kJoinThreads / 64];
+  __shared__ float red[kJoinThreads / 64], weight[kMaxSegments], head_m[32], head_r[32];
+  __shared__ float4 sums[kJoinThreads];
   const int tid = threadIdx.x, outs = a.pool.batch * a.H;
   const bool joins = int(blockIdx.x) < outs;
   int b, h = 0, kvh = 0, block = 0;
@@ -78,28 +102,47 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
   const int row0 = span.lo / kTile * kTile + block * kWeightRows;
   if (!joins && row0 >= span.n) return;
   int first, total;
-  place(a, b, red, &first, &total);
+  place(a, b, red64, &first, &total);
   const int per = tiles_per_wg(total, a.W);
-  const int w0 = first / per, w1 = (first + span.tiles - 1) / per;
+  const int w0 = first / per, n = (first + span.tiles - 1) / per - w0 + 1;
+  const int64_t slot0 = w0 + b;
+  float m;
   if (joins) {
-    if (w0 == w1) return;  // written by the attention kernel
-    float m, l;
-    head_sum(a, b, h, w0, w1, &m, &l);
-    for (int d = tid; d < D; d += kJoinThreads) {
-      float o = 0.0f;
-      for (int w = w0; w <= w1; ++w) {
-        const float pm = a.part_m[int64_t(w + b) * a.H + h];
-        const float s = pm == -INFINITY ? 0.0f : exp2f(pm - m);
-        o = fmaf(s, a.part_o[(int64_t(w + b) * a.H + h) * D + d], o);
+    if (n == 1) return;  // written by the attention kernel
+    const float l = segment_weights(a, slot0, n, h, weight, red, &m);
+    const int quad = tid % kQuads, deal = tid / kQuads;
+    const float* po = a.part_o + (slot0 * a.H + h) * D + 4 * quad;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int s = deal; s < n; s += kDeal) {
+      const float w = weight[s];
+      const float4 y = *reinterpret_cast<const float4*>(po + int64_t(s) * a.H * D);
+      o.x = fmaf(w, y.x, o.x);
+      o.y = fmaf(w, y.y, o.y);
+      o.z = fmaf(w, y.z, o.z);
+      o.w = fmaf(w, y.w, o.w);
+    }
+    sums[tid] = o;
+    __syncthreads();
+    if (deal == 0) {
+      for (int i = 1; i < kDeal; ++i) {
+        const float4 y = sums[i * kQuads + quad];
+        o.x += y.x;
+        o.y += y.y;
+        o.z += y.z;
+        o.w += y.w;
       }
-      a.out[int64_t(blockIdx.x) * D + d] = f32_to_bf16(l == 0.0f ? 0.0f : o / l);
+      const float inv = 1.0f / l;
+      const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+      uint16_t* out = a.out + int64_t(blockIdx.x) * D + 4 * quad;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[i] = f32_to_bf16(l == 0.0f ? 0.0f : v[i]);
     }
     return;
   }
-  for (int i = tid / 64; i < a.G; i += kJoinThreads / 64) {
-    float m, l;
-    head_sum(a, b, kvh * a.G + i, w0, w1, &m, &l);
-    if (tid % 64 == 0) {
+  for (int i = 0; i < a.G; ++i) {
+    const float l = segment_weights(a, slot0, n, kvh * a.G + i, weight, red, &m);
+    if (tid == 0) {
       head_m[i] = m == -INFINITY ? 0.0f : m + kDown;
       head_r[i] = l == 0.0f ? 0.0f : 1.0f / l;
     }
@@ -118,6 +161,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
 
 // Workgroups wanted over all KV heads: enough that every CU has several.
 constexpr int kTargetWgs = 1024;
+static_assert(kTargetWgs <= kMaxSegments, "a join holds a sequence's segments");
 
 struct Plan {
   int groups16, W;
@@ -234,8 +278,15 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
     }
   }
   TQKV_LAUNCHED();
-  hipLaunchKernelGGL(paged_join_kernel, dim3(unsigned(blocks)), dim3(kJoinThreads), 0, st, a, D,
-                     row_blocks);
+  auto join = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(kJoinThreads), 0, st, a, row_blocks);
+  };
+  switch (D) {
+    case 64: join(paged_join_kernel<64>); break;
+    case 128: join(paged_join_kernel<128>); break;
+    case 256: join(paged_join_kernel<256>); break;
+    default: join(paged_join_kernel<512>); break;
+  }
   TQKV_LAUNCHED();
   return ok();
 }

@@ -24,11 +24,12 @@
 // Weights enter as a bf16 pair hi + lo, 16 bits, so their rounding stays below
 // the bf16 output's; the softmax sum is of the unrounded f32 weights.
 //
-// Affine rows: scores use the codes themselves, exact in bf16, one product a
-// group: s = sum_g scale_g (q.c)_g + bias_g sum(q_g). 4-bit codes become
-// bf16 128 + c by one AND-OR a pair, and the 128 goes into the bias. Values
-// are dequantized in f32 and rounded once to bf16, the rows that
-// tqkv_affine_dequantize gives.
+// Affine rows: scores use the codes themselves as f16 subnormals (one AND a
+// pair; the queries enter as f16 in a unit of their own), one product a group,
+// s = sum_g scale_g (q.c)_g + bias_g sum(q_g), and the bias part of all groups
+// is one more product, of the biases as they lie and the query sums in three
+// bf16 parts. Values are dequantized in f32 (one mixed multiply-add a code)
+// and rounded once to bf16, the rows that tqkv_affine_dequantize gives.
 //
 // Bound by HBM: the live rows once. At G heads of 16 the matrix cores do
 // 16 / G times the work that is needed and are still far from busy.
@@ -106,22 +107,36 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 __device__ __forceinline__ float low_f32(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_f32(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
+// Loads of the stream are buffer loads at a wavefront-uniform base (scalar
+// registers) plus a 32-bit lane offset plus a constant. With plain pointers the
+// compiler keeps a 64-bit lane address a load across the loop, tens of
+// registers.
+typedef __amdgpu_buffer_rsrc_t rsrc;
+__device__ __forceinline__ rsrc uniform(const void* p, int64_t offset) {
+  uint64_t x = reinterpret_cast<uint64_t>(p) + uint64_t(offset);
+  asm("" : "+s"(x));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(x), 0, 0x40000000, 0x00027000);
+}
+
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
 // A load of N bytes (2, 4, 8 or a multiple of 16) into words.
 template <int N>
-__device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
+__device__ __forceinline__ void load_words(rsrc base, uint32_t off, uint32_t* w) {
   if constexpr (N == 2) {
-    w[0] = *reinterpret_cast<const uint16_t*>(p);
+    w[0] = __builtin_amdgcn_raw_buffer_load_b16(base, off, 0, 0);
   } else if constexpr (N == 4) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
+    w[0] = __builtin_amdgcn_raw_buffer_load_b32(base, off, 0, 0);
   } else if constexpr (N == 8) {
-    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    const uintx2 x = __builtin_amdgcn_raw_buffer_load_b64(base, off, 0, 0);
     w[0] = x.x;
     w[1] = x.y;
   } else {
     static_assert(N % 16 == 0, "whole 16-byte loads");
 #pragma unroll
     for (int i = 0; i < N / 16; ++i) {
-      const uint4 x = *reinterpret_cast<const uint4*>(p + 16 * i);
+      const uintx4 x = __builtin_amdgcn_raw_buffer_load_b128(base, off + 16 * i, 0, 0);
       w[4 * i] = x.x;
       w[4 * i + 1] = x.y;
       w[4 * i + 2] = x.z;
@@ -130,26 +145,51 @@ __device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
   }
 }
 
-// The two pool row blocks (page, KV head) of a tile's 16-row halves.
-struct Halves {
-  int64_t row[2];  // pool row of the half's first row
-  bool ok[2];
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ halfx8 as_halfx8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint4 x = make_uint4(a, b, c, d);
+  return __builtin_bit_cast(halfx8, x);
+}
+
+// Output += V^T P^T over a step's rows: 8 rows a lane (two halves) or 4.
+template <int HALVES>
+__device__ __forceinline__ floatx4 mfma_pv(const uint32_t (&v)[2 * HALVES],
+                                           const uint32_t (&p)[2 * HALVES], floatx4 c) {
+  if constexpr (HALVES == 2) {
+    return mfma(as_bf16x8(v[0], v[1], v[2], v[3]), as_bf16x8(p[0], p[1], p[2], p[3]), c);
+  } else {
+    const uint2 x = make_uint2(v[0], v[1]), y = make_uint2(p[0], p[1]);
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(shortx4, x),
+                                                     __builtin_bit_cast(shortx4, y), c, 0, 0, 0);
+  }
+}
+
+// The pool rows of a step's 16-row halves (uniform over the wavefront).
+template <int HALVES>
+struct Step {
+  int64_t row[HALVES];  // pool row of the half's first row
+  bool ok[HALVES];
 };
-__device__ __forceinline__ Halves halves_of(const Pool& p, const int32_t* table, int kvh, int tile,
-                                            int n) {
-  Halves h;
+template <int HALVES>
+__device__ __forceinline__ Step<HALVES> step_of(const Pool& p, const int32_t* table, int kvh,
+                                                int step, int n) {
+  Step<HALVES> h;
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int r = tile * kTile + s * 16;
+  for (int s = 0; s < HALVES; ++s) {
+    const int r = (step * HALVES + s) * 16;
     int page = -1;
-    if (r < n) page = table[r >> p.shift];
+    if (r < n) page = __builtin_amdgcn_readfirstlane(table[r >> p.shift]);
     h.ok[s] = page >= 0 && page < p.num_pages;
     h.row[s] = pool_row(p, h.ok[s] ? page : 0, kvh, h.ok[s] ? r & ((1 << p.shift) - 1) : 0);
   }
   return h;
 }
 
-// Channel layout of the values: MFMA j's output row r is channel_of(j, r).
+// Channel layout of the values: product j's output row r is channel
+// (j / kCpl) * 16 kCpl + r * kCpl + j % kCpl.
 template <int D>
 struct Chan {
   static constexpr int kCpl = D >= 128 ? 8 : 4;      // consecutive channels a lane and piece
@@ -161,48 +201,59 @@ struct Chan {
 template <int D>
 struct Bf16Rows {
   static constexpr int kD = D;
+  static constexpr int kHalves = D <= 128 ? 2 : 1;
+  static constexpr int kOcc = D == 64 ? 4 : D == 128 ? 3 : D == 256 ? 2 : 1;  // wavefronts a SIMD
   using C = Chan<D>;
+  using S = Step<kHalves>;
   static constexpr int kChunks = D / 32;
+  static constexpr int kVWords = C::kPieces * C::kCpl / 2;
   struct Q {
     bf16x8 op[kChunks];
+    float mul;
   };
   struct K {
-    uint32_t w[2][D / 32 * 4];
+    uint32_t w[kHalves][kChunks * 4];
   };
   struct V {
-    uint32_t w[8][C::kPieces * C::kCpl / 2];
+    uint32_t w[4 * kHalves][kVWords];
   };
 
   // Channels of (chunk, quarter): 32 chunk + 8 quarter.
-  static __device__ __forceinline__ void load_q(Q& q, const uint16_t* p, bool live, int g) {
+  static __device__ __forceinline__ void load_q(Q& q, rsrc p, bool live, int r, int g,
+                                                float scale_log2) {
+    const uint32_t off = r * (2 * D) + g * 16;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       uint32_t w[4] = {0, 0, 0, 0};
-      if (live) load_words<16>(reinterpret_cast<const char*>(p + c * 32 + g * 8), w);
+      if (live) load_words<16>(p, off + c * 64, w);
       q.op[c] = as_bf16x8(w[0], w[1], w[2], w[3]);
     }
+    q.mul = scale_log2;
   }
-  static __device__ __forceinline__ void load_k(K& k, const DecodeArgs& a, const Halves& h, int r,
+  static __device__ __forceinline__ void load_k(K& k, const DecodeArgs& a, const S& h, int r,
                                                 int g) {
+    const uint32_t off = r * (2 * D) + g * 16;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const char* p = static_cast<const char*>(a.slot[0]) + (h.row[s] + r) * (2 * D) + g * 16;
+    for (int s = 0; s < kHalves; ++s) {
+      const rsrc p = uniform(a.slot[0], h.row[s] * (2 * D));
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) load_words<16>(p + c * 64, k.w[s] + 4 * c);
+      for (int c = 0; c < kChunks; ++c) load_words<16>(p, off + c * 64, k.w[s] + 4 * c);
     }
   }
-  static __device__ __forceinline__ void load_v(V& v, const DecodeArgs& a, const Halves& h, int r,
+  static __device__ __forceinline__ void load_v(V& v, const DecodeArgs& a, const S& h, int r,
                                                 int g) {
+    const uint32_t off = 4 * g * (2 * D) + r * (2 * C::kCpl);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const char* p = static_cast<const char*>(a.slot[1]) +
-                      (h.row[e / 4] + 4 * g + e % 4) * (2 * D) + r * (2 * C::kCpl);
+    for (int s = 0; s < kHalves; ++s) {
+      const rsrc p = uniform(a.slot[1], h.row[s] * (2 * D));
 #pragma unroll
-      for (int x = 0; x < C::kPieces; ++x)
-        load_words<2 * C::kCpl>(p + x * 256, v.w[e] + x * (C::kCpl / 2));
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int x = 0; x < C::kPieces; ++x)
+          load_words<2 * C::kCpl>(p, off + e * (2 * D) + x * 256, v.w[4 * s + e] + x * (C::kCpl / 2));
     }
   }
-  // Scores of half s, unscaled.
+  // Scores of half s, to be multiplied by q.mul.
   static __device__ __forceinline__ floatx4 scores(const Q& q, const K& k, int s) {
     floatx4 acc = {0, 0, 0, 0};
 #pragma unroll
@@ -214,19 +265,22 @@ struct Bf16Rows {
   // The rows for which dead is set hold nothing: zero, whatever lies there.
   static __device__ __forceinline__ void clear(V& v, uint32_t dead) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < 4 * kHalves; ++e)
 #pragma unroll
-      for (int i = 0; i < C::kPieces * C::kCpl / 2; ++i)
-        if (dead >> e & 1) v.w[e][i] = 0;
+      for (int i = 0; i < kVWords; ++i) v.w[e][i] = dead >> e & 1 ? 0 : v.w[e][i];
   }
   template <typename F>
   static __device__ __forceinline__ void values(const V& v, int, F&& product) {
 #pragma unroll
-    for (int i = 0; i < C::kPieces * C::kCpl / 2; ++i) {
-      product(2 * i, as_bf16x8(lows(v.w[0][i], v.w[1][i]), lows(v.w[2][i], v.w[3][i]),
-                               lows(v.w[4][i], v.w[5][i]), lows(v.w[6][i], v.w[7][i])));
-      product(2 * i + 1, as_bf16x8(highs(v.w[0][i], v.w[1][i]), highs(v.w[2][i], v.w[3][i]),
-                                   highs(v.w[4][i], v.w[5][i]), highs(v.w[6][i], v.w[7][i])));
+    for (int i = 0; i < kVWords; ++i) {
+      uint32_t lo[2 * kHalves], hi[2 * kHalves];
+#pragma unroll
+      for (int e = 0; e < 2 * kHalves; ++e) {
+        lo[e] = lows(v.w[2 * e][i], v.w[2 * e + 1][i]);
+        hi[e] = highs(v.w[2 * e][i], v.w[2 * e + 1][i]);
+      }
+      product(2 * i, lo);
+      product(2 * i + 1, hi);
     }
   }
 };
@@ -235,100 +289,136 @@ struct Bf16Rows {
 template <int D, int BK, int BV, int GS>
 struct AffineRows {
   static constexpr int kD = D;
+  static constexpr int kHalves = D <= 128 ? 2 : 1;
+  static constexpr int kOcc = D <= 64 ? 4 : D <= 128 ? 3 : D <= 256 ? 2 : 1;
   using C = Chan<D>;
+  using S = Step<kHalves>;
   static constexpr int NG = D / GS;          // groups a row
   static constexpr int CPG = GS / 32;        // products a group
   static constexpr int kGroupBytes = GS / 4 * BK / 8;  // a lane's codes of a group
-  static constexpr int kGroupWords = (kGroupBytes + 3) / 4;
+  static constexpr int kGroupWords = kGroupBytes / 4;
   static constexpr int kPieceBytes = C::kCpl * BV / 8;
   static constexpr int kPieceWords = (kPieceBytes + 3) / 4;
-  static constexpr int kGpp = 16 * C::kCpl / GS > 0 ? 16 * C::kCpl / GS : 1;  // groups a piece
+  static constexpr int kGpp = 16 * C::kCpl > GS ? 16 * C::kCpl / GS : 1;  // groups a piece
+  static constexpr int kSets = (NG + 7) / 8;           // bias products
+  static constexpr int kBiasBytes = 2 * NG < 16 ? 2 * NG : 16;
   struct Q {
-    bf16x8 op[D / 32];
-    float sum[NG];  // of a group's channels, log2-scaled later with the rest
+    halfx8 op[D / 32];
+    bf16x8 sum[kSets];
+    float mul;
   };
   struct K {
-    uint32_t w[2][NG * kGroupWords];
-    uint32_t s[2][2 * NG], b[2][2 * NG];  // 4 rows x NG scales and biases of each half
+    uint32_t w[kHalves][NG * kGroupWords];
+    uint32_t s[kHalves][2 * NG];     // scales of rows [4 g, 4 g + 4)
+    uint32_t b[kHalves][kSets * 4];  // biases of row r
   };
   struct V {
-    uint32_t w[8][C::kPieces * kPieceWords];
-    uint32_t s[2][2 * NG], b[2][2 * NG];
+    uint32_t w[4 * kHalves][C::kPieces * kPieceWords];
+    uint32_t s[kHalves][2 * NG], b[kHalves][2 * NG];  // of rows [4 g, 4 g + 4)
   };
 
-  // Channels of (group, quarter): group GS + quarter GS / 4, then in order; a
-  // product's eight in the order that unpack() gives the codes.
-  static __device__ __forceinline__ void load_q(Q& q, const uint16_t* p, bool live, int g) {
-#pragma unroll
-    for (int n = 0; n < NG; ++n) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int c = 0; c < CPG; ++c) {
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (live) load_words<16>(reinterpret_cast<const char*>(p + n * GS + g * (GS / 4) + c * 8), w);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum += low_f32(w[i]) + high_f32(w[i]);
-        if (BK == 4)  // (0,4) (1,5) (2,6) (3,7)
-          q.op[n * CPG + c] = as_bf16x8(lows(w[0], w[2]), highs(w[0], w[2]), lows(w[1], w[3]),
-                                        highs(w[1], w[3]));
-        else
-          q.op[n * CPG + c] = as_bf16x8(w[0], w[1], w[2], w[3]);
-      }
-      sum += __shfl_xor(sum, 16, 64);
-      sum += __shfl_xor(sum, 32, 64);
-      q.sum[n] = sum;
-    }
-  }
-  // Scales (or biases) of rows [4 g, 4 g + 4) of both halves.
-  static __device__ __forceinline__ void load_scales(uint32_t (&w)[2][2 * NG], const void* slot,
-                                                     const Halves& h, int g) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const char* p = static_cast<const char*>(slot) + (h.row[s] + 4 * g) * (2 * NG);
-      load_words<8 * NG>(p, w[s]);
-    }
-  }
-  static __device__ __forceinline__ void load_k(K& k, const DecodeArgs& a, const Halves& h, int r,
-                                                int g) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const char* p = static_cast<const char*>(a.slot[0]) + (h.row[s] + r) * (D * BK / 8) +
-                      g * kGroupBytes;
-#pragma unroll
-      for (int n = 0; n < NG; ++n)
-        load_words<kGroupBytes>(p + n * (GS * BK / 8), k.w[s] + n * kGroupWords);
-    }
-    load_scales(k.s, a.slot[1], h, g);
-    load_scales(k.b, a.slot[2], h, g);
-  }
-  static __device__ __forceinline__ void load_v(V& v, const DecodeArgs& a, const Halves& h, int r,
-                                                int g) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const char* p = static_cast<const char*>(a.slot[3]) +
-                      (h.row[e / 4] + 4 * g + e % 4) * (D * BV / 8) + r * kPieceBytes;
-#pragma unroll
-      for (int x = 0; x < C::kPieces; ++x)
-        load_words<kPieceBytes>(p + x * (16 * kPieceBytes), v.w[e] + x * kPieceWords);
-    }
-    load_scales(v.s, a.slot[4], h, g);
-    load_scales(v.b, a.slot[5], h, g);
-  }
-  // Eight codes as bf16: 4 bits, 128 + c of codes (0,4) (1,5) (2,6) (3,7);
-  // 8 bits, the codes in order.
-  static __device__ __forceinline__ bf16x8 unpack(const uint32_t* w) {
+  // The f16 pairs of eight codes, as subnormals c 2^-24 (4-bit codes with an
+  // odd place in their half word: c 2^-20): one AND a pair. 4 bits: codes
+  // (0,4) (1,5)* (2,6) (3,7)*; 8 bits: (0,2) (1,3) (4,6) (5,7).
+  static __device__ __forceinline__ halfx8 unpack(const uint32_t* w) {
     if constexpr (BK == 4) {
-      constexpr uint32_t m = 0x000f000fu, one = 0x43004300u;
-      return as_bf16x8((w[0] & m) | one, ((w[0] >> 4) & m) | one, ((w[0] >> 8) & m) | one,
-                       ((w[0] >> 12) & m) | one);
+      const uint32_t x = w[0], y = x >> 8;
+      return as_halfx8(x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u);
     } else {
-      uint32_t o[4];
+      return as_halfx8(w[0] & 0x00ff00ffu, (w[0] >> 8) & 0x00ff00ffu, w[1] & 0x00ff00ffu,
+                       (w[1] >> 8) & 0x00ff00ffu);
+    }
+  }
+  // Queries as f16 times 2^(14 - E), E the head's largest exponent (so they
+  // lie below 2^15; parts below 2^-28 of the largest lose bits), in unpack's
+  // order; the sums of the groups in the same unit as three bf16 parts, which
+  // hold all bits of an f32, one a quarter. Channels of (group, quarter):
+  // group GS + quarter GS / 4, then in order.
+  static __device__ __forceinline__ void load_q(Q& q, rsrc p, bool live, int r, int g,
+                                                float scale_log2) {
+    const uint32_t off = r * (2 * D) + g * (GS / 2);
+    uint32_t w[D / 32][4];
+    float top = 0.0f;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[c][i] = 0;
+      if (live)
+        load_words<16>(p, off + c / CPG * (2 * GS) + c % CPG * 16, w[c]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        top = fmaxf(top, fmaxf(fabsf(low_f32(w[c][i])), fabsf(high_f32(w[c][i]))));
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    int E = int(__float_as_uint(top) >> 23) - 127;
+    E = E < -100 ? -100 : E;
+    const float up = __uint_as_float(uint32_t(127 + 14 - E) << 23);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      float x[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t x = w[i / 2] >> (16 * (i % 2));
-        o[i] = highs(__float_as_uint(float(x & 0xffu)), __float_as_uint(float((x >> 8) & 0xffu)));
+        x[2 * i] = low_f32(w[c][i]) * up;
+        x[2 * i + 1] = high_f32(w[c][i]) * up;
       }
-      return as_bf16x8(o[0], o[1], o[2], o[3]);
+      halfx8 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int lo = BK == 4 ? i : i / 2 * 4 + i % 2, hi = lo + (BK == 4 ? 4 : 2);
+        const float down = BK == 4 && i % 2 ? 0x1p-4f : 1.0f;
+        o[2 * i] = _Float16(x[lo] * down);
+        o[2 * i + 1] = _Float16(x[hi] * down);
+      }
+      q.op[c] = o;
+    }
+#pragma unroll
+    for (int n = 0; n < 8 * kSets; ++n) {
+      float sum = 0.0f;
+      if (n < NG) {
+#pragma unroll
+        for (int c = n * CPG; c < (n + 1) * CPG; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum += low_f32(w[c][i]) + high_f32(w[c][i]);
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        sum *= up * 0x1p-24f;
+      }
+      const float hi = __bf16(sum), mid = __bf16(sum - hi), lo = __bf16(sum - hi - mid);
+      q.sum[n / 8][n % 8] = __bf16(g == 0 ? hi : g == 1 ? mid : g == 2 ? lo : 0.0f);
+    }
+    q.mul = ldexpf(scale_log2, E + 10);
+  }
+  static __device__ __forceinline__ void load_k(K& k, const DecodeArgs& a, const S& h, int r,
+                                                int g) {
+    const uint32_t off = r * (D * BK / 8) + g * kGroupBytes;
+    const uint32_t soff = g * (8 * NG), boff = r * (2 * NG);
+#pragma unroll
+    for (int s = 0; s < kHalves; ++s) {
+      const rsrc p = uniform(a.slot[0], h.row[s] * (D * BK / 8));
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+        load_words<kGroupBytes>(p, off + n * (GS * BK / 8), k.w[s] + n * kGroupWords);
+      load_words<8 * NG>(uniform(a.slot[1], h.row[s] * (2 * NG)), soff, k.s[s]);
+      const rsrc b = uniform(a.slot[2], h.row[s] * (2 * NG));
+#pragma unroll
+      for (int i = 0; i < kSets; ++i) load_words<kBiasBytes>(b, boff + 16 * i, k.b[s] + 4 * i);
+    }
+  }
+  static __device__ __forceinline__ void load_v(V& v, const DecodeArgs& a, const S& h, int r,
+                                                int g) {
+    const uint32_t off = 4 * g * (D * BV / 8) + r * kPieceBytes, soff = g * (8 * NG);
+#pragma unroll
+    for (int s = 0; s < kHalves; ++s) {
+      const rsrc p = uniform(a.slot[3], h.row[s] * (D * BV / 8));
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int x = 0; x < C::kPieces; ++x)
+          load_words<kPieceBytes>(p, off + e * (D * BV / 8) + x * (16 * kPieceBytes),
+                                  v.w[4 * s + e] + x * kPieceWords);
+      load_words<8 * NG>(uniform(a.slot[4], h.row[s] * (2 * NG)), soff, v.s[s]);
+      load_words<8 * NG>(uniform(a.slot[5], h.row[s] * (2 * NG)), soff, v.b[s]);
     }
   }
   // The f32 of entry (row i of four, group n) of four rows' scales.
@@ -336,70 +426,91 @@ struct AffineRows {
     const int at = i * NG + n;
     return at % 2 ? high_f32(w[at / 2]) : low_f32(w[at / 2]);
   }
+  // The biases' part of all groups in a product, then a scale a group.
   static __device__ __forceinline__ floatx4 scores(const Q& q, const K& k, int s) {
     floatx4 out = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kSets; ++i) {
+      uint32_t b[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int x = 0; x < (kBiasBytes + 3) / 4; ++x) b[x] = k.b[s][4 * i + x];
+      out = mfma(as_bf16x8(b[0], b[1], b[2], b[3]), q.sum[i], out);
+    }
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       floatx4 acc = {0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < CPG; ++c)
-        acc = mfma(unpack(k.w[s] + n * kGroupWords + c * (BK / 4)), q.op[n * CPG + c], acc);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(unpack(k.w[s] + n * kGroupWords + c * (BK / 4)),
+                                                     q.op[n * CPG + c], acc, 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float sc = entry(k.s[s], i, n);
-        float bi = entry(k.b[s], i, n);
-        if (BK == 4) bi = fmaf(-128.0f, sc, bi);
-        out[i] = fmaf(sc, acc[i], fmaf(bi, q.sum[n], out[i]));
-      }
+      for (int i = 0; i < 4; ++i) out[i] = fmaf(entry(k.s[s], i, n), acc[i], out[i]);
     }
     return out;
   }
-  // Dead rows: codes of 0, a scale and a bias of 0.
+  // Dead rows: a scale and a bias of 0.
   static __device__ __forceinline__ void clear(V& v, uint32_t dead) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (!(dead >> e & 1)) continue;
+    for (int e = 0; e < 4 * kHalves; ++e) {
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         const int at = e % 4 * NG + n;
-        const uint32_t keep = at % 2 ? 0x0000ffffu : 0xffff0000u;
+        const uint32_t keep = dead >> e & 1 ? (at % 2 ? 0x0000ffffu : 0xffff0000u) : 0xffffffffu;
         v.s[e / 4][at / 2] &= keep;
         v.b[e / 4][at / 2] &= keep;
       }
     }
   }
-  // The scale of (row e, the lane's group of piece x): of the kGpp
-  // candidates, the one of lane row r.
-  static __device__ __forceinline__ float lane_entry(const uint32_t (&w)[2][2 * NG], int e, int x,
-                                                     int r) {
-    const int first = x * (16 * C::kCpl) / GS;
-    float f = entry(w[e / 4], e % 4, first);
-#pragma unroll
-    for (int c = 1; c < kGpp; ++c)
-      f = r * C::kCpl / GS == c ? entry(w[e / 4], e % 4, first + c) : f;
-    return f;
+  // The f32 of (row e, the lane's group of piece x): sel picks the lane's
+  // half word of the piece's (at most four groups) by one byte permute.
+  static __device__ __forceinline__ float lane_entry(const uint32_t* w, int e, int x, uint32_t sel) {
+    const int first = e % 4 * NG + x * (16 * C::kCpl) / GS;
+    if constexpr (kGpp == 1) {
+      return first % 2 ? high_f32(w[first / 2]) : low_f32(w[first / 2]);
+    } else if constexpr (kGpp == 2) {
+      return __uint_as_float(__builtin_amdgcn_perm(0u, w[first / 2], sel));
+    } else {
+      return __uint_as_float(__builtin_amdgcn_perm(w[first / 2 + 1], w[first / 2], sel));
+    }
+  }
+  // Channel j's f16 subnormal in word-and-mask form.
+  static __device__ __forceinline__ float code(const uint32_t* w, int j, float s24, float s20,
+                                               float b) {
+    uint32_t x;
+    int half;
+    if constexpr (BV == 4) {
+      x = (w[j / 8] >> (j & 2 ? 8 : 0)) & (j & 1 ? 0x00f000f0u : 0x000f000fu);
+      half = j % 8 / 4;
+    } else {
+      x = (w[j / 4] >> (j & 1 ? 8 : 0)) & 0x00ff00ffu;
+      half = j % 4 / 2;
+    }
+    return fmaf(float(__builtin_bit_cast(halfx2, x)[half]), BV == 4 && (j & 1) ? s20 : s24, b);
   }
   template <typename F>
   static __device__ __forceinline__ void values(const V& v, int r, F&& product) {
+    const uint32_t grp = r * C::kCpl / GS;  // the lane's group of a piece
+    const uint32_t sel = ((2 * grp + 1) << 24) | ((2 * grp) << 16) | 0x0c0cu;
 #pragma unroll
     for (int x = 0; x < C::kPieces; ++x) {
-      uint32_t o[C::kCpl][4];
+      uint32_t o[C::kCpl][2 * kHalves];
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float s0 = lane_entry(v.s, e, x, r), b0 = lane_entry(v.b, e, x, r);
-        const float s1 = lane_entry(v.s, e + 1, x, r), b1 = lane_entry(v.b, e + 1, x, r);
+      for (int e = 0; e < 4 * kHalves; e += 2) {
+        float s24[2], s20[2], b[2];
 #pragma unroll
-        for (int j = 0; j < C::kCpl; ++j) {
-          const int bit = j * BV;
-          const uint32_t m = (1u << BV) - 1;
-          const float c0 = float((v.w[e][x * kPieceWords + bit / 32] >> (bit % 32)) & m);
-          const float c1 = float((v.w[e + 1][x * kPieceWords + bit / 32] >> (bit % 32)) & m);
-          o[j][e / 2] = pack_bf16(fmaf(c0, s0, b0), fmaf(c1, s1, b1));
+        for (int i = 0; i < 2; ++i) {
+          const float s = lane_entry(v.s[e / 4], e + i, x, sel);
+          s24[i] = s * 0x1p24f;
+          s20[i] = s * 0x1p20f;
+          b[i] = lane_entry(v.b[e / 4], e + i, x, sel);
         }
+#pragma unroll
+        for (int j = 0; j < C::kCpl; ++j)
+          o[j][e / 2] = pack_bf16(code(v.w[e] + x * kPieceWords, j, s24[0], s20[0], b[0]),
+                                  code(v.w[e + 1] + x * kPieceWords, j, s24[1], s20[1], b[1]));
       }
 #pragma unroll
-      for (int j = 0; j < C::kCpl; ++j)
-        product(x * C::kCpl + j, as_bf16x8(o[j][0], o[j][1], o[j][2], o[j][3]));
+      for (int j = 0; j < C::kCpl; ++j) product(x * C::kCpl + j, o[j]);
     }
   }
 };
@@ -445,8 +556,9 @@ constexpr float kTau = 8.0f;  // log2 by which a score may pass the running maxi
 constexpr float kDown = 40.0f;
 
 template <typename Rows>
-__global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const DecodeArgs a) {
-  constexpr int D = Rows::kD;
+__global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(const DecodeArgs a) {
+  constexpr int D = Rows::kD, HALVES = Rows::kHalves, kRows = 16 * HALVES;  // rows a step
+  constexpr int kSteps = kTile / kRows;                                     // steps a tile
   using C = Chan<D>;
   constexpr int kPiece = 16 * C::kCpl;      // channels the epilogue joins at a time
   constexpr int kStride = kPiece + 4;
@@ -482,14 +594,15 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const DecodeA
     const int end = s1 < x1 ? s1 : x1;
     const bool whole = x == s0 && end == s1;
     const Span span = span_of(a, b);
-    const int n = span.n, lo = span.lo;
-    const int t1 = end - s0 + lo / kTile;
-    int t = __builtin_amdgcn_readfirstlane(x - s0 + lo / kTile + wave);
+    const int n = __builtin_amdgcn_readfirstlane(span.n), lo = __builtin_amdgcn_readfirstlane(span.lo);
+    // Steps: a wavefront takes every fourth.
+    const int t1 = (end - s0 + lo / kTile) * kSteps;
+    int t = __builtin_amdgcn_readfirstlane((x - s0 + lo / kTile) * kSteps + wave);
     x = end;
     const int32_t* table = p.table + b * p.tstride;
 
     typename Rows::Q q;
-    Rows::load_q(q, a.q + b * a.qstride + int64_t(head0 + r) * D, r < live, g);
+    Rows::load_q(q, uniform(a.q, 2 * (b * a.qstride + int64_t(head0) * D)), r < live, r, g, a.scale_log2);
     floatx4 acc[C::kJ];
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) acc[j] = floatx4{0, 0, 0, 0};
@@ -497,27 +610,28 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const DecodeA
 
     typename Rows::K kr;
     typename Rows::V vr;
-    Halves h{};
+    Step<HALVES> h{};
     if (t < t1) {
-      h = halves_of(p, table, kvh, t, n);
+      h = step_of<HALVES>(p, table, kvh, t, n);
       Rows::load_k(kr, a, h, r, g);
       Rows::load_v(vr, a, h, r, g);
     }
     for (; t < t1; t += kWaves) {
-      const Halves hn = t + kWaves < t1 ? halves_of(p, table, kvh, t + kWaves, n) : h;
-      float sc[8];
+      Step<HALVES> hn = h;
+      if (t + kWaves < t1) hn = step_of<HALVES>(p, table, kvh, t + kWaves, n);
+      float sc[4 * HALVES];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < HALVES; ++s) {
         const floatx4 y = Rows::scores(q, kr, s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[4 * s + i] = y[i] * a.scale_log2;
+        for (int i = 0; i < 4; ++i) sc[4 * s + i] = y[i] * q.mul;
       }
       if (t + kWaves < t1) Rows::load_k(kr, a, hn, r, g);
-      const int row0 = t * kTile;
-      if (!(row0 >= lo && row0 + kTile <= n && h.ok[0] && h.ok[1])) {
+      const int row0 = t * kRows;
+      if (!(row0 >= lo && row0 + kRows <= n && h.ok[0] && h.ok[HALVES - 1])) {
         uint32_t dead = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 4 * HALVES; ++e) {
           const int row = row0 + (e / 4) * 16 + 4 * g + e % 4;
           if (row < lo || row >= n || !h.ok[e / 4]) {
             dead |= 1u << e;
@@ -528,26 +642,28 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const DecodeA
       }
       if (a.scores && r < live) {
         float* dst = a.scores + (int64_t(b) * a.H + head0 + r) * a.srows + row0 + 4 * g;
-        *reinterpret_cast<float4*>(dst) = make_float4(sc[0], sc[1], sc[2], sc[3]);
-        *reinterpret_cast<float4*>(dst + 16) = make_float4(sc[4], sc[5], sc[6], sc[7]);
+#pragma unroll
+        for (int s = 0; s < HALVES; ++s)
+          *reinterpret_cast<float4*>(dst + 16 * s) =
+              make_float4(sc[4 * s], sc[4 * s + 1], sc[4 * s + 2], sc[4 * s + 3]);
       }
       float top = sc[0];
 #pragma unroll
-      for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[e]);
+      for (int e = 1; e < 4 * HALVES; ++e) top = fmaxf(top, sc[e]);
       if (__any(top > m + kTau)) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float next = fmaxf(m, top);
-        const float scale = m == -INFINITY ? 0.0f : exp2f(m - next);
+        const float scale = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
         m = next;
         l *= scale;
 #pragma unroll
         for (int j = 0; j < C::kJ; ++j) acc[j] *= scale;
       }
       const float base = m == -INFINITY ? 0.0f : m + kDown;
-      uint32_t hi[4], lw[4];
+      uint32_t hi[2 * HALVES], lw[2 * HALVES];
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
+      for (int e = 0; e < 4 * HALVES; e += 2) {
         const float p0 = __builtin_amdgcn_exp2f(sc[e] - base);
         const float p1 = __builtin_amdgcn_exp2f(sc[e + 1] - base);
         l += p0 + p1;
@@ -555,11 +671,9 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const DecodeA
         hi[e / 2] = w;
         lw[e / 2] = pack_bf16(p0 - low_f32(w), p1 - high_f32(w));
       }
-      const bf16x8 ph = as_bf16x8(hi[0], hi[1], hi[2], hi[3]);
-      const bf16x8 pl = as_bf16x8(lw[0], lw[1], lw[2], lw[3]);
-      Rows::values(vr, r, [&](int j, bf16x8 v) {
-        acc[j] = mfma(v, ph, acc[j]);
-        acc[j] = mfma(v, pl, acc[j]);
+      Rows::values(vr, r, [&](int j, const uint32_t (&v)[2 * HALVES]) {
+        acc[j] = mfma_pv<HALVES>(v, hi, acc[j]);
+        acc[j] = mfma_pv<HALVES>(v, lw, acc[j]);
       });
       if (t + kWaves < t1) Rows::load_v(vr, a, hn, r, g);
       h = hn;
