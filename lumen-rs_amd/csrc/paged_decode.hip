@@ -5,10 +5,10 @@
 namespace tqkv {
 namespace paged {
 
-extern template void launch_affine<64>(const DecodeArgs&, int, int, int, dim3, hipStream_t);
-extern template void launch_affine<128>(const DecodeArgs&, int, int, int, dim3, hipStream_t);
-extern template void launch_affine<256>(const DecodeArgs&, int, int, int, dim3, hipStream_t);
-extern template void launch_affine<512>(const DecodeArgs&, int, int, int, dim3, hipStream_t);
+extern template int launch_affine<64>(const DecodeArgs&, int, int, int, dim3, hipStream_t, bool);
+extern template int launch_affine<128>(const DecodeArgs&, int, int, int, dim3, hipStream_t, bool);
+extern template int launch_affine<256>(const DecodeArgs&, int, int, int, dim3, hipStream_t, bool);
+extern template int launch_affine<512>(const DecodeArgs&, int, int, int, dim3, hipStream_t, bool);
 
 namespace {
 
@@ -16,12 +16,12 @@ constexpr int kJoinThreads = 256;
 constexpr int kWeightRows = 1024;  // rows whose weights a workgroup adds
 constexpr int kMaxSegments = 1024;  // of one sequence: the workgroups of a KV head
 
-// Where sequence b's segments lie: its first tile of all, and the totals.
+// Where sequence b's segments lie: its first unit of all, and the total.
 __device__ __forceinline__ void place(const DecodeArgs& a, int b, int64_t* red, int* first,
                                       int* total) {
-  int64_t mine = 0;  // tiles before b in the high half, all in the low
+  int64_t mine = 0;  // units before b in the high half, all in the low
   for (int i = threadIdx.x; i < a.pool.batch; i += kJoinThreads) {
-    const int64_t t = span_of(a, i).tiles;
+    const int64_t t = span_of(a, i).units;
     mine += t + (i < b ? t << 32 : 0);
   }
   for (int off = 32; off > 0; off >>= 1) mine += __shfl_xor(mine, off, 64);
@@ -99,12 +99,12 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
     for (int d = tid; d < D; d += kJoinThreads) a.out[int64_t(blockIdx.x) * D + d] = 0;
     return;
   }
-  const int row0 = span.lo / kTile * kTile + block * kWeightRows;
+  const int row0 = span.lo + block * kWeightRows;
   if (!joins && row0 >= span.n) return;
   int first, total;
   place(a, b, red64, &first, &total);
-  const int per = tiles_per_wg(total, a.W);
-  const int w0 = first / per, n = (first + span.tiles - 1) / per - w0 + 1;
+  const int per = units_per_wg(total, a.W);
+  const int w0 = (first + a.over) / per, n = (first + span.units - 1) / per - w0 + 1;
   const int64_t slot0 = w0 + b;
   float m;
   if (joins) {
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
   for (int i = 0; i < a.G; ++i) {
     const float l = segment_weights(a, slot0, n, kvh * a.G + i, weight, red, &m);
     if (tid == 0) {
-      head_m[i] = m == -INFINITY ? 0.0f : m + kDown;
+      head_m[i] = m == -INFINITY ? 0.0f : m + a.down;
       head_r[i] = l == 0.0f ? 0.0f : 1.0f / l;
     }
   }
@@ -151,7 +151,6 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
   float* weights = a.pool.weights + (int64_t(b) * a.pool.Hkv + kvh) * a.pool.wstride;
   const float* scores = a.scores + (int64_t(b) * a.H + kvh * a.G) * a.srows;
   for (int row = row0 + tid; row < row0 + kWeightRows && row < span.n; row += kJoinThreads) {
-    if (row < span.lo) continue;
     float sum = 0.0f;
     for (int i = 0; i < a.G; ++i)
       sum += __builtin_amdgcn_exp2f(scores[i * a.srows + row] - head_m[i]) * head_r[i];
@@ -159,30 +158,65 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
   }
 }
 
-// Workgroups wanted over all KV heads: enough that every CU has several.
-constexpr int kTargetWgs = 1024;
-static_assert(kTargetWgs <= kMaxSegments, "a join holds a sequence's segments");
+// The attention kernel of a layout, launched; or only its wavefronts a SIMD.
+int launch(const tqkv_paged_kv* kv, const DecodeArgs& a, dim3 grid, hipStream_t st,
+           bool occupancy) {
+  if (kv->kind == TQKV_CACHE_BF16) {
+    switch (kv->dim) {
+      case 64: return launch_rows<Bf16Rows<64>>(a, grid, st, occupancy);
+      case 128: return launch_rows<Bf16Rows<128>>(a, grid, st, occupancy);
+      case 256: return launch_rows<Bf16Rows<256>>(a, grid, st, occupancy);
+      default: return launch_rows<Bf16Rows<512>>(a, grid, st, occupancy);
+    }
+  }
+  const int bk = kv->bits_k, bv = kv->bits_v, gs = kv->group_size;
+  switch (kv->dim) {
+    case 64: return launch_affine<64>(a, bk, bv, gs, grid, st, occupancy);
+    case 128: return launch_affine<128>(a, bk, bv, gs, grid, st, occupancy);
+    case 256: return launch_affine<256>(a, bk, bv, gs, grid, st, occupancy);
+    default: return launch_affine<512>(a, bk, bv, gs, grid, st, occupancy);
+  }
+}
 
-struct Plan {
-  int groups16, W;
+// Workgroups a CU: as many as fit at once for affine rows, whose loads leave
+// little in flight (16 x 32,768 4-bit rows at D = 256: 240 us with two, 320
+// with one); one for bf16 rows, which fill the memory system with it (131,071
+// rows at D = 128: 95 us, 100 with two, 107 with three).
+int workgroups_a_cu(const tqkv_paged_kv* kv) {
+  if (kv->kind == TQKV_CACHE_BF16) return 1;
+  return launch(kv, DecodeArgs{}, dim3(1), nullptr, true);
+}
+
+// Workgroups wanted over all KV heads: one round of them on 256 CUs.
+constexpr int kCus = 256;
+// Tiles that a sequence's start counts as: its segment's own latencies. 32
+// sequences of 17 to 16,000 4-bit rows: 53 us at 0, 48 at 4, 37 at 8, 34 at
+// 16; 16 of 17 to 8,192 bf16 rows: 29, 19, 17, 20; 8 windows of 1,024 8-bit
+// rows: 17, 18, 18, 20.
+constexpr int kOver = 8;
+static_assert(4 * kCus <= kMaxSegments, "a join holds a sequence's segments");
+
+struct HostPlan {
+  int groups16, W, tile;
   int64_t srows;
   size_t slots, bytes;
 };
 
 // Host plan of a call that check() accepted. False where H or max_rows is out
 // of range.
-bool plan_of(const tqkv_paged_kv* kv, int32_t H, int64_t max_rows, Plan* out) {
+bool plan_of(const tqkv_paged_kv* kv, int32_t H, int64_t max_rows, HostPlan* out) {
   if (H < 1 || H % kv->kv_heads != 0 || H / kv->kv_heads > 32 || max_rows < 1 ||
       max_rows > kv->table_stride * kv->page_rows)
     return false;
-  Plan p;
+  HostPlan p;
+  p.tile = kv->dim == 512 ? kWideTile : kTile;
   p.groups16 = (H / kv->kv_heads + 15) / 16;
-  p.srows = (max_rows + kTile - 1) / kTile * kTile;
+  p.srows = (max_rows + p.tile - 1) / p.tile * p.tile;
   const int64_t units = int64_t(kv->kv_heads) * p.groups16;
-  int64_t W = (kTargetWgs + units - 1) / units;
+  int64_t W = (workgroups_a_cu(kv) * kCus + units - 1) / units;
   // No more than the longest possible batch fills.
-  const int64_t most = (int64_t(kv->batch) * (p.srows / kTile) + kMinTiles - 1) / kMinTiles;
-  if (W > most) W = most;
+  const int64_t most = int64_t(kv->batch) * (p.srows / p.tile + kOver);
+  if (W > (most + kMinUnits - 1) / kMinUnits) W = (most + kMinUnits - 1) / kMinUnits;
   p.W = int(W);
   p.slots = size_t(p.W) + kv->batch;
   size_t floats = p.slots * H * (size_t(kv->dim) + 2);
@@ -200,7 +234,7 @@ bool plan_of(const tqkv_paged_kv* kv, int32_t H, int64_t max_rows, Plan* out) {
 extern "C" size_t tqkv_paged_decode_workspace_size(const tqkv_paged_kv* kv, int32_t H,
                                                    int64_t max_rows) {
   tqkv::paged::Pool pool;
-  tqkv::paged::Plan plan;
+  tqkv::paged::HostPlan plan;
   if (tqkv::paged::check(kv, &pool) != TQKV_OK || !tqkv::paged::plan_of(kv, H, max_rows, &plan))
     return 0;
   return plan.bytes;
@@ -219,19 +253,19 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
   if (!aligned(q, 16) || !aligned(out, 2) || q_stride % 8 != 0)
     return fail(TQKV_EINVAL_ARG, "q is 16-byte aligned and q_stride (%lld) a multiple of 8",
                 (long long)q_stride);
-  Plan plan;
+  HostPlan plan;
   if (H >= 1 && H % kv->kv_heads == 0 && H / kv->kv_heads > 32)
     return fail(TQKV_EUNSUPPORTED, "%d query heads a KV head", H / kv->kv_heads);
   if (!plan_of(kv, H, max_rows, &plan))
     return fail(TQKV_EINVAL_SHAPE, "H=%d kv_heads=%d max_rows=%lld", H, kv->kv_heads,
                 (long long)max_rows);
   a.window = window > 0 && window < max_rows ? int(window) : 0;
-  const int64_t seen = a.window > 0 ? a.window + kTile : plan.srows;
+  const int64_t seen = a.window > 0 ? a.window : max_rows;
   const int row_blocks = kv->weights ? int((seen + kWeightRows - 1) / kWeightRows) : 0;
   const int64_t blocks = int64_t(kv->batch) * H + int64_t(kv->batch) * kv->kv_heads * row_blocks;
   // Tile numbers over the whole batch are 32-bit in the kernels, and a grid
   // holds below 2^32 threads.
-  if (int64_t(kv->batch) * (plan.srows / kTile + 1) > 0x7fffffffLL ||
+  if (int64_t(kv->batch) * (plan.srows / plan.tile + kOver + 1) > 0x7fffffffLL ||
       blocks > 0xffffffffLL / kJoinThreads)
     return fail(TQKV_EUNSUPPORTED, "batch=%d max_rows=%lld", kv->batch, (long long)max_rows);
   if (!workspace) {
@@ -250,7 +284,10 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
   a.groups16 = plan.groups16;
   a.max_rows = int(max_rows);
   a.W = plan.W;
+  a.tile = plan.tile;
+  a.over = kOver;
   a.scale_log2 = scale * 1.44269504088896340736f;
+  a.down = kv->kind == TQKV_CACHE_BF16 ? Bf16Rows<128>::kDown : AffineRows<128, 4, 4, 64>::kDown;
   a.part_o = static_cast<float*>(workspace);
   a.part_m = a.part_o + plan.slots * H * D;
   a.part_l = a.part_m + plan.slots * H;
@@ -259,24 +296,7 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
     a.scores = static_cast<float*>(workspace) + (plan.slots * H * (size_t(D) + 2) + 3) / 4 * 4;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(unsigned(a.W), unsigned(kv->kv_heads * a.groups16));
-  if (kv->kind == TQKV_CACHE_BF16) {
-    auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, st, a);
-    };
-    switch (D) {
-      case 64: go(paged_decode_kernel<Bf16Rows<64>>); break;
-      case 128: go(paged_decode_kernel<Bf16Rows<128>>); break;
-      case 256: go(paged_decode_kernel<Bf16Rows<256>>); break;
-      default: go(paged_decode_kernel<Bf16Rows<512>>); break;
-    }
-  } else {
-    switch (D) {
-      case 64: launch_affine<64>(a, kv->bits_k, kv->bits_v, kv->group_size, grid, st); break;
-      case 128: launch_affine<128>(a, kv->bits_k, kv->bits_v, kv->group_size, grid, st); break;
-      case 256: launch_affine<256>(a, kv->bits_k, kv->bits_v, kv->group_size, grid, st); break;
-      default: launch_affine<512>(a, kv->bits_k, kv->bits_v, kv->group_size, grid, st); break;
-    }
-  }
+  launch(kv, a, grid, st, false);
   TQKV_LAUNCHED();
   auto join = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(kJoinThreads), 0, st, a, row_blocks);

@@ -21,15 +21,17 @@
 //     running maximum, sum and rescaling are the lane's own.
 // V's operand is a channel's eight rows: a lane loads 8 (4 at D = 64)
 // consecutive channels of its eight rows and pairs rows by byte permutes.
-// Weights enter as a bf16 pair hi + lo, 16 bits, so their rounding stays below
-// the bf16 output's; the softmax sum is of the unrounded f32 weights.
+// bf16 rows take the weights as a bf16 pair hi + lo, 16 bits, so their rounding
+// stays below the bf16 output's; the softmax sum is of the unrounded f32
+// weights.
 //
 // Affine rows: scores use the codes themselves as f16 subnormals (one AND a
 // pair; the queries enter as f16 in a unit of their own), one product a group,
 // s = sum_g scale_g (q.c)_g + bias_g sum(q_g), and the bias part of all groups
 // is one more product, of the biases as they lie and the query sums in three
-// bf16 parts. Values are dequantized in f32 (one mixed multiply-add a code)
-// and rounded once to bf16, the rows that tqkv_affine_dequantize gives.
+// bf16 parts. Values are dequantized by one mixed multiply-add a code, f32 to
+// f16 in a unit of the wavefront's, and weights enter as f16 too (each
+// rounded by at most 2^-12 of itself, a sixteenth of a bf16 step).
 //
 // Bound by HBM: the live rows once. At G heads of 16 the matrix cores do
 // 16 / G times the work that is needed and are still far from busy.
@@ -43,8 +45,9 @@ namespace tqkv {
 namespace paged {
 
 constexpr int kWaves = 4;
-constexpr int kTile = 32;
-constexpr int kMinTiles = 4;  // tiles a workgroup at least: one a wavefront
+constexpr int kTile = 32;      // rows of a tile
+constexpr int kWideTile = 64;  // at head dim 512
+constexpr int kMinUnits = 4;   // of a workgroup: a tile a wavefront
 
 struct DecodeArgs {
   Pool pool;
@@ -55,7 +58,10 @@ struct DecodeArgs {
   int H, G, groups16;  // query heads, of a KV head, 16-head sets of those
   int max_rows, window;
   int W;               // workgroups a (KV head, set)
+  int tile;            // rows of a tile
+  int over;            // tiles that a sequence's start counts as
   float scale_log2;
+  float down;      // log2 by which the row format's weights are held lower
   float* part_o;  // [W + batch, H, D]
   float* part_m;  // [W + batch, H]: log2 units
   float* part_l;
@@ -63,21 +69,24 @@ struct DecodeArgs {
   int64_t srows;
 };
 
-// The tiles of sequence b: n rows held, from the window's first.
+// The tiles of sequence b: n rows held, from the window's first, and its units,
+// which the batch is divided by: its tiles and `over` for starting on it.
 struct Span {
-  int n, lo, tiles;
+  int n, lo, tiles, units;
 };
-__device__ __forceinline__ Span span_of(const DecodeArgs& a, int b) {
-  const int most = a.max_rows < a.pool.cap ? a.max_rows : a.pool.cap;
-  const int n = held(a.pool, b, most);
+__device__ __forceinline__ Span span_of_rows(const DecodeArgs& a, int n) {
   const int lo = a.window > 0 && n > a.window ? n - a.window : 0;
-  return {n, lo, n > 0 ? (n + kTile - 1) / kTile - lo / kTile : 0};
+  const int tiles = n > 0 ? (n + a.tile - 1) / a.tile - lo / a.tile : 0;
+  return {n, lo, tiles, n > 0 ? tiles + a.over : 0};
+}
+__device__ __forceinline__ Span span_of(const DecodeArgs& a, int b) {
+  return span_of_rows(a, held(a.pool, b, a.max_rows < a.pool.cap ? a.max_rows : a.pool.cap));
 }
 
-// Tiles a workgroup takes of `total`.
-__device__ __forceinline__ int tiles_per_wg(int total, int W) {
+// Units a workgroup takes of `total`.
+__device__ __forceinline__ int units_per_wg(int total, int W) {
   const int per = (total + W - 1) / W;
-  return per < kMinTiles ? kMinTiles : per;
+  return per < kMinUnits ? kMinUnits : per;
 }
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -114,6 +123,8 @@ __device__ __forceinline__ float high_f32(uint32_t w) { return __uint_as_float(w
 typedef __amdgpu_buffer_rsrc_t rsrc;
 __device__ __forceinline__ rsrc uniform(const void* p, int64_t offset) {
   uint64_t x = reinterpret_cast<uint64_t>(p) + uint64_t(offset);
+  x = uint32_t(__builtin_amdgcn_readfirstlane(int(x))) |
+      uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(x >> 32)))) << 32;
   asm("" : "+s"(x));
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(x), 0, 0x40000000, 0x00027000);
 }
@@ -147,6 +158,7 @@ __device__ __forceinline__ void load_words(rsrc base, uint32_t off, uint32_t* w)
 
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ halfx8 as_halfx8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -154,18 +166,56 @@ __device__ __forceinline__ halfx8 as_halfx8(uint32_t a, uint32_t b, uint32_t c, 
   return __builtin_bit_cast(halfx8, x);
 }
 
-// Output += V^T P^T over a step's rows: 8 rows a lane (two halves) or 4.
-template <int HALVES>
+// Output += V^T P^T over a step's rows, 8 rows a lane (two halves) or 4, of
+// bf16 or f16 operands.
+template <int HALVES, bool F16>
 __device__ __forceinline__ floatx4 mfma_pv(const uint32_t (&v)[2 * HALVES],
                                            const uint32_t (&p)[2 * HALVES], floatx4 c) {
-  if constexpr (HALVES == 2) {
+  if constexpr (HALVES == 2 && F16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(as_halfx8(v[0], v[1], v[2], v[3]),
+                                                  as_halfx8(p[0], p[1], p[2], p[3]), c, 0, 0, 0);
+  } else if constexpr (HALVES == 2) {
     return mfma(as_bf16x8(v[0], v[1], v[2], v[3]), as_bf16x8(p[0], p[1], p[2], p[3]), c);
   } else {
     const uint2 x = make_uint2(v[0], v[1]), y = make_uint2(p[0], p[1]);
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(shortx4, x),
-                                                     __builtin_bit_cast(shortx4, y), c, 0, 0, 0);
+    if constexpr (F16)
+      return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(halfx4, x),
+                                                   __builtin_bit_cast(halfx4, y), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(shortx4, x),
+                                                       __builtin_bit_cast(shortx4, y), c, 0, 0, 0);
   }
 }
+
+// The pages of a wavefront's coming steps, a table entry a lane, two blocks of
+// 64: a step takes its page by a lane read. (Loaded when a step needs it, an
+// entry's wait is also one for every load before it, the step's own values.)
+struct Pages {
+  const int32_t* table;
+  int most;        // entries that may be read
+  int first;       // entry of lane 0 of `now`; `next` holds the 64 behind
+  int now, next;
+  __device__ __forceinline__ int load(int at) const {
+    const int i = at + int(threadIdx.x % 64);
+    return i < most ? table[i] : -1;
+  }
+  __device__ __forceinline__ void start(const int32_t* t, int n, int at) {
+    table = t;
+    most = n;
+    first = at;
+    now = load(at);
+    next = load(at + 64);
+  }
+  // Entry i, not below those asked for before.
+  __device__ __forceinline__ int entry(int i) {
+    while (i >= first + 64) {
+      first += 64;
+      now = next;
+      next = load(first + 64);
+    }
+    return __builtin_amdgcn_readlane(now, i - first);
+  }
+};
 
 // The pool rows of a step's 16-row halves (uniform over the wavefront).
 template <int HALVES>
@@ -174,14 +224,13 @@ struct Step {
   bool ok[HALVES];
 };
 template <int HALVES>
-__device__ __forceinline__ Step<HALVES> step_of(const Pool& p, const int32_t* table, int kvh,
-                                                int step, int n) {
+__device__ __forceinline__ Step<HALVES> step_of(const Pool& p, Pages& pages, int kvh, int step,
+                                                int n) {
   Step<HALVES> h;
 #pragma unroll
   for (int s = 0; s < HALVES; ++s) {
     const int r = (step * HALVES + s) * 16;
-    int page = -1;
-    if (r < n) page = __builtin_amdgcn_readfirstlane(table[r >> p.shift]);
+    const int page = r < n ? pages.entry(r >> p.shift) : -1;
     h.ok[s] = page >= 0 && page < p.num_pages;
     h.row[s] = pool_row(p, h.ok[s] ? page : 0, kvh, h.ok[s] ? r & ((1 << p.shift) - 1) : 0);
   }
@@ -269,18 +318,82 @@ struct Bf16Rows {
 #pragma unroll
       for (int i = 0; i < kVWords; ++i) v.w[e][i] = dead >> e & 1 ? 0 : v.w[e][i];
   }
-  template <typename F>
-  static __device__ __forceinline__ void values(const V& v, int, F&& product) {
+  // Weights are held times 2^-40 (their sum too, so it cancels): 2^30 rows of
+  // weight 2^kTau and values of bf16's largest magnitude stay within f32.
+  // Weights below 2^-86 of the largest vanish.
+  static constexpr float kDown = 40.0f;
+  struct Unit {  // of the accumulators
+    __device__ __forceinline__ float of() const { return 1.0f; }
+  };
+  static __device__ __forceinline__ void accumulate(const V& v, const float (&p)[4 * kHalves],
+                                                    floatx4 (&acc)[C::kJ], Unit&, int) {
+    uint32_t hi[2 * kHalves], lw[2 * kHalves];
+#pragma unroll
+    for (int e = 0; e < 2 * kHalves; ++e) {
+      hi[e] = pack_bf16(p[2 * e], p[2 * e + 1]);
+      lw[e] = pack_bf16(p[2 * e] - low_f32(hi[e]), p[2 * e + 1] - high_f32(hi[e]));
+    }
 #pragma unroll
     for (int i = 0; i < kVWords; ++i) {
-      uint32_t lo[2 * kHalves], hi[2 * kHalves];
+      uint32_t x[2 * kHalves], y[2 * kHalves];
 #pragma unroll
       for (int e = 0; e < 2 * kHalves; ++e) {
-        lo[e] = lows(v.w[2 * e][i], v.w[2 * e + 1][i]);
-        hi[e] = highs(v.w[2 * e][i], v.w[2 * e + 1][i]);
+        x[e] = lows(v.w[2 * e][i], v.w[2 * e + 1][i]);
+        y[e] = highs(v.w[2 * e][i], v.w[2 * e + 1][i]);
       }
-      product(2 * i, lo);
-      product(2 * i + 1, hi);
+      acc[2 * i] = mfma_pv<kHalves, false>(x, hi, acc[2 * i]);
+      acc[2 * i] = mfma_pv<kHalves, false>(x, lw, acc[2 * i]);
+      acc[2 * i + 1] = mfma_pv<kHalves, false>(y, hi, acc[2 * i + 1]);
+      acc[2 * i + 1] = mfma_pv<kHalves, false>(y, lw, acc[2 * i + 1]);
+    }
+  }
+  // The wide kernel's share of the values: the lane's 16 rows of a 64-row tile
+  // at eight channels of the wavefront's 128.
+  static constexpr int kWideOcc = 1;
+  struct Wide {
+    uint32_t w[16][4];
+  };
+  static __device__ __forceinline__ void load_wide(Wide& v, const DecodeArgs& a, const Step<4>& h,
+                                                   int wave, int r, int g) {
+    const uint32_t off = 4 * g * (2 * D) + wave * 256 + r * 16;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const rsrc p = uniform(a.slot[1], h.row[s] * (2 * D));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) load_words<16>(p, off + e * (2 * D), v.w[4 * s + e]);
+    }
+  }
+  static __device__ __forceinline__ void clear_wide(Wide& v, uint32_t dead) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v.w[e][i] = dead >> e & 1 ? 0 : v.w[e][i];
+  }
+  static __device__ __forceinline__ void accumulate_wide(const Wide& v, const float (&p)[16],
+                                                         floatx4 (&acc)[8], Unit&) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t hi[4], lw[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = p[8 * k + 2 * e], p1 = p[8 * k + 2 * e + 1];
+        hi[e] = pack_bf16(p0, p1);
+        lw[e] = pack_bf16(p0 - low_f32(hi[e]), p1 - high_f32(hi[e]));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t x[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = lows(v.w[8 * k + 2 * e][i], v.w[8 * k + 2 * e + 1][i]);
+          y[e] = highs(v.w[8 * k + 2 * e][i], v.w[8 * k + 2 * e + 1][i]);
+        }
+        acc[2 * i] = mfma_pv<2, false>(x, hi, acc[2 * i]);
+        acc[2 * i] = mfma_pv<2, false>(x, lw, acc[2 * i]);
+        acc[2 * i + 1] = mfma_pv<2, false>(y, hi, acc[2 * i + 1]);
+        acc[2 * i + 1] = mfma_pv<2, false>(y, lw, acc[2 * i + 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -290,7 +403,6 @@ template <int D, int BK, int BV, int GS>
 struct AffineRows {
   static constexpr int kD = D;
   static constexpr int kHalves = D <= 128 ? 2 : 1;
-  static constexpr int kOcc = D <= 64 ? 4 : D <= 128 ? 3 : D <= 256 ? 2 : 1;
   using C = Chan<D>;
   using S = Step<kHalves>;
   static constexpr int NG = D / GS;          // groups a row
@@ -316,6 +428,13 @@ struct AffineRows {
     uint32_t w[4 * kHalves][C::kPieces * kPieceWords];
     uint32_t s[kHalves][2 * NG], b[kHalves][2 * NG];  // of rows [4 g, 4 g + 4)
   };
+
+  // Wavefronts a SIMD: by the registers that live across a step, so that none
+  // of them spill in the loop.
+  static constexpr int kLive = kHalves * (NG * kGroupWords + 2 * NG + (NG + 1) / 2) +
+                               4 * kHalves * C::kPieces * kPieceWords + kHalves * 4 * NG + 4 * C::kJ +
+                               D / 8 + 4 * kSets + 1;
+  static constexpr int kOcc = kLive <= 64 ? 4 : kLive <= 100 ? 3 : kLive <= 165 ? 2 : 1;
 
   // The f16 pairs of eight codes, as subnormals c 2^-24 (4-bit codes with an
   // odd place in their half word: c 2^-20): one AND a pair. 4 bits: codes
@@ -473,9 +592,11 @@ struct AffineRows {
       return __uint_as_float(__builtin_amdgcn_perm(w[first / 2 + 1], w[first / 2], sel));
     }
   }
-  // Channel j's f16 subnormal in word-and-mask form.
-  static __device__ __forceinline__ float code(const uint32_t* w, int j, float s24, float s20,
-                                               float b) {
+  // Channel j of a row's piece: scale * code + bias as f16, one mixed
+  // multiply-add. s24: the scale times 2^24 (2^20 for a code with an odd place
+  // in its half word).
+  static __device__ __forceinline__ _Float16 value(const uint32_t* w, int j, float s24, float s20,
+                                                   float b) {
     uint32_t x;
     int half;
     if constexpr (BV == 4) {
@@ -485,49 +606,174 @@ struct AffineRows {
       x = (w[j / 4] >> (j & 1 ? 8 : 0)) & 0x00ff00ffu;
       half = j % 4 / 2;
     }
-    return fmaf(float(__builtin_bit_cast(halfx2, x)[half]), BV == 4 && (j & 1) ? s20 : s24, b);
+    return _Float16(fmaf(float(__builtin_bit_cast(halfx2, x)[half]), BV == 4 && (j & 1) ? s20 : s24, b));
   }
-  template <typename F>
-  static __device__ __forceinline__ void values(const V& v, int r, F&& product) {
+  // Weights are held times 2^7: they reach 2^(7 + kTau) in f16, and those that
+  // f16 loses lie below 2^-32 of the largest, 2^-15 in all at 2^17 rows.
+  static constexpr float kDown = -7.0f;
+  // The accumulators hold values times `up`, a power of two, the wavefront's:
+  // f16 values are at most 2^15, and the largest magnitude that the rows gave
+  // when the unit was taken is near 2^6, so it is taken anew only when a
+  // bound on a value (its scale times the largest code, plus its bias) passes
+  // `cap`, 2^9 times that.
+  struct Unit {
+    float up = 1.0f, cap = 0.0f;
+    __device__ __forceinline__ float of() const { return 1.0f / up; }
+    template <int N>
+    __device__ __forceinline__ void admit(float most, floatx4 (&acc)[N]) {
+      if (!__any(most > cap)) return;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+      int E = int(__float_as_uint(most) >> 23) - 127;
+      E = E < -100 ? -100 : E;
+      const float next = __uint_as_float(uint32_t(127 + 5 - E) << 23);
+      const float turn = next / up;  // both powers of two
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] *= turn;
+      up = next;
+      cap = 0x1p15f / up;
+    }
+  };
+  static __device__ __forceinline__ void accumulate(const V& v, const float (&p)[4 * kHalves],
+                                                    floatx4 (&acc)[C::kJ], Unit& unit, int r) {
+    uint32_t pw[2 * kHalves];
+#pragma unroll
+    for (int e = 0; e < 2 * kHalves; ++e) {
+      const floatx2 x = {p[2 * e], p[2 * e + 1]};
+      pw[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, halfx2));
+    }
     const uint32_t grp = r * C::kCpl / GS;  // the lane's group of a piece
     const uint32_t sel = ((2 * grp + 1) << 24) | ((2 * grp) << 16) | 0x0c0cu;
 #pragma unroll
     for (int x = 0; x < C::kPieces; ++x) {
-      uint32_t o[C::kCpl][2 * kHalves];
+      float s[4 * kHalves], b[4 * kHalves], most = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 4 * kHalves; e += 2) {
-        float s24[2], s20[2], b[2];
+      for (int e = 0; e < 4 * kHalves; ++e) {
+        s[e] = lane_entry(v.s[e / 4], e, x, sel);
+        b[e] = lane_entry(v.b[e / 4], e, x, sel);
+        most = fmaxf(most, fmaf(fabsf(s[e]), float((1 << BV) - 1), fabsf(b[e])));
+      }
+      unit.admit(most, acc);
+      const float up24 = unit.up * 0x1p24f;
+      float s20[4 * kHalves];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float s = lane_entry(v.s[e / 4], e + i, x, sel);
-          s24[i] = s * 0x1p24f;
-          s20[i] = s * 0x1p20f;
-          b[i] = lane_entry(v.b[e / 4], e + i, x, sel);
-        }
-#pragma unroll
-        for (int j = 0; j < C::kCpl; ++j)
-          o[j][e / 2] = pack_bf16(code(v.w[e] + x * kPieceWords, j, s24[0], s20[0], b[0]),
-                                  code(v.w[e + 1] + x * kPieceWords, j, s24[1], s20[1], b[1]));
+      for (int e = 0; e < 4 * kHalves; ++e) {
+        s[e] *= up24;
+        s20[e] = s[e] * 0x1p-4f;
+        b[e] *= unit.up;
       }
 #pragma unroll
-      for (int j = 0; j < C::kCpl; ++j) product(x * C::kCpl + j, o[j]);
+      for (int j = 0; j < C::kCpl; ++j) {
+        uint32_t o[2 * kHalves];
+#pragma unroll
+        for (int e = 0; e < 2 * kHalves; ++e) {
+          const halfx2 y = {
+              value(v.w[2 * e] + x * kPieceWords, j, s[2 * e], s20[2 * e], b[2 * e]),
+              value(v.w[2 * e + 1] + x * kPieceWords, j, s[2 * e + 1], s20[2 * e + 1], b[2 * e + 1])};
+          o[e] = __builtin_bit_cast(uint32_t, y);
+        }
+        acc[x * C::kCpl + j] = mfma_pv<kHalves, true>(o, pw, acc[x * C::kCpl + j]);
+        if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  // The wide kernel's share of the values, as Bf16Rows': codes, and the scale
+  // and bias of the lane's own group of each row.
+  static constexpr int kWideOcc = 1;
+  struct Wide {
+    uint32_t w[16][kPieceWords];
+    uint32_t s[16], b[16];  // bf16
+  };
+  static __device__ __forceinline__ void load_wide(Wide& v, const DecodeArgs& a, const Step<4>& h,
+                                                   int wave, int r, int g) {
+    const uint32_t off = 4 * g * (D * BV / 8) + (16 * wave + r) * kPieceBytes;
+    const uint32_t soff = 4 * g * (2 * NG) + (128 * wave + 8 * r) / GS * 2;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const rsrc p = uniform(a.slot[3], h.row[s] * (D * BV / 8));
+      const rsrc ps = uniform(a.slot[4], h.row[s] * (2 * NG));
+      const rsrc pb = uniform(a.slot[5], h.row[s] * (2 * NG));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        load_words<kPieceBytes>(p, off + e * (D * BV / 8), v.w[4 * s + e]);
+        load_words<2>(ps, soff + e * (2 * NG), &v.s[4 * s + e]);
+        load_words<2>(pb, soff + e * (2 * NG), &v.b[4 * s + e]);
+      }
+    }
+  }
+  static __device__ __forceinline__ void clear_wide(Wide& v, uint32_t dead) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      v.s[e] = dead >> e & 1 ? 0 : v.s[e];
+      v.b[e] = dead >> e & 1 ? 0 : v.b[e];
+    }
+  }
+  static __device__ __forceinline__ void accumulate_wide(const Wide& v, const float (&p)[16],
+                                                         floatx4 (&acc)[8], Unit& unit) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t pw[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const floatx2 x = {p[8 * k + 2 * e], p[8 * k + 2 * e + 1]};
+        pw[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, halfx2));
+      }
+      float s[8], s20[8], b[8], most = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s[e] = low_f32(v.s[8 * k + e]);
+        b[e] = low_f32(v.b[8 * k + e]);
+        most = fmaxf(most, fmaf(fabsf(s[e]), float((1 << BV) - 1), fabsf(b[e])));
+      }
+      unit.admit(most, acc);
+      const float up24 = unit.up * 0x1p24f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s[e] *= up24;
+        s20[e] = s[e] * 0x1p-4f;
+        b[e] *= unit.up;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const halfx2 y = {value(v.w[8 * k + 2 * e], j, s[2 * e], s20[2 * e], b[2 * e]),
+                            value(v.w[8 * k + 2 * e + 1], j, s[2 * e + 1], s20[2 * e + 1], b[2 * e + 1])};
+          o[e] = __builtin_bit_cast(uint32_t, y);
+        }
+        acc[j] = mfma_pv<2, true>(o, pw, acc[j]);
+        if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
 };
 
 // ------------------------------------------------------------------- kernel
-// Exclusive prefix over the batch of the tiles of each sequence, into LDS:
-// start[b], start[batch] = all. All threads call it; batch <= 4 kThreads.
-template <int kThreads>
-__device__ __forceinline__ void lay_out(const DecodeArgs& a, int32_t* start, int32_t* waves) {
+// What the workgroup takes, found from lens: the units of the sequences laid
+// end to end.
+struct Plan {
+  int32_t start[kMaxBatch + 1];  // first unit of each sequence; [batch]: all
+  int32_t rows[kMaxBatch];       // held
+  int32_t waves[kWaves];
+};
+
+// Fills the plan in LDS. All 64 kWaves threads call it.
+__device__ __forceinline__ void lay_out(const DecodeArgs& a, Plan& plan) {
+  constexpr int kThreads = 64 * kWaves, kMost = kMaxBatch / kThreads;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, B = a.pool.batch;
   const int per = (B + kThreads - 1) / kThreads;
-  int mine = 0, t[kMaxBatch / kThreads];
+  int mine = 0, units[kMost];
 #pragma unroll
-  for (int i = 0; i < kMaxBatch / kThreads; ++i) {
+  for (int i = 0; i < kMost; ++i) {
     const int b = tid * per + i;
-    t[i] = i < per && b < B ? span_of(a, b).tiles : 0;
-    mine += t[i];
+    units[i] = 0;
+    if (i < per && b < B) {
+      const Span s = span_of(a, b);
+      plan.rows[b] = s.n;
+      units[i] = s.units;
+    }
+    mine += units[i];
   }
   int incl = mine;
 #pragma unroll
@@ -535,25 +781,62 @@ __device__ __forceinline__ void lay_out(const DecodeArgs& a, int32_t* start, int
     const int y = __shfl_up(incl, off, 64);
     if (lane >= off) incl += y;
   }
-  if (lane == 63) waves[wave] = incl;
+  if (lane == 63) plan.waves[wave] = incl;
   __syncthreads();
   int at = incl - mine;
-  for (int w = 0; w < wave; ++w) at += waves[w];
+  for (int w = 0; w < wave; ++w) at += plan.waves[w];
 #pragma unroll
-  for (int i = 0; i < kMaxBatch / kThreads; ++i) {
+  for (int i = 0; i < kMost; ++i) {
     const int b = tid * per + i;
-    if (i < per && b < B) start[b] = at;
-    at += t[i];
+    if (i < per && b < B) plan.start[b] = at;
+    at += units[i];
   }
-  if (tid == kThreads - 1) start[B] = at;
+  if (tid == kThreads - 1) plan.start[B] = at;
   __syncthreads();
 }
 
+// The workgroup's segments, one after the other (all values uniform).
+struct Walk {
+  int x, x1, b;          // next unit, the end, the sequence it is in
+  int seq, n, lo;        // the segment's sequence, its rows held and first row
+  int t0, t1;            // its tiles
+  bool whole;            // the whole sequence
+  // Kept in scalar registers: the loops over it branch as one.
+  static __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+  __device__ __forceinline__ void start(const Plan& plan, int batch, int W) {
+    const int total = scalar(plan.start[batch]), per = units_per_wg(total, W);
+    x = int(blockIdx.x) * per;
+    x1 = x + per < total ? x + per : total;
+    b = 0;
+    int hi = batch;  // b: the last sequence that starts at or before x
+    while (hi - b > 1) {
+      const int mid = (b + hi) / 2;
+      if (scalar(plan.start[mid]) <= x) b = mid;
+      else hi = mid;
+    }
+  }
+  __device__ __forceinline__ bool next(const DecodeArgs& a, const Plan& plan) {
+    while (x < x1) {
+      const int s0 = scalar(plan.start[b]), s1 = scalar(plan.start[b + 1]);
+      seq = b++;
+      if (s1 <= x) continue;
+      const int end = s1 < x1 ? s1 : x1;
+      const int u0 = x - s0 - a.over, u1 = end - s0 - a.over;
+      x = end;
+      if (u1 <= 0) continue;  // only the units for starting on it
+      const Span s = span_of_rows(a, scalar(plan.rows[seq]));
+      n = s.n;
+      lo = s.lo;
+      t0 = (u0 < 0 ? 0 : u0) + lo / a.tile;
+      t1 = u1 + lo / a.tile;
+      whole = u0 <= 0 && u1 == s.tiles;
+      return true;
+    }
+    return false;
+  }
+};
+
 constexpr float kTau = 8.0f;  // log2 by which a score may pass the running maximum
-// Weights are held times 2^-40 (their sum too, so it cancels): 2^30 rows of
-// weight 2^8 and values of bf16's largest magnitude stay within f32. Weights
-// below 2^-86 of the largest vanish.
-constexpr float kDown = 40.0f;
 
 template <typename Rows>
 __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(const DecodeArgs a) {
@@ -562,8 +845,7 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
   using C = Chan<D>;
   constexpr int kPiece = 16 * C::kCpl;      // channels the epilogue joins at a time
   constexpr int kStride = kPiece + 4;
-  __shared__ int32_t start[kMaxBatch + 1];
-  __shared__ int32_t wsum[kWaves];
+  __shared__ Plan plan;
   __shared__ float ml[2][kWaves][16];
   __shared__ __attribute__((aligned(16))) float joint[kWaves][16][kStride];
   const Pool& p = a.pool;
@@ -573,33 +855,18 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
   const int live = a.G - 16 * set < 16 ? a.G - 16 * set : 16;  // heads here
   const int head0 = kvh * a.G + 16 * set;
 
-  lay_out<64 * kWaves>(a, start, wsum);
-  const int total = start[p.batch], per = tiles_per_wg(total, a.W);
-  int x = int(blockIdx.x) * per;
-  const int x1 = x + per < total ? x + per : total;
-  if (x >= x1) return;
-  int b = 0;
-  {  // the last sequence that starts at or before x
-    int hi = p.batch;
-    while (hi - b > 1) {
-      const int mid = (b + hi) / 2;
-      if (start[mid] <= x) b = mid;
-      else hi = mid;
-    }
-  }
-  for (; x < x1; ++b) {
-    b = __builtin_amdgcn_readfirstlane(b);
-    const int s0 = start[b], s1 = start[b + 1];
-    if (s1 <= x) continue;
-    const int end = s1 < x1 ? s1 : x1;
-    const bool whole = x == s0 && end == s1;
-    const Span span = span_of(a, b);
-    const int n = __builtin_amdgcn_readfirstlane(span.n), lo = __builtin_amdgcn_readfirstlane(span.lo);
+  lay_out(a, plan);
+  Walk walk;
+  walk.start(plan, p.batch, a.W);
+  while (walk.next(a, plan)) {
+    const int b = walk.seq, n = walk.n, lo = walk.lo;
     // Steps: a wavefront takes every fourth.
-    const int t1 = (end - s0 + lo / kTile) * kSteps;
-    int t = __builtin_amdgcn_readfirstlane((x - s0 + lo / kTile) * kSteps + wave);
-    x = end;
-    const int32_t* table = p.table + b * p.tstride;
+    const int t1 = walk.t1 * kSteps;
+    int t = walk.t0 * kSteps + wave;
+
+    Pages pages;
+    pages.start(p.table + b * p.tstride, (n + (1 << p.shift) - 1) >> p.shift,
+                (t * kRows) >> p.shift);
 
     typename Rows::Q q;
     Rows::load_q(q, uniform(a.q, 2 * (b * a.qstride + int64_t(head0) * D)), r < live, r, g, a.scale_log2);
@@ -607,26 +874,29 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) acc[j] = floatx4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
+    typename Rows::Unit unit;
 
     typename Rows::K kr;
     typename Rows::V vr;
     Step<HALVES> h{};
     if (t < t1) {
-      h = step_of<HALVES>(p, table, kvh, t, n);
+      h = step_of<HALVES>(p, pages, kvh, t, n);
       Rows::load_k(kr, a, h, r, g);
       Rows::load_v(vr, a, h, r, g);
     }
     for (; t < t1; t += kWaves) {
       Step<HALVES> hn = h;
-      if (t + kWaves < t1) hn = step_of<HALVES>(p, table, kvh, t + kWaves, n);
+      if (t + kWaves < t1) hn = step_of<HALVES>(p, pages, kvh, t + kWaves, n);
       float sc[4 * HALVES];
 #pragma unroll
       for (int s = 0; s < HALVES; ++s) {
         const floatx4 y = Rows::scores(q, kr, s);
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[4 * s + i] = y[i] * q.mul;
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (t + kWaves < t1) Rows::load_k(kr, a, hn, r, g);
+      Rows::load_k(kr, a, hn, r, g);
+      __builtin_amdgcn_sched_barrier(0);
       const int row0 = t * kRows;
       if (!(row0 >= lo && row0 + kRows <= n && h.ok[0] && h.ok[HALVES - 1])) {
         uint32_t dead = 0;
@@ -660,22 +930,17 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
 #pragma unroll
         for (int j = 0; j < C::kJ; ++j) acc[j] *= scale;
       }
-      const float base = m == -INFINITY ? 0.0f : m + kDown;
-      uint32_t hi[2 * HALVES], lw[2 * HALVES];
+      const float base = m == -INFINITY ? 0.0f : m + Rows::kDown;
+      float pr[4 * HALVES];
 #pragma unroll
-      for (int e = 0; e < 4 * HALVES; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(sc[e] - base);
-        const float p1 = __builtin_amdgcn_exp2f(sc[e + 1] - base);
-        l += p0 + p1;
-        const uint32_t w = pack_bf16(p0, p1);
-        hi[e / 2] = w;
-        lw[e / 2] = pack_bf16(p0 - low_f32(w), p1 - high_f32(w));
+      for (int e = 0; e < 4 * HALVES; ++e) {
+        pr[e] = __builtin_amdgcn_exp2f(sc[e] - base);
+        l += pr[e];
       }
-      Rows::values(vr, r, [&](int j, const uint32_t (&v)[2 * HALVES]) {
-        acc[j] = mfma_pv<HALVES>(v, hi, acc[j]);
-        acc[j] = mfma_pv<HALVES>(v, lw, acc[j]);
-      });
-      if (t + kWaves < t1) Rows::load_v(vr, a, hn, r, g);
+      Rows::accumulate(vr, pr, acc, unit, r);
+      __builtin_amdgcn_sched_barrier(0);
+      Rows::load_v(vr, a, hn, r, g);
+      __builtin_amdgcn_sched_barrier(0);
       h = hn;
     }
 
@@ -690,7 +955,7 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml[0][w][r]);
-    const float mine = m == -INFINITY ? 0.0f : exp2f(m - top);
+    const float mine = m == -INFINITY ? 0.0f : exp2f(m - top) * unit.of();
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
       sum += ml[0][w][r] == -INFINITY ? 0.0f * ml[1][w][r] : ml[1][w][r] * exp2f(ml[0][w][r] - top);
@@ -725,7 +990,7 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) o += joint[w][hd][ch];
         const int d = x0 * kPiece + ch;
-        if (whole) {
+        if (walk.whole) {
           const float all = ml[1][0][hd];
           a.out[(int64_t(b) * a.H + head0 + hd) * D + d] = f32_to_bf16(all == 0.0f ? 0.0f : o / all);
         } else {
@@ -737,22 +1002,185 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
   }
 }
 
+// A workgroup barrier for LDS only: loads of the stream stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// The 16 rows of a 64-row tile that a wavefront scores. By selects of values: an
+// index would put the tile's rows into memory.
+__device__ __forceinline__ Step<1> quarter_of(const Step<4>& h, int wave) {
+  const int64_t r0 = h.row[0], r1 = h.row[1], r2 = h.row[2], r3 = h.row[3];
+  const int64_t lo = wave & 1 ? r1 : r0, hi = wave & 1 ? r3 : r2;
+  return Step<1>{{wave & 2 ? hi : lo}, {true}};
+}
+
+// Head dim 512. A wavefront of the kernel above would hold 128 accumulators
+// beside 64 query and 64 key registers; here the four wavefronts of a
+// workgroup share a 64-row tile: each scores 16 rows over all channels, the
+// scores meet in LDS (two buffers, one barrier a tile), and each goes over the
+// softmax of all 64 rows by itself and accumulates 128 output channels, which
+// it also writes.
+template <typename Rows>
+__global__ __launch_bounds__(64 * kWaves, Rows::kWideOcc) void paged_wide_kernel(const DecodeArgs a) {
+  constexpr int D = Rows::kD;
+  static_assert(D == 128 * kWaves && Rows::kHalves == 1, "a wavefront takes 128 channels");
+  __shared__ Plan plan;
+  __shared__ float4 tiles[2][16][16];
+  const Pool& p = a.pool;
+  const int tid = threadIdx.x, lane = tid % 64, r = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int kvh = blockIdx.y / a.groups16, set = blockIdx.y % a.groups16;
+  const int live = a.G - 16 * set < 16 ? a.G - 16 * set : 16;
+  const int head0 = kvh * a.G + 16 * set;
+  lay_out(a, plan);
+  Walk walk;
+  walk.start(plan, p.batch, a.W);
+  int buf = 0;
+  while (walk.next(a, plan)) {
+    const int b = walk.seq, n = walk.n, lo = walk.lo, t1 = walk.t1;
+    int t = walk.t0;
+    Pages pages;
+    pages.start(p.table + b * p.tstride, (n + (1 << p.shift) - 1) >> p.shift,
+                (t * kWideTile) >> p.shift);
+    typename Rows::Q q;
+    Rows::load_q(q, uniform(a.q, 2 * (b * a.qstride + int64_t(head0) * D)), r < live, r, g, a.scale_log2);
+    floatx4 acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = floatx4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+    typename Rows::Unit unit;
+    typename Rows::K kr;
+    typename Rows::Wide vr;
+    Step<4> h = step_of<4>(p, pages, kvh, t, n);
+    Rows::load_k(kr, a, quarter_of(h, wave), r, g);
+    Rows::load_wide(vr, a, h, wave, r, g);
+    for (; t < t1; ++t) {
+      Step<4> hn = h;
+      if (t + 1 < t1) hn = step_of<4>(p, pages, kvh, t + 1, n);
+      const floatx4 y = Rows::scores(q, kr, 0);
+      float4 mine = make_float4(y[0] * q.mul, y[1] * q.mul, y[2] * q.mul, y[3] * q.mul);
+      __builtin_amdgcn_sched_barrier(0);
+      Rows::load_k(kr, a, quarter_of(hn, wave), r, g);
+      __builtin_amdgcn_sched_barrier(0);
+      const int row0 = t * kWideTile;
+      const bool full = row0 >= lo && row0 + kWideTile <= n && h.ok[0] && h.ok[1] && h.ok[2] && h.ok[3];
+      uint32_t dead = 0;  // of the lane's 16 rows
+      if (!full) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int row = row0 + (e / 4) * 16 + 4 * g + e % 4;
+          dead |= uint32_t(row < lo || row >= n || !h.ok[e / 4]) << e;
+        }
+        const uint32_t d = dead >> (4 * wave);
+        mine.x = d & 1 ? -INFINITY : mine.x;
+        mine.y = d & 2 ? -INFINITY : mine.y;
+        mine.z = d & 4 ? -INFINITY : mine.z;
+        mine.w = d & 8 ? -INFINITY : mine.w;
+        Rows::clear_wide(vr, dead);
+      }
+      tiles[buf][4 * wave + g][r] = mine;
+      if (a.scores && r < live)
+        *reinterpret_cast<float4*>(a.scores + (int64_t(b) * a.H + head0 + r) * a.srows + row0 +
+                                   16 * wave + 4 * g) = mine;
+      lds_barrier();
+      float pr[16];
+      float top = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const float4 x = tiles[buf][4 * s + g][r];
+        pr[4 * s] = x.x;
+        pr[4 * s + 1] = x.y;
+        pr[4 * s + 2] = x.z;
+        pr[4 * s + 3] = x.w;
+        top = fmaxf(top, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
+      }
+      buf ^= 1;
+      if (__any(top > m + kTau)) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float next = fmaxf(m, top);
+        const float scale = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l *= scale;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] *= scale;
+      }
+      const float base = m == -INFINITY ? 0.0f : m + Rows::kDown;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        pr[e] = __builtin_amdgcn_exp2f(pr[e] - base);
+        l += pr[e];
+      }
+      Rows::accumulate_wide(vr, pr, acc, unit);
+      __builtin_amdgcn_sched_barrier(0);
+      Rows::load_wide(vr, a, hn, wave, r, g);
+      __builtin_amdgcn_sched_barrier(0);
+      h = hn;
+    }
+    // Every wavefront holds the same maximum and sum.
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const int64_t slot = int64_t(blockIdx.x) + b;
+    if (tid < live) {
+      a.part_m[slot * a.H + head0 + tid] = m;
+      a.part_l[slot * a.H + head0 + tid] = l;
+    }
+    if (r < live) {
+      const float of = unit.of(), inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 128 * wave + (4 * g + i) * 8;
+        if (walk.whole) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            w[j] = f32_to_bf16(acc[2 * j][i] * of * inv) |
+                   uint32_t(f32_to_bf16(acc[2 * j + 1][i] * of * inv)) << 16;
+          uint16_t* out = a.out + (int64_t(b) * a.H + head0 + r) * D + d;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) out[j] = uint16_t(w[j / 2] >> (16 * (j % 2)));
+        } else {
+          float4* out = reinterpret_cast<float4*>(a.part_o + (slot * a.H + head0 + r) * D + d);
+          out[0] = make_float4(acc[0][i] * of, acc[1][i] * of, acc[2][i] * of, acc[3][i] * of);
+          out[1] = make_float4(acc[4][i] * of, acc[5][i] * of, acc[6][i] * of, acc[7][i] * of);
+        }
+      }
+    }
+  }
+}
+
 // One affine layout's launch; a unit a head dim (paged_decode_d*.hip).
+// occupancy: no launch, but the wavefronts a SIMD of the layout's kernel.
+template <typename Rows>
+int launch_rows(const DecodeArgs& a, dim3 grid, hipStream_t st, bool occupancy) {
+  if constexpr (Rows::kD == 512) {
+    if (!occupancy)
+      hipLaunchKernelGGL(paged_wide_kernel<Rows>, grid, dim3(64 * kWaves), 0, st, a);
+    return Rows::kWideOcc;
+  } else {
+    if (!occupancy)
+      hipLaunchKernelGGL(paged_decode_kernel<Rows>, grid, dim3(64 * kWaves), 0, st, a);
+    return Rows::kOcc;
+  }
+}
+
 template <int D>
-void launch_affine(const DecodeArgs& a, int bk, int bv, int gs, dim3 grid, hipStream_t st) {
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, st, a);
-  };
+int launch_affine(const DecodeArgs& a, int bk, int bv, int gs, dim3 grid, hipStream_t st,
+                  bool occupancy) {
   auto width = [&](auto group) {
     constexpr int GS = decltype(group)::value;
-    if (bk == 4 && bv == 4) go(paged_decode_kernel<AffineRows<D, 4, 4, GS>>);
-    else if (bk == 4) go(paged_decode_kernel<AffineRows<D, 4, 8, GS>>);
-    else if (bv == 4) go(paged_decode_kernel<AffineRows<D, 8, 4, GS>>);
-    else go(paged_decode_kernel<AffineRows<D, 8, 8, GS>>);
+    if (bk == 4 && bv == 4) return launch_rows<AffineRows<D, 4, 4, GS>>(a, grid, st, occupancy);
+    if (bk == 4) return launch_rows<AffineRows<D, 4, 8, GS>>(a, grid, st, occupancy);
+    if (bv == 4) return launch_rows<AffineRows<D, 8, 4, GS>>(a, grid, st, occupancy);
+    return launch_rows<AffineRows<D, 8, 8, GS>>(a, grid, st, occupancy);
   };
-  if (gs == 32) width(std::integral_constant<int, 32>{});
-  else if (gs == 64) width(std::integral_constant<int, 64>{});
-  else if constexpr (D >= 128) width(std::integral_constant<int, 128>{});
+  if (gs == 32) return width(std::integral_constant<int, 32>{});
+  if (gs == 64) return width(std::integral_constant<int, 64>{});
+  if constexpr (D >= 128) return width(std::integral_constant<int, 128>{});
+  return 1;
 }
 
 }  // namespace paged

@@ -3,6 +3,6 @@
 
 namespace tqkv {
 namespace paged {
-template void launch_affine<64>(const DecodeArgs&, int, int, int, dim3, hipStream_t);
+template int launch_affine<64>(const DecodeArgs&, int, int, int, dim3, hipStream_t, bool);
 }  // namespace paged
 }  // namespace tqkv
