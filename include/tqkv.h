@@ -332,8 +332,8 @@ size_t tqkv_sparse_workspace_size(int32_t B, int32_t H, int32_t H_kv, int32_t D,
  * dim in {64, 128, 256, 512}; page_rows in {16, 32, 64, 128, 256}; batch at
  * most 1024; affine: bits_k and bits_v 4 or 8 each, group_size in {32, 64,
  * 128} dividing dim (bf16 ignores the three). TQKV_EUNSUPPORTED otherwise.
- * slot pointers are 16-byte aligned, and the pool, table, lens and weights
- * belong to the calling thread's current device.
+ * slot pointers and weights are 16-byte aligned, and the pool, table, lens and
+ * weights belong to the calling thread's current device.
  */
 typedef struct tqkv_paged_kv {
   int32_t kind; /* TQKV_CACHE_BF16 or TQKV_CACHE_AFFINE */

@@ -51,10 +51,10 @@ __device__ __forceinline__ void load_lane(const uint16_t* p, float (&v)[kLaneEle
 // takes the exact division only where the product lies within 2^-20 of
 // its value from a rounding boundary k + 1/2 (where the two could round to
 // different integers). The codes are the same bits either way.
-template <int N, bool kFastQuotient = false>
-__device__ __forceinline__ void quantize_elems(const float (&v)[N], int lpg, int bits,
-                                               float& scale_out, float& bias_out,
-                                               uint64_t (&chunk)[N / 8]) {
+// The group's f32 scale and bias, before the bf16 store.
+template <int N>
+__device__ __forceinline__ void group_scale(const float (&v)[N], int lpg, int bits,
+                                            float& scale_out, float& bias_out) {
   // The Metal kernel starts w_min at the dtype's max and w_max at 0.
   float w_min = __uint_as_float(0x7f7f0000u);
   float w_max = 0.0f;
@@ -75,8 +75,17 @@ __device__ __forceinline__ void quantize_elems(const float (&v)[N], int lpg, int
   const float edge = side ? w_min : w_max;
   const float q0 = roundf(edge / scale);
   const bool at_zero = q0 == 0.0f;
-  scale = at_zero ? scale : edge / q0;
-  const float bias = at_zero ? 0.0f : edge;
+  scale_out = at_zero ? scale : edge / q0;
+  bias_out = at_zero ? 0.0f : edge;
+}
+
+template <int N, bool kFastQuotient = false>
+__device__ __forceinline__ void quantize_elems(const float (&v)[N], int lpg, int bits,
+                                               float& scale_out, float& bias_out,
+                                               uint64_t (&chunk)[N / 8]) {
+  float scale, bias;
+  group_scale(v, lpg, bits, scale, bias);
+  const float n_bins = float((1 << bits) - 1);
 
   scale_out = scale;
   bias_out = bias;
@@ -119,6 +128,46 @@ __device__ __forceinline__ void quantize_elems(const float (&v)[N], int lpg, int
 __device__ __forceinline__ LaneCodes quantize_lane(const float (&v)[kLaneElems], int gs, int bits) {
   LaneCodes r;
   quantize_elems<kLaneElems>(v, gs / kLaneElems, bits, r.scale, r.bias, r.chunk);
+  return r;
+}
+
+// The same bits as quantize_lane without a division an element. With y =
+// RN(1 / scale), each step q += (num - q scale) y (the difference exact in an
+// fma) brings q nearer; after the first q is within an ulp of num / scale,
+// and the second then gives the correctly rounded quotient (Markstein, 1990).
+// y must be normal and the scale finite: other groups divide. A code is the
+// quotient clamped at the top (a NaN to the top, as fminf does) and rounded,
+// halves up: adding the float below 1/2 and truncating rounds every value of
+// [0, 255] so, 1/2 less an ulp included; a value below 0 truncates to 0.
+__device__ __forceinline__ LaneCodes quantize_lane_refined(const float (&v)[kLaneElems], int gs,
+                                                           int bits) {
+  LaneCodes r;
+  group_scale(v, gs / kLaneElems, bits, r.scale, r.bias);
+  const float n_bins = float((1 << bits) - 1);
+  const float y = 1.0f / r.scale;
+  float q[kLaneElems];
+  if (__builtin_expect(!(fabsf(r.scale) < 0x1p100f), 0)) {
+#pragma unroll
+    for (int e = 0; e < kLaneElems; ++e) q[e] = (v[e] - r.bias) / r.scale;
+  } else {
+#pragma unroll
+    for (int e = 0; e < kLaneElems; ++e) {
+      const float num = v[e] - r.bias;
+      float x = num * y;
+      x = fmaf(fmaf(-x, r.scale, num), y, x);
+      q[e] = fmaf(fmaf(-x, r.scale, num), y, x);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < kLaneElems / 8; ++h) {
+    uint64_t c = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = fmaxf(fminf(q[8 * h + e], n_bins), 0.0f);
+      c |= uint64_t(uint32_t(x + 0x1.fffffep-2f)) << (bits * e);
+    }
+    r.chunk[h] = c;
+  }
   return r;
 }
 

@@ -41,8 +41,8 @@ int32_t check(const tqkv_paged_kv* kv, Pool* out) {
   for (int i = 0; i < (affine ? 6 : 2); ++i)
     if (!kv->slot[i] || !aligned(kv->slot[i], 16))
       return fail(TQKV_EINVAL_ARG, "slot %d is null or not 16-byte aligned", i);
-  if (!aligned(kv->table, 4) || !aligned(kv->lens, 4) || !aligned(kv->weights, 4))
-    return fail(TQKV_EINVAL_ARG, "table, lens or weights not 4-byte aligned");
+  if (!aligned(kv->table, 4) || !aligned(kv->lens, 4) || !aligned(kv->weights, 16))
+    return fail(TQKV_EINVAL_ARG, "table or lens not 4-byte aligned, or weights not 16-byte");
   int shift = 4;
   while ((1 << shift) < R) ++shift;
   *out = Pool{kv->table,   kv->lens,        kv->weights,
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(kThreads) void append_bf16_kernel(const AppendArgs 
   clear_weights(p, dest, n);
 }
 
-// Affine rows: a lane quantizes 16 elements (aq::quantize_lane, the bits of
+// Affine rows: a lane quantizes 16 elements (the bits of
 // tqkv_affine_quantize), whose 4- or 8-bit codes are whole words, so they are
 // stored from registers. blockIdx.y: K or V.
 template <int D, int BK, int BV>
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kThreads) void append_affine_kernel(const AppendArg
     const int c = i % LPR, h = (i / LPR) % p.Hkv, t = i / LPR / p.Hkv;
     float v[aq::kLaneElems];
     aq::load_lane(x + (t0 + t) * a.ts + h * a.hs + c * aq::kLaneElems, v);
-    const aq::LaneCodes q = aq::quantize_lane(v, a.gs, bits);
+    const aq::LaneCodes q = aq::quantize_lane_refined(v, a.gs, bits);
     if (dest[t].row < 0 || i0 + int(threadIdx.x) >= items) continue;
     const int64_t row = dest[t].row + (int64_t(h) << p.shift);
     uint32_t* out = packed + row * (D * bits / 32) + c * (bits / 2);

@@ -13,7 +13,7 @@ extern template int launch_affine<512>(const DecodeArgs&, int, int, int, dim3, h
 namespace {
 
 constexpr int kJoinThreads = 256;
-constexpr int kWeightRows = 1024;  // rows whose weights a workgroup adds
+constexpr int kWeightRows = 4 * kJoinThreads;  // rows whose weights a workgroup adds
 constexpr int kMaxSegments = 1024;  // of one sequence: the workgroups of a KV head
 
 // Where sequence b's segments lie: its first unit of all, and the total.
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
     for (int d = tid; d < D; d += kJoinThreads) a.out[int64_t(blockIdx.x) * D + d] = 0;
     return;
   }
-  const int row0 = span.lo + block * kWeightRows;
+  const int row0 = span.lo / 4 * 4 + block * kWeightRows;
   if (!joins && row0 >= span.n) return;
   int first, total;
   place(a, b, red64, &first, &total);
@@ -140,9 +140,24 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
     }
     return;
   }
-  for (int i = 0; i < a.G; ++i) {
-    const float l = segment_weights(a, slot0, n, kvh * a.G + i, weight, red, &m);
-    if (tid == 0) {
+  // A wavefront a head.
+  for (int i = tid / 64; i < a.G; i += kJoinThreads / 64) {
+    const int at = kvh * a.G + i, lane = tid % 64;
+    float top = -INFINITY, l = 0.0f;
+    for (int s = lane; s < n; s += 64) {  // the running maximum and sum of the lane's segments
+      const float pm = a.part_m[(slot0 + s) * a.H + at], pl = a.part_l[(slot0 + s) * a.H + at];
+      const float next = fmaxf(top, pm);
+      if (next > -INFINITY)
+        l = l * __builtin_amdgcn_exp2f(top - next) + pl * __builtin_amdgcn_exp2f(pm - next);
+      else
+        l += pl;  // a NaN sum stays one
+      top = next;
+    }
+    m = top;
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    l = top == -INFINITY ? 0.0f * l : l * __builtin_amdgcn_exp2f(top - m);
+    for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
+    if (lane == 0) {
       head_m[i] = m == -INFINITY ? 0.0f : m + a.down;
       head_r[i] = l == 0.0f ? 0.0f : 1.0f / l;
     }
@@ -150,12 +165,24 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
   __syncthreads();
   float* weights = a.pool.weights + (int64_t(b) * a.pool.Hkv + kvh) * a.pool.wstride;
   const float* scores = a.scores + (int64_t(b) * a.H + kvh * a.G) * a.srows;
-  for (int row = row0 + tid; row < row0 + kWeightRows && row < span.n; row += kJoinThreads) {
-    float sum = 0.0f;
-    for (int i = 0; i < a.G; ++i)
-      sum += __builtin_amdgcn_exp2f(scores[i * a.srows + row] - head_m[i]) * head_r[i];
-    weights[row] += sum;
+  const int row = row0 + 4 * tid;
+  if (row >= span.n) return;
+  // Four rows a thread; the scores of rows outside the span are -inf or unset.
+  const float4 old = *reinterpret_cast<const float4*>(weights + row);
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int i = 0; i < a.G; ++i) {
+    const float4 x = *reinterpret_cast<const float4*>(scores + i * a.srows + row);
+    const float hm = head_m[i], hr = head_r[i];
+    sum[0] += __builtin_amdgcn_exp2f(x.x - hm) * hr;
+    sum[1] += __builtin_amdgcn_exp2f(x.y - hm) * hr;
+    sum[2] += __builtin_amdgcn_exp2f(x.z - hm) * hr;
+    sum[3] += __builtin_amdgcn_exp2f(x.w - hm) * hr;
   }
+  const float v[4] = {old.x + sum[0], old.y + sum[1], old.z + sum[2], old.w + sum[3]};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (row + e >= span.lo && row + e < span.n) weights[row + e] = v[e];
 }
 
 // The attention kernel of a layout, launched; or only its wavefronts a SIMD.
@@ -260,7 +287,7 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
     return fail(TQKV_EINVAL_SHAPE, "H=%d kv_heads=%d max_rows=%lld", H, kv->kv_heads,
                 (long long)max_rows);
   a.window = window > 0 && window < max_rows ? int(window) : 0;
-  const int64_t seen = a.window > 0 ? a.window : max_rows;
+  const int64_t seen = a.window > 0 ? a.window + 3 : max_rows;  // from a row of four
   const int row_blocks = kv->weights ? int((seen + kWeightRows - 1) / kWeightRows) : 0;
   const int64_t blocks = int64_t(kv->batch) * H + int64_t(kv->batch) * kv->kv_heads * row_blocks;
   // Tile numbers over the whole batch are 32-bit in the kernels, and a grid

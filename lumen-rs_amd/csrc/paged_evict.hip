@@ -1,13 +1,15 @@
 // Paged cache: eviction by gathered attention weight.
 //
 // Two launches. (1) One workgroup per (sequence, KV head) finds the weight of
-// the last row that still fits (a radix select over the weights' bits, 11, 11
-// and 10 a pass, histograms in LDS), then goes over the rows once more in
-// their order and writes the kept positions, ascending: forced rows (the
-// first `sinks`, the last `recent`) and heavier rows all, rows of exactly that
-// weight while there is room. Bound by latency and by LDS atomics: 4 bytes a
-// row, read four times, from the caches after the first. (2) The gather moves
-// the rows to their new pages, 16 bytes a thread, bound by HBM.
+// the last row that still fits: a radix select over the weights' bits, 11, 11
+// and 10 a pass, histograms in LDS. Then it goes over the rows in their order
+// and writes the kept positions, ascending: heavier rows all, rows of exactly
+// that weight while there is room. The rows that stay anyhow (the first
+// `sinks`, the last `recent`) take part as the heaviest of all. Up to 32,768
+// rows stay in registers between the passes; more are read again, from the
+// caches. Bound by one CU's vector units (every operation a row costs 16
+// cycles a 1,024 rows) and the passes' barriers. (2) The gather moves the rows to their new pages, bound by
+// HBM.
 #include <cmath>
 
 #include "paged.hpp"
@@ -16,46 +18,110 @@ namespace tqkv {
 namespace paged {
 namespace {
 
-constexpr int kSel = 1024;   // threads of the selection
-constexpr int kPer = 4;      // rows a thread an iteration of the last pass
+constexpr int kSel = 1024;        // threads of the selection
+constexpr int kWaves = kSel / 64;
+constexpr int kQuads = 8;         // quads of rows a thread holds
+constexpr int kChunk = kSel * 4 * kQuads;
 constexpr int kBins = 2048;
 
 // Bits that order like the weights: larger is heavier; NaN counts as -inf and
-// -0 as 0.
+// -0 as 0. Between 0x007fffff (-inf) and 0xff800000 (inf).
 __device__ __forceinline__ uint32_t order_bits(float w) {
   w = w != w ? -INFINITY : w + 0.0f;
   const uint32_t u = __float_as_uint(w);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
 
-// Sums x over the workgroup, exclusive, and the total. All threads call it.
-__device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* waves, uint64_t* total) {
+// Sums x over the workgroup, exclusive. All threads call it.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* waves) {
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  uint64_t incl = x;
+  uint32_t incl = x;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t y = __shfl_up(incl, off, 64);
+    const uint32_t y = __shfl_up(incl, off, 64);
     if (lane >= off) incl += y;
   }
-  __syncthreads();  // the last call's sums are read
   if (lane == 63) waves[wave] = incl;
   __syncthreads();
-  uint64_t base = 0, all = 0;
-  for (int w = 0; w < kSel / 64; ++w) {
-    const uint64_t y = waves[w];
-    if (w < wave) base += y;
-    all += y;
+  uint32_t base = incl - x;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) base += w < wave ? waves[w] : 0;
+  return base;
+}
+
+// A wavefront's rows of a chunk: quad k of lane l is the four rows from
+// first + 256 k + 4 l.
+struct Held {
+  uint32_t u[4 * kQuads];
+};
+// Forced rows get all bits set, rows past the end none.
+__device__ __forceinline__ void load_rows(Held& x, const float* w, int first, int quads, int n,
+                                          int lo, int hi) {
+  const int at = first + 4 * int(threadIdx.x % 64);
+  float4 f[kQuads];
+#pragma unroll
+  for (int k = 0; k < kQuads; ++k) {
+    f[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // A quad that starts before n ends within the weights: they are whole pages.
+    if (k < quads && at + 256 * k < n) f[k] = *reinterpret_cast<const float4*>(w + at + 256 * k);
   }
-  *total = all;
-  return base + incl - x;
+#pragma unroll
+  for (int k = 0; k < kQuads; ++k) {
+    const float y[4] = {f[k].x, f[k].y, f[k].z, f[k].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = at + 256 * k + e;
+      uint32_t u = order_bits(y[e]);
+      u = i < lo || i >= hi ? 0xffffffffu : u;
+      x.u[4 * k + e] = k < quads && i < n ? u : 0;
+    }
+  }
+}
+
+// Writes the kept rows of a wavefront's part of a chunk, from out[at] on; ties
+// (rows of bits `edge`) while fewer than `room` came before.
+template <bool kTies>
+__device__ __forceinline__ void write_rows(const Held& x, int first, int quads, uint32_t edge,
+                                           uint32_t room, uint32_t at, uint32_t ties,
+                                           int32_t* out) {
+  const int i0 = first + 4 * int(threadIdx.x % 64);
+#pragma unroll
+  for (int k = 0; k < kQuads; ++k) {
+    if (k >= quads) break;
+    uint64_t stay[4], tie[4];
+    uint32_t s = at, t = ties;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      stay[e] = __ballot(x.u[4 * k + e] > edge);
+      s = __builtin_amdgcn_mbcnt_hi(uint32_t(stay[e] >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(stay[e]), s));
+      at += __popcll(stay[e]);
+      if (kTies) {
+        tie[e] = __ballot(x.u[4 * k + e] == edge);
+        t = __builtin_amdgcn_mbcnt_hi(uint32_t(tie[e] >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(tie[e]), t));
+        ties += __popcll(tie[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t u = x.u[4 * k + e];
+      if (kTies) {
+        if (u > edge || (u == edge && t < room)) out[s + (t < room ? t : room)] = i0 + 256 * k + e;
+        t += u == edge;
+      } else if (u > edge) {
+        out[s] = i0 + 256 * k + e;
+      }
+      s += u > edge;
+    }
+  }
 }
 
 __global__ __launch_bounds__(kSel) void evict_select_kernel(const Pool p, int budget, int sinks,
                                                             int recent, int32_t* __restrict__ kept) {
   __shared__ uint32_t hist[kBins];
-  __shared__ uint64_t waves[kSel / 64];
-  __shared__ uint32_t found[2];  // the digit, and the rows wanted within it
-  const int unit = blockIdx.x, b = unit / p.Hkv, tid = threadIdx.x;
+  __shared__ uint32_t waves[kWaves], counts[2][kWaves];
+  __shared__ uint32_t found[3];  // the digit, the rows wanted within it, the rows it has
+  const int unit = blockIdx.x, b = unit / p.Hkv, tid = threadIdx.x, lane = tid % 64;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int n = held(p, b, p.cap);
   int32_t* out = kept + int64_t(unit) * budget;
   if (n <= budget) {
@@ -64,73 +130,90 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(const Pool p, int bu
   }
   const float* w = p.weights + unit * p.wstride;
   const int lo = sinks, hi = n - recent;  // the rows that compete
-  uint32_t room = uint32_t(budget - sinks - recent);
-  // The threshold: the room-th heaviest of [lo, hi). With no room, above all.
-  uint32_t prefix = 0xffffffffu, mask = 0;
-  if (room > 0) {
-    prefix = 0;
-    const int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
-    for (int pass = 0; pass < 3; ++pass) {
-      const int sh = shifts[pass], bins = 1 << widths[pass];
-      for (int i = tid; i < bins; i += kSel) hist[i] = 0;
-      __syncthreads();
-      for (int i = lo + tid; i < hi; i += kSel) {
-        const uint32_t u = order_bits(w[i]);
-        if ((u & mask) == prefix) atomicAdd(&hist[(u >> sh) & (bins - 1)], 1u);
-      }
-      __syncthreads();
-      // Counts from the heaviest digit down: thread t takes the digits
-      // bins - 1 - 2t and below it.
-      const int d0 = bins - 1 - 2 * tid;
-      const uint32_t c0 = d0 >= 0 ? hist[d0] : 0, c1 = d0 >= 1 ? hist[d0 - 1] : 0;
-      uint64_t all;
-      const uint32_t above = uint32_t(block_scan(c0 + c1, waves, &all));
-      if (above < room && above + c0 >= room) {
-        found[0] = uint32_t(d0);
-        found[1] = room - above;
-      } else if (above + c0 < room && above + c0 + c1 >= room) {
-        found[0] = uint32_t(d0 - 1);
-        found[1] = room - above - c0;
-      }
-      __syncthreads();
-      prefix |= found[0] << sh;
-      mask |= uint32_t(bins - 1) << sh;
-      room = found[1];
-      __syncthreads();
-    }
-  }
-  // room: the rows of exactly the threshold's weight that stay.
-  uint32_t sure0 = 0, ties0 = 0;  // before this iteration
-  for (int base = 0; base < n; base += kSel * kPer) {
-    const int i0 = base + tid * kPer;
-    uint32_t kind[kPer], sure = 0, ties = 0;  // 2 stays, 1 ties, 0 goes
+  // Quads a wavefront: the rows dealt evenly, or a chunk at a time.
+  const bool one = n <= kChunk;
+  const int quads = one ? (n + 256 * kWaves - 1) / (256 * kWaves) : kQuads;
+  const int step = 256 * kWaves * quads, first = 256 * quads * wave;
+  Held x;
+  if (one) load_rows(x, w, first, quads, n, lo, hi);
+  // The threshold: the budget-th heaviest.
+  uint32_t edge = 0, mask = 0, room = uint32_t(budget), have = 0;
+  for (int pass = 0; pass < 3; ++pass) {
+    const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass < 2 ? 2048 : 1024;
+    hist[tid] = 0;
+    hist[tid + kSel] = 0;
+    __syncthreads();
+    for (int base = 0; base < n; base += step) {
+      if (!one) load_rows(x, w, base + first, quads, n, lo, hi);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const int i = i0 + e;
-      kind[e] = 0;
-      if (i < n) {
-        if (i < lo || i >= hi) {
-          kind[e] = 2;
-        } else if (mask) {
-          const uint32_t u = order_bits(w[i]);
-          kind[e] = u > prefix ? 2 : u == prefix ? 1 : 0;
+      for (int k = 0; k < kQuads; ++k) {
+        if (k >= quads) break;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t u = x.u[4 * k + e];
+          if ((u & mask) == edge) atomicAdd(&hist[(u >> sh) & (bins - 1)], 1u);
         }
       }
-      sure += kind[e] == 2;
-      ties += kind[e] == 1;
     }
-    uint64_t all;
-    const uint64_t before = block_scan((uint64_t(sure) << 32) | ties, waves, &all);
-    uint32_t s = sure0 + uint32_t(before >> 32), t = ties0 + uint32_t(before);
+    __syncthreads();
+    // Counts from the heaviest digit down: thread t takes the digits
+    // bins - 1 - 2t and below it.
+    const int d0 = bins - 1 - 2 * tid;
+    const uint32_t c0 = d0 >= 0 ? hist[d0] : 0, c1 = d0 >= 1 ? hist[d0 - 1] : 0;
+    const uint32_t above = block_scan(c0 + c1, waves);
+    if (above < room && above + c0 >= room) {
+      found[0] = uint32_t(d0);
+      found[1] = room - above;
+      found[2] = c0;
+    } else if (above + c0 < room && above + c0 + c1 >= room) {
+      found[0] = uint32_t(d0 - 1);
+      found[1] = room - above - c0;
+      found[2] = c1;
+    }
+    __syncthreads();
+    edge |= found[0] << sh;
+    mask |= uint32_t(bins - 1) << sh;
+    room = found[1];
+    have = found[2];
+  }
+  // Of the `have` rows at the edge, the first `room` stay. Where all do, they
+  // count as above it.
+  const bool ties = have > room;
+  if (!ties) edge -= 1;
+  uint32_t at = 0, tied = 0;  // before this chunk
+  for (int base = 0; base < n; base += step) {
+    if (!one) load_rows(x, w, base + first, quads, n, lo, hi);
+    uint32_t s = 0, t = 0;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const uint32_t at = s + (t < room ? t : room);
-      if (kind[e] == 2 || (kind[e] == 1 && t < room)) out[at] = i0 + e;
-      s += kind[e] == 2;
-      t += kind[e] == 1;
+    for (int k = 0; k < kQuads; ++k) {
+      if (k >= quads) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s += __popcll(__ballot(x.u[4 * k + e] > edge));
+        if (ties) t += __popcll(__ballot(x.u[4 * k + e] == edge));
+      }
     }
-    sure0 += uint32_t(all >> 32);
-    ties0 += uint32_t(all);
+    if (lane == 0) {
+      counts[0][wave] = s;
+      counts[1][wave] = t;
+    }
+    __syncthreads();
+    uint32_t s0 = at, t0 = tied;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const uint32_t cs = counts[0][v], ct = counts[1][v];
+      if (v < wave) {
+        s0 += cs;
+        t0 += ct;
+      }
+      at += cs;
+      tied += ct;
+    }
+    if (ties)
+      write_rows<true>(x, base + first, quads, edge, room, s0, t0, out);
+    else
+      write_rows<false>(x, base + first, quads, edge, 0, s0, 0, out);
+    __syncthreads();
   }
 }
 
@@ -142,13 +225,48 @@ struct MoveArgs {
   int32_t* dst_lens;
   float* dst_weights;
   int budget;
-  void* slot[6];
-  int row_bytes[6];
-  int n_slots;
+  int slots;  // buffers a side
+  void* k[3];
+  void* v[3];
+  int k_shift[3], v_shift[3];  // log2 of a row's bytes: all are powers of two
 };
+
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));  // a 16-byte unit
+
+int log2_of(int x) { return 31 - __builtin_clz(unsigned(x)); }
 
 constexpr int kThreads = 256;
 constexpr int kRows = 64;  // kept rows a workgroup
+
+// Rows of one buffer (2^ks units of type T each) and of another (2^vs), four
+// loads of each in flight a thread. src is a row that can be read also where
+// dst is -1.
+template <typename T>
+__device__ __forceinline__ void move_rows(T* kb, int ks, T* vb, int vs, const int64_t* src,
+                                          const int64_t* dst) {
+  const int items = kRows << (ks > vs ? ks : vs);
+  auto load = [&](const T* buf, int shift, int i) {
+    return buf[(src[(i >> shift) % kRows] << shift) + (i & ((1 << shift) - 1))];
+  };
+  auto store = [&](T* buf, int shift, int i, T x) {
+    const int r = i >> shift;
+    if (r < kRows && dst[r] >= 0) buf[(dst[r] << shift) + (i & ((1 << shift) - 1))] = x;
+  };
+  for (int i = threadIdx.x; i < items; i += 4 * kThreads) {
+    const T x0 = load(kb, ks, i), x1 = load(kb, ks, i + kThreads);
+    const T x2 = load(kb, ks, i + 2 * kThreads), x3 = load(kb, ks, i + 3 * kThreads);
+    const T y0 = load(vb, vs, i), y1 = load(vb, vs, i + kThreads);
+    const T y2 = load(vb, vs, i + 2 * kThreads), y3 = load(vb, vs, i + 3 * kThreads);
+    store(kb, ks, i, x0);
+    store(kb, ks, i + kThreads, x1);
+    store(kb, ks, i + 2 * kThreads, x2);
+    store(kb, ks, i + 3 * kThreads, x3);
+    store(vb, vs, i, y0);
+    store(vb, vs, i + kThreads, y1);
+    store(vb, vs, i + 2 * kThreads, y2);
+    store(vb, vs, i + 3 * kThreads, y3);
+  }
+}
 
 __global__ __launch_bounds__(kThreads) void evict_move_kernel(const MoveArgs a) {
   __shared__ int64_t src[kRows], dst[kRows];
@@ -159,7 +277,7 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(const MoveArgs a) 
   if (tid < kRows) {
     const int i = i0 + tid;
     const int r = i < a.budget ? a.kept[unit * a.budget + i] : -1;
-    int64_t s = -1, d = -1;
+    int64_t s = 0, d = -1;
     if (r >= 0) {
       const int ps = p.table[b * p.tstride + (r >> p.shift)];
       const int pd = a.dst_table[b * a.dst_stride + (i >> p.shift)];
@@ -180,26 +298,19 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(const MoveArgs a) 
     a.dst_lens[b] = n < a.budget ? n : a.budget;
   }
   __syncthreads();
-  for (int k = 0; k < a.n_slots; ++k) {
-    const int bytes = a.row_bytes[k];
-    char* buf = static_cast<char*>(a.slot[k]);
-    if (bytes % 16 == 0) {
-      const int per = bytes / 16;
-      for (int i = tid; i < kRows * per; i += kThreads) {
-        const int r = i / per, c = i % per;
-        if (dst[r] >= 0)
-          *reinterpret_cast<uint4*>(buf + dst[r] * bytes + c * 16) =
-              *reinterpret_cast<const uint4*>(buf + src[r] * bytes + c * 16);
-      }
-    } else {
-      const int per = bytes / 2;
-      for (int i = tid; i < kRows * per; i += kThreads) {
-        const int r = i / per, c = i % per;
-        if (dst[r] >= 0)
-          *reinterpret_cast<uint16_t*>(buf + dst[r] * bytes + c * 2) =
-              *reinterpret_cast<const uint16_t*>(buf + src[r] * bytes + c * 2);
-      }
-    }
+  // Keys and values side by side, so that their loads are in flight together.
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    if (i >= a.slots) break;
+    const int ks = a.k_shift[i], vs = a.v_shift[i];
+    if (ks >= 4 && vs >= 4)
+      move_rows(static_cast<uintx4*>(a.k[i]), ks - 4, static_cast<uintx4*>(a.v[i]), vs - 4, src, dst);
+    else if (ks >= 2)  // scales and biases: rows of one length
+      move_rows(static_cast<uint32_t*>(a.k[i]), ks - 2, static_cast<uint32_t*>(a.v[i]), vs - 2, src,
+                dst);
+    else
+      move_rows(static_cast<uint16_t*>(a.k[i]), ks - 1, static_cast<uint16_t*>(a.v[i]), vs - 1, src,
+                dst);
   }
 }
 
@@ -248,17 +359,14 @@ extern "C" int32_t tqkv_paged_evict(const tqkv_paged_kv* kv, int64_t budget, int
   a.dst_weights = dst_weights;
   a.budget = int(budget);
   const int D = kv->dim;
-  if (kv->kind == TQKV_CACHE_BF16) {
-    a.n_slots = 2;
-    a.row_bytes[0] = a.row_bytes[1] = 2 * D;
-  } else {
-    a.n_slots = 6;
-    for (int s = 0; s < 2; ++s) {
-      a.row_bytes[3 * s] = D * (s ? kv->bits_v : kv->bits_k) / 8;
-      a.row_bytes[3 * s + 1] = a.row_bytes[3 * s + 2] = D / kv->group_size * 2;
-    }
+  a.slots = kv->kind == TQKV_CACHE_BF16 ? 1 : 3;
+  for (int i = 0; i < a.slots; ++i) {
+    a.k[i] = kv->slot[i];
+    a.v[i] = kv->slot[a.slots + i];
+    const int scales = 2 * D / (i > 0 ? kv->group_size : 1);  // bf16 rows also
+    a.k_shift[i] = log2_of(i > 0 || a.slots == 1 ? scales : D * kv->bits_k / 8);
+    a.v_shift[i] = log2_of(i > 0 || a.slots == 1 ? scales : D * kv->bits_v / 8);
   }
-  for (int i = 0; i < a.n_slots; ++i) a.slot[i] = kv->slot[i];
   hipLaunchKernelGGL(evict_move_kernel,
                      dim3(unsigned((budget + kRows - 1) / kRows), unsigned(kv->kv_heads),
                           unsigned(kv->batch)),

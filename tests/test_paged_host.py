@@ -33,7 +33,7 @@ BAD_VIEWS = [
     (dict(dim=64, group_size=128), T.EUNSUPPORTED), (dict(bits_k=3), T.EUNSUPPORTED),
     (dict(bits_v=16), T.EUNSUPPORTED), (dict(table=None), T.EINVAL_ARG),
     (dict(lens=None), T.EINVAL_ARG), (dict(slots=[A] * 5 + [None]), T.EINVAL_ARG),
-    (dict(slots=[A, A + 8] + [A] * 4), T.EINVAL_ARG), (dict(weights=A + 2), T.EINVAL_ARG),
+    (dict(slots=[A, A + 8] + [A] * 4), T.EINVAL_ARG), (dict(weights=A + 4), T.EINVAL_ARG),
     (dict(kind=T.CACHE_BF16, slots=[A, None] + [None] * 4), T.EINVAL_ARG),
 ]
 
