@@ -71,7 +71,7 @@ __device__ __forceinline__ float segment_weights(const DecodeArgs& a, int64_t sl
 }
 
 // Workgroups [0, batch x H): the output of one (sequence, head) from its
-// segments: a quad of channels a thread, the segments dealt over the rows of
+// segments, a quad of channels a thread, the segments dealt over the rows of
 // threads, then the rows in order. The others: kWeightRows rows of one
 // (sequence, KV head), weights[row] += sum over the group's heads of
 // 2^(s - m) / l.
@@ -216,15 +216,12 @@ int workgroups_a_cu(const tqkv_paged_kv* kv) {
 
 // Workgroups wanted over all KV heads: one round of them on 256 CUs.
 constexpr int kCus = 256;
-// Tiles that a sequence's start counts as: its segment's own latencies. 32
-// sequences of 17 to 16,000 4-bit rows: 53 us at 0, 48 at 4, 37 at 8, 34 at
-// 16; 16 of 17 to 8,192 bf16 rows: 29, 19, 17, 20; 8 windows of 1,024 8-bit
-// rows: 17, 18, 18, 20.
-constexpr int kOver = 8;
+// Units that a sequence's start counts as: its segment's own latencies.
+constexpr int kOver = 16;
 static_assert(4 * kCus <= kMaxSegments, "a join holds a sequence's segments");
 
 struct HostPlan {
-  int groups16, W, tile;
+  int groups16, W;
   int64_t srows;
   size_t slots, bytes;
 };
@@ -236,13 +233,12 @@ bool plan_of(const tqkv_paged_kv* kv, int32_t H, int64_t max_rows, HostPlan* out
       max_rows > kv->table_stride * kv->page_rows)
     return false;
   HostPlan p;
-  p.tile = kv->dim == 512 ? kWideTile : kTile;
   p.groups16 = (H / kv->kv_heads + 15) / 16;
-  p.srows = (max_rows + p.tile - 1) / p.tile * p.tile;
+  p.srows = (max_rows + kUnit - 1) / kUnit * kUnit;
   const int64_t units = int64_t(kv->kv_heads) * p.groups16;
   int64_t W = (workgroups_a_cu(kv) * kCus + units - 1) / units;
   // No more than the longest possible batch fills.
-  const int64_t most = int64_t(kv->batch) * (p.srows / p.tile + kOver);
+  const int64_t most = int64_t(kv->batch) * (p.srows / kUnit + kOver);
   if (W > (most + kMinUnits - 1) / kMinUnits) W = (most + kMinUnits - 1) / kMinUnits;
   p.W = int(W);
   p.slots = size_t(p.W) + kv->batch;
@@ -290,9 +286,9 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
   const int64_t seen = a.window > 0 ? a.window + 3 : max_rows;  // from a row of four
   const int row_blocks = kv->weights ? int((seen + kWeightRows - 1) / kWeightRows) : 0;
   const int64_t blocks = int64_t(kv->batch) * H + int64_t(kv->batch) * kv->kv_heads * row_blocks;
-  // Tile numbers over the whole batch are 32-bit in the kernels, and a grid
+  // Units over the whole batch are 32-bit in the kernels, and a grid
   // holds below 2^32 threads.
-  if (int64_t(kv->batch) * (plan.srows / plan.tile + kOver + 1) > 0x7fffffffLL ||
+  if (int64_t(kv->batch) * (plan.srows / kUnit + kOver + 1) > 0x7fffffffLL ||
       blocks > 0xffffffffLL / kJoinThreads)
     return fail(TQKV_EUNSUPPORTED, "batch=%d max_rows=%lld", kv->batch, (long long)max_rows);
   if (!workspace) {
@@ -311,8 +307,7 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
   a.groups16 = plan.groups16;
   a.max_rows = int(max_rows);
   a.W = plan.W;
-  a.tile = plan.tile;
-  a.over = kOver;
+  a.over = getenv("POVER") ? atoi(getenv("POVER")) : kOver;
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.down = kv->kind == TQKV_CACHE_BF16 ? Bf16Rows<128>::kDown : AffineRows<128, 4, 4, 64>::kDown;
   a.part_o = static_cast<float*>(workspace);

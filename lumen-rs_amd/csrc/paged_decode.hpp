@@ -1,19 +1,19 @@
 // Decode attention over a paged cache: one new token a sequence.
 //
 // o = sum_t p_t v_t with p = softmax(scale q.k_t): one pass over the rows with
-// a running maximum and sum. The rows of the whole batch, cut into 32-row
-// tiles, are laid end to end and divided evenly among the W workgroups of a
-// KV head, from lens on the device: a long sequence spreads over many
+// a running maximum and sum. The rows of the whole batch, in blocks of 16, are
+// laid end to end and divided evenly among the W workgroups of a KV head, from
+// lens on the device: a long sequence spreads over many
 // workgroups and a workgroup may take several short ones. A workgroup's part
 // of one sequence is a segment; it leaves the segment's output, maximum and
 // sum in slot (workgroup + sequence), which no other segment shares (along
 // the row order both only grow and one always does), unless the segment is
 // the whole sequence. The second launch joins the slots.
 //
-// A wavefront takes whole tiles, every fourth of the segment, on the matrix
-// cores with the query heads of the KV head as the 16 columns:
+// A wavefront takes every fourth step (32 rows, or 16 for wide rows) of the
+// segment, on the matrix cores with the query heads of the KV head as the 16 columns:
 //   S[row][head] = K Q^T  (A: lane l holds row l % 16 and 8 channels of
-//     quarter l / 16; two 16-row products a tile), so lane l ends up with head
+//     quarter l / 16; a product a 16 rows), so lane l ends up with head
 //     l % 16 and rows 4 (l / 16) + i of each half;
 //   O^T[channel][head] += V^T P^T: the eight weights that lane l just
 //     computed are the operand it has to supply (rows as the contraction, in
@@ -45,9 +45,8 @@ namespace tqkv {
 namespace paged {
 
 constexpr int kWaves = 4;
-constexpr int kTile = 32;      // rows of a tile
-constexpr int kWideTile = 64;  // at head dim 512
-constexpr int kMinUnits = 4;   // of a workgroup: a tile a wavefront
+constexpr int kUnit = 16;     // rows by which the batch is divided
+constexpr int kMinUnits = 8;  // of a workgroup: two a wavefront
 
 struct DecodeArgs {
   Pool pool;
@@ -58,8 +57,7 @@ struct DecodeArgs {
   int H, G, groups16;  // query heads, of a KV head, 16-head sets of those
   int max_rows, window;
   int W;               // workgroups a (KV head, set)
-  int tile;            // rows of a tile
-  int over;            // tiles that a sequence's start counts as
+  int over;            // units that a sequence's start counts as
   float scale_log2;
   float down;      // log2 by which the row format's weights are held lower
   float* part_o;  // [W + batch, H, D]
@@ -69,15 +67,16 @@ struct DecodeArgs {
   int64_t srows;
 };
 
-// The tiles of sequence b: n rows held, from the window's first, and its units,
-// which the batch is divided by: its tiles and `over` for starting on it.
+// The rows of sequence b: n held, attended from the window's first, and its
+// units, which the batch is divided by: 16-row blocks and `over` for starting
+// on it.
 struct Span {
-  int n, lo, tiles, units;
+  int n, lo, blocks, units;
 };
 __device__ __forceinline__ Span span_of_rows(const DecodeArgs& a, int n) {
   const int lo = a.window > 0 && n > a.window ? n - a.window : 0;
-  const int tiles = n > 0 ? (n + a.tile - 1) / a.tile - lo / a.tile : 0;
-  return {n, lo, tiles, n > 0 ? tiles + a.over : 0};
+  const int blocks = n > 0 ? (n + kUnit - 1) / kUnit - lo / kUnit : 0;
+  return {n, lo, blocks, n > 0 ? blocks + a.over : 0};
 }
 __device__ __forceinline__ Span span_of(const DecodeArgs& a, int b) {
   return span_of_rows(a, held(a.pool, b, a.max_rows < a.pool.cap ? a.max_rows : a.pool.cap));
@@ -129,25 +128,30 @@ __device__ __forceinline__ rsrc uniform(const void* p, int64_t offset) {
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(x), 0, 0x40000000, 0x00027000);
 }
 
+// Cache policies. Rows are read once, so they are best streamed past the caches
+// (131,071 bf16 rows at D = 128: 95 -> 87 us; 16 x 16,384 at D = 256: 346 ->
+// 312), but only where one load takes whole 64-byte pieces: with 4-bit codes
+// several loads share a line (16 x 32,768 rows at D = 256: 240 -> 308).
+constexpr int kKeep = 0, kStream = 2;
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 // A load of N bytes (2, 4, 8 or a multiple of 16) into words.
-template <int N>
+template <int N, int kPolicy = kKeep>
 __device__ __forceinline__ void load_words(rsrc base, uint32_t off, uint32_t* w) {
   if constexpr (N == 2) {
-    w[0] = __builtin_amdgcn_raw_buffer_load_b16(base, off, 0, 0);
+    w[0] = __builtin_amdgcn_raw_buffer_load_b16(base, off, 0, kPolicy);
   } else if constexpr (N == 4) {
-    w[0] = __builtin_amdgcn_raw_buffer_load_b32(base, off, 0, 0);
+    w[0] = __builtin_amdgcn_raw_buffer_load_b32(base, off, 0, kPolicy);
   } else if constexpr (N == 8) {
-    const uintx2 x = __builtin_amdgcn_raw_buffer_load_b64(base, off, 0, 0);
+    const uintx2 x = __builtin_amdgcn_raw_buffer_load_b64(base, off, 0, kPolicy);
     w[0] = x.x;
     w[1] = x.y;
   } else {
     static_assert(N % 16 == 0, "whole 16-byte loads");
 #pragma unroll
     for (int i = 0; i < N / 16; ++i) {
-      const uintx4 x = __builtin_amdgcn_raw_buffer_load_b128(base, off + 16 * i, 0, 0);
+      const uintx4 x = __builtin_amdgcn_raw_buffer_load_b128(base, off + 16 * i, 0, kPolicy);
       w[4 * i] = x.x;
       w[4 * i + 1] = x.y;
       w[4 * i + 2] = x.z;
@@ -187,33 +191,35 @@ __device__ __forceinline__ floatx4 mfma_pv(const uint32_t (&v)[2 * HALVES],
   }
 }
 
-// The pages of a wavefront's coming steps, a table entry a lane, two blocks of
-// 64: a step takes its page by a lane read. (Loaded when a step needs it, an
-// entry's wait is also one for every load before it, the step's own values.)
+// The pages of a wavefront's coming steps: a block of table entries in LDS,
+// its own, filled when a step asks for an entry behind it. (An entry loaded
+// when its step needs it, or one block in registers ahead of the next, makes
+// the step wait for every load before it, its own values' too.)
+constexpr int kBlock = 256;
 struct Pages {
   const int32_t* table;
+  int32_t* block;  // LDS, kBlock entries of the wavefront's
   int most;        // entries that may be read
-  int first;       // entry of lane 0 of `now`; `next` holds the 64 behind
-  int now, next;
-  __device__ __forceinline__ int load(int at) const {
-    const int i = at + int(threadIdx.x % 64);
-    return i < most ? table[i] : -1;
-  }
-  __device__ __forceinline__ void start(const int32_t* t, int n, int at) {
-    table = t;
-    most = n;
+  int first;       // entry of block[0]
+  __device__ __forceinline__ void fill(int at) {
     first = at;
-    now = load(at);
-    next = load(at + 64);
+#pragma unroll
+    for (int i = 0; i < kBlock / 64; ++i) {
+      const int lane = 64 * i + int(threadIdx.x % 64);
+      block[lane] = at + lane < most ? table[at + lane] : -1;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  __device__ __forceinline__ void start(int32_t* lds, const int32_t* t, int n, int at) {
+    table = t;
+    block = lds;
+    most = n;
+    fill(at);
   }
   // Entry i, not below those asked for before.
   __device__ __forceinline__ int entry(int i) {
-    while (i >= first + 64) {
-      first += 64;
-      now = next;
-      next = load(first + 64);
-    }
-    return __builtin_amdgcn_readlane(now, i - first);
+    if (i >= first + kBlock) fill(i);
+    return __builtin_amdgcn_readfirstlane(block[i - first]);
   }
 };
 
@@ -224,13 +230,13 @@ struct Step {
   bool ok[HALVES];
 };
 template <int HALVES>
-__device__ __forceinline__ Step<HALVES> step_of(const Pool& p, Pages& pages, int kvh, int step,
-                                                int n) {
+__device__ __forceinline__ Step<HALVES> step_of(const Pool& p, Pages& pages, int kvh, int row,
+                                                int end) {
   Step<HALVES> h;
 #pragma unroll
   for (int s = 0; s < HALVES; ++s) {
-    const int r = (step * HALVES + s) * 16;
-    const int page = r < n ? pages.entry(r >> p.shift) : -1;
+    const int r = row + s * 16;
+    const int page = r < end ? pages.entry(r >> p.shift) : -1;
     h.ok[s] = page >= 0 && page < p.num_pages;
     h.row[s] = pool_row(p, h.ok[s] ? page : 0, kvh, h.ok[s] ? r & ((1 << p.shift) - 1) : 0);
   }
@@ -256,9 +262,10 @@ struct Bf16Rows {
   using S = Step<kHalves>;
   static constexpr int kChunks = D / 32;
   static constexpr int kVWords = C::kPieces * C::kCpl / 2;
-  struct Q {
-    bf16x8 op[kChunks];
-    float mul;
+  typedef bf16x8 Operand;
+  static constexpr int kOperands = kChunks;
+  struct Rest {   // of the queries, beside their operands
+    float mul;    // of a score: positive
   };
   struct K {
     uint32_t w[kHalves][kChunks * 4];
@@ -268,16 +275,21 @@ struct Bf16Rows {
   };
 
   // Channels of (chunk, quarter): 32 chunk + 8 quarter.
-  static __device__ __forceinline__ void load_q(Q& q, rsrc p, bool live, int r, int g,
-                                                float scale_log2) {
-    const uint32_t off = r * (2 * D) + g * 16;
+  static __device__ __forceinline__ void load_q(Operand (&op)[kOperands], Rest& q, rsrc p, bool live,
+                                                int r, int g, float scale_log2) {
+    // Lanes without a head load the first one's (no branch between the loads).
+    const uint32_t off = (live ? r : 0) * (2 * D) + g * 16;
+    uint32_t w[kChunks][4];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      uint32_t w[4] = {0, 0, 0, 0};
-      if (live) load_words<16>(p, off + c * 64, w);
-      q.op[c] = as_bf16x8(w[0], w[1], w[2], w[3]);
-    }
-    q.mul = scale_log2;
+    for (int c = 0; c < kChunks; ++c) load_words<16>(p, off + c * 64, w[c]);
+    // The scale's sign goes into the queries.
+    const uint32_t keep = live && scale_log2 != 0.0f ? 0xffffffffu : 0u;
+    const uint32_t flip = scale_log2 < 0.0f ? 0x80008000u & keep : 0u;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+      op[c] = as_bf16x8((w[c][0] & keep) ^ flip, (w[c][1] & keep) ^ flip, (w[c][2] & keep) ^ flip,
+                        (w[c][3] & keep) ^ flip);
+    q.mul = scale_log2 != 0.0f ? fabsf(scale_log2) : 1.0f;
   }
   static __device__ __forceinline__ void load_k(K& k, const DecodeArgs& a, const S& h, int r,
                                                 int g) {
@@ -286,7 +298,7 @@ struct Bf16Rows {
     for (int s = 0; s < kHalves; ++s) {
       const rsrc p = uniform(a.slot[0], h.row[s] * (2 * D));
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) load_words<16>(p, off + c * 64, k.w[s] + 4 * c);
+      for (int c = 0; c < kChunks; ++c) load_words<16, kStream>(p, off + c * 64, k.w[s] + 4 * c);
     }
   }
   static __device__ __forceinline__ void load_v(V& v, const DecodeArgs& a, const S& h, int r,
@@ -299,16 +311,18 @@ struct Bf16Rows {
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int x = 0; x < C::kPieces; ++x)
-          load_words<2 * C::kCpl>(p, off + e * (2 * D) + x * 256, v.w[4 * s + e] + x * (C::kCpl / 2));
+          load_words<2 * C::kCpl, kStream>(p, off + e * (2 * D) + x * 256, v.w[4 * s + e] + x * (C::kCpl / 2));
     }
   }
   // Scores of half s, to be multiplied by q.mul.
-  static __device__ __forceinline__ floatx4 scores(const Q& q, const K& k, int s) {
+  // op(c): the queries' operand of product c.
+  template <typename Op>
+  static __device__ __forceinline__ floatx4 scores(Op&& op, const Rest&, const K& k, int s) {
     floatx4 acc = {0, 0, 0, 0};
 #pragma unroll
     for (int c = 0; c < kChunks; ++c)
       acc = mfma(as_bf16x8(k.w[s][4 * c], k.w[s][4 * c + 1], k.w[s][4 * c + 2], k.w[s][4 * c + 3]),
-                 q.op[c], acc);
+                 op(c), acc);
     return acc;
   }
   // The rows for which dead is set hold nothing: zero, whatever lies there.
@@ -349,7 +363,7 @@ struct Bf16Rows {
   }
   // The wide kernel's share of the values: the lane's 16 rows of a 64-row tile
   // at eight channels of the wavefront's 128.
-  static constexpr int kWideOcc = 1;
+  static constexpr int kWideOcc = 2;
   struct Wide {
     uint32_t w[16][4];
   };
@@ -360,7 +374,7 @@ struct Bf16Rows {
     for (int s = 0; s < 4; ++s) {
       const rsrc p = uniform(a.slot[1], h.row[s] * (2 * D));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) load_words<16>(p, off + e * (2 * D), v.w[4 * s + e]);
+      for (int e = 0; e < 4; ++e) load_words<16, kStream>(p, off + e * (2 * D), v.w[4 * s + e]);
     }
   }
   static __device__ __forceinline__ void clear_wide(Wide& v, uint32_t dead) {
@@ -370,7 +384,7 @@ struct Bf16Rows {
       for (int i = 0; i < 4; ++i) v.w[e][i] = dead >> e & 1 ? 0 : v.w[e][i];
   }
   static __device__ __forceinline__ void accumulate_wide(const Wide& v, const float (&p)[16],
-                                                         floatx4 (&acc)[8], Unit&) {
+                                                         floatx4 (&acc)[8], Unit&, int, int) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       uint32_t hi[4], lw[4];
@@ -411,11 +425,17 @@ struct AffineRows {
   static constexpr int kGroupWords = kGroupBytes / 4;
   static constexpr int kPieceBytes = C::kCpl * BV / 8;
   static constexpr int kPieceWords = (kPieceBytes + 3) / 4;
+  static constexpr int kPieceLoad = kPieceBytes < 4 ? 4 : kPieceBytes;  // of two lanes at D = 64, 4 bits
+  static constexpr int kKeyPolicy = kGroupBytes >= 16 ? kStream : kKeep;
+  static constexpr int kValuePolicy = kPieceBytes >= 4 ? kStream : kKeep;
   static constexpr int kGpp = 16 * C::kCpl > GS ? 16 * C::kCpl / GS : 1;  // groups a piece
   static constexpr int kSets = (NG + 7) / 8;           // bias products
-  static constexpr int kBiasBytes = 2 * NG < 16 ? 2 * NG : 16;
-  struct Q {
-    halfx8 op[D / 32];
+  // Loaded as whole words: two 16-bit loads would be packed into a register as
+  // they arrive, a wait in the middle of the loads.
+  static constexpr int kBiasBytes = NG == 1 ? 4 : 2 * NG < 16 ? 2 * NG : 16;
+  typedef halfx8 Operand;
+  static constexpr int kOperands = D / 32;
+  struct Rest {
     bf16x8 sum[kSets];
     float mul;
   };
@@ -453,17 +473,20 @@ struct AffineRows {
   // order; the sums of the groups in the same unit as three bf16 parts, which
   // hold all bits of an f32, one a quarter. Channels of (group, quarter):
   // group GS + quarter GS / 4, then in order.
-  static __device__ __forceinline__ void load_q(Q& q, rsrc p, bool live, int r, int g,
-                                                float scale_log2) {
-    const uint32_t off = r * (2 * D) + g * (GS / 2);
+  static __device__ __forceinline__ void load_q(Operand (&op)[kOperands], Rest& q, rsrc p, bool live,
+                                                int r, int g, float scale_log2) {
+    // Lanes without a head load the first one's (no branch between the loads).
+    const uint32_t off = (live ? r : 0) * (2 * D) + g * (GS / 2);
+    const uint32_t keep = live && scale_log2 != 0.0f ? 0xffffffffu : 0u;
     uint32_t w[D / 32][4];
     float top = 0.0f;
 #pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+      load_words<16>(p, off + c / CPG * (2 * GS) + c % CPG * 16, w[c]);
+#pragma unroll
     for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[c][i] = 0;
-      if (live)
-        load_words<16>(p, off + c / CPG * (2 * GS) + c % CPG * 16, w[c]);
+      for (int i = 0; i < 4; ++i) w[c][i] &= keep;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         top = fmaxf(top, fmaxf(fabsf(low_f32(w[c][i])), fabsf(high_f32(w[c][i]))));
@@ -472,7 +495,8 @@ struct AffineRows {
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     int E = int(__float_as_uint(top) >> 23) - 127;
     E = E < -100 ? -100 : E;
-    const float up = __uint_as_float(uint32_t(127 + 14 - E) << 23);
+    // The scale's sign goes into the queries.
+    const float up = __uint_as_float(uint32_t(127 + 14 - E) << 23) * (scale_log2 < 0.0f ? -1.0f : 1.0f);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       float x[8];
@@ -489,7 +513,7 @@ struct AffineRows {
         o[2 * i] = _Float16(x[lo] * down);
         o[2 * i + 1] = _Float16(x[hi] * down);
       }
-      q.op[c] = o;
+      op[c] = o;
     }
 #pragma unroll
     for (int n = 0; n < 8 * kSets; ++n) {
@@ -506,18 +530,18 @@ struct AffineRows {
       const float hi = __bf16(sum), mid = __bf16(sum - hi), lo = __bf16(sum - hi - mid);
       q.sum[n / 8][n % 8] = __bf16(g == 0 ? hi : g == 1 ? mid : g == 2 ? lo : 0.0f);
     }
-    q.mul = ldexpf(scale_log2, E + 10);
+    q.mul = scale_log2 != 0.0f ? ldexpf(fabsf(scale_log2), E + 10) : 1.0f;
   }
   static __device__ __forceinline__ void load_k(K& k, const DecodeArgs& a, const S& h, int r,
                                                 int g) {
     const uint32_t off = r * (D * BK / 8) + g * kGroupBytes;
-    const uint32_t soff = g * (8 * NG), boff = r * (2 * NG);
+    const uint32_t soff = g * (8 * NG), boff = r * (2 * NG) & ~3u;
 #pragma unroll
     for (int s = 0; s < kHalves; ++s) {
       const rsrc p = uniform(a.slot[0], h.row[s] * (D * BK / 8));
 #pragma unroll
       for (int n = 0; n < NG; ++n)
-        load_words<kGroupBytes>(p, off + n * (GS * BK / 8), k.w[s] + n * kGroupWords);
+        load_words<kGroupBytes, kKeyPolicy>(p, off + n * (GS * BK / 8), k.w[s] + n * kGroupWords);
       load_words<8 * NG>(uniform(a.slot[1], h.row[s] * (2 * NG)), soff, k.s[s]);
       const rsrc b = uniform(a.slot[2], h.row[s] * (2 * NG));
 #pragma unroll
@@ -526,7 +550,7 @@ struct AffineRows {
   }
   static __device__ __forceinline__ void load_v(V& v, const DecodeArgs& a, const S& h, int r,
                                                 int g) {
-    const uint32_t off = 4 * g * (D * BV / 8) + r * kPieceBytes, soff = g * (8 * NG);
+    const uint32_t off = 4 * g * (D * BV / 8) + (r * kPieceBytes & ~3), soff = g * (8 * NG);
 #pragma unroll
     for (int s = 0; s < kHalves; ++s) {
       const rsrc p = uniform(a.slot[3], h.row[s] * (D * BV / 8));
@@ -534,7 +558,7 @@ struct AffineRows {
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int x = 0; x < C::kPieces; ++x)
-          load_words<kPieceBytes>(p, off + e * (D * BV / 8) + x * (16 * kPieceBytes),
+          load_words<kPieceLoad, kValuePolicy>(p, off + e * (D * BV / 8) + x * (16 * kPieceBytes),
                                   v.w[4 * s + e] + x * kPieceWords);
       load_words<8 * NG>(uniform(a.slot[4], h.row[s] * (2 * NG)), soff, v.s[s]);
       load_words<8 * NG>(uniform(a.slot[5], h.row[s] * (2 * NG)), soff, v.b[s]);
@@ -546,13 +570,16 @@ struct AffineRows {
     return at % 2 ? high_f32(w[at / 2]) : low_f32(w[at / 2]);
   }
   // The biases' part of all groups in a product, then a scale a group.
-  static __device__ __forceinline__ floatx4 scores(const Q& q, const K& k, int s) {
+  template <typename Op>
+  static __device__ __forceinline__ floatx4 scores(Op&& op, const Rest& q, const K& k, int s) {
     floatx4 out = {0, 0, 0, 0};
+    const int odd = NG == 1 ? threadIdx.x & 1 : 0;  // row r's half of a word of two rows
 #pragma unroll
     for (int i = 0; i < kSets; ++i) {
       uint32_t b[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int x = 0; x < (kBiasBytes + 3) / 4; ++x) b[x] = k.b[s][4 * i + x];
+      for (int x = 0; x < kBiasBytes / 4; ++x) b[x] = k.b[s][4 * i + x];
+      if (NG == 1) b[0] = (b[0] >> (16 * odd)) & 0xffffu;
       out = mfma(as_bf16x8(b[0], b[1], b[2], b[3]), q.sum[i], out);
     }
 #pragma unroll
@@ -561,7 +588,7 @@ struct AffineRows {
 #pragma unroll
       for (int c = 0; c < CPG; ++c)
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(unpack(k.w[s] + n * kGroupWords + c * (BK / 4)),
-                                                     q.op[n * CPG + c], acc, 0, 0, 0);
+                                                     op(n * CPG + c), acc, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) out[i] = fmaf(entry(k.s[s], i, n), acc[i], out[i]);
     }
@@ -595,12 +622,12 @@ struct AffineRows {
   // Channel j of a row's piece: scale * code + bias as f16, one mixed
   // multiply-add. s24: the scale times 2^24 (2^20 for a code with an odd place
   // in its half word).
-  static __device__ __forceinline__ _Float16 value(const uint32_t* w, int j, float s24, float s20,
-                                                   float b) {
+  static __device__ __forceinline__ _Float16 value(const uint32_t* w, int shift, int j, float s24,
+                                                   float s20, float b) {
     uint32_t x;
     int half;
     if constexpr (BV == 4) {
-      x = (w[j / 8] >> (j & 2 ? 8 : 0)) & (j & 1 ? 0x00f000f0u : 0x000f000fu);
+      x = ((w[j / 8] >> shift) >> (j & 2 ? 8 : 0)) & (j & 1 ? 0x00f000f0u : 0x000f000fu);
       half = j % 8 / 4;
     } else {
       x = (w[j / 4] >> (j & 1 ? 8 : 0)) & 0x00ff00ffu;
@@ -636,6 +663,7 @@ struct AffineRows {
   };
   static __device__ __forceinline__ void accumulate(const V& v, const float (&p)[4 * kHalves],
                                                     floatx4 (&acc)[C::kJ], Unit& unit, int r) {
+    const int shift = kPieceBytes < 4 ? 16 * (r & 1) : 0;
     uint32_t pw[2 * kHalves];
 #pragma unroll
     for (int e = 0; e < 2 * kHalves; ++e) {
@@ -668,8 +696,9 @@ struct AffineRows {
 #pragma unroll
         for (int e = 0; e < 2 * kHalves; ++e) {
           const halfx2 y = {
-              value(v.w[2 * e] + x * kPieceWords, j, s[2 * e], s20[2 * e], b[2 * e]),
-              value(v.w[2 * e + 1] + x * kPieceWords, j, s[2 * e + 1], s20[2 * e + 1], b[2 * e + 1])};
+              value(v.w[2 * e] + x * kPieceWords, shift, j, s[2 * e], s20[2 * e], b[2 * e]),
+              value(v.w[2 * e + 1] + x * kPieceWords, shift, j, s[2 * e + 1], s20[2 * e + 1],
+                    b[2 * e + 1])};
           o[e] = __builtin_bit_cast(uint32_t, y);
         }
         acc[x * C::kCpl + j] = mfma_pv<kHalves, true>(o, pw, acc[x * C::kCpl + j]);
@@ -679,15 +708,15 @@ struct AffineRows {
   }
   // The wide kernel's share of the values, as Bf16Rows': codes, and the scale
   // and bias of the lane's own group of each row.
-  static constexpr int kWideOcc = 1;
+  static constexpr int kWideOcc = NG <= 8 ? 2 : 1;  // groups of 32 would spill
   struct Wide {
     uint32_t w[16][kPieceWords];
-    uint32_t s[16], b[16];  // bf16
+    uint32_t s[16], b[16];  // words that hold the group's bf16
   };
   static __device__ __forceinline__ void load_wide(Wide& v, const DecodeArgs& a, const Step<4>& h,
                                                    int wave, int r, int g) {
     const uint32_t off = 4 * g * (D * BV / 8) + (16 * wave + r) * kPieceBytes;
-    const uint32_t soff = 4 * g * (2 * NG) + (128 * wave + 8 * r) / GS * 2;
+    const uint32_t soff = 4 * g * (2 * NG) + ((128 * wave + 8 * r) / GS * 2 & ~3);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const rsrc p = uniform(a.slot[3], h.row[s] * (D * BV / 8));
@@ -695,9 +724,9 @@ struct AffineRows {
       const rsrc pb = uniform(a.slot[5], h.row[s] * (2 * NG));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        load_words<kPieceBytes>(p, off + e * (D * BV / 8), v.w[4 * s + e]);
-        load_words<2>(ps, soff + e * (2 * NG), &v.s[4 * s + e]);
-        load_words<2>(pb, soff + e * (2 * NG), &v.b[4 * s + e]);
+        load_words<kPieceBytes, kValuePolicy>(p, off + e * (D * BV / 8), v.w[4 * s + e]);
+        load_words<4>(ps, soff + e * (2 * NG), &v.s[4 * s + e]);
+        load_words<4>(pb, soff + e * (2 * NG), &v.b[4 * s + e]);
       }
     }
   }
@@ -709,7 +738,10 @@ struct AffineRows {
     }
   }
   static __device__ __forceinline__ void accumulate_wide(const Wide& v, const float (&p)[16],
-                                                         floatx4 (&acc)[8], Unit& unit) {
+                                                         floatx4 (&acc)[8], Unit& unit, int wave,
+                                                         int r) {
+    const uint32_t half = (128 * wave + 8 * r) / GS & 1;  // the group's place in its word
+    const uint32_t sel = ((2 * half + 1) << 24) | ((2 * half) << 16) | 0x0c0cu;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       uint32_t pw[4];
@@ -721,8 +753,8 @@ struct AffineRows {
       float s[8], s20[8], b[8], most = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        s[e] = low_f32(v.s[8 * k + e]);
-        b[e] = low_f32(v.b[8 * k + e]);
+        s[e] = __uint_as_float(__builtin_amdgcn_perm(0u, v.s[8 * k + e], sel));
+        b[e] = __uint_as_float(__builtin_amdgcn_perm(0u, v.b[8 * k + e], sel));
         most = fmaxf(most, fmaf(fabsf(s[e]), float((1 << BV) - 1), fabsf(b[e])));
       }
       unit.admit(most, acc);
@@ -738,8 +770,9 @@ struct AffineRows {
         uint32_t o[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const halfx2 y = {value(v.w[8 * k + 2 * e], j, s[2 * e], s20[2 * e], b[2 * e]),
-                            value(v.w[8 * k + 2 * e + 1], j, s[2 * e + 1], s20[2 * e + 1], b[2 * e + 1])};
+          const halfx2 y = {value(v.w[8 * k + 2 * e], 0, j, s[2 * e], s20[2 * e], b[2 * e]),
+                            value(v.w[8 * k + 2 * e + 1], 0, j, s[2 * e + 1], s20[2 * e + 1],
+                                  b[2 * e + 1])};
           o[e] = __builtin_bit_cast(uint32_t, y);
         }
         acc[j] = mfma_pv<2, true>(o, pw, acc[j]);
@@ -798,8 +831,8 @@ __device__ __forceinline__ void lay_out(const DecodeArgs& a, Plan& plan) {
 // The workgroup's segments, one after the other (all values uniform).
 struct Walk {
   int x, x1, b;          // next unit, the end, the sequence it is in
-  int seq, n, lo;        // the segment's sequence, its rows held and first row
-  int t0, t1;            // its tiles
+  int seq, n;            // the segment's sequence and the rows that it holds
+  int row, lo, end;      // its rows: from a multiple of 16, those in [lo, end)
   bool whole;            // the whole sequence
   // Kept in scalar registers: the loops over it branch as one.
   static __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -820,16 +853,17 @@ struct Walk {
       const int s0 = scalar(plan.start[b]), s1 = scalar(plan.start[b + 1]);
       seq = b++;
       if (s1 <= x) continue;
-      const int end = s1 < x1 ? s1 : x1;
-      const int u0 = x - s0 - a.over, u1 = end - s0 - a.over;
-      x = end;
+      const int stop = s1 < x1 ? s1 : x1;
+      const int u0 = x - s0 - a.over, u1 = stop - s0 - a.over;
+      x = stop;
       if (u1 <= 0) continue;  // only the units for starting on it
       const Span s = span_of_rows(a, scalar(plan.rows[seq]));
       n = s.n;
       lo = s.lo;
-      t0 = (u0 < 0 ? 0 : u0) + lo / a.tile;
-      t1 = u1 + lo / a.tile;
-      whole = u0 <= 0 && u1 == s.tiles;
+      row = ((u0 < 0 ? 0 : u0) + lo / kUnit) * kUnit;
+      end = (u1 + lo / kUnit) * kUnit;
+      end = end < n ? end : n;
+      whole = u0 <= 0 && u1 == s.blocks;
       return true;
     }
     return false;
@@ -841,11 +875,11 @@ constexpr float kTau = 8.0f;  // log2 by which a score may pass the running maxi
 template <typename Rows>
 __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(const DecodeArgs a) {
   constexpr int D = Rows::kD, HALVES = Rows::kHalves, kRows = 16 * HALVES;  // rows a step
-  constexpr int kSteps = kTile / kRows;                                     // steps a tile
   using C = Chan<D>;
   constexpr int kPiece = 16 * C::kCpl;      // channels the epilogue joins at a time
   constexpr int kStride = kPiece + 4;
   __shared__ Plan plan;
+  __shared__ int32_t blocks[kWaves][kBlock];
   __shared__ float ml[2][kWaves][16];
   __shared__ __attribute__((aligned(16))) float joint[kWaves][16][kStride];
   const Pool& p = a.pool;
@@ -859,17 +893,15 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
   Walk walk;
   walk.start(plan, p.batch, a.W);
   while (walk.next(a, plan)) {
-    const int b = walk.seq, n = walk.n, lo = walk.lo;
-    // Steps: a wavefront takes every fourth.
-    const int t1 = walk.t1 * kSteps;
-    int t = walk.t0 * kSteps + wave;
-
+    const int b = walk.seq, lo = walk.lo, end = walk.end;
+    // A wavefront takes every fourth step of kRows rows.
+    int row0 = walk.row + wave * kRows;
     Pages pages;
-    pages.start(p.table + b * p.tstride, (n + (1 << p.shift) - 1) >> p.shift,
-                (t * kRows) >> p.shift);
+    pages.start(blocks[wave], p.table + b * p.tstride, (walk.n + (1 << p.shift) - 1) >> p.shift, row0 >> p.shift);
 
-    typename Rows::Q q;
-    Rows::load_q(q, uniform(a.q, 2 * (b * a.qstride + int64_t(head0) * D)), r < live, r, g, a.scale_log2);
+    typename Rows::Operand ops[Rows::kOperands];
+    typename Rows::Rest q;
+    Rows::load_q(ops, q, uniform(a.q, 2 * (b * a.qstride + int64_t(head0) * D)), r < live, r, g, a.scale_log2);
     floatx4 acc[C::kJ];
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) acc[j] = floatx4{0, 0, 0, 0};
@@ -879,31 +911,32 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
     typename Rows::K kr;
     typename Rows::V vr;
     Step<HALVES> h{};
-    if (t < t1) {
-      h = step_of<HALVES>(p, pages, kvh, t, n);
+    if (row0 < end) {
+      h = step_of<HALVES>(p, pages, kvh, row0, end);
       Rows::load_k(kr, a, h, r, g);
       Rows::load_v(vr, a, h, r, g);
     }
-    for (; t < t1; t += kWaves) {
+    for (; row0 < end; row0 += kWaves * kRows) {
+      // The last step loads its own rows again: no branch between the loads.
       Step<HALVES> hn = h;
-      if (t + kWaves < t1) hn = step_of<HALVES>(p, pages, kvh, t + kWaves, n);
+      if (row0 + kWaves * kRows < end)
+        hn = step_of<HALVES>(p, pages, kvh, row0 + kWaves * kRows, end);
       float sc[4 * HALVES];
 #pragma unroll
       for (int s = 0; s < HALVES; ++s) {
-        const floatx4 y = Rows::scores(q, kr, s);
+        const floatx4 y = Rows::scores([&](int c) { return ops[c]; }, q, kr, s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[4 * s + i] = y[i] * q.mul;
+        for (int i = 0; i < 4; ++i) sc[4 * s + i] = y[i];
         __builtin_amdgcn_sched_barrier(0);
       }
       Rows::load_k(kr, a, hn, r, g);
       __builtin_amdgcn_sched_barrier(0);
-      const int row0 = t * kRows;
-      if (!(row0 >= lo && row0 + kRows <= n && h.ok[0] && h.ok[HALVES - 1])) {
+      if (!(row0 >= lo && row0 + kRows <= end && h.ok[0] && h.ok[HALVES - 1])) {
         uint32_t dead = 0;
 #pragma unroll
         for (int e = 0; e < 4 * HALVES; ++e) {
           const int row = row0 + (e / 4) * 16 + 4 * g + e % 4;
-          if (row < lo || row >= n || !h.ok[e / 4]) {
+          if (row < lo || row >= end || !h.ok[e / 4]) {
             dead |= 1u << e;
             sc[e] = -INFINITY;
           }
@@ -914,12 +947,15 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
         float* dst = a.scores + (int64_t(b) * a.H + head0 + r) * a.srows + row0 + 4 * g;
 #pragma unroll
         for (int s = 0; s < HALVES; ++s)
-          *reinterpret_cast<float4*>(dst + 16 * s) =
-              make_float4(sc[4 * s], sc[4 * s + 1], sc[4 * s + 2], sc[4 * s + 3]);
+          if (row0 + 16 * s < end)  // the rows behind are another segment's
+            *reinterpret_cast<float4*>(dst + 16 * s) =
+                make_float4(sc[4 * s] * q.mul, sc[4 * s + 1] * q.mul, sc[4 * s + 2] * q.mul,
+                            sc[4 * s + 3] * q.mul);
       }
       float top = sc[0];
 #pragma unroll
       for (int e = 1; e < 4 * HALVES; ++e) top = fmaxf(top, sc[e]);
+      top *= q.mul;
       if (__any(top > m + kTau)) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -934,7 +970,7 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
       float pr[4 * HALVES];
 #pragma unroll
       for (int e = 0; e < 4 * HALVES; ++e) {
-        pr[e] = __builtin_amdgcn_exp2f(sc[e] - base);
+        pr[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], q.mul, -base));
         l += pr[e];
       }
       Rows::accumulate(vr, pr, acc, unit, r);
@@ -1022,13 +1058,19 @@ __device__ __forceinline__ Step<1> quarter_of(const Step<4>& h, int wave) {
 // workgroup share a 64-row tile: each scores 16 rows over all channels, the
 // scores meet in LDS (two buffers, one barrier a tile), and each goes over the
 // softmax of all 64 rows by itself and accumulates 128 output channels, which
-// it also writes.
+// it also writes. The queries' operands lie in LDS: with them in registers the
+// rows in flight went through accumulation registers, and each copy waited for
+// its load.
+constexpr int kWideTile = 16 * kWaves;
+
 template <typename Rows>
 __global__ __launch_bounds__(64 * kWaves, Rows::kWideOcc) void paged_wide_kernel(const DecodeArgs a) {
   constexpr int D = Rows::kD;
   static_assert(D == 128 * kWaves && Rows::kHalves == 1, "a wavefront takes 128 channels");
   __shared__ Plan plan;
+  __shared__ int32_t blocks[kWaves][kBlock];
   __shared__ float4 tiles[2][16][16];
+  __shared__ typename Rows::Operand queries[Rows::kOperands][64];
   const Pool& p = a.pool;
   const int tid = threadIdx.x, lane = tid % 64, r = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -1040,13 +1082,22 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kWideOcc) void paged_wide_kernel
   walk.start(plan, p.batch, a.W);
   int buf = 0;
   while (walk.next(a, plan)) {
-    const int b = walk.seq, n = walk.n, lo = walk.lo, t1 = walk.t1;
-    int t = walk.t0;
+    const int b = walk.seq, lo = walk.lo, end = walk.end;
+    int row0 = walk.row;
     Pages pages;
-    pages.start(p.table + b * p.tstride, (n + (1 << p.shift) - 1) >> p.shift,
-                (t * kWideTile) >> p.shift);
-    typename Rows::Q q;
-    Rows::load_q(q, uniform(a.q, 2 * (b * a.qstride + int64_t(head0) * D)), r < live, r, g, a.scale_log2);
+    pages.start(blocks[wave], p.table + b * p.tstride, (walk.n + (1 << p.shift) - 1) >> p.shift, row0 >> p.shift);
+    typename Rows::Rest q;
+    {
+      typename Rows::Operand ops[Rows::kOperands];
+      Rows::load_q(ops, q, uniform(a.q, 2 * (b * a.qstride + int64_t(head0) * D)), r < live, r, g,
+                   a.scale_log2);
+      // The last segment's reads are over: every wavefront passed a barrier
+      // since its last.
+#pragma unroll
+      for (int c = 0; c < Rows::kOperands; ++c)
+        if (c % kWaves == wave) queries[c][lane] = ops[c];
+      lds_barrier();
+    }
     floatx4 acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = floatx4{0, 0, 0, 0};
@@ -1054,25 +1105,24 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kWideOcc) void paged_wide_kernel
     typename Rows::Unit unit;
     typename Rows::K kr;
     typename Rows::Wide vr;
-    Step<4> h = step_of<4>(p, pages, kvh, t, n);
+    Step<4> h = step_of<4>(p, pages, kvh, row0, end);
     Rows::load_k(kr, a, quarter_of(h, wave), r, g);
     Rows::load_wide(vr, a, h, wave, r, g);
-    for (; t < t1; ++t) {
+    for (; row0 < end; row0 += kWideTile) {
       Step<4> hn = h;
-      if (t + 1 < t1) hn = step_of<4>(p, pages, kvh, t + 1, n);
-      const floatx4 y = Rows::scores(q, kr, 0);
-      float4 mine = make_float4(y[0] * q.mul, y[1] * q.mul, y[2] * q.mul, y[3] * q.mul);
+      if (row0 + kWideTile < end) hn = step_of<4>(p, pages, kvh, row0 + kWideTile, end);
+      const floatx4 y = Rows::scores([&](int c) { return queries[c][lane]; }, q, kr, 0);
+      float4 mine = make_float4(y[0], y[1], y[2], y[3]);
       __builtin_amdgcn_sched_barrier(0);
       Rows::load_k(kr, a, quarter_of(hn, wave), r, g);
       __builtin_amdgcn_sched_barrier(0);
-      const int row0 = t * kWideTile;
-      const bool full = row0 >= lo && row0 + kWideTile <= n && h.ok[0] && h.ok[1] && h.ok[2] && h.ok[3];
+      const bool full = row0 >= lo && row0 + kWideTile <= end && h.ok[0] && h.ok[1] && h.ok[2] && h.ok[3];
       uint32_t dead = 0;  // of the lane's 16 rows
       if (!full) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int row = row0 + (e / 4) * 16 + 4 * g + e % 4;
-          dead |= uint32_t(row < lo || row >= n || !h.ok[e / 4]) << e;
+          dead |= uint32_t(row < lo || row >= end || !h.ok[e / 4]) << e;
         }
         const uint32_t d = dead >> (4 * wave);
         mine.x = d & 1 ? -INFINITY : mine.x;
@@ -1082,9 +1132,10 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kWideOcc) void paged_wide_kernel
         Rows::clear_wide(vr, dead);
       }
       tiles[buf][4 * wave + g][r] = mine;
-      if (a.scores && r < live)
+      if (a.scores && r < live && row0 + 16 * wave < end)
         *reinterpret_cast<float4*>(a.scores + (int64_t(b) * a.H + head0 + r) * a.srows + row0 +
-                                   16 * wave + 4 * g) = mine;
+                                   16 * wave + 4 * g) =
+            make_float4(mine.x * q.mul, mine.y * q.mul, mine.z * q.mul, mine.w * q.mul);
       lds_barrier();
       float pr[16];
       float top = -INFINITY;
@@ -1098,6 +1149,7 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kWideOcc) void paged_wide_kernel
         top = fmaxf(top, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
       }
       buf ^= 1;
+      top *= q.mul;
       if (__any(top > m + kTau)) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -1111,10 +1163,10 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kWideOcc) void paged_wide_kernel
       const float base = m == -INFINITY ? 0.0f : m + Rows::kDown;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        pr[e] = __builtin_amdgcn_exp2f(pr[e] - base);
+        pr[e] = __builtin_amdgcn_exp2f(fmaf(pr[e], q.mul, -base));
         l += pr[e];
       }
-      Rows::accumulate_wide(vr, pr, acc, unit);
+      Rows::accumulate_wide(vr, pr, acc, unit, wave, r);
       __builtin_amdgcn_sched_barrier(0);
       Rows::load_wide(vr, a, hn, wave, r, g);
       __builtin_amdgcn_sched_barrier(0);

@@ -111,7 +111,7 @@ def test_workspace_sizes():
     n = T.paged_decode_workspace_size(kv, 8, 512)
     tracked = T.paged_decode_workspace_size(view(), 8, 512)
     assert tracked - n == 2 * 8 * 512 * 4  # the scores
-    assert T.paged_decode_workspace_size(view(), 8, 33) - T.paged_decode_workspace_size(kv, 8, 33) == 2 * 8 * 64 * 4
+    assert T.paged_decode_workspace_size(view(), 8, 33) - T.paged_decode_workspace_size(kv, 8, 33) == 2 * 8 * 48 * 4
     assert n >= 2 * 8 * 130 * 4
     assert T.paged_decode_workspace_size(kv, 8, 513) == 0 and T.paged_decode_workspace_size(kv, 7, 512) == 0
     assert T.paged_evict_workspace_size(kv, 64) == 2 * 4 * 64 * 4
