@@ -146,9 +146,11 @@ __device__ __forceinline__ LaneCodes quantize_lane_refined(const float (&v)[kLan
   const float n_bins = float((1 << bits) - 1);
   const float y = 1.0f / r.scale;
   float q[kLaneElems];
-  if (__builtin_expect(!(fabsf(r.scale) < 0x1p100f), 0)) {
+  if (__any(!(fabsf(r.scale) < 0x1p100f))) {
+    float scale = r.scale;
+    asm volatile("" : "+v"(scale));  // or the compiler divides for every row, ahead of the branch
 #pragma unroll
-    for (int e = 0; e < kLaneElems; ++e) q[e] = (v[e] - r.bias) / r.scale;
+    for (int e = 0; e < kLaneElems; ++e) q[e] = (v[e] - r.bias) / scale;
   } else {
 #pragma unroll
     for (int e = 0; e < kLaneElems; ++e) {

@@ -119,6 +119,10 @@ __device__ __forceinline__ void clear_weights(const Pool& p, const Dest* dest, i
 // bf16 rows: a thread moves 16 bytes of K and of V; a row is D / 8 threads.
 // kTokens tokens a workgroup.
 constexpr int kTokens = 4;
+// Quantized prompts: a workgroup's rows of a head lie side by side in a page
+// (13,548 tokens of 8 heads, 4 bits: 27 us at 4 tokens a workgroup, 24 at 8,
+// 25 at 16, 28 at 32); few tokens keep the smaller workgroups, for latency.
+constexpr int kMany = 8, kManyTokens = 2048;
 
 template <int D>
 __global__ __launch_bounds__(kThreads) void append_bf16_kernel(const AppendArgs a) {
@@ -127,18 +131,31 @@ __global__ __launch_bounds__(kThreads) void append_bf16_kernel(const AppendArgs 
   const Pool& p = a.pool;
   const int64_t t0 = int64_t(blockIdx.x) * kTokens;
   const int n = a.tokens - t0 < kTokens ? int(a.tokens - t0) : kTokens;
-  find_dests(p, a.starts, t0, n, sstarts, dest);
   constexpr int LPR = D / 8;
-  const int items = n * p.Hkv * LPR;
-  for (int i = threadIdx.x; i < items; i += kThreads) {
-    const int c = i % LPR, h = (i / LPR) % p.Hkv, t = i / LPR / p.Hkv;
+  const int c = threadIdx.x % LPR;
+  // Rows are heads within tokens: a token's heads lie side by side where they
+  // are read.
+  auto source = [&](int row) {
+    row = row < n * p.Hkv ? row : n * p.Hkv - 1;
+    return (t0 + row / p.Hkv) * a.ts + (row % p.Hkv) * a.hs + c * 8;
+  };
+  // The first rows are on their way while their places are found.
+  const int64_t first = source(threadIdx.x / LPR);
+  uint4 x = *reinterpret_cast<const uint4*>(a.k + first);
+  uint4 y = *reinterpret_cast<const uint4*>(a.v + first);
+  find_dests(p, a.starts, t0, n, sstarts, dest);
+  for (int r = threadIdx.x / LPR; r < n * p.Hkv; r += kThreads / LPR) {
+    const int t = r / p.Hkv, h = r % p.Hkv;
+    const uint4 xs = x, ys = y;
+    if (r + kThreads / LPR < n * p.Hkv) {
+      const int64_t next = source(r + kThreads / LPR);
+      x = *reinterpret_cast<const uint4*>(a.k + next);
+      y = *reinterpret_cast<const uint4*>(a.v + next);
+    }
     if (dest[t].row < 0) continue;
-    const int64_t src = (t0 + t) * a.ts + h * a.hs + c * 8;
     const int64_t dst = (dest[t].row + (int64_t(h) << p.shift)) * D + c * 8;
-    const uint4 x = *reinterpret_cast<const uint4*>(a.k + src);
-    const uint4 y = *reinterpret_cast<const uint4*>(a.v + src);
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.slot[0]) + dst) = x;
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.slot[1]) + dst) = y;
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.slot[0]) + dst) = xs;
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.slot[1]) + dst) = ys;
   }
   clear_weights(p, dest, n);
 }
@@ -146,14 +163,13 @@ __global__ __launch_bounds__(kThreads) void append_bf16_kernel(const AppendArgs 
 // Affine rows: a lane quantizes 16 elements (the bits of
 // tqkv_affine_quantize), whose 4- or 8-bit codes are whole words, so they are
 // stored from registers. blockIdx.y: K or V.
-template <int D, int BK, int BV>
+template <int D, int BK, int BV, int kTokens>
 __global__ __launch_bounds__(kThreads) void append_affine_kernel(const AppendArgs a) {
   __shared__ int32_t sstarts[kMaxBatch + 1];
   __shared__ Dest dest[kTokens];
   const Pool& p = a.pool;
   const int64_t t0 = int64_t(blockIdx.x) * kTokens;
   const int n = a.tokens - t0 < kTokens ? int(a.tokens - t0) : kTokens;
-  find_dests(p, a.starts, t0, n, sstarts, dest);
   constexpr int LPR = D / aq::kLaneElems;
   const int side = blockIdx.y, bits = side ? BV : BK;
   const uint16_t* x = side ? a.v : a.k;
@@ -161,17 +177,25 @@ __global__ __launch_bounds__(kThreads) void append_affine_kernel(const AppendArg
   uint16_t* scales = static_cast<uint16_t*>(a.slot[3 * side + 1]);
   uint16_t* biases = static_cast<uint16_t*>(a.slot[3 * side + 2]);
   const int lpg = a.gs / aq::kLaneElems, groups = D / a.gs;
-  const int items = n * p.Hkv * LPR;
-  // Whole wavefronts go round (the groups' butterflies exchange across
-  // lanes); lanes past the end repeat the last item and store nothing.
-  for (int i0 = 0; i0 < items; i0 += kThreads) {
-    const int i = i0 + int(threadIdx.x) < items ? i0 + int(threadIdx.x)
-                                                : items - LPR + int(threadIdx.x) % LPR;
-    const int c = i % LPR, h = (i / LPR) % p.Hkv, t = i / LPR / p.Hkv;
-    float v[aq::kLaneElems];
-    aq::load_lane(x + (t0 + t) * a.ts + h * a.hs + c * aq::kLaneElems, v);
+  // Lane c of a row; rows are tokens within heads, so that a wavefront's rows
+  // lie side by side in a page.
+  const int c = threadIdx.x % LPR, rows = p.Hkv * kTokens;
+  auto load = [&](int row, float (&v)[aq::kLaneElems]) {
+    // Whole wavefronts go round (the groups' butterflies exchange across
+    // lanes): rows past the end load the last ones and are not stored.
+    row = row < rows ? row : rows - 1;
+    const int t = row % kTokens < n ? row % kTokens : n - 1;
+    aq::load_lane(x + (t0 + t) * a.ts + (row / kTokens) * a.hs + c * aq::kLaneElems, v);
+  };
+  // The first rows are on their way while their places are found.
+  float v[aq::kLaneElems];
+  load(threadIdx.x / LPR, v);
+  find_dests(p, a.starts, t0, n, sstarts, dest);
+  for (int row0 = 0; row0 < rows; row0 += kThreads / LPR) {
+    const int r = row0 + threadIdx.x / LPR, t = r % kTokens, h = r / kTokens;
     const aq::LaneCodes q = aq::quantize_lane_refined(v, a.gs, bits);
-    if (dest[t].row < 0 || i0 + int(threadIdx.x) >= items) continue;
+    if (row0 + kThreads / LPR < rows) load(r + kThreads / LPR, v);
+    if (r >= rows || t >= n || dest[t].row < 0) continue;
     const int64_t row = dest[t].row + (int64_t(h) << p.shift);
     uint32_t* out = packed + row * (D * bits / 32) + c * (bits / 2);
     if (bits == 4)
@@ -187,17 +211,27 @@ __global__ __launch_bounds__(kThreads) void append_affine_kernel(const AppendArg
   if (side == 0) clear_weights(p, dest, n);
 }
 
+template <int D, int kTokens>
+void launch_affine(const tqkv_paged_kv* kv, const AppendArgs& a, hipStream_t st) {
+  const unsigned blocks = unsigned((a.tokens + kTokens - 1) / kTokens);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(blocks, 2), dim3(kThreads), 0, st, a);
+  };
+  if (kv->bits_k == 4 && kv->bits_v == 4) go(append_affine_kernel<D, 4, 4, kTokens>);
+  else if (kv->bits_k == 4) go(append_affine_kernel<D, 4, 8, kTokens>);
+  else if (kv->bits_v == 4) go(append_affine_kernel<D, 8, 4, kTokens>);
+  else go(append_affine_kernel<D, 8, 8, kTokens>);
+}
+
 template <int D>
 void launch_append(const tqkv_paged_kv* kv, const AppendArgs& a, hipStream_t st) {
-  const unsigned blocks = unsigned((a.tokens + kTokens - 1) / kTokens);
-  auto go = [&](auto kernel, unsigned y) {
-    hipLaunchKernelGGL(kernel, dim3(blocks, y), dim3(kThreads), 0, st, a);
-  };
-  if (kv->kind == TQKV_CACHE_BF16) go(append_bf16_kernel<D>, 1);
-  else if (kv->bits_k == 4 && kv->bits_v == 4) go(append_affine_kernel<D, 4, 4>, 2);
-  else if (kv->bits_k == 4) go(append_affine_kernel<D, 4, 8>, 2);
-  else if (kv->bits_v == 4) go(append_affine_kernel<D, 8, 4>, 2);
-  else go(append_affine_kernel<D, 8, 8>, 2);
+  if (kv->kind == TQKV_CACHE_BF16)
+    hipLaunchKernelGGL(append_bf16_kernel<D>, dim3(unsigned((a.tokens + kTokens - 1) / kTokens)),
+                       dim3(kThreads), 0, st, a);
+  else if (a.tokens >= kManyTokens)
+    launch_affine<D, kMany>(kv, a, st);
+  else
+    launch_affine<D, kTokens>(kv, a, st);
 }
 
 }  // namespace

@@ -206,9 +206,10 @@ int launch(const tqkv_paged_kv* kv, const DecodeArgs& a, dim3 grid, hipStream_t 
 }
 
 // Workgroups a CU: as many as fit at once for affine rows, whose loads leave
-// little in flight (16 x 32,768 4-bit rows at D = 256: 240 us with two, 320
-// with one); one for bf16 rows, which fill the memory system with it (131,071
-// rows at D = 128: 95 us, 100 with two, 107 with three).
+// little in flight (16 x 16,384 4-bit rows at D = 128: 94 us with one, 75 with
+// two, 76 with three, 91 with six); one for bf16 rows, which fill the memory
+// system with it (131,071 rows at D = 128: 90 us, 102 with two, 110 with
+// three; 4 x 8,179 at D = 512: 35 and 45).
 int workgroups_a_cu(const tqkv_paged_kv* kv) {
   if (kv->kind == TQKV_CACHE_BF16) return 1;
   return launch(kv, DecodeArgs{}, dim3(1), nullptr, true);
@@ -216,9 +217,14 @@ int workgroups_a_cu(const tqkv_paged_kv* kv) {
 
 // Workgroups wanted over all KV heads: one round of them on 256 CUs.
 constexpr int kCus = 256;
-// Units that a sequence's start counts as: its segment's own latencies.
+// Units that a sequence's start counts as: its segment's own latencies. 32
+// sequences of 17 to 16,000 4-bit rows: 49 us at 0, 40 at 8, 36 at 16, 33 at
+// 32; 16 of 17 to 8,192 bf16 rows: 26, 21, 19, 20; 8 windows of 1,024 8-bit
+// rows: 16, 18, 18, 20.
 constexpr int kOver = 16;
 static_assert(4 * kCus <= kMaxSegments, "a join holds a sequence's segments");
+
+constexpr int64_t kKeptBytes = int64_t(192) << 20;  // of the 256 MB memory-side cache
 
 struct HostPlan {
   int groups16, W;
@@ -307,13 +313,14 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
   a.groups16 = plan.groups16;
   a.max_rows = int(max_rows);
   a.W = plan.W;
-  a.over = getenv("POVER") ? atoi(getenv("POVER")) : kOver;
+  a.over = kOver;
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.down = kv->kind == TQKV_CACHE_BF16 ? Bf16Rows<128>::kDown : AffineRows<128, 4, 4, 64>::kDown;
   a.part_o = static_cast<float*>(workspace);
   a.part_m = a.part_o + plan.slots * H * D;
   a.part_l = a.part_m + plan.slots * H;
   a.srows = plan.srows;
+  a.kept_units = int(kKeptBytes / (int64_t(kUnit) * kv->kv_heads * 4 * D));
   if (kv->weights)
     a.scores = static_cast<float*>(workspace) + (plan.slots * H * (size_t(D) + 2) + 3) / 4 * 4;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

@@ -58,6 +58,7 @@ struct DecodeArgs {
   int max_rows, window;
   int W;               // workgroups a (KV head, set)
   int over;            // units that a sequence's start counts as
+  int kept_units;      // bf16 rows beyond these are streamed
   float scale_log2;
   float down;      // log2 by which the row format's weights are held lower
   float* part_o;  // [W + batch, H, D]
@@ -128,10 +129,9 @@ __device__ __forceinline__ rsrc uniform(const void* p, int64_t offset) {
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(x), 0, 0x40000000, 0x00027000);
 }
 
-// Cache policies. Rows are read once, so they are best streamed past the caches
-// (131,071 bf16 rows at D = 128: 95 -> 87 us; 16 x 16,384 at D = 256: 346 ->
-// 312), but only where one load takes whole 64-byte pieces: with 4-bit codes
-// several loads share a line (16 x 32,768 rows at D = 256: 240 -> 308).
+// Cache policies. Streaming past the caches pays where one load takes whole
+// 64-byte pieces; with 4-bit codes several loads share a line (16 x 32,768
+// rows at D = 256: 240 us kept, 308 streamed).
 constexpr int kKeep = 0, kStream = 2;
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
@@ -253,11 +253,14 @@ struct Chan {
 };
 
 // ---------------------------------------------------------------- bf16 rows
-template <int D>
+// POLICY: of the rows' loads; the launched kernel holds both and chooses.
+template <int D, int POLICY = kStream>
 struct Bf16Rows {
   static constexpr int kD = D;
+  static constexpr bool kChooses = true;
+  typedef Bf16Rows<D, kKeep> Kept;
   static constexpr int kHalves = D <= 128 ? 2 : 1;
-  static constexpr int kOcc = D == 64 ? 4 : D == 128 ? 3 : D == 256 ? 2 : 1;  // wavefronts a SIMD
+  static constexpr int kOcc = 2;  // wavefronts a SIMD that there are registers for
   using C = Chan<D>;
   using S = Step<kHalves>;
   static constexpr int kChunks = D / 32;
@@ -275,13 +278,17 @@ struct Bf16Rows {
   };
 
   // Channels of (chunk, quarter): 32 chunk + 8 quarter.
-  static __device__ __forceinline__ void load_q(Operand (&op)[kOperands], Rest& q, rsrc p, bool live,
-                                                int r, int g, float scale_log2) {
-    // Lanes without a head load the first one's (no branch between the loads).
+  // A head's queries: lanes without a head load the first one's (no branch
+  // between the loads), and prepare() clears them.
+  static __device__ __forceinline__ void load_q(uint32_t (&w)[D / 32][4], rsrc p, bool live, int r,
+                                                int g) {
     const uint32_t off = (live ? r : 0) * (2 * D) + g * 16;
-    uint32_t w[kChunks][4];
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) load_words<16>(p, off + c * 64, w[c]);
+  }
+  static __device__ __forceinline__ void prepare(Operand (&op)[kOperands], Rest& q,
+                                                 const uint32_t (&w)[D / 32][4], bool live, int,
+                                                 float scale_log2) {
     // The scale's sign goes into the queries.
     const uint32_t keep = live && scale_log2 != 0.0f ? 0xffffffffu : 0u;
     const uint32_t flip = scale_log2 < 0.0f ? 0x80008000u & keep : 0u;
@@ -298,7 +305,7 @@ struct Bf16Rows {
     for (int s = 0; s < kHalves; ++s) {
       const rsrc p = uniform(a.slot[0], h.row[s] * (2 * D));
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) load_words<16, kStream>(p, off + c * 64, k.w[s] + 4 * c);
+      for (int c = 0; c < kChunks; ++c) load_words<16, POLICY>(p, off + c * 64, k.w[s] + 4 * c);
     }
   }
   static __device__ __forceinline__ void load_v(V& v, const DecodeArgs& a, const S& h, int r,
@@ -311,7 +318,7 @@ struct Bf16Rows {
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int x = 0; x < C::kPieces; ++x)
-          load_words<2 * C::kCpl, kStream>(p, off + e * (2 * D) + x * 256, v.w[4 * s + e] + x * (C::kCpl / 2));
+          load_words<2 * C::kCpl, POLICY>(p, off + e * (2 * D) + x * 256, v.w[4 * s + e] + x * (C::kCpl / 2));
     }
   }
   // Scores of half s, to be multiplied by q.mul.
@@ -363,7 +370,7 @@ struct Bf16Rows {
   }
   // The wide kernel's share of the values: the lane's 16 rows of a 64-row tile
   // at eight channels of the wavefront's 128.
-  static constexpr int kWideOcc = 2;
+  static constexpr int kWideOcc = 1;
   struct Wide {
     uint32_t w[16][4];
   };
@@ -374,7 +381,7 @@ struct Bf16Rows {
     for (int s = 0; s < 4; ++s) {
       const rsrc p = uniform(a.slot[1], h.row[s] * (2 * D));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) load_words<16, kStream>(p, off + e * (2 * D), v.w[4 * s + e]);
+      for (int e = 0; e < 4; ++e) load_words<16, POLICY>(p, off + e * (2 * D), v.w[4 * s + e]);
     }
   }
   static __device__ __forceinline__ void clear_wide(Wide& v, uint32_t dead) {
@@ -416,6 +423,8 @@ struct Bf16Rows {
 template <int D, int BK, int BV, int GS>
 struct AffineRows {
   static constexpr int kD = D;
+  static constexpr bool kChooses = false;
+  typedef AffineRows Kept;
   static constexpr int kHalves = D <= 128 ? 2 : 1;
   using C = Chan<D>;
   using S = Step<kHalves>;
@@ -473,16 +482,18 @@ struct AffineRows {
   // order; the sums of the groups in the same unit as three bf16 parts, which
   // hold all bits of an f32, one a quarter. Channels of (group, quarter):
   // group GS + quarter GS / 4, then in order.
-  static __device__ __forceinline__ void load_q(Operand (&op)[kOperands], Rest& q, rsrc p, bool live,
-                                                int r, int g, float scale_log2) {
-    // Lanes without a head load the first one's (no branch between the loads).
+  static __device__ __forceinline__ void load_q(uint32_t (&w)[D / 32][4], rsrc p, bool live, int r,
+                                                int g) {
     const uint32_t off = (live ? r : 0) * (2 * D) + g * (GS / 2);
-    const uint32_t keep = live && scale_log2 != 0.0f ? 0xffffffffu : 0u;
-    uint32_t w[D / 32][4];
-    float top = 0.0f;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
       load_words<16>(p, off + c / CPG * (2 * GS) + c % CPG * 16, w[c]);
+  }
+  static __device__ __forceinline__ void prepare(Operand (&op)[kOperands], Rest& q,
+                                                 uint32_t (&w)[D / 32][4], bool live, int g,
+                                                 float scale_log2) {
+    const uint32_t keep = live && scale_log2 != 0.0f ? 0xffffffffu : 0u;
+    float top = 0.0f;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
@@ -872,16 +883,23 @@ struct Walk {
 
 constexpr float kTau = 8.0f;  // log2 by which a score may pass the running maximum
 
+// What a workgroup keeps in LDS.
 template <typename Rows>
-__global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(const DecodeArgs a) {
+struct Shared {
+  static constexpr int kPiece = 16 * Chan<Rows::kD>::kCpl;  // channels joined at a time
+  Plan plan;
+  int32_t blocks[kWaves][kBlock];
+  float ml[2][kWaves][16];
+  __attribute__((aligned(16))) float joint[kWaves][16][kPiece + 4];
+};
+
+template <typename Rows>
+__device__ __forceinline__ void attend(const DecodeArgs& a, Shared<Rows>& lds) {
   constexpr int D = Rows::kD, HALVES = Rows::kHalves, kRows = 16 * HALVES;  // rows a step
   using C = Chan<D>;
-  constexpr int kPiece = 16 * C::kCpl;      // channels the epilogue joins at a time
-  constexpr int kStride = kPiece + 4;
-  __shared__ Plan plan;
-  __shared__ int32_t blocks[kWaves][kBlock];
-  __shared__ float ml[2][kWaves][16];
-  __shared__ __attribute__((aligned(16))) float joint[kWaves][16][kStride];
+  constexpr int kPiece = Shared<Rows>::kPiece;
+  auto& ml = lds.ml;
+  auto& joint = lds.joint;
   const Pool& p = a.pool;
   const int tid = threadIdx.x, lane = tid % 64, r = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -889,33 +907,32 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
   const int live = a.G - 16 * set < 16 ? a.G - 16 * set : 16;  // heads here
   const int head0 = kvh * a.G + 16 * set;
 
-  lay_out(a, plan);
   Walk walk;
-  walk.start(plan, p.batch, a.W);
-  while (walk.next(a, plan)) {
+  walk.start(lds.plan, p.batch, a.W);
+  while (walk.next(a, lds.plan)) {
     const int b = walk.seq, lo = walk.lo, end = walk.end;
     // A wavefront takes every fourth step of kRows rows.
     int row0 = walk.row + wave * kRows;
+    // The queries and the table first, then the first step's rows, and the
+    // queries' operands are prepared while these are on their way.
+    uint32_t qw[D / 32][4];
+    Rows::load_q(qw, uniform(a.q, 2 * (b * a.qstride + int64_t(head0) * D)), r < live, r, g);
     Pages pages;
-    pages.start(blocks[wave], p.table + b * p.tstride, (walk.n + (1 << p.shift) - 1) >> p.shift, row0 >> p.shift);
-
+    pages.start(lds.blocks[wave], p.table + b * p.tstride, (walk.n + (1 << p.shift) - 1) >> p.shift,
+                row0 >> p.shift);
+    typename Rows::K kr;
+    typename Rows::V vr;
+    Step<HALVES> h = step_of<HALVES>(p, pages, kvh, row0, end);
+    Rows::load_k(kr, a, h, r, g);
+    Rows::load_v(vr, a, h, r, g);
     typename Rows::Operand ops[Rows::kOperands];
     typename Rows::Rest q;
-    Rows::load_q(ops, q, uniform(a.q, 2 * (b * a.qstride + int64_t(head0) * D)), r < live, r, g, a.scale_log2);
+    Rows::prepare(ops, q, qw, r < live, g, a.scale_log2);
     floatx4 acc[C::kJ];
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) acc[j] = floatx4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
     typename Rows::Unit unit;
-
-    typename Rows::K kr;
-    typename Rows::V vr;
-    Step<HALVES> h{};
-    if (row0 < end) {
-      h = step_of<HALVES>(p, pages, kvh, row0, end);
-      Rows::load_k(kr, a, h, r, g);
-      Rows::load_v(vr, a, h, r, g);
-    }
     for (; row0 < end; row0 += kWaves * kRows) {
       // The last step loads its own rows again: no branch between the loads.
       Step<HALVES> hn = h;
@@ -1038,6 +1055,27 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(c
   }
 }
 
+// Whether the batch's rows are more than the memory-side cache may still hold
+// from an earlier call: then they are streamed. (16 ragged sequences, 70 MB in
+// turn with two other pools: 17 us kept, 23 streamed; 131,071 rows, 537 MB:
+// 95 us kept, 88 streamed; 268 MB: 50 and 46; 134 MB: 33 and 35.)
+__device__ __forceinline__ bool streams(const DecodeArgs& a, const Plan& plan) {
+  return __builtin_amdgcn_readfirstlane(plan.start[a.pool.batch]) > a.kept_units;
+}
+
+template <typename Rows>
+__global__ __launch_bounds__(64 * kWaves, Rows::kOcc) void paged_decode_kernel(const DecodeArgs a) {
+  __shared__ Shared<Rows> lds;
+  lay_out(a, lds.plan);
+  if constexpr (Rows::kChooses) {
+    if (!streams(a, lds.plan)) {
+      attend<typename Rows::Kept>(a, reinterpret_cast<Shared<typename Rows::Kept>&>(lds));
+      return;
+    }
+  }
+  attend<Rows>(a, lds);
+}
+
 // A workgroup barrier for LDS only: loads of the stream stay in flight.
 __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -1064,38 +1102,51 @@ __device__ __forceinline__ Step<1> quarter_of(const Step<4>& h, int wave) {
 constexpr int kWideTile = 16 * kWaves;
 
 template <typename Rows>
-__global__ __launch_bounds__(64 * kWaves, Rows::kWideOcc) void paged_wide_kernel(const DecodeArgs a) {
+struct SharedWide {
+  Plan plan;
+  int32_t blocks[kWaves][kBlock];
+  float4 tiles[2][16][16];
+  typename Rows::Operand queries[Rows::kOperands][64];
+};
+
+template <typename Rows>
+__device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows>& lds) {
   constexpr int D = Rows::kD;
   static_assert(D == 128 * kWaves && Rows::kHalves == 1, "a wavefront takes 128 channels");
-  __shared__ Plan plan;
-  __shared__ int32_t blocks[kWaves][kBlock];
-  __shared__ float4 tiles[2][16][16];
-  __shared__ typename Rows::Operand queries[Rows::kOperands][64];
+  auto& tiles = lds.tiles;
+  auto& queries = lds.queries;
   const Pool& p = a.pool;
   const int tid = threadIdx.x, lane = tid % 64, r = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int kvh = blockIdx.y / a.groups16, set = blockIdx.y % a.groups16;
   const int live = a.G - 16 * set < 16 ? a.G - 16 * set : 16;
   const int head0 = kvh * a.G + 16 * set;
-  lay_out(a, plan);
   Walk walk;
-  walk.start(plan, p.batch, a.W);
+  walk.start(lds.plan, p.batch, a.W);
   int buf = 0;
-  while (walk.next(a, plan)) {
+  while (walk.next(a, lds.plan)) {
     const int b = walk.seq, lo = walk.lo, end = walk.end;
     int row0 = walk.row;
+    uint32_t qw[D / 32][4];
+    Rows::load_q(qw, uniform(a.q, 2 * (b * a.qstride + int64_t(head0) * D)), r < live, r, g);
     Pages pages;
-    pages.start(blocks[wave], p.table + b * p.tstride, (walk.n + (1 << p.shift) - 1) >> p.shift, row0 >> p.shift);
+    pages.start(lds.blocks[wave], p.table + b * p.tstride, (walk.n + (1 << p.shift) - 1) >> p.shift,
+                row0 >> p.shift);
+    typename Rows::K kr;
+    typename Rows::Wide vr;
+    Step<4> h = step_of<4>(p, pages, kvh, row0, end);
+    Rows::load_k(kr, a, quarter_of(h, wave), r, g);
     typename Rows::Rest q;
     {
       typename Rows::Operand ops[Rows::kOperands];
-      Rows::load_q(ops, q, uniform(a.q, 2 * (b * a.qstride + int64_t(head0) * D)), r < live, r, g,
-                   a.scale_log2);
+      Rows::prepare(ops, q, qw, r < live, g, a.scale_log2);
       // The last segment's reads are over: every wavefront passed a barrier
       // since its last.
 #pragma unroll
       for (int c = 0; c < Rows::kOperands; ++c)
         if (c % kWaves == wave) queries[c][lane] = ops[c];
+      __builtin_amdgcn_sched_barrier(0);
+      Rows::load_wide(vr, a, h, wave, r, g);  // after it: no registers for both
       lds_barrier();
     }
     floatx4 acc[8];
@@ -1103,11 +1154,6 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kWideOcc) void paged_wide_kernel
     for (int j = 0; j < 8; ++j) acc[j] = floatx4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
     typename Rows::Unit unit;
-    typename Rows::K kr;
-    typename Rows::Wide vr;
-    Step<4> h = step_of<4>(p, pages, kvh, row0, end);
-    Rows::load_k(kr, a, quarter_of(h, wave), r, g);
-    Rows::load_wide(vr, a, h, wave, r, g);
     for (; row0 < end; row0 += kWideTile) {
       Step<4> hn = h;
       if (row0 + kWideTile < end) hn = step_of<4>(p, pages, kvh, row0 + kWideTile, end);
@@ -1202,6 +1248,19 @@ __global__ __launch_bounds__(64 * kWaves, Rows::kWideOcc) void paged_wide_kernel
       }
     }
   }
+}
+
+template <typename Rows>
+__global__ __launch_bounds__(64 * kWaves, Rows::kWideOcc) void paged_wide_kernel(const DecodeArgs a) {
+  __shared__ SharedWide<Rows> lds;
+  lay_out(a, lds.plan);
+  if constexpr (Rows::kChooses) {
+    if (!streams(a, lds.plan)) {
+      attend_wide<typename Rows::Kept>(a, reinterpret_cast<SharedWide<typename Rows::Kept>&>(lds));
+      return;
+    }
+  }
+  attend_wide<Rows>(a, lds);
 }
 
 // One affine layout's launch; a unit a head dim (paged_decode_d*.hip).

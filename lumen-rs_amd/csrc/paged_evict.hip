@@ -23,6 +23,7 @@ constexpr int kWaves = kSel / 64;
 constexpr int kQuads = 8;         // quads of rows a thread holds
 constexpr int kChunk = kSel * 4 * kQuads;
 constexpr int kBins = 2048;
+constexpr int kCopies = 4;        // of the histogram, by lane: weights crowd few digits
 
 // Bits that order like the weights: larger is heavier; NaN counts as -inf and
 // -0 as 0. Between 0x007fffff (-inf) and 0xff800000 (inf).
@@ -117,7 +118,7 @@ __device__ __forceinline__ void write_rows(const Held& x, int first, int quads, 
 
 __global__ __launch_bounds__(kSel) void evict_select_kernel(const Pool p, int budget, int sinks,
                                                             int recent, int32_t* __restrict__ kept) {
-  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t hist[kCopies][kBins + 1];
   __shared__ uint32_t waves[kWaves], counts[2][kWaves];
   __shared__ uint32_t found[3];  // the digit, the rows wanted within it, the rows it has
   const int unit = blockIdx.x, b = unit / p.Hkv, tid = threadIdx.x, lane = tid % 64;
@@ -140,8 +141,11 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(const Pool p, int bu
   uint32_t edge = 0, mask = 0, room = uint32_t(budget), have = 0;
   for (int pass = 0; pass < 3; ++pass) {
     const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass < 2 ? 2048 : 1024;
-    hist[tid] = 0;
-    hist[tid + kSel] = 0;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      hist[c][tid] = 0;
+      hist[c][tid + kSel] = 0;
+    }
     __syncthreads();
     for (int base = 0; base < n; base += step) {
       if (!one) load_rows(x, w, base + first, quads, n, lo, hi);
@@ -151,7 +155,7 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(const Pool p, int bu
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t u = x.u[4 * k + e];
-          if ((u & mask) == edge) atomicAdd(&hist[(u >> sh) & (bins - 1)], 1u);
+          if ((u & mask) == edge) atomicAdd(&hist[tid % kCopies][(u >> sh) & (bins - 1)], 1u);
         }
       }
     }
@@ -159,7 +163,12 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(const Pool p, int bu
     // Counts from the heaviest digit down: thread t takes the digits
     // bins - 1 - 2t and below it.
     const int d0 = bins - 1 - 2 * tid;
-    const uint32_t c0 = d0 >= 0 ? hist[d0] : 0, c1 = d0 >= 1 ? hist[d0 - 1] : 0;
+    uint32_t c0 = 0, c1 = 0;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      c0 += d0 >= 0 ? hist[c][d0] : 0;
+      c1 += d0 >= 1 ? hist[c][d0 - 1] : 0;
+    }
     const uint32_t above = block_scan(c0 + c1, waves);
     if (above < room && above + c0 >= room) {
       found[0] = uint32_t(d0);
