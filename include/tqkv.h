@@ -374,8 +374,8 @@ int32_t tqkv_paged_append(const tqkv_paged_kv* kv, const uint16_t* k, const uint
  * Attention of one new token a sequence over its pages, softmax(scale * q.K^T)
  * . V: tqkv_decode_attend_affine with a length and pages for each sequence.
  * q: bf16, head h of sequence b at q + b * q_stride + h * dim (16-byte
- * aligned, q_stride a multiple of 8); out: bf16 [batch, H, dim]. H / kv_heads
- * from 1 to 32. window > 0: the last `window` rows only; otherwise all.
+ * aligned, q_stride a multiple of 8); out: bf16 [batch, H, dim], not over q.
+ * H / kv_heads from 1 to 32 (more than 16 read the rows twice). window > 0: the last `window` rows only; otherwise all.
  * max_rows: the host's bound on lens (at most table_stride * page_rows); it
  * sizes the grid and the workspace, and a sequence that holds more attends
  * its first max_rows rows as if it held no more. A sequence without rows gets

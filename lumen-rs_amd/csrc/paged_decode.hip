@@ -14,6 +14,10 @@ namespace {
 
 constexpr int kJoinThreads = 256;
 constexpr int kWeightRows = 4 * kJoinThreads;  // rows whose weights a workgroup adds
+constexpr float kPartDown = 40.0f;  // log2 by which parts hold weights and their sums lower
+static_assert(Bf16Rows<128>::kDown == kPartDown, "as the parts are");
+static_assert(AffineRows<128, 4, 4, 64>::kLast == 0x1p-47f && AffineRows<128, 4, 4, 64>::kDown == kPartDown - 47,
+              "as the parts are");
 constexpr int kMaxSegments = 1024;  // of one sequence: the workgroups of a KV head
 
 // Where sequence b's segments lie: its first unit of all, and the total.
@@ -132,8 +136,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
         o.z += y.z;
         o.w += y.w;
       }
-      const float inv = 1.0f / l;
-      const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+      const float v[4] = {o.x / l, o.y / l, o.z / l, o.w / l};
       uint16_t* out = a.out + int64_t(blockIdx.x) * D + 4 * quad;
 #pragma unroll
       for (int i = 0; i < 4; ++i) out[i] = f32_to_bf16(l == 0.0f ? 0.0f : v[i]);
@@ -158,7 +161,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
     l = top == -INFINITY ? 0.0f * l : l * __builtin_amdgcn_exp2f(top - m);
     for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
     if (lane == 0) {
-      head_m[i] = m == -INFINITY ? 0.0f : m + a.down;
+      head_m[i] = m == -INFINITY ? 0.0f : m + kPartDown;
       head_r[i] = l == 0.0f ? 0.0f : 1.0f / l;
     }
   }
@@ -315,7 +318,6 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
   a.W = plan.W;
   a.over = kOver;
   a.scale_log2 = scale * 1.44269504088896340736f;
-  a.down = kv->kind == TQKV_CACHE_BF16 ? Bf16Rows<128>::kDown : AffineRows<128, 4, 4, 64>::kDown;
   a.part_o = static_cast<float*>(workspace);
   a.part_m = a.part_o + plan.slots * H * D;
   a.part_l = a.part_m + plan.slots * H;

@@ -60,7 +60,6 @@ struct DecodeArgs {
   int over;            // units that a sequence's start counts as
   int kept_units;      // bf16 rows beyond these are streamed
   float scale_log2;
-  float down;      // log2 by which the row format's weights are held lower
   float* part_o;  // [W + batch, H, D]
   float* part_m;  // [W + batch, H]: log2 units
   float* part_l;
@@ -342,7 +341,7 @@ struct Bf16Rows {
   // Weights are held times 2^-40 (their sum too, so it cancels): 2^30 rows of
   // weight 2^kTau and values of bf16's largest magnitude stay within f32.
   // Weights below 2^-86 of the largest vanish.
-  static constexpr float kDown = 40.0f;
+  static constexpr float kDown = 40.0f, kLast = 1.0f;
   struct Unit {  // of the accumulators
     __device__ __forceinline__ float of() const { return 1.0f; }
   };
@@ -647,8 +646,9 @@ struct AffineRows {
     return _Float16(fmaf(float(__builtin_bit_cast(halfx2, x)[half]), BV == 4 && (j & 1) ? s20 : s24, b));
   }
   // Weights are held times 2^7: they reach 2^(7 + kTau) in f16, and those that
-  // f16 loses lie below 2^-32 of the largest, 2^-15 in all at 2^17 rows.
-  static constexpr float kDown = -7.0f;
+  // f16 loses lie below 2^-32 of the largest, 2^-15 in all at 2^17 rows. At a
+  // segment's end they and their sum go down by 2^-47, to bf16 rows' 2^-40.
+  static constexpr float kDown = -7.0f, kLast = 0x1p-47f;
   // The accumulators hold values times `up`, a power of two, the wavefront's:
   // f16 values are at most 2^15, and the largest magnitude that the rows gave
   // when the unit was taken is near 2^6, so it is taken anew only when a
@@ -656,14 +656,14 @@ struct AffineRows {
   // `cap`, 2^9 times that.
   struct Unit {
     float up = 1.0f, cap = 0.0f;
-    __device__ __forceinline__ float of() const { return 1.0f / up; }
+    __device__ __forceinline__ float of() const { return kLast / up; }
     template <int N>
     __device__ __forceinline__ void admit(float most, floatx4 (&acc)[N]) {
       if (!__any(most > cap)) return;
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
       int E = int(__float_as_uint(most) >> 23) - 127;
-      E = E < -100 ? -100 : E;
+      E = E < -90 ? -90 : E;  // up * 2^24 stays finite
       const float next = __uint_as_float(uint32_t(127 + 5 - E) << 23);
       const float turn = next / up;  // both powers of two
 #pragma unroll
@@ -1000,6 +1000,7 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, Shared<Rows>& lds) {
     // The four wavefronts' parts, joined in their order.
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
+    l *= Rows::kLast;
     if (lane < 16) {
       ml[0][wave][r] = m;
       ml[1][wave][r] = l;
@@ -1221,13 +1222,14 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
     // Every wavefront holds the same maximum and sum.
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
+    l *= Rows::kLast;
     const int64_t slot = int64_t(blockIdx.x) + b;
     if (tid < live) {
       a.part_m[slot * a.H + head0 + tid] = m;
       a.part_l[slot * a.H + head0 + tid] = l;
     }
     if (r < live) {
-      const float of = unit.of(), inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float of = unit.of();
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = 128 * wave + (4 * g + i) * 8;
@@ -1235,8 +1237,8 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
           uint32_t w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            w[j] = f32_to_bf16(acc[2 * j][i] * of * inv) |
-                   uint32_t(f32_to_bf16(acc[2 * j + 1][i] * of * inv)) << 16;
+            w[j] = f32_to_bf16(l == 0.0f ? 0.0f : acc[2 * j][i] * of / l) |
+                   uint32_t(f32_to_bf16(l == 0.0f ? 0.0f : acc[2 * j + 1][i] * of / l)) << 16;
           uint16_t* out = a.out + (int64_t(b) * a.H + head0 + r) * D + d;
 #pragma unroll
           for (int j = 0; j < 8; ++j) out[j] = uint16_t(w[j / 2] >> (16 * (j % 2)));

@@ -347,6 +347,9 @@ extern "C" int32_t tqkv_paged_evict(const tqkv_paged_kv* kv, int64_t budget, int
     return fail(TQKV_EINVAL_SHAPE, "budget=%lld sinks=%lld recent=%lld of %lld new pages a sequence",
                 (long long)budget, (long long)sinks, (long long)recent, (long long)dst_stride);
   if (!kv->weights || !dst_table || !dst_lens) return fail(TQKV_EINVAL_ARG, "null pointer");
+  if (!aligned(dst_table, 4) || !aligned(dst_lens, 4) || !aligned(dst_weights, 4) ||
+      !aligned(kept, 4))
+    return fail(TQKV_EINVAL_ARG, "dst_table, dst_lens, dst_weights or kept not 4-byte aligned");
   if (dst_weights == kv->weights) return fail(TQKV_EINVAL_ARG, "dst_weights is the pool's weights");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const size_t need = tqkv_paged_evict_workspace_size(kv, budget);

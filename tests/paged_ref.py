@@ -108,10 +108,12 @@ class Paged:
     def attend(self, q, scale, window=-1, max_rows=None):
         """q bf16 [B, H, D]: (output f64, its tolerance, weights to add f64,
         theirs). The tolerances count roundings: half a bf16 step of the
-        output (2^-8 of it) and, on affine rows, of each value; 2^-16 of each
-        weight's hi + lo pair; the f32 score sums (a step 2^-24 an addition
-        of the products' magnitudes) and exp2's argument and result, which
-        move a weight by their size."""
+        output (2^-8 of it); each weight's, 2^-16 as a bf16 pair, 2^-12 as the
+        f16 that affine rows take, and there each value's as f16 too, with
+        what f16 loses of small weights (2^-32 of the largest) and small
+        values (2^-30 of the largest); the f32 score sums (a step 2^-24 an
+        addition of the products' magnitudes) and exp2's argument and result,
+        which move a weight by their size."""
         H, D = q.shape[1], self.D
         G = H // self.Hkv
         qf = O.bf16_to_f32(q).astype(np.float64)
@@ -137,8 +139,10 @@ class Paged:
                     sums = (D + 16) * 2.0 ** -24 * (big @ np.abs(qf[b, e])).max() * abs(scale)
                     d = 2 * (sums + 2.0 ** -22 * (np.abs(s).max() + 4))  # of a weight, and of their sum
                     out[b, e] = p @ v
-                    each = (2.0 ** -8 if self.bv != 16 else 0.0) + 2.0 ** -16 + d + n * 2.0 ** -24
+                    each = (2.0 ** -11 if self.bv != 16 else 2.0 ** -16) + d + n * 2.0 ** -24
                     tol[b, e] = 2.0 ** -8 * np.abs(out[b, e]) + 1.01 * each * (p @ np.abs(v)) + 1e-30
+                    if self.bv != 16:
+                        tol[b, e] += (n * 2.0 ** -32 * p.max() + 2.0 ** -30) * np.abs(v).max()
                     gain[b, h, r] += p
                     gtol[b, h, r] += (d + n * 2.0 ** -24) * p + 1e-12
         return out, tol, gain, gtol

@@ -8,7 +8,7 @@ import pytest
 
 import oracle_lib as O
 from inputs import kv_bf16
-from paged_ref import AFFINE, BF16, GUARD, Paged, check
+from paged_ref import AFFINE, BF16, Paged, check
 from test_gpu_capture import captured
 
 pytestmark = pytest.mark.gpu
@@ -29,7 +29,6 @@ def say(*a):
 def append(T, p, counts, seed, heads_before=0, pad=0, gap=0):
     """lens already count the new rows: host and device appended, compared
     byte for byte, rows behind and pages beside included."""
-    rng = np.random.default_rng(seed)
     total = sum(counts)
     heads = heads_before + 2 * p.Hkv
     width = heads * p.D + pad
@@ -49,7 +48,6 @@ def append(T, p, counts, seed, heads_before=0, pad=0, gap=0):
             assert np.array_equal(g, w)
     if p.weights is not None:
         assert np.array_equal(d.weights.numpy(), p.weights)
-    del rng
 
 
 APPENDS = [
@@ -243,6 +241,35 @@ def test_attend_type_extremes_in_bf16_rows(T):
     assert np.all(np.abs(got[0] - want) <= 2.0 ** -7 * (w / w.sum() @ np.abs(v[keep])))
 
 
+@pytest.mark.parametrize("D", [128, 512])
+@pytest.mark.parametrize("power", [-75, -14, 14, 60, 118])
+def test_attend_values_of_any_magnitude(T, D, power):
+    """Affine values times powers of two, one sequence's pages larger than the
+    others' by 2^20 half way: the f16 unit follows them."""
+    say("magnitude", D, power)
+    p = Paged([700, 33], 1, D, 16, AFFINE, 4, 8, 64, seed=power % 97).fill(3)
+    late = p.table[0, 20:44]
+    for t in p.sides[1][1:]:
+        x = O.bf16_to_f32(t) * np.float32(2.0 ** min(power, 100)) * np.float32(2.0 ** max(power - 100, 0))
+        x[late] *= np.float32(2.0 ** (-20 if power > 100 else 20))
+        t[...] = O.bf16_from_f32(x)
+    q = kv_bf16((2, 4, D), 8)
+    out, tol, _, _ = p.attend(q, 0.05)
+    check(O.bf16_to_f32(p.device(T).attend(q, 0.05)), out, tol, f"2^{power}")
+
+
+@pytest.mark.parametrize("power", [-60, 40])
+def test_attend_queries_of_any_magnitude(T, power):
+    """Queries times a power of two, the scale times its inverse."""
+    for kind in (BF16, AFFINE):
+        p = Paged([300, 40], 2, 128, 32, kind, seed=19).fill(19)
+        q = kv_bf16((2, 4, 128), 8)
+        d = p.device(T)
+        big = O.bf16_from_f32(O.bf16_to_f32(q) * np.float32(2.0 ** power))
+        say("queries", kind, power)
+        assert np.array_equal(d.attend(q, 0.09), d.attend(big, float(np.float32(0.09) * 2.0 ** -power)))
+
+
 def test_attend_shared_pages(T):
     """A prompt's pages shared by every sequence, their weights apart."""
     for kind in (BF16, AFFINE):
@@ -425,7 +452,6 @@ def test_prompt_steps_and_evictions(T, kind, D, H, Hkv, R):
     p = Paged([0, 0, 0], Hkv, D, R, kind, stride=10, seed=51, spare=400, track=True)
     say("in use", kind, D)
     free = list(p.spare)
-    ids = np.random.default_rng(1)
 
     def grow():
         for b in range(p.B):
@@ -458,7 +484,6 @@ def test_prompt_steps_and_evictions(T, kind, D, H, Hkv, R):
             k = min(neww.shape[2], p.weights.shape[2])
             p.weights[:, :, :k] = neww[:, :, :k]
             free = [f for f in free if f not in set(dst[dst >= 0].tolist())]
-    del ids
 
 
 def test_captured_steps_follow_the_device_lengths(T):
@@ -548,4 +573,3 @@ def test_two_streams_at_once(T):
         assert np.array_equal(out.numpy(), w)
     for s in streams:
         hip.h.hipStreamDestroy(ctypes.c_void_p(s))
-    assert GUARD

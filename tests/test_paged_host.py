@@ -96,7 +96,9 @@ def test_evict_refusals():
               dst_weights=2 * A, kept=A)
     for other, status in [(dict(kv=view(weights=None)), T.EINVAL_ARG),
                           (dict(dst_table=None), T.EINVAL_ARG), (dict(dst_lens=None), T.EINVAL_ARG),
-                          (dict(dst_weights=A), T.EINVAL_ARG), (dict(budget=0), T.EINVAL_SHAPE),
+                          (dict(dst_weights=A), T.EINVAL_ARG), (dict(dst_table=A + 2), T.EINVAL_ARG),
+                          (dict(dst_weights=A + 2), T.EINVAL_ARG), (dict(kept=A + 1), T.EINVAL_ARG),
+                          (dict(dst_lens=A + 3), T.EINVAL_ARG), (dict(budget=0), T.EINVAL_SHAPE),
                           (dict(sinks=-1), T.EINVAL_SHAPE), (dict(recent=-1), T.EINVAL_SHAPE),
                           (dict(sinks=60, recent=5), T.EINVAL_SHAPE),
                           (dict(sinks=1 << 62, recent=1 << 62), T.EINVAL_SHAPE),
