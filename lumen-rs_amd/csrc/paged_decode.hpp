@@ -31,10 +31,14 @@
 // is one more product, of the biases as they lie and the query sums in three
 // bf16 parts. Values are dequantized by one mixed multiply-add a code, f32 to
 // f16 in a unit of the wavefront's, and weights enter as f16 too (each
-// rounded by at most 2^-12 of itself, a sixteenth of a bf16 step).
+// rounded by at most 2^-11 of itself, an eighth of the output's own rounding).
 //
 // Bound by HBM: the live rows once. At G heads of 16 the matrix cores do
-// 16 / G times the work that is needed and are still far from busy.
+// 16 / G times the work that is needed and are still far from busy (7 to 20%).
+// Measured, with the join: bf16, 131,071 rows x 8 KV heads at D = 128 (537 MB)
+// 88 us, 6.1 TB/s; 4 bits, 16 x 32,768 x 8 at D = 256 (1.21 GB) 245 us, 4.9
+// TB/s, where unpacking keeps the vector units 72% busy. Short calls are bound
+// by latencies: 777 rows take 7.8 us and the join's 4.5.
 #pragma once
 
 #include <type_traits>
@@ -540,7 +544,8 @@ struct AffineRows {
       const float hi = __bf16(sum), mid = __bf16(sum - hi), lo = __bf16(sum - hi - mid);
       q.sum[n / 8][n % 8] = __bf16(g == 0 ? hi : g == 1 ? mid : g == 2 ? lo : 0.0f);
     }
-    q.mul = scale_log2 != 0.0f ? ldexpf(fabsf(scale_log2), E + 10) : 1.0f;
+    // Above 0: masked scores are -inf times it.
+    q.mul = scale_log2 != 0.0f ? fmaxf(ldexpf(fabsf(scale_log2), E + 10), 0x1p-126f) : 1.0f;
   }
   static __device__ __forceinline__ void load_k(K& k, const DecodeArgs& a, const S& h, int r,
                                                 int g) {

@@ -108,8 +108,10 @@ class Paged:
     def attend(self, q, scale, window=-1, max_rows=None):
         """q bf16 [B, H, D]: (output f64, its tolerance, weights to add f64,
         theirs). The tolerances count roundings: half a bf16 step of the
-        output (2^-8 of it); each weight's, 2^-16 as a bf16 pair, 2^-12 as the
-        f16 that affine rows take, and there each value's as f16 too, with
+        output (2^-8 of it); each weight's, 2^-16 as a bf16 pair (2^-8 of what
+        the first part's 2^-8 left), 2^-11 as the f16 that affine rows take,
+        and there each value's as f16 too (half a step of 10 stored bits,
+        2^-11: 2^-11 + 2^-11 = 2^-10 of a term), with
         what f16 loses of small weights (2^-32 of the largest) and small
         values (2^-30 of the largest); the f32 score sums (a step 2^-24 an
         addition of the products' magnitudes) and exp2's argument and result,
@@ -139,7 +141,7 @@ class Paged:
                     sums = (D + 16) * 2.0 ** -24 * (big @ np.abs(qf[b, e])).max() * abs(scale)
                     d = 2 * (sums + 2.0 ** -22 * (np.abs(s).max() + 4))  # of a weight, and of their sum
                     out[b, e] = p @ v
-                    each = (2.0 ** -11 if self.bv != 16 else 2.0 ** -16) + d + n * 2.0 ** -24
+                    each = (2.0 ** -10 if self.bv != 16 else 2.0 ** -16) + d + n * 2.0 ** -24
                     tol[b, e] = 2.0 ** -8 * np.abs(out[b, e]) + 1.01 * each * (p @ np.abs(v)) + 1e-30
                     if self.bv != 16:
                         tol[b, e] += (n * 2.0 ** -32 * p.max() + 2.0 ** -30) * np.abs(v).max()

@@ -270,6 +270,20 @@ def test_attend_queries_of_any_magnitude(T, power):
         assert np.array_equal(d.attend(q, 0.09), d.attend(big, float(np.float32(0.09) * 2.0 ** -power)))
 
 
+@pytest.mark.parametrize("kind", [BF16, AFFINE])
+@pytest.mark.parametrize("power", [-126, -100, 0])
+def test_attend_scales_and_queries_that_vanish(T, kind, power):
+    """Scores of nothing, and of a factor below f32's smallest, beside rows
+    that are masked: every row of the window has the same weight."""
+    p = Paged([17, 50, 3], 2, 128, 16, kind, 8, 4, 32, seed=21, spare=1).fill(22)
+    q = kv_bf16((3, 4, 128), 23)
+    q[0] = 0
+    q[1] = O.bf16_from_f32(O.bf16_to_f32(q[1]) * np.float32(2.0 ** power))
+    for scale in (2.0 ** -60, 0.0):
+        out, tol, _, _ = p.attend(q, scale, 33)
+        check(O.bf16_to_f32(p.device(T).attend(q, scale, 33)), out, tol, f"2^{power} x {scale}")
+
+
 def test_attend_shared_pages(T):
     """A prompt's pages shared by every sequence, their weights apart."""
     for kind in (BF16, AFFINE):
