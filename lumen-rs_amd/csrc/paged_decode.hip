@@ -20,24 +20,6 @@ static_assert(AffineRows<128, 4, 4, 64>::kLast == 0x1p-47f && AffineRows<128, 4,
               "as the parts are");
 constexpr int kMaxSegments = 1024;  // of one sequence: the workgroups of a KV head
 
-// Where sequence b's segments lie: its first unit of all, and the total.
-__device__ __forceinline__ void place(const DecodeArgs& a, int b, int64_t* red, int* first,
-                                      int* total) {
-  int64_t mine = 0;  // units before b in the high half, all in the low
-  for (int i = threadIdx.x; i < a.pool.batch; i += kJoinThreads) {
-    const int64_t t = span_of(a, i).units;
-    mine += t + (i < b ? t << 32 : 0);
-  }
-  for (int off = 32; off > 0; off >>= 1) mine += __shfl_xor(mine, off, 64);
-  __syncthreads();
-  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = mine;
-  __syncthreads();
-  mine = 0;
-  for (int w = 0; w < kJoinThreads / 64; ++w) mine += red[w];
-  *first = int(mine >> 32);
-  *total = int(mine & 0xffffffff);
-}
-
 // 2^(m_s - m) of every segment s of one (sequence, head) into LDS, and the sum
 // of the segments' sums by those. All threads call it.
 __device__ __forceinline__ float segment_weights(const DecodeArgs& a, int64_t slot0, int n, int h,
@@ -74,61 +56,92 @@ __device__ __forceinline__ float segment_weights(const DecodeArgs& a, int64_t sl
   return l;
 }
 
-// Workgroups [0, batch x H): the output of one (sequence, head) from its
-// segments, a quad of channels a thread, the segments dealt over the rows of
-// threads, then the rows in order. The others: kWeightRows rows of one
-// (sequence, KV head), weights[row] += sum over the group's heads of
-// 2^(s - m) / l.
+// Channels that a workgroup joins, a quad a thread, and the threads that the
+// segments are dealt over.
+template <int D>
+struct JoinShape {
+  static constexpr int kPart = D < 128 ? D : 128, kParts = D / kPart;
+  static constexpr int kQuads = kPart / 4, kDeal = kJoinThreads / kQuads;
+};
+// Segments whose weights a wavefront holds, one a lane.
+constexpr int kFew = 64;
+
+// Workgroups [0, batch x H x parts): channels of the output of one (sequence,
+// head) from its segments. The others: kWeightRows rows of one (sequence, KV
+// head), weights[row] += sum over the group's heads of 2^(s - m) / l. Bound by
+// a chain of loads: the starts, then all that depends on them at once.
 template <int D>
 __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeArgs a,
                                                                   int row_blocks) {
-  constexpr int kQuads = D / 4, kDeal = kJoinThreads / kQuads;
-  __shared__ int64_t red64[kJoinThreads / 64];
+  using J = JoinShape<D>;
+  constexpr int kQuads = J::kQuads, kDeal = J::kDeal;
   __shared__ float red[kJoinThreads / 64], weight[kMaxSegments], head_m[32], head_r[32];
   __shared__ float4 sums[kJoinThreads];
-  const int tid = threadIdx.x, outs = a.pool.batch * a.H;
+  const int tid = threadIdx.x, lane = tid % 64, outs = a.pool.batch * a.H * J::kParts;
   const bool joins = int(blockIdx.x) < outs;
-  int b, h = 0, kvh = 0, block = 0;
+  int b, h = 0, kvh = 0, block = 0, part = 0;
   if (joins) {
-    b = blockIdx.x / a.H;
-    h = blockIdx.x % a.H;
+    part = blockIdx.x % J::kParts;
+    h = blockIdx.x / J::kParts % a.H;
+    b = blockIdx.x / J::kParts / a.H;
   } else {
     const int i = blockIdx.x - outs;
     block = i % row_blocks;
     kvh = i / row_blocks % a.pool.Hkv;
     b = i / row_blocks / a.pool.Hkv;
   }
-  const Span span = span_of(a, b);
-  if (joins && span.n == 0) {
-    for (int d = tid; d < D; d += kJoinThreads) a.out[int64_t(blockIdx.x) * D + d] = 0;
-    return;
-  }
-  const int row0 = span.lo / 4 * 4 + block * kWeightRows;
-  if (!joins && row0 >= span.n) return;
-  int first, total;
-  place(a, b, red64, &first, &total);
+  const int first = a.starts[b], next = a.starts[b + 1], total = a.starts[a.pool.batch];
   const int per = units_per_wg(total, a.W);
-  const int w0 = (first + a.over) / per, n = (first + span.units - 1) / per - w0 + 1;
+  const int w0 = (first + a.over) / per, n = (next - 1) / per - w0 + 1;
   const int64_t slot0 = w0 + b;
   float m;
   if (joins) {
+    const int quad = tid % kQuads, deal = tid / kQuads, d = part * J::kPart + 4 * quad;
+    uint16_t* out = a.out + (int64_t(b) * a.H + h) * D + d;
+    if (next == first) {  // no rows
+      if (deal == 0)
+        for (int i = 0; i < 4; ++i) out[i] = 0;
+      return;
+    }
     if (n == 1) return;  // written by the attention kernel
-    const float l = segment_weights(a, slot0, n, h, weight, red, &m);
-    const int quad = tid % kQuads, deal = tid / kQuads;
-    const float* po = a.part_o + (slot0 * a.H + h) * D + 4 * quad;
+    const float* po = a.part_o + (slot0 * a.H + h) * D + d;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int s = deal; s < n; s += kDeal) {
-      const float w = weight[s];
-      const float4 y = *reinterpret_cast<const float4*>(po + int64_t(s) * a.H * D);
+    float l;
+    auto add = [&](float w, const float4& y) {
       o.x = fmaf(w, y.x, o.x);
       o.y = fmaf(w, y.y, o.y);
       o.z = fmaf(w, y.z, o.z);
       o.w = fmaf(w, y.w, o.w);
+    };
+    if (n <= kFew) {
+      const int seg = lane < n ? lane : n - 1;
+      const float pm = a.part_m[(slot0 + seg) * a.H + h], pl = a.part_l[(slot0 + seg) * a.H + h];
+      float4 y[kFew / kDeal];
+#pragma unroll
+      for (int i = 0; i < kFew / kDeal; ++i) {
+        const int s = deal + i * kDeal < n ? deal + i * kDeal : n - 1;
+        y[i] = *reinterpret_cast<const float4*>(po + int64_t(s) * a.H * D);
+      }
+      m = pm;
+      for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+      const float w = pm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm - m);
+      l = lane < n ? w * pl : 0.0f;  // a NaN sum stays one
+      for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
+#pragma unroll
+      for (int i = 0; i < kFew / kDeal; ++i) {
+        const float ws = __shfl(w, deal + i * kDeal, 64);
+        if (deal + i * kDeal < n) add(ws, y[i]);
+      }
+    } else {
+      l = segment_weights(a, slot0, n, h, weight, red, &m);
+#pragma unroll 8
+      for (int s = deal; s < n; s += kDeal)
+        add(weight[s], *reinterpret_cast<const float4*>(po + int64_t(s) * a.H * D));
     }
     sums[tid] = o;
     __syncthreads();
     if (deal == 0) {
+#pragma unroll
       for (int i = 1; i < kDeal; ++i) {
         const float4 y = sums[i * kQuads + quad];
         o.x += y.x;
@@ -137,18 +150,32 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
         o.w += y.w;
       }
       const float v[4] = {o.x / l, o.y / l, o.z / l, o.w / l};
-      uint16_t* out = a.out + int64_t(blockIdx.x) * D + 4 * quad;
 #pragma unroll
       for (int i = 0; i < 4; ++i) out[i] = f32_to_bf16(l == 0.0f ? 0.0f : v[i]);
     }
     return;
   }
+  const Span span = span_of(a, b);
+  const int row0 = span.lo / 4 * 4 + block * kWeightRows, row = row0 + 4 * tid;
+  if (row0 >= span.n) return;
+  float* weights = a.pool.weights + (int64_t(b) * a.pool.Hkv + kvh) * a.pool.wstride;
+  const float* scores = a.scores + (int64_t(b) * a.H + kvh * a.G) * a.srows;
+  // Four rows a thread; the scores of rows outside the span are -inf or unset.
+  // The first heads' are on their way while the heads' sums are found; rows
+  // past the end load the first ones.
+  const int at = row < span.n ? row : row0;
+  const float4 old = *reinterpret_cast<const float4*>(weights + at);
+  constexpr int kAhead = 4;
+  float4 x[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    x[i] = *reinterpret_cast<const float4*>(scores + (i < a.G ? i : 0) * a.srows + at);
   // A wavefront a head.
   for (int i = tid / 64; i < a.G; i += kJoinThreads / 64) {
-    const int at = kvh * a.G + i, lane = tid % 64;
+    const int head = kvh * a.G + i;
     float top = -INFINITY, l = 0.0f;
     for (int s = lane; s < n; s += 64) {  // the running maximum and sum of the lane's segments
-      const float pm = a.part_m[(slot0 + s) * a.H + at], pl = a.part_l[(slot0 + s) * a.H + at];
+      const float pm = a.part_m[(slot0 + s) * a.H + head], pl = a.part_l[(slot0 + s) * a.H + head];
       const float next = fmaxf(top, pm);
       if (next > -INFINITY)
         l = l * __builtin_amdgcn_exp2f(top - next) + pl * __builtin_amdgcn_exp2f(pm - next);
@@ -166,22 +193,21 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
     }
   }
   __syncthreads();
-  float* weights = a.pool.weights + (int64_t(b) * a.pool.Hkv + kvh) * a.pool.wstride;
-  const float* scores = a.scores + (int64_t(b) * a.H + kvh * a.G) * a.srows;
-  const int row = row0 + 4 * tid;
   if (row >= span.n) return;
-  // Four rows a thread; the scores of rows outside the span are -inf or unset.
-  const float4 old = *reinterpret_cast<const float4*>(weights + row);
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int i = 0; i < a.G; ++i) {
-    const float4 x = *reinterpret_cast<const float4*>(scores + i * a.srows + row);
+  auto add = [&](const float4& y, int i) {
     const float hm = head_m[i], hr = head_r[i];
-    sum[0] += __builtin_amdgcn_exp2f(x.x - hm) * hr;
-    sum[1] += __builtin_amdgcn_exp2f(x.y - hm) * hr;
-    sum[2] += __builtin_amdgcn_exp2f(x.z - hm) * hr;
-    sum[3] += __builtin_amdgcn_exp2f(x.w - hm) * hr;
-  }
+    sum[0] += __builtin_amdgcn_exp2f(y.x - hm) * hr;
+    sum[1] += __builtin_amdgcn_exp2f(y.y - hm) * hr;
+    sum[2] += __builtin_amdgcn_exp2f(y.z - hm) * hr;
+    sum[3] += __builtin_amdgcn_exp2f(y.w - hm) * hr;
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (i < a.G) add(x[i], i);
+#pragma unroll 4
+  for (int i = kAhead; i < a.G; ++i)
+    add(*reinterpret_cast<const float4*>(scores + i * a.srows + row), i);
   const float v[4] = {old.x + sum[0], old.y + sum[1], old.z + sum[2], old.w + sum[3]};
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -252,7 +278,7 @@ bool plan_of(const tqkv_paged_kv* kv, int32_t H, int64_t max_rows, HostPlan* out
   p.W = int(W);
   p.slots = size_t(p.W) + kv->batch;
   size_t floats = p.slots * H * (size_t(kv->dim) + 2);
-  floats = (floats + 3) / 4 * 4;
+  floats = (floats + 3) / 4 * 4 + (size_t(kv->batch) + 4) / 4 * 4;
   if (kv->weights) floats += size_t(kv->batch) * H * size_t(p.srows);
   p.bytes = floats * sizeof(float);
   *out = p;
@@ -294,7 +320,9 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
   a.window = window > 0 && window < max_rows ? int(window) : 0;
   const int64_t seen = a.window > 0 ? a.window + 3 : max_rows;  // from a row of four
   const int row_blocks = kv->weights ? int((seen + kWeightRows - 1) / kWeightRows) : 0;
-  const int64_t blocks = int64_t(kv->batch) * H + int64_t(kv->batch) * kv->kv_heads * row_blocks;
+  const int parts = kv->dim > 128 ? kv->dim / 128 : 1;  // JoinShape's
+  const int64_t blocks =
+      int64_t(kv->batch) * H * parts + int64_t(kv->batch) * kv->kv_heads * row_blocks;
   // Units over the whole batch are 32-bit in the kernels, and a grid
   // holds below 2^32 threads.
   if (int64_t(kv->batch) * (plan.srows / kUnit + kOver + 1) > 0x7fffffffLL ||
@@ -323,8 +351,10 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
   a.part_l = a.part_m + plan.slots * H;
   a.srows = plan.srows;
   a.kept_units = int(kKeptBytes / (int64_t(kUnit) * kv->kv_heads * 4 * D));
+  a.starts = reinterpret_cast<int32_t*>(static_cast<float*>(workspace) +
+                                        (plan.slots * H * (size_t(D) + 2) + 3) / 4 * 4);
   if (kv->weights)
-    a.scores = static_cast<float*>(workspace) + (plan.slots * H * (size_t(D) + 2) + 3) / 4 * 4;
+    a.scores = reinterpret_cast<float*>(a.starts) + (kv->batch + 4) / 4 * 4;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(unsigned(a.W), unsigned(kv->kv_heads * a.groups16));
   launch(kv, a, grid, st, false);

@@ -67,6 +67,7 @@ struct DecodeArgs {
   float* part_o;  // [W + batch, H, D]
   float* part_m;  // [W + batch, H]: log2 units
   float* part_l;
+  int32_t* starts;  // [batch + 1]: units before each sequence, all; for the join
   float* scores;  // [batch, H, srows] log2 units, or NULL
   int64_t srows;
 };
@@ -807,11 +808,13 @@ struct Plan {
   int32_t waves[kWaves];
 };
 
-// Fills the plan in LDS. All 64 kWaves threads call it.
+// Fills the plan in LDS, the first workgroup the join's copy too. All 64 kWaves
+// threads call it.
 __device__ __forceinline__ void lay_out(const DecodeArgs& a, Plan& plan) {
   constexpr int kThreads = 64 * kWaves, kMost = kMaxBatch / kThreads;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, B = a.pool.batch;
   const int per = (B + kThreads - 1) / kThreads;
+  const bool writes = blockIdx.x == 0 && blockIdx.y == 0;
   int mine = 0, units[kMost];
 #pragma unroll
   for (int i = 0; i < kMost; ++i) {
@@ -837,10 +840,16 @@ __device__ __forceinline__ void lay_out(const DecodeArgs& a, Plan& plan) {
 #pragma unroll
   for (int i = 0; i < kMost; ++i) {
     const int b = tid * per + i;
-    if (i < per && b < B) plan.start[b] = at;
+    if (i < per && b < B) {
+      plan.start[b] = at;
+      if (writes) a.starts[b] = at;
+    }
     at += units[i];
   }
-  if (tid == kThreads - 1) plan.start[B] = at;
+  if (tid == kThreads - 1) {
+    plan.start[B] = at;
+    if (writes) a.starts[B] = at;
+  }
   __syncthreads();
 }
 
