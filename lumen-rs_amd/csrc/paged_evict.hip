@@ -8,10 +8,12 @@
 // `sinks`, the last `recent`) take part as the heaviest of all. Up to 32,768
 // rows stay in registers between the passes; more are read again, from the
 // caches. Bound by one CU's vector units (every operation a row costs 16
-// cycles a 1,024 rows) and the passes' barriers: 15 us for 16,384 rows to 2,048
-// (8 workgroups), 18 for 16 sequences of up to 30,000 to 4,096 (128). (2) The
-// gather moves the rows to their new pages, bound by HBM: 16 x 4,096 x 8 rows
-// of 4 bits 28 us, in pieces of a row's 64 bytes.
+// cycles a 1,024 rows) and the passes' barriers: 13 us for 16,384 rows to 2,048
+// (8 workgroups), 16 for 16 sequences of up to 30,000 to 4,096 (128); the third
+// pass, which most selections do not need, took 2. (2) The gather moves the rows
+// to their new pages, bound by HBM: 16 sequences cut to 4,096 rows x 8 heads of
+// 4 bits 24 us, in pieces of a row's 64 bytes (28 with four wavefronts a
+// workgroup).
 #include <cmath>
 
 #include "paged.hpp"
@@ -186,9 +188,11 @@ __global__ __launch_bounds__(kSel) void evict_select_kernel(const Pool p, int bu
     mask |= uint32_t(bins - 1) << sh;
     room = found[1];
     have = found[2];
+    if (have == room) break;  // the digits below decide nothing
   }
   // Of the `have` rows at the edge, the first `room` stay. Where all do, they
-  // count as above it.
+  // count as above it (the edge is then the least of its digits, and not 0: the
+  // lightest weight's bits are above).
   const bool ties = have > room;
   if (!ties) edge -= 1;
   uint32_t at = 0, tied = 0;  // before this chunk
@@ -237,6 +241,7 @@ struct MoveArgs {
   float* dst_weights;
   int budget;
   int slots;  // buffers a side
+  int rows;   // kept rows a workgroup: a power of two
   void* k[3];
   void* v[3];
   int k_shift[3], v_shift[3];  // log2 of a row's bytes: all are powers of two
@@ -246,22 +251,24 @@ typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));  // a 16-byte unit
 
 int log2_of(int x) { return 31 - __builtin_clz(unsigned(x)); }
 
-constexpr int kThreads = 256;
-constexpr int kRows = 64;  // kept rows a workgroup
+// A wavefront a workgroup, so that the most of them have their chains of loads
+// (positions, pages, rows) going at once.
+constexpr int kThreads = 64;
+constexpr int kRows = 64;  // kept rows a workgroup at most
 
 // Rows of one buffer (2^ks units of type T each) and of another (2^vs), four
 // loads of each in flight a thread. src is a row that can be read also where
 // dst is -1.
 template <typename T>
 __device__ __forceinline__ void move_rows(T* kb, int ks, T* vb, int vs, const int64_t* src,
-                                          const int64_t* dst) {
-  const int items = kRows << (ks > vs ? ks : vs);
+                                          const int64_t* dst, int rows) {
+  const int items = rows << (ks > vs ? ks : vs);
   auto load = [&](const T* buf, int shift, int i) {
-    return buf[(src[(i >> shift) % kRows] << shift) + (i & ((1 << shift) - 1))];
+    return buf[(src[(i >> shift) & (rows - 1)] << shift) + (i & ((1 << shift) - 1))];
   };
   auto store = [&](T* buf, int shift, int i, T x) {
     const int r = i >> shift;
-    if (r < kRows && dst[r] >= 0) buf[(dst[r] << shift) + (i & ((1 << shift) - 1))] = x;
+    if (r < rows && dst[r] >= 0) buf[(dst[r] << shift) + (i & ((1 << shift) - 1))] = x;
   };
   for (int i = threadIdx.x; i < items; i += 4 * kThreads) {
     const T x0 = load(kb, ks, i), x1 = load(kb, ks, i + kThreads);
@@ -283,9 +290,9 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(const MoveArgs a) 
   __shared__ int64_t src[kRows], dst[kRows];
   const Pool& p = a.pool;
   const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-  const int i0 = blockIdx.x * kRows, rmask = (1 << p.shift) - 1;
+  const int i0 = blockIdx.x * a.rows, rmask = (1 << p.shift) - 1;
   const int64_t unit = int64_t(b) * p.Hkv + h;
-  if (tid < kRows) {
+  if (tid < a.rows) {
     const int i = i0 + tid;
     const int r = i < a.budget ? a.kept[unit * a.budget + i] : -1;
     int64_t s = 0, d = -1;
@@ -315,13 +322,14 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(const MoveArgs a) 
     if (i >= a.slots) break;
     const int ks = a.k_shift[i], vs = a.v_shift[i];
     if (ks >= 4 && vs >= 4)
-      move_rows(static_cast<uintx4*>(a.k[i]), ks - 4, static_cast<uintx4*>(a.v[i]), vs - 4, src, dst);
+      move_rows(static_cast<uintx4*>(a.k[i]), ks - 4, static_cast<uintx4*>(a.v[i]), vs - 4, src, dst,
+                a.rows);
     else if (ks >= 2)  // scales and biases: rows of one length
       move_rows(static_cast<uint32_t*>(a.k[i]), ks - 2, static_cast<uint32_t*>(a.v[i]), vs - 2, src,
-                dst);
+                dst, a.rows);
     else
       move_rows(static_cast<uint16_t*>(a.k[i]), ks - 1, static_cast<uint16_t*>(a.v[i]), vs - 1, src,
-                dst);
+                dst, a.rows);
   }
 }
 
@@ -353,6 +361,22 @@ extern "C" int32_t tqkv_paged_evict(const tqkv_paged_kv* kv, int64_t budget, int
       !aligned(kept, 4))
     return fail(TQKV_EINVAL_ARG, "dst_table, dst_lens, dst_weights or kept not 4-byte aligned");
   if (dst_weights == kv->weights) return fail(TQKV_EINVAL_ARG, "dst_weights is the pool's weights");
+  const int D = kv->dim;
+  a.slots = kv->kind == TQKV_CACHE_BF16 ? 1 : 3;
+  for (int i = 0; i < a.slots; ++i) {
+    a.k[i] = kv->slot[i];
+    a.v[i] = kv->slot[a.slots + i];
+    const int scales = 2 * D / (i > 0 ? kv->group_size : 1);  // bf16 rows also
+    a.k_shift[i] = log2_of(i > 0 || a.slots == 1 ? scales : D * kv->bits_k / 8);
+    a.v_shift[i] = log2_of(i > 0 || a.slots == 1 ? scales : D * kv->bits_v / 8);
+  }
+  // Four 16-byte pieces of the wider rows a thread.
+  const int wide = a.k_shift[0] > a.v_shift[0] ? a.k_shift[0] : a.v_shift[0];
+  a.rows = 4 * kThreads >> (wide - 4);
+  if (a.rows > kRows) a.rows = kRows;
+  const int64_t blocks = (budget + a.rows - 1) / a.rows;
+  if (blocks > 0xffffffffLL / kThreads)  // a grid: below 2^32 threads
+    return fail(TQKV_EUNSUPPORTED, "budget=%lld", (long long)budget);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const size_t need = tqkv_paged_evict_workspace_size(kv, budget);
   if (!kept) {
@@ -372,18 +396,8 @@ extern "C" int32_t tqkv_paged_evict(const tqkv_paged_kv* kv, int64_t budget, int
   a.dst_lens = dst_lens;
   a.dst_weights = dst_weights;
   a.budget = int(budget);
-  const int D = kv->dim;
-  a.slots = kv->kind == TQKV_CACHE_BF16 ? 1 : 3;
-  for (int i = 0; i < a.slots; ++i) {
-    a.k[i] = kv->slot[i];
-    a.v[i] = kv->slot[a.slots + i];
-    const int scales = 2 * D / (i > 0 ? kv->group_size : 1);  // bf16 rows also
-    a.k_shift[i] = log2_of(i > 0 || a.slots == 1 ? scales : D * kv->bits_k / 8);
-    a.v_shift[i] = log2_of(i > 0 || a.slots == 1 ? scales : D * kv->bits_v / 8);
-  }
   hipLaunchKernelGGL(evict_move_kernel,
-                     dim3(unsigned((budget + kRows - 1) / kRows), unsigned(kv->kv_heads),
-                          unsigned(kv->batch)),
+                     dim3(unsigned(blocks), unsigned(kv->kv_heads), unsigned(kv->batch)),
                      dim3(kThreads), 0, st, a);
   TQKV_LAUNCHED();
   return ok();
