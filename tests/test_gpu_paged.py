@@ -156,6 +156,24 @@ def test_attend_lengths_of_one_sequence(T, n, kind):
     attend(T, p.fill(n), 4, f"n={n}")
 
 
+@pytest.mark.parametrize("kind,D,n,G", [(BF16, 64, 33001, 3), (BF16, 512, 20011, 2), (AFFINE, 128, 70007, 1),
+                                        (AFFINE, 512, 12345, 17)])
+def test_attend_one_sequence_over_the_whole_card(T, kind, D, n, G):
+    """A KV head's rows in more parts than a wavefront has lanes."""
+    say("attend long", kind, D, n, G)
+    p = Paged([n], 1, D, 256, kind, seed=n, track=G != 2)
+    attend(T, p.fill(n), G, f"n={n}")
+
+
+def test_attend_more_pages_than_a_block_of_the_table(T):
+    """Many KV heads, so that a part of the sequence has hundreds of pages,
+    some of them invalid."""
+    say("attend pages")
+    p = Paged([17600, 300], 64, 64, 16, BF16, seed=14)
+    p.table[0, 270] = p.table[0, 511] = p.table[0, 800] = -1
+    attend(T, p.fill(15), 64, "pages")
+
+
 @pytest.mark.parametrize("window", [1, 15, 32, 33, 200, 299, 300, 5000])
 @pytest.mark.parametrize("kind", [BF16, AFFINE])
 def test_attend_windows(T, window, kind):
@@ -442,6 +460,28 @@ def test_evict_orders_weights(T, which):
         p.weights[...] = r.standard_normal(p.weights.shape)
     for budget in (1234, 250):
         evict(T, p, budget, 3, 100, budget)
+
+
+@pytest.mark.parametrize("kind,bk,bv,gs", LAYOUTS)
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_evict_moves_every_row_format(T, kind, bk, bv, gs, D):
+    if gs > D:
+        pytest.skip("a group is at most a row")
+    say("evict format", kind, bk, bv, gs, D)
+    p = Paged([333, 7, 150], 3, D, 16, kind, bk, bv, gs, spare=24, seed=D + gs, track=True).fill(D)
+    p.weights[...] = p.rng.random(p.weights.shape)
+    evict(T, p, 131, 3, 20, D)
+
+
+@pytest.mark.parametrize("budget", [5000, 40001])
+@pytest.mark.parametrize("ties", [False, True])
+def test_evict_long_sequences(T, budget, ties):
+    """More rows than the selection holds in registers."""
+    say("evict long", budget, ties)
+    p = Paged([70001, 33000, 32769], 1, 64, 256, AFFINE, spare=500, seed=45, track=True)
+    w = p.rng.random(p.weights.shape)
+    p.weights[...] = np.floor(8 * w) if ties else w
+    evict(T, p, budget, 4, 1000, budget)
 
 
 def test_evict_with_invalid_pages_and_lengths(T):
