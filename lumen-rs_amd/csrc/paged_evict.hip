@@ -12,8 +12,8 @@
 // (8 workgroups), 16 for 16 sequences of up to 30,000 to 4,096 (128); the third
 // pass, which most selections do not need, took 2. (2) The gather moves the rows
 // to their new pages, bound by HBM: 16 sequences cut to 4,096 rows x 8 heads of
-// 4 bits 24 us, in pieces of a row's 64 bytes (28 with four wavefronts a
-// workgroup).
+// 4 bits 22 us (28 with four wavefronts a workgroup), where a row's 64 bytes
+// come in lines of 128.
 #include <cmath>
 
 #include "paged.hpp"
@@ -254,9 +254,9 @@ int log2_of(int x) { return 31 - __builtin_clz(unsigned(x)); }
 // A wavefront a workgroup, so that the most of them have their chains of loads
 // (positions, pages, rows) going at once.
 constexpr int kThreads = 64;
-constexpr int kRows = 64;  // kept rows a workgroup at most
+constexpr int kRows = 64;  // kept rows a workgroup at most, and threads that place them
 
-// Rows of one buffer (2^ks units of type T each) and of another (2^vs), four
+// Rows of one buffer (2^ks units of type T each) and of another (2^vs), two
 // loads of each in flight a thread. src is a row that can be read also where
 // dst is -1.
 template <typename T>
@@ -270,19 +270,13 @@ __device__ __forceinline__ void move_rows(T* kb, int ks, T* vb, int vs, const in
     const int r = i >> shift;
     if (r < rows && dst[r] >= 0) buf[(dst[r] << shift) + (i & ((1 << shift) - 1))] = x;
   };
-  for (int i = threadIdx.x; i < items; i += 4 * kThreads) {
+  for (int i = threadIdx.x; i < items; i += 2 * kThreads) {
     const T x0 = load(kb, ks, i), x1 = load(kb, ks, i + kThreads);
-    const T x2 = load(kb, ks, i + 2 * kThreads), x3 = load(kb, ks, i + 3 * kThreads);
     const T y0 = load(vb, vs, i), y1 = load(vb, vs, i + kThreads);
-    const T y2 = load(vb, vs, i + 2 * kThreads), y3 = load(vb, vs, i + 3 * kThreads);
     store(kb, ks, i, x0);
     store(kb, ks, i + kThreads, x1);
-    store(kb, ks, i + 2 * kThreads, x2);
-    store(kb, ks, i + 3 * kThreads, x3);
     store(vb, vs, i, y0);
     store(vb, vs, i + kThreads, y1);
-    store(vb, vs, i + 2 * kThreads, y2);
-    store(vb, vs, i + 3 * kThreads, y3);
   }
 }
 
@@ -370,9 +364,10 @@ extern "C" int32_t tqkv_paged_evict(const tqkv_paged_kv* kv, int64_t budget, int
     a.k_shift[i] = log2_of(i > 0 || a.slots == 1 ? scales : D * kv->bits_k / 8);
     a.v_shift[i] = log2_of(i > 0 || a.slots == 1 ? scales : D * kv->bits_v / 8);
   }
-  // Four 16-byte pieces of the wider rows a thread.
+  // Two 16-byte pieces of the wider rows a thread (2,048 bf16 rows x 8 heads and
+  // a batch's 4-bit rows: 5.0 and 23.2 us; four 5.7 and 24.6, eight 5.9 and 24.1).
   const int wide = a.k_shift[0] > a.v_shift[0] ? a.k_shift[0] : a.v_shift[0];
-  a.rows = 4 * kThreads >> (wide - 4);
+  a.rows = 2 * kThreads >> (wide - 4);
   if (a.rows > kRows) a.rows = kRows;
   const int64_t blocks = (budget + a.rows - 1) / a.rows;
   if (blocks > 0xffffffffLL / kThreads)  // a grid: below 2^32 threads
