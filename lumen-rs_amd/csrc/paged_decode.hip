@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
     b = i / row_blocks / a.pool.Hkv;
   }
   const int first = a.starts[b], next = a.starts[b + 1], total = a.starts[a.pool.batch];
-  const int per = units_per_wg(total, a.W);
+  const int per = units_per_wg(a, total);
   const int w0 = (first + a.over) / per, n = (next - 1) / per - w0 + 1;
   const int64_t slot0 = w0 + b;
   float m;
@@ -255,8 +255,13 @@ static_assert(4 * kCus <= kMaxSegments, "a join holds a sequence's segments");
 
 constexpr int64_t kKeptBytes = int64_t(192) << 20;  // of the 256 MB memory-side cache
 
+// Units a workgroup takes at least: a step of each of its wavefronts, of 32 rows,
+// or 16 for wide ones (2 x 600 bf16 rows at D = 256: 9.7 us with 8 units, 8.4 with
+// 4; 5 x 300 8- and 4-bit rows at D = 512: 18.5 and 17.8).
+int least_units(const tqkv_paged_kv* kv) { return kv->dim <= 128 ? 8 : 4; }
+
 struct HostPlan {
-  int groups16, W;
+  int groups16, W, least;
   int64_t srows;
   size_t slots, bytes;
 };
@@ -274,7 +279,8 @@ bool plan_of(const tqkv_paged_kv* kv, int32_t H, int64_t max_rows, HostPlan* out
   int64_t W = (workgroups_a_cu(kv) * kCus + units - 1) / units;
   // No more than the longest possible batch fills.
   const int64_t most = int64_t(kv->batch) * (p.srows / kUnit + kOver);
-  if (W > (most + kMinUnits - 1) / kMinUnits) W = (most + kMinUnits - 1) / kMinUnits;
+  p.least = least_units(kv);
+  if (W > (most + p.least - 1) / p.least) W = (most + p.least - 1) / p.least;
   p.W = int(W);
   p.slots = size_t(p.W) + kv->batch;
   size_t floats = p.slots * H * (size_t(kv->dim) + 2);
@@ -345,6 +351,7 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
   a.max_rows = int(max_rows);
   a.W = plan.W;
   a.over = kOver;
+  a.least = plan.least;
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.part_o = static_cast<float*>(workspace);
   a.part_m = a.part_o + plan.slots * H * D;

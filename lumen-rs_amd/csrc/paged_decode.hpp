@@ -50,7 +50,6 @@ namespace paged {
 
 constexpr int kWaves = 4;
 constexpr int kUnit = 16;     // rows by which the batch is divided
-constexpr int kMinUnits = 8;  // of a workgroup: two a wavefront
 
 struct DecodeArgs {
   Pool pool;
@@ -62,6 +61,7 @@ struct DecodeArgs {
   int max_rows, window;
   int W;               // workgroups a (KV head, set)
   int over;            // units that a sequence's start counts as
+  int least;           // units of a workgroup
   int kept_units;      // bf16 rows beyond these are streamed
   float scale_log2;
   float* part_o;  // [W + batch, H, D]
@@ -88,9 +88,9 @@ __device__ __forceinline__ Span span_of(const DecodeArgs& a, int b) {
 }
 
 // Units a workgroup takes of `total`.
-__device__ __forceinline__ int units_per_wg(int total, int W) {
-  const int per = (total + W - 1) / W;
-  return per < kMinUnits ? kMinUnits : per;
+__device__ __forceinline__ int units_per_wg(const DecodeArgs& a, int total) {
+  const int per = (total + a.W - 1) / a.W;
+  return per < a.least ? a.least : per;
 }
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -861,8 +861,8 @@ struct Walk {
   bool whole;            // the whole sequence
   // Kept in scalar registers: the loops over it branch as one.
   static __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
-  __device__ __forceinline__ void start(const Plan& plan, int batch, int W) {
-    const int total = scalar(plan.start[batch]), per = units_per_wg(total, W);
+  __device__ __forceinline__ void start(const DecodeArgs& a, const Plan& plan) {
+    const int batch = a.pool.batch, total = scalar(plan.start[batch]), per = units_per_wg(a, total);
     x = int(blockIdx.x) * per;
     x1 = x + per < total ? x + per : total;
     b = 0;
@@ -922,7 +922,7 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, Shared<Rows>& lds) {
   const int head0 = kvh * a.G + 16 * set;
 
   Walk walk;
-  walk.start(lds.plan, p.batch, a.W);
+  walk.start(a, lds.plan);
   while (walk.next(a, lds.plan)) {
     const int b = walk.seq, lo = walk.lo, end = walk.end;
     // A wavefront takes every fourth step of kRows rows.
@@ -1137,7 +1137,7 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
   const int live = a.G - 16 * set < 16 ? a.G - 16 * set : 16;
   const int head0 = kvh * a.G + 16 * set;
   Walk walk;
-  walk.start(lds.plan, p.batch, a.W);
+  walk.start(a, lds.plan);
   int buf = 0;
   while (walk.next(a, lds.plan)) {
     const int b = walk.seq, lo = walk.lo, end = walk.end;
