@@ -36,9 +36,9 @@
 // Bound by HBM: the live rows once. At G heads of 16 the matrix cores do
 // 16 / G times the work that is needed and are still far from busy (7 to 20%).
 // Measured, with the join: bf16, 131,071 rows x 8 KV heads at D = 128 (537 MB)
-// 88 us, 6.1 TB/s; 4 bits, 16 x 32,768 x 8 at D = 256 (1.21 GB) 245 us, 4.9
+// 86 us, 6.2 TB/s; 4 bits, 16 x 32,768 x 8 at D = 256 (1.21 GB) 244 us, 5.0
 // TB/s, where unpacking keeps the vector units 72% busy. Short calls are bound
-// by latencies: 777 rows take 7.8 us and the join's 4.5.
+// by latencies: 777 rows take 7.4 us and the join's 2.9.
 #pragma once
 
 #include <type_traits>
