@@ -326,11 +326,11 @@ size_t tqkv_sparse_workspace_size(int32_t B, int32_t H, int32_t H_kv, int32_t D,
  * weights (optional, NULL for none): f32 [batch, kv_heads, table_stride *
  * page_rows], the attention weight that row t of sequence b has gathered so
  * far: tqkv_paged_append clears the rows it writes, tqkv_paged_decode_attend
- * adds to them and tqkv_paged_evict ranks by them. They belong to the sequence and not to
- * the page, so sequences that share pages gather their own.
+ * adds to them and tqkv_paged_evict ranks by them. They belong to the sequence
+ * and not to the page, so sequences that share pages gather their own.
  *
- * dim in {64, 128, 256, 512}; page_rows in {16, 32, 64, 128, 256}; batch at
- * most 1024; affine: bits_k and bits_v 4 or 8 each, group_size in {32, 64,
+ * dim in {64, 128, 256, 512}; page_rows in {16, 32, 64, 128, 256}; batch and
+ * kv_heads at most 1024; affine: bits_k and bits_v 4 or 8 each, group_size in {32, 64,
  * 128} dividing dim (bf16 ignores the three). TQKV_EUNSUPPORTED otherwise.
  * slot pointers and weights are 16-byte aligned, and the pool, table, lens and
  * weights belong to the calling thread's current device.
@@ -375,7 +375,8 @@ int32_t tqkv_paged_append(const tqkv_paged_kv* kv, const uint16_t* k, const uint
  * . V: tqkv_decode_attend_affine with a length and pages for each sequence.
  * q: bf16, head h of sequence b at q + b * q_stride + h * dim (16-byte
  * aligned, q_stride a multiple of 8); out: bf16 [batch, H, dim], not over q.
- * H / kv_heads from 1 to 32 (more than 16 read the rows twice). window > 0: the last `window` rows only; otherwise all.
+ * H / kv_heads from 1 to 32 (more than 16 read the rows twice). window > 0: the
+ * last `window` rows only; otherwise all.
  * max_rows: the host's bound on lens (at most table_stride * page_rows); it
  * sizes the grid and the workspace, and a sequence that holds more attends
  * its first max_rows rows as if it held no more. A sequence without rows gets
@@ -412,7 +413,7 @@ size_t tqkv_paged_decode_workspace_size(const tqkv_paged_kv* kv, int32_t H, int6
  * must not be among the pages of kv->table nor twice in dst_table, and
  * dst_weights must not overlap kv->weights; dst_lens may be kv->lens. Rows
  * whose old or new page is invalid are not moved (their weights are).
- * budget >= 1, sinks + recent <= budget <= dst_stride * page_rows.
+ * budget >= 1, sinks + recent <= budget <= dst_stride * page_rows and 2^29.
  * workspace: tqkv_paged_evict_workspace_size() bytes (the kept positions) or
  * NULL for the library's scratch; neither is used where kept is given. Two
  * launches.
