@@ -198,6 +198,17 @@ def test_attend_leaves_out_invalid_pages(T, kind):
     assert np.all(got[2] == 0)
 
 
+@pytest.mark.parametrize("D", [128, 512])
+@pytest.mark.parametrize("kind", [BF16, AFFINE])
+def test_attend_a_page_named_twice(T, kind, D):
+    """Its rows count twice, each place with weights of its own."""
+    say("attend page twice", kind, D)
+    p = Paged([100, 50], 2, D, 16, kind, seed=5, track=True).fill(5)
+    p.table[0, 4] = p.table[0, 1]
+    p.table[1, :3] = p.table[0, 1]
+    attend(T, p, 8, "page twice", max_rows=93)
+
+
 @pytest.mark.parametrize("kind", [BF16, AFFINE])
 def test_attend_lengths_outside_the_table(T, kind):
     say("attend lens", kind)
