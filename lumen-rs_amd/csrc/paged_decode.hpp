@@ -247,6 +247,14 @@ __device__ __forceinline__ Step<HALVES> step_of(const Pool& p, Pages& pages, int
   return h;
 }
 
+// Two weights as bf16 words hi + lo, 16 bits of each: hi the upper bits, and
+// lo the rest and 2^-23 of the weight. Both parts of a weight above 0 are above
+// 0, so that an infinite value times each is infinite and not NaN.
+__device__ __forceinline__ void split(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+  hi = highs(__float_as_uint(p0), __float_as_uint(p1));
+  lo = pack_bf16(fmaf(p0, 1.0f + 0x1p-23f, -low_f32(hi)), fmaf(p1, 1.0f + 0x1p-23f, -high_f32(hi)));
+}
+
 // Channel layout of the values: product j's output row r is channel
 // (j / kCpl) * 16 kCpl + r * kCpl + j % kCpl.
 template <int D>
@@ -354,10 +362,7 @@ struct Bf16Rows {
                                                     floatx4 (&acc)[C::kJ], Unit&, int) {
     uint32_t hi[2 * kHalves], lw[2 * kHalves];
 #pragma unroll
-    for (int e = 0; e < 2 * kHalves; ++e) {
-      hi[e] = pack_bf16(p[2 * e], p[2 * e + 1]);
-      lw[e] = pack_bf16(p[2 * e] - low_f32(hi[e]), p[2 * e + 1] - high_f32(hi[e]));
-    }
+    for (int e = 0; e < 2 * kHalves; ++e) split(p[2 * e], p[2 * e + 1], hi[e], lw[e]);
 #pragma unroll
     for (int i = 0; i < kVWords; ++i) {
       uint32_t x[2 * kHalves], y[2 * kHalves];
@@ -400,11 +405,7 @@ struct Bf16Rows {
     for (int k = 0; k < 2; ++k) {
       uint32_t hi[4], lw[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p0 = p[8 * k + 2 * e], p1 = p[8 * k + 2 * e + 1];
-        hi[e] = pack_bf16(p0, p1);
-        lw[e] = pack_bf16(p0 - low_f32(hi[e]), p1 - high_f32(hi[e]));
-      }
+      for (int e = 0; e < 4; ++e) split(p[8 * k + 2 * e], p[8 * k + 2 * e + 1], hi[e], lw[e]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t x[4], y[4];

@@ -1,6 +1,6 @@
 """Paged decode attention within the bounds of paged_bounds.py, which are tight
 enough to tell a wrong answer from a rounded one: every layout, windows, long
-and many sequences."""
+and many sequences, infinite values."""
 import numpy as np
 import pytest
 
@@ -73,3 +73,18 @@ def test_sharp_softmax(T, kind, D):
     p = Paged([500, 129], 2, D, 64, kind, seed=12, track=True).fill(12)
     for scale in (0.5, -0.3, 0.0):
         attend(T, p, 4, f"sharp {kind} {D} {scale}", scale=scale)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("n", [1, 40, 9000])
+def test_infinite_values_of_bf16_rows(T, D, n):
+    """A channel with an infinite value is infinite, of that sign; with both
+    signs, or a NaN, it is NaN; the other channels are as they would be."""
+    p = Paged([n, 33], 2, D, 16, BF16, seed=n).fill(n)
+    v = p.sides[1][0]
+    for row, ch, bits in [(0, 0, 0x7F80), (n // 2, 3, 0xFF80), (n - 1, D - 1, 0x7FC0), (0, 9, 0x7F80),
+                          (n - 1, 9, 0xFF80), (n // 3, 20, 0x7F80), (n // 2, 20, 0x7F80)]:
+        v[p.table[0, row // 16], 1, row % 16, ch] = bits
+    got = attend(T, p, 4, f"infinite values {D} {n}", scale=0.1 * D ** -0.5)
+    assert got[0, 2, 0] == np.inf and got[0, 3, 3] == -np.inf and np.isnan(got[0, 2, D - 1])
+    assert np.all(np.isfinite(got[0, :2])) and np.count_nonzero(~np.isfinite(got)) == 2 * 5
