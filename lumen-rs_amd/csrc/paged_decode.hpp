@@ -32,6 +32,8 @@
 // bf16 parts. Values are dequantized by one mixed multiply-add a code, f32 to
 // f16 in a unit of the wavefront's, and weights enter as f16 too (each
 // rounded by at most 2^-11 of itself, an eighth of the output's own rounding).
+// Where a wavefront's values are of magnitudes too far apart for f16, it goes
+// over its rows once more and takes values and weights as bf16 pairs.
 //
 // Bound by HBM: the live rows once. At G heads of 16 the matrix cores do
 // 16 / G times the work that is needed and are still far from busy (7 to 20%).
@@ -195,6 +197,14 @@ __device__ __forceinline__ floatx4 mfma_pv(const uint32_t (&v)[2 * HALVES],
   }
 }
 
+// The lane, counted anew: a thread index kept for its rare uses would be spilled,
+// and every reload waits for the loads before it.
+__device__ __forceinline__ int lane_anew() {
+  uint32_t all = ~0u;
+  asm volatile("" : "+s"(all));
+  return int(__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0)));
+}
+
 // The pages of a wavefront's coming steps: a block of table entries in LDS,
 // its own, filled when a step asks for an entry behind it. (An entry loaded
 // when its step needs it, or one block in registers ahead of the next, makes
@@ -207,9 +217,10 @@ struct Pages {
   int first;       // entry of block[0]
   __device__ __forceinline__ void fill(int at) {
     first = at;
+    const int me = lane_anew();
 #pragma unroll
     for (int i = 0; i < kBlock / 64; ++i) {
-      const int lane = 64 * i + int(threadIdx.x % 64);
+      const int lane = 64 * i + me;
       block[lane] = at + lane < most ? table[at + lane] : -1;
     }
     __builtin_amdgcn_wave_barrier();
@@ -345,7 +356,7 @@ struct Bf16Rows {
     return acc;
   }
   // The rows for which dead is set hold nothing: zero, whatever lies there.
-  static __device__ __forceinline__ void clear(V& v, uint32_t dead) {
+  static __device__ __forceinline__ void clear(V& v, uint32_t dead, uint32_t) {
 #pragma unroll
     for (int e = 0; e < 4 * kHalves; ++e)
 #pragma unroll
@@ -355,8 +366,10 @@ struct Bf16Rows {
   // weight 2^kTau and values of bf16's largest magnitude stay within f32.
   // Weights below 2^-86 of the largest vanish.
   static constexpr float kDown = 40.0f, kLast = 1.0f;
+  static constexpr bool kPairs = false;  // values are exact: no second pass
   struct Unit {  // of the accumulators
     __device__ __forceinline__ float of() const { return 1.0f; }
+    __device__ __forceinline__ uint32_t filler() const { return 0; }
   };
   static __device__ __forceinline__ void accumulate(const V& v, const float (&p)[4 * kHalves],
                                                     floatx4 (&acc)[C::kJ], Unit&, int) {
@@ -393,7 +406,7 @@ struct Bf16Rows {
       for (int e = 0; e < 4; ++e) load_words<16, POLICY>(p, off + e * (2 * D), v.w[4 * s + e]);
     }
   }
-  static __device__ __forceinline__ void clear_wide(Wide& v, uint32_t dead) {
+  static __device__ __forceinline__ void clear_wide(Wide& v, uint32_t dead, uint32_t) {
 #pragma unroll
     for (int e = 0; e < 16; ++e)
 #pragma unroll
@@ -611,8 +624,9 @@ struct AffineRows {
     }
     return out;
   }
-  // Dead rows: a scale and a bias of 0.
-  static __device__ __forceinline__ void clear(V& v, uint32_t dead) {
+  // Dead rows: a scale of 0, and the unit's filler for a bias (their weights
+  // are 0).
+  static __device__ __forceinline__ void clear(V& v, uint32_t dead, uint32_t filler) {
 #pragma unroll
     for (int e = 0; e < 4 * kHalves; ++e) {
 #pragma unroll
@@ -620,7 +634,7 @@ struct AffineRows {
         const int at = e % 4 * NG + n;
         const uint32_t keep = dead >> e & 1 ? (at % 2 ? 0x0000ffffu : 0xffff0000u) : 0xffffffffu;
         v.s[e / 4][at / 2] &= keep;
-        v.b[e / 4][at / 2] &= keep;
+        v.b[e / 4][at / 2] = (v.b[e / 4][at / 2] & keep) | (filler & ~keep);
       }
     }
   }
@@ -636,7 +650,7 @@ struct AffineRows {
       return __uint_as_float(__builtin_amdgcn_perm(w[first / 2 + 1], w[first / 2], sel));
     }
   }
-  // Channel j of a row's piece: scale * code + bias as f16, one mixed
+  // Channel j of a row's piece: scale * code + bias, as f16 one mixed
   // multiply-add. s24: the scale times 2^24 (2^20 for a code with an odd place
   // in its half word).
   static __device__ __forceinline__ _Float16 value(const uint32_t* w, int shift, int j, float s24,
@@ -652,31 +666,79 @@ struct AffineRows {
     }
     return _Float16(fmaf(float(__builtin_bit_cast(halfx2, x)[half]), BV == 4 && (j & 1) ? s20 : s24, b));
   }
+  // The same in f32, of any magnitude.
+  static __device__ __forceinline__ float plain_value(const uint32_t* w, int shift, int j, float s,
+                                                      float b) {
+    const uint32_t code = BV == 4 ? w[j / 8] >> (shift + 4 * (j % 8)) & 0xfu : w[j / 4] >> (8 * (j % 4)) & 0xffu;
+    return fmaf(float(code), s, b);
+  }
   // Weights are held times 2^7: they reach 2^(7 + kTau) in f16, and those that
   // f16 loses lie below 2^-32 of the largest, 2^-15 in all at 2^17 rows. At a
   // segment's end they and their sum go down by 2^-47, to bf16 rows' 2^-40.
   static constexpr float kDown = -7.0f, kLast = 0x1p-47f;
-  // The accumulators hold values times `up`, a power of two, the wavefront's:
-  // f16 values are at most 2^15, and the largest magnitude that the rows gave
-  // when the unit was taken is near 2^6, so it is taken anew only when a
-  // bound on a value (its scale times the largest code, plus its bias) passes
-  // `cap`, 2^9 times that.
+  // The accumulators hold values times `up`, a power of two, the wavefront's.
+  // A bound on the values of a row's group is its scale times the largest code,
+  // plus its bias. The unit puts a bound of the first rows that are not all 0 at
+  // 2^4. As long as all bounds lie within 2^-4 and 2^12, each f16 value is off by
+  // at most 2^-11 of itself or 2^-21 of its bound, none overflows, and no row is
+  // so much larger than another that what f16 loses of its weight would matter
+  // to the other's. Otherwise (infinite bounds too) the sums are given up, and
+  // the second pass makes them: calls with such rows in every wavefront's part
+  // take 1.6 to 2.3 times as long (16 x 16,384 rows of 4 bits at D = 128: 147 us
+  // for 80). Pairs in the loop itself spilled, and cost every call (32 sequences
+  // of 17 to 16,000 rows: 57 us for 39).
+  static constexpr bool kPairs = true;
   struct Unit {
-    float up = 1.0f, cap = 0.0f;
+    float up = 1.0f;
+    float low = INFINITY, high = 0.0f;  // 2^-4 and 2^12 in this unit; none yet
+    int given_up = 0;
     __device__ __forceinline__ float of() const { return kLast / up; }
-    template <int N>
-    __device__ __forceinline__ void admit(float most, floatx4 (&acc)[N]) {
-      if (!__any(most > cap)) return;
+    // A scalar, and so a branch: in lanes masked off matrix products run all the
+    // same.
+    __device__ __forceinline__ bool gave_up() const {
+      return __builtin_amdgcn_readfirstlane(given_up) != 0;
+    }
+    // Two bf16 of 1 in this unit (0 without one): biases of rows that hold
+    // nothing, within the bounds.
+    __device__ __forceinline__ uint32_t filler() const {
+      const uint32_t one = __float_as_uint(low * 0x1p4f);
+      return low == INFINITY ? 0 : one | one >> 16;
+    }
+    // The unit for a step's groups. (Without shuffles: the first rows of every
+    // segment come through its second half. A NaN passes: it stays in its
+    // channel.)
+    template <int M, int N>
+    __device__ __forceinline__ void admit(const float (&s)[M], const float (&b)[M],
+                                          const floatx4 (&acc)[N]) {
+      float bound[M], most = 0.0f, least = INFINITY;
 #pragma unroll
-      for (int off = 1; off < 64; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
-      int E = int(__float_as_uint(most) >> 23) - 127;
-      E = E < -90 ? -90 : E;  // up * 2^24 stays finite
-      const float next = __uint_as_float(uint32_t(127 + 5 - E) << 23);
-      const float turn = next / up;  // both powers of two
+      for (int e = 0; e < M; ++e) {
+        bound[e] = fmaf(fabsf(s[e]), float((1 << BV) - 1), fabsf(b[e]));
+        most = fmaxf(most, bound[e]);
+        least = fminf(least, bound[e]);
+      }
+      if (__builtin_expect(!__any(least < low || most > high), 1)) return;
+      const uint64_t some = __ballot(most > 0.0f);
+      if (some == 0) return;  // rows of 0 alone
+      bool empty = true;
+      if (low < INFINITY) {  // rows of zeros, stored as steps of 1e-7, leave the choice open
 #pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] *= turn;
-      up = next;
-      cap = 0x1p15f / up;
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) empty &= acc[j][i] == 0.0f;
+      }
+      if (__all(empty)) {
+        const uint32_t first = __builtin_amdgcn_readlane(__float_as_uint(most), __builtin_ctzll(some));
+        int E = int(first >> 23) - 127 - 4;
+        E = E < -94 ? -94 : E > 96 ? 96 : E;  // up * 2^24 and low stay normal
+        up = __uint_as_float(uint32_t(127 - E) << 23);
+        low = __uint_as_float(uint32_t(127 - 4 + E) << 23);
+        high = __uint_as_float(uint32_t(127 + 12 + E) << 23);
+      }
+      bool out = most > high;
+#pragma unroll
+      for (int e = 0; e < M; ++e) out |= bound[e] > 0.0f && bound[e] < low;
+      if (__any(out)) given_up = 1;
     }
   };
   static __device__ __forceinline__ void accumulate(const V& v, const float (&p)[4 * kHalves],
@@ -692,14 +754,13 @@ struct AffineRows {
     const uint32_t sel = ((2 * grp + 1) << 24) | ((2 * grp) << 16) | 0x0c0cu;
 #pragma unroll
     for (int x = 0; x < C::kPieces; ++x) {
-      float s[4 * kHalves], b[4 * kHalves], most = 0.0f;
+      float s[4 * kHalves], b[4 * kHalves];
 #pragma unroll
       for (int e = 0; e < 4 * kHalves; ++e) {
         s[e] = lane_entry(v.s[e / 4], e, x, sel);
         b[e] = lane_entry(v.b[e / 4], e, x, sel);
-        most = fmaxf(most, fmaf(fabsf(s[e]), float((1 << BV) - 1), fabsf(b[e])));
       }
-      unit.admit(most, acc);
+      unit.admit(s, b, acc);
       const float up24 = unit.up * 0x1p24f;
       float s20[4 * kHalves];
 #pragma unroll
@@ -723,6 +784,52 @@ struct AffineRows {
         if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
     }
+  }
+  // The second pass: values and weights as bf16 pairs, hi + lo, 16 bits of each
+  // (an infinite value is its hi alone), in the unit of bf16 rows' sums.
+  static __device__ __forceinline__ void split_values(float x, float y, uint32_t& hi, uint32_t& lo) {
+    hi = highs(__float_as_uint(x), __float_as_uint(y));
+    const float a = x - low_f32(hi), b = y - high_f32(hi);
+    lo = pack_bf16(fabsf(x) < INFINITY ? a : 0.0f, fabsf(y) < INFINITY ? b : 0.0f);
+  }
+  template <int HALVES>
+  struct Weights {
+    uint32_t hi[2 * HALVES], lo[2 * HALVES];
+  };
+  template <int HALVES>
+  static __device__ __forceinline__ Weights<HALVES> weights_of(const float* p) {
+    Weights<HALVES> w;
+#pragma unroll
+    for (int e = 0; e < 2 * HALVES; ++e) split(p[2 * e] * kLast, p[2 * e + 1] * kLast, w.hi[e], w.lo[e]);
+    return w;
+  }
+  template <int HALVES, typename Value>
+  static __device__ __forceinline__ floatx4 pairs(Value&& value_of, const Weights<HALVES>& w, floatx4 acc) {
+    uint32_t hi[2 * HALVES], lo[2 * HALVES];
+#pragma unroll
+    for (int e = 0; e < 2 * HALVES; ++e) split_values(value_of(2 * e), value_of(2 * e + 1), hi[e], lo[e]);
+    acc = mfma_pv<HALVES, false>(hi, w.hi, acc);
+    acc = mfma_pv<HALVES, false>(hi, w.lo, acc);
+    return mfma_pv<HALVES, false>(lo, w.hi, acc);
+  }
+  static __device__ __forceinline__ void accumulate_pairs(const V& v, const float (&p)[4 * kHalves],
+                                                          floatx4 (&acc)[C::kJ], int r) {
+    const int shift = kPieceBytes < 4 ? 16 * (r & 1) : 0;
+    const uint32_t grp = r * C::kCpl / GS;
+    const uint32_t sel = ((2 * grp + 1) << 24) | ((2 * grp) << 16) | 0x0c0cu;
+    const Weights<kHalves> w = weights_of<kHalves>(p);
+#pragma unroll
+    for (int x = 0; x < C::kPieces; ++x)
+#pragma unroll
+      for (int j = 0; j < C::kCpl; ++j) {
+        acc[x * C::kCpl + j] = pairs<kHalves>(
+            [&](int e) {
+              const float s = lane_entry(v.s[e / 4], e, x, sel), b = lane_entry(v.b[e / 4], e, x, sel);
+              return plain_value(v.w[e] + x * kPieceWords, shift, j, s, b);
+            },
+            w, acc[x * C::kCpl + j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
   }
   // The wide kernel's share of the values, as Bf16Rows': codes, and the scale
   // and bias of the lane's own group of each row.
@@ -748,11 +855,11 @@ struct AffineRows {
       }
     }
   }
-  static __device__ __forceinline__ void clear_wide(Wide& v, uint32_t dead) {
+  static __device__ __forceinline__ void clear_wide(Wide& v, uint32_t dead, uint32_t filler) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       v.s[e] = dead >> e & 1 ? 0 : v.s[e];
-      v.b[e] = dead >> e & 1 ? 0 : v.b[e];
+      v.b[e] = dead >> e & 1 ? filler : v.b[e];
     }
   }
   static __device__ __forceinline__ void accumulate_wide(const Wide& v, const float (&p)[16],
@@ -768,14 +875,13 @@ struct AffineRows {
         const floatx2 x = {p[8 * k + 2 * e], p[8 * k + 2 * e + 1]};
         pw[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, halfx2));
       }
-      float s[8], s20[8], b[8], most = 0.0f;
+      float s[8], s20[8], b[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         s[e] = __uint_as_float(__builtin_amdgcn_perm(0u, v.s[8 * k + e], sel));
         b[e] = __uint_as_float(__builtin_amdgcn_perm(0u, v.b[8 * k + e], sel));
-        most = fmaxf(most, fmaf(fabsf(s[e]), float((1 << BV) - 1), fabsf(b[e])));
       }
-      unit.admit(most, acc);
+      unit.admit(s, b, acc);
       const float up24 = unit.up * 0x1p24f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -795,6 +901,26 @@ struct AffineRows {
         }
         acc[j] = mfma_pv<2, true>(o, pw, acc[j]);
         if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  static __device__ __forceinline__ void accumulate_wide_pairs(const Wide& v, const float (&p)[16],
+                                                               floatx4 (&acc)[8], int wave, int r) {
+    const uint32_t half = (128 * wave + 8 * r) / GS & 1;
+    const uint32_t sel = ((2 * half + 1) << 24) | ((2 * half) << 16) | 0x0c0cu;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const Weights<2> w = weights_of<2>(p + 8 * k);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        acc[j] = pairs<2>(
+            [&](int e) {
+              const float s = __uint_as_float(__builtin_amdgcn_perm(0u, v.s[8 * k + e], sel));
+              const float b = __uint_as_float(__builtin_amdgcn_perm(0u, v.b[8 * k + e], sel));
+              return plain_value(v.w[8 * k + e], 0, j, s, b);
+            },
+            w, acc[j]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -973,7 +1099,7 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, Shared<Rows>& lds) {
             sc[e] = -INFINITY;
           }
         }
-        Rows::clear(vr, dead);
+        Rows::clear(vr, dead, unit.filler());
       }
       if (a.scores && r < live) {
         float* dst = a.scores + (int64_t(b) * a.H + head0 + r) * a.srows + row0 + 4 * g;
@@ -1012,6 +1138,38 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, Shared<Rows>& lds) {
       h = hn;
     }
 
+    float of = unit.of();
+    if constexpr (Rows::kPairs) {
+      if (__builtin_expect(unit.gave_up(), 0)) {  // again, with the maximum known
+        of = 1.0f;
+#pragma unroll
+        for (int j = 0; j < C::kJ; ++j) acc[j] = floatx4{0, 0, 0, 0};
+        const float base = m == -INFINITY ? 0.0f : m + Rows::kDown;
+        row0 = walk.row + wave * kRows;
+        pages.fill(row0 >> p.shift);
+        for (; row0 < end; row0 += kWaves * kRows) {
+          h = step_of<HALVES>(p, pages, kvh, row0, end);
+          Rows::load_k(kr, a, h, r, g);
+          Rows::load_v(vr, a, h, r, g);
+          float pr[4 * HALVES];
+          uint32_t dead = 0;
+#pragma unroll
+          for (int s = 0; s < HALVES; ++s) {
+            const floatx4 y = Rows::scores([&](int c) { return ops[c]; }, q, kr, s);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = row0 + s * 16 + 4 * g + i;
+              const bool none = row < lo || row >= end || !h.ok[s];
+              dead |= uint32_t(none) << (4 * s + i);
+              pr[4 * s + i] = none ? 0.0f : __builtin_amdgcn_exp2f(fmaf(y[i], q.mul, -base));
+            }
+          }
+          Rows::clear(vr, dead, 0);
+          Rows::accumulate_pairs(vr, pr, acc, r);
+        }
+      }
+    }
+
     // The four wavefronts' parts, joined in their order.
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -1024,7 +1182,7 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, Shared<Rows>& lds) {
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml[0][w][r]);
-    const float mine = m == -INFINITY ? 0.0f : exp2f(m - top) * unit.of();
+    const float mine = m == -INFINITY ? 0.0f : exp2f(m - top) * of;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
       sum += ml[0][w][r] == -INFINITY ? 0.0f * ml[1][w][r] : ml[1][w][r] * exp2f(ml[0][w][r] - top);
@@ -1157,7 +1315,7 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
       typename Rows::Operand ops[Rows::kOperands];
       Rows::prepare(ops, q, qw, r < live, g, a.scale_log2);
       // The last segment's reads are over: every wavefront passed a barrier
-      // since its last.
+      // since its last (for scores, and of a second pass).
 #pragma unroll
       for (int c = 0; c < Rows::kOperands; ++c)
         if (c % kWaves == wave) queries[c][lane] = ops[c];
@@ -1191,7 +1349,7 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
         mine.y = d & 2 ? -INFINITY : mine.y;
         mine.z = d & 4 ? -INFINITY : mine.z;
         mine.w = d & 8 ? -INFINITY : mine.w;
-        Rows::clear_wide(vr, dead);
+        Rows::clear_wide(vr, dead, unit.filler());
       }
       tiles[buf][4 * wave + g][r] = mine;
       if (a.scores && r < live && row0 + 16 * wave < end)
@@ -1234,6 +1392,39 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
       __builtin_amdgcn_sched_barrier(0);
       h = hn;
     }
+    float of = unit.of();
+    if constexpr (Rows::kPairs) {
+      if (__builtin_expect(unit.gave_up(), 0)) {  // again, with the maximum known, all scores its own
+        of = 1.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = floatx4{0, 0, 0, 0};
+        const float base = m == -INFINITY ? 0.0f : m + Rows::kDown;
+        row0 = walk.row;
+        pages.fill(row0 >> p.shift);
+        for (; row0 < end; row0 += kWideTile) {
+          h = step_of<4>(p, pages, kvh, row0, end);
+          Rows::load_wide(vr, a, h, wave, r, g);
+          float pr[16];
+          uint32_t dead = 0;
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            Rows::load_k(kr, a, quarter_of(h, s), r, g);
+            const floatx4 y = Rows::scores([&](int c) { return queries[c][lane]; }, q, kr, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = row0 + s * 16 + 4 * g + i;
+              const bool none = row < lo || row >= end || !h.ok[s];
+              dead |= uint32_t(none) << (4 * s + i);
+              pr[4 * s + i] = none ? 0.0f : __builtin_amdgcn_exp2f(fmaf(y[i], q.mul, -base));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          Rows::clear_wide(vr, dead, 0);
+          Rows::accumulate_wide_pairs(vr, pr, acc, wave, r);
+        }
+      }
+      lds_barrier();  // the queries are written again
+    }
     // Every wavefront holds the same maximum and sum.
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -1244,7 +1435,6 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
       a.part_l[slot * a.H + head0 + tid] = l;
     }
     if (r < live) {
-      const float of = unit.of();
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = 128 * wave + (4 * g + i) * 8;
