@@ -14,9 +14,9 @@ namespace {
 
 constexpr int kJoinThreads = 256;
 constexpr int kWeightRows = 4 * kJoinThreads;  // rows whose weights a workgroup adds
-constexpr float kPartDown = 40.0f;  // log2 by which parts hold weights and their sums lower
-static_assert(Bf16Rows<128>::kDown == kPartDown, "as the parts are");
-static_assert(AffineRows<128, 4, 4, 64>::kLast == 0x1p-47f && AffineRows<128, 4, 4, 64>::kDown == kPartDown - 47,
+constexpr float kPartDown = 0x1p-40f;  // parts hold weights and their sums times it
+static_assert(Bf16Rows<128>::kDown == 40, "as the parts are");
+static_assert(AffineRows<128, 4, 4, 64>::kLast == 0x1p-47f && AffineRows<128, 4, 4, 64>::kDown == 40 - 47,
               "as the parts are");
 constexpr int kMaxSegments = 1024;  // of one sequence: the workgroups of a KV head
 
@@ -188,8 +188,8 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const DecodeAr
     l = top == -INFINITY ? 0.0f * l : l * __builtin_amdgcn_exp2f(top - m);
     for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
     if (lane == 0) {
-      head_m[i] = m == -INFINITY ? 0.0f : m + kPartDown;
-      head_r[i] = l == 0.0f ? 0.0f : 1.0f / l;
+      head_m[i] = m == -INFINITY ? 0.0f : m;
+      head_r[i] = l == 0.0f ? 0.0f : kPartDown / l;
     }
   }
   __syncthreads();

@@ -312,14 +312,23 @@ struct Bf16Rows {
   static __device__ __forceinline__ void prepare(Operand (&op)[kOperands], Rest& q,
                                                  const uint32_t (&w)[D / 32][4], bool live, int,
                                                  float scale_log2) {
-    // The scale's sign goes into the queries.
+    // The scale's sign goes into the queries, and its power of two if it makes
+    // them smaller (both exact): products stay within f32 where scores do.
     const uint32_t keep = live && scale_log2 != 0.0f ? 0xffffffffu : 0u;
-    const uint32_t flip = scale_log2 < 0.0f ? 0x80008000u & keep : 0u;
+    int e = int(__float_as_uint(scale_log2) >> 23 & 255) - 127;
+    e = e > 0 ? 0 : e < -64 ? -64 : e;
+    const float times = ldexpf(scale_log2 < 0.0f ? -1.0f : 1.0f, e);
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-      op[c] = as_bf16x8((w[c][0] & keep) ^ flip, (w[c][1] & keep) ^ flip, (w[c][2] & keep) ^ flip,
-                        (w[c][3] & keep) ^ flip);
-    q.mul = scale_log2 != 0.0f ? fabsf(scale_log2) : 1.0f;
+    for (int c = 0; c < kChunks; ++c) {
+      uint32_t x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t y = w[c][i] & keep;
+        x[i] = highs(__float_as_uint(low_f32(y) * times), __float_as_uint(high_f32(y) * times));
+      }
+      op[c] = as_bf16x8(x[0], x[1], x[2], x[3]);
+    }
+    q.mul = scale_log2 != 0.0f ? ldexpf(fabsf(scale_log2), -e) : 1.0f;
   }
   static __device__ __forceinline__ void load_k(K& k, const DecodeArgs& a, const S& h, int r,
                                                 int g) {
@@ -559,8 +568,11 @@ struct AffineRows {
       const float hi = __bf16(sum), mid = __bf16(sum - hi), lo = __bf16(sum - hi - mid);
       q.sum[n / 8][n % 8] = __bf16(g == 0 ? hi : g == 1 ? mid : g == 2 ? lo : 0.0f);
     }
-    // Above 0: masked scores are -inf times it.
-    q.mul = scale_log2 != 0.0f ? fmaxf(ldexpf(fabsf(scale_log2), E + 10), 0x1p-126f) : 1.0f;
+    // Above 0: masked scores are -inf times it. Finite: queries above 2^90 only
+    // have their scores' differences understated, and these decide at 2^100 too.
+    q.mul = scale_log2 != 0.0f
+                ? fminf(fmaxf(ldexpf(fabsf(scale_log2), E + 10), 0x1p-126f), 0x1p100f)
+                : 1.0f;
   }
   static __device__ __forceinline__ void load_k(K& k, const DecodeArgs& a, const S& h, int r,
                                                 int g) {
@@ -1072,6 +1084,8 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, Shared<Rows>& lds) {
     floatx4 acc[C::kJ];
 #pragma unroll
     for (int j = 0; j < C::kJ; ++j) acc[j] = floatx4{0, 0, 0, 0};
+    // The maximum of the scores before their factor: differences to it are exact
+    // where they matter, however large the scores.
     float m = -INFINITY, l = 0.0f;
     typename Rows::Unit unit;
     for (; row0 < end; row0 += kWaves * kRows) {
@@ -1113,22 +1127,21 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, Shared<Rows>& lds) {
       float top = sc[0];
 #pragma unroll
       for (int e = 1; e < 4 * HALVES; ++e) top = fmaxf(top, sc[e]);
-      top *= q.mul;
-      if (__any(top > m + kTau)) {
+      if (__any((top - m) * q.mul > kTau)) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float next = fmaxf(m, top);
-        const float scale = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+        const float scale = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - next) * q.mul);
         m = next;
         l *= scale;
 #pragma unroll
         for (int j = 0; j < C::kJ; ++j) acc[j] *= scale;
       }
-      const float base = m == -INFINITY ? 0.0f : m + Rows::kDown;
+      const float base = m == -INFINITY ? 0.0f : m;
       float pr[4 * HALVES];
 #pragma unroll
       for (int e = 0; e < 4 * HALVES; ++e) {
-        pr[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], q.mul, -base));
+        pr[e] = __builtin_amdgcn_exp2f(fmaf(sc[e] - base, q.mul, -Rows::kDown));
         l += pr[e];
       }
       Rows::accumulate(vr, pr, acc, unit, r);
@@ -1144,7 +1157,7 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, Shared<Rows>& lds) {
         of = 1.0f;
 #pragma unroll
         for (int j = 0; j < C::kJ; ++j) acc[j] = floatx4{0, 0, 0, 0};
-        const float base = m == -INFINITY ? 0.0f : m + Rows::kDown;
+        const float base = m == -INFINITY ? 0.0f : m;
         row0 = walk.row + wave * kRows;
         pages.fill(row0 >> p.shift);
         for (; row0 < end; row0 += kWaves * kRows) {
@@ -1161,7 +1174,7 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, Shared<Rows>& lds) {
               const int row = row0 + s * 16 + 4 * g + i;
               const bool none = row < lo || row >= end || !h.ok[s];
               dead |= uint32_t(none) << (4 * s + i);
-              pr[4 * s + i] = none ? 0.0f : __builtin_amdgcn_exp2f(fmaf(y[i], q.mul, -base));
+              pr[4 * s + i] = none ? 0.0f : __builtin_amdgcn_exp2f(fmaf(y[i] - base, q.mul, -Rows::kDown));
             }
           }
           Rows::clear(vr, dead, 0);
@@ -1171,6 +1184,7 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, Shared<Rows>& lds) {
     }
 
     // The four wavefronts' parts, joined in their order.
+    m *= q.mul;
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     l *= Rows::kLast;
@@ -1326,6 +1340,8 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
     floatx4 acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = floatx4{0, 0, 0, 0};
+    // The maximum of the scores before their factor: differences to it are exact
+    // where they matter, however large the scores.
     float m = -INFINITY, l = 0.0f;
     typename Rows::Unit unit;
     for (; row0 < end; row0 += kWideTile) {
@@ -1369,21 +1385,20 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
         top = fmaxf(top, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
       }
       buf ^= 1;
-      top *= q.mul;
-      if (__any(top > m + kTau)) {
+      if (__any((top - m) * q.mul > kTau)) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float next = fmaxf(m, top);
-        const float scale = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+        const float scale = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - next) * q.mul);
         m = next;
         l *= scale;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j] *= scale;
       }
-      const float base = m == -INFINITY ? 0.0f : m + Rows::kDown;
+      const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        pr[e] = __builtin_amdgcn_exp2f(fmaf(pr[e], q.mul, -base));
+        pr[e] = __builtin_amdgcn_exp2f(fmaf(pr[e] - base, q.mul, -Rows::kDown));
         l += pr[e];
       }
       Rows::accumulate_wide(vr, pr, acc, unit, wave, r);
@@ -1398,7 +1413,7 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
         of = 1.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j] = floatx4{0, 0, 0, 0};
-        const float base = m == -INFINITY ? 0.0f : m + Rows::kDown;
+        const float base = m == -INFINITY ? 0.0f : m;
         row0 = walk.row;
         pages.fill(row0 >> p.shift);
         for (; row0 < end; row0 += kWideTile) {
@@ -1415,7 +1430,7 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
               const int row = row0 + s * 16 + 4 * g + i;
               const bool none = row < lo || row >= end || !h.ok[s];
               dead |= uint32_t(none) << (4 * s + i);
-              pr[4 * s + i] = none ? 0.0f : __builtin_amdgcn_exp2f(fmaf(y[i], q.mul, -base));
+              pr[4 * s + i] = none ? 0.0f : __builtin_amdgcn_exp2f(fmaf(y[i] - base, q.mul, -Rows::kDown));
             }
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -1426,6 +1441,7 @@ __device__ __forceinline__ void attend_wide(const DecodeArgs& a, SharedWide<Rows
       lds_barrier();  // the queries are written again
     }
     // Every wavefront holds the same maximum and sum.
+    m *= q.mul;
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     l *= Rows::kLast;

@@ -1,6 +1,6 @@
 """Paged decode attention within the bounds of paged_bounds.py, which are tight
 enough to tell a wrong answer from a rounded one: every layout, windows, long
-and many sequences, infinite values."""
+and many sequences, infinite values and extreme queries."""
 import numpy as np
 import pytest
 
@@ -88,3 +88,27 @@ def test_infinite_values_of_bf16_rows(T, D, n):
     got = attend(T, p, 4, f"infinite values {D} {n}", scale=0.1 * D ** -0.5)
     assert got[0, 2, 0] == np.inf and got[0, 3, 3] == -np.inf and np.isnan(got[0, 2, D - 1])
     assert np.all(np.isfinite(got[0, :2])) and np.count_nonzero(~np.isfinite(got)) == 2 * 5
+
+
+@pytest.mark.parametrize("kind,bk,bv,gs", LAYOUTS[:3])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("power", [90, 120, 122])
+def test_queries_near_the_largest_of_the_type(T, kind, bk, bv, gs, D, power):
+    """Scores of up to 2^126: the row of the largest one has all the weight."""
+    n = 200
+    p = Paged([n], 1, D, 32, kind, bk, bv, gs, seed=D, track=True).fill(D)
+    q = O.bf16_to_f32(kv_bf16((1, 4, D), 17)) * np.float32(2.0 ** power)
+    _, k, v, _ = p.rows(0, 0, n)
+    s = k @ q[0].T.astype(np.float64) * D ** -0.5
+    first, second = np.sort(s, 0)[-1], np.sort(s, 0)[-2]
+    x = np.abs(q[0].T.astype(np.float64))
+    ck, zk, _ = PB.parts_of(p, p.sides[0], p.bk, 0, 0, n)
+    sure = first - second > 4 * (D + 64) * 2.0 ** -24 * ((ck + zk) @ x).max(0) * D ** -0.5
+    assert np.count_nonzero(sure) >= 3 and np.abs(s).max() < 2.0 ** 126
+    d = p.device(T)
+    print("[numerics] large queries", kind, D, power, flush=True)
+    got = O.bf16_to_f32(d.attend(O.bf16_from_f32(q), D ** -0.5))
+    for h in np.nonzero(sure)[0]:
+        want = v[s[:, h].argmax()]
+        assert np.all(np.abs(got[0, h] - want) <= (2.0 ** -8 + 2.0 ** -9) * np.abs(want) + 2.0 ** -20)
+    assert np.all(np.isfinite(d.weights.numpy())) and abs(d.weights.numpy().sum() - 4) < 1e-3
