@@ -400,7 +400,7 @@ int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint16_t* q, int
                                  tqkv_stream stream);
 /* Its workspace: split partials, and f32 scores [batch, H, max_rows] where
  * kv->weights is set. Host arithmetic only; 0 for arguments that the call
- * refuses. */
+ * refuses whatever its window. */
 size_t tqkv_paged_decode_workspace_size(const tqkv_paged_kv* kv, int32_t H, int64_t max_rows);
 
 /*
@@ -427,6 +427,7 @@ int32_t tqkv_paged_evict(const tqkv_paged_kv* kv, int64_t budget, int64_t sinks,
                          const int32_t* dst_table, int64_t dst_stride, int32_t* dst_lens,
                          float* dst_weights, int32_t* kept, void* workspace,
                          size_t workspace_bytes, tqkv_stream stream);
+/* Host arithmetic only; 0 for a pool or a budget that the call refuses. */
 size_t tqkv_paged_evict_workspace_size(const tqkv_paged_kv* kv, int64_t budget);
 
 /*

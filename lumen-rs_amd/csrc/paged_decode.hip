@@ -291,17 +291,33 @@ bool plan_of(const tqkv_paged_kv* kv, int32_t H, int64_t max_rows, HostPlan* out
   return true;
 }
 
+// Workgroups of the join a sequence and KV head whose weights it adds: `seen` rows.
+int row_blocks_of(const tqkv_paged_kv* kv, int64_t seen) {
+  return kv->weights ? int((seen + kWeightRows - 1) / kWeightRows) : 0;
+}
+int64_t join_blocks(const tqkv_paged_kv* kv, int32_t H, int row_blocks) {
+  const int parts = kv->dim > 128 ? kv->dim / 128 : 1;  // JoinShape's
+  return int64_t(kv->batch) * H * parts + int64_t(kv->batch) * kv->kv_heads * row_blocks;
+}
+// Units over the whole batch are 32-bit in the kernels, and a grid holds below
+// 2^32 threads.
+bool fits(const tqkv_paged_kv* kv, const HostPlan& plan, int64_t blocks) {
+  return int64_t(kv->batch) * (plan.srows / kUnit + kOver + 1) <= 0x7fffffffLL &&
+         blocks <= 0xffffffffLL / kJoinThreads;
+}
+
 }  // namespace
 }  // namespace paged
 }  // namespace tqkv
 
 extern "C" size_t tqkv_paged_decode_workspace_size(const tqkv_paged_kv* kv, int32_t H,
                                                    int64_t max_rows) {
-  tqkv::paged::Pool pool;
-  tqkv::paged::HostPlan plan;
-  if (tqkv::paged::check(kv, &pool) != TQKV_OK || !tqkv::paged::plan_of(kv, H, max_rows, &plan))
-    return 0;
-  return plan.bytes;
+  using namespace tqkv::paged;
+  Pool pool;
+  HostPlan plan;
+  if (check(kv, &pool) != TQKV_OK || !plan_of(kv, H, max_rows, &plan)) return 0;
+  // The least that a window leaves of the weights' rows.
+  return fits(kv, plan, join_blocks(kv, H, row_blocks_of(kv, 1))) ? plan.bytes : 0;
 }
 
 extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint16_t* q,
@@ -325,14 +341,9 @@ extern "C" int32_t tqkv_paged_decode_attend(const tqkv_paged_kv* kv, const uint1
                 (long long)max_rows);
   a.window = window > 0 && window < max_rows ? int(window) : 0;
   const int64_t seen = a.window > 0 ? a.window + 3 : max_rows;  // from a row of four
-  const int row_blocks = kv->weights ? int((seen + kWeightRows - 1) / kWeightRows) : 0;
-  const int parts = kv->dim > 128 ? kv->dim / 128 : 1;  // JoinShape's
-  const int64_t blocks =
-      int64_t(kv->batch) * H * parts + int64_t(kv->batch) * kv->kv_heads * row_blocks;
-  // Units over the whole batch are 32-bit in the kernels, and a grid
-  // holds below 2^32 threads.
-  if (int64_t(kv->batch) * (plan.srows / kUnit + kOver + 1) > 0x7fffffffLL ||
-      blocks > 0xffffffffLL / kJoinThreads)
+  const int row_blocks = row_blocks_of(kv, seen);
+  const int64_t blocks = join_blocks(kv, H, row_blocks);
+  if (!fits(kv, plan, blocks))
     return fail(TQKV_EUNSUPPORTED, "batch=%d max_rows=%lld", kv->batch, (long long)max_rows);
   if (!workspace) {
     if (int32_t rc = scratch_for_current_device(plan.bytes, &workspace)) return rc;

@@ -28,6 +28,7 @@ constexpr int kQuads = 8;         // quads of rows a thread holds
 constexpr int kChunk = kSel * 4 * kQuads;
 constexpr int kBins = 2048;
 constexpr int kCopies = 4;        // of the histogram, by lane: weights crowd few digits
+constexpr int64_t kMostBudget = int64_t(1) << 29;
 
 // Bits that order like the weights: larger is heavier; NaN counts as -inf and
 // -0 as 0. Between 0x007fffff (-inf) and 0xff800000 (inf).
@@ -333,7 +334,7 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(const MoveArgs a) 
 
 extern "C" size_t tqkv_paged_evict_workspace_size(const tqkv_paged_kv* kv, int64_t budget) {
   tqkv::paged::Pool p;
-  if (tqkv::paged::check(kv, &p) != TQKV_OK || budget < 1 || budget > 0x7fffffffLL) return 0;
+  if (tqkv::paged::check(kv, &p) != TQKV_OK || budget < 1 || budget > kMostBudget) return 0;
   return size_t(p.batch) * p.Hkv * size_t(budget) * sizeof(int32_t);
 }
 
@@ -347,7 +348,7 @@ extern "C" int32_t tqkv_paged_evict(const tqkv_paged_kv* kv, int64_t budget, int
   if (int32_t rc = check(kv, &a.pool)) return rc;
   if (dst_stride < 1 || dst_stride > (int64_t(1) << 30) / kv->page_rows || budget < 1 || sinks < 0 ||
       recent < 0 || sinks > budget || recent > budget - sinks ||
-      budget > dst_stride * kv->page_rows || budget > (int64_t(1) << 29))
+      budget > dst_stride * kv->page_rows || budget > kMostBudget)
     return fail(TQKV_EINVAL_SHAPE, "budget=%lld sinks=%lld recent=%lld of %lld new pages a sequence",
                 (long long)budget, (long long)sinks, (long long)recent, (long long)dst_stride);
   if (!kv->weights || !dst_table || !dst_lens) return fail(TQKV_EINVAL_ARG, "null pointer");
