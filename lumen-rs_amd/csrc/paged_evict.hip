@@ -333,8 +333,9 @@ __global__ __launch_bounds__(kThreads) void evict_move_kernel(const MoveArgs a) 
 }  // namespace tqkv
 
 extern "C" size_t tqkv_paged_evict_workspace_size(const tqkv_paged_kv* kv, int64_t budget) {
-  tqkv::paged::Pool p;
-  if (tqkv::paged::check(kv, &p) != TQKV_OK || budget < 1 || budget > kMostBudget) return 0;
+  using namespace tqkv::paged;
+  Pool p;
+  if (check(kv, &p) != TQKV_OK || budget < 1 || budget > kMostBudget) return 0;
   return size_t(p.batch) * p.Hkv * size_t(budget) * sizeof(int32_t);
 }
 
