@@ -356,7 +356,12 @@ extern "C" int32_t tqkv_paged_evict(const tqkv_paged_kv* kv, int64_t budget, int
   if (!aligned(dst_table, 4) || !aligned(dst_lens, 4) || !aligned(dst_weights, 4) ||
       !aligned(kept, 4))
     return fail(TQKV_EINVAL_ARG, "dst_table, dst_lens, dst_weights or kept not 4-byte aligned");
-  if (dst_weights == kv->weights) return fail(TQKV_EINVAL_ARG, "dst_weights is the pool's weights");
+  // Rows move while others' weights are still read.
+  const uintptr_t old_at = reinterpret_cast<uintptr_t>(kv->weights), new_at = reinterpret_cast<uintptr_t>(dst_weights);
+  const uint64_t units = uint64_t(kv->batch) * uint64_t(kv->kv_heads) * sizeof(float);
+  if (dst_weights && new_at < old_at + units * uint64_t(a.pool.wstride) &&
+      old_at < new_at + units * uint64_t(dst_stride * kv->page_rows))
+    return fail(TQKV_EINVAL_ARG, "dst_weights overlaps the pool's weights");
   const int D = kv->dim;
   a.slots = kv->kind == TQKV_CACHE_BF16 ? 1 : 3;
   for (int i = 0; i < a.slots; ++i) {

@@ -25,3 +25,18 @@ def test_no_eviction_workspace_for_a_budget_that_is_refused():
         refused(T.EINVAL_SHAPE, T.paged_evict, kv, budget, 0, 0, A, stride, A)
         assert T.paged_evict_workspace_size(kv, budget) == 0
     assert T.paged_evict_workspace_size(kv, 1 << 29) == 2 * 4 * 4 << 29
+
+
+def test_eviction_refuses_overlapping_weights():
+    """The rows' new weights may touch the old ones' end or begin, and no more."""
+    kv = view(weights=16 * A)  # 2 x 4 x 512 weights: 16 KB
+    ok = dict(kv=kv, budget=64, sinks=4, recent=8, dst_table=A, dst_stride=4, dst_lens=A, kept=None,
+              workspace=A, workspace_bytes=0)  # too small a workspace: refused in any case
+    new = 2 * 4 * 256 * 4
+    for at in (16 * A, 16 * A + 4, 16 * A + (1 << 14) - 4, 16 * A - new + 4):
+        with pytest.raises(T.TqkvError, match="overlaps") as e:
+            T.paged_evict(**ok, dst_weights=at)
+        assert e.value.status == T.EINVAL_ARG
+    for at in (16 * A + (1 << 14), 16 * A - new, None):
+        with pytest.raises(T.TqkvError, match="workspace"):
+            T.paged_evict(**ok, dst_weights=at)
