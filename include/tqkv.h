@@ -417,7 +417,11 @@ size_t tqkv_paged_decode_workspace_size(const tqkv_paged_kv* kv, int32_t H, int6
  * dst_weights behind the last row, stay as they were. The destination pages
  * must not be among the pages of kv->table nor twice in dst_table, and
  * dst_weights must not overlap kv->weights; dst_lens may be kv->lens. Rows
- * whose old or new page is invalid are not moved (their weights are).
+ * whose old or new page is invalid are not moved (their weights are): a row
+ * without an old page ranks and takes a place like any other, and that place
+ * holds what the new page held before and is attended to from then on. So cut
+ * back only sequences that have valid pages for all of their rows, or clear the
+ * new pages first.
  * budget >= 1, sinks + recent <= budget <= dst_stride * page_rows and 2^29.
  * workspace: tqkv_paged_evict_workspace_size() bytes (the kept positions) or
  * NULL for the library's scratch; neither is used where kept is given. Two
