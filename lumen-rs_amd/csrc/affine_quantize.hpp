@@ -39,19 +39,9 @@ __device__ __forceinline__ void load_lane(const uint16_t* p, float (&v)[kLaneEle
   }
 }
 
-// Quantizes N (a multiple of 8) consecutive elements of a row held by each
-// lane; a group is `lpg` adjacent lanes (a power of two), whose min and max
-// meet in a butterfly. Writes the group's f32 scale and bias and the lane's
-// codes as N / 8 chunks of 8. Every lane of the wavefront must call it (the
-// butterfly exchanges across lanes).
-//
-// kFastQuotient: the code of an element is roundf(RN((v - bias) / scale))
-// clamped; instead of the correctly rounded division it multiplies by
-// RN(1 / scale), whose product is within 3 ulp of the rounded quotient, and
-// takes the exact division only where the product lies within 2^-20 of
-// its value from a rounding boundary k + 1/2 (where the two could round to
-// different integers). The codes are the same bits either way.
-// The group's f32 scale and bias, before the bf16 store.
+// The f32 scale and bias, before the bf16 store, of a group of `lpg` adjacent
+// lanes (a power of two) that hold N elements each; their min and max meet in a
+// butterfly, so every lane of the wavefront must call it.
 template <int N>
 __device__ __forceinline__ void group_scale(const float (&v)[N], int lpg, int bits,
                                             float& scale_out, float& bias_out) {
@@ -79,6 +69,18 @@ __device__ __forceinline__ void group_scale(const float (&v)[N], int lpg, int bi
   bias_out = at_zero ? 0.0f : edge;
 }
 
+// Quantizes N (a multiple of 8) consecutive elements of a row held by each
+// lane; a group is `lpg` adjacent lanes (a power of two), whose min and max
+// meet in a butterfly. Writes the group's f32 scale and bias and the lane's
+// codes as N / 8 chunks of 8. Every lane of the wavefront must call it (the
+// butterfly exchanges across lanes).
+//
+// kFastQuotient: the code of an element is roundf(RN((v - bias) / scale))
+// clamped; instead of the correctly rounded division it multiplies by
+// RN(1 / scale), whose product is within 3 ulp of the rounded quotient, and
+// takes the exact division only where the product lies within 2^-20 of
+// its value from a rounding boundary k + 1/2 (where the two could round to
+// different integers). The codes are the same bits either way.
 template <int N, bool kFastQuotient = false>
 __device__ __forceinline__ void quantize_elems(const float (&v)[N], int lpg, int bits,
                                                float& scale_out, float& bias_out,

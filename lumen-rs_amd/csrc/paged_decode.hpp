@@ -142,12 +142,10 @@ constexpr int kKeep = 0, kStream = 2;
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
-// A load of N bytes (2, 4, 8 or a multiple of 16) into words.
+// A load of N bytes (4, 8 or a multiple of 16) into words.
 template <int N, int kPolicy = kKeep>
 __device__ __forceinline__ void load_words(rsrc base, uint32_t off, uint32_t* w) {
-  if constexpr (N == 2) {
-    w[0] = __builtin_amdgcn_raw_buffer_load_b16(base, off, 0, kPolicy);
-  } else if constexpr (N == 4) {
+  if constexpr (N == 4) {
     w[0] = __builtin_amdgcn_raw_buffer_load_b32(base, off, 0, kPolicy);
   } else if constexpr (N == 8) {
     const uintx2 x = __builtin_amdgcn_raw_buffer_load_b64(base, off, 0, kPolicy);
