@@ -386,8 +386,9 @@ int32_t tqkv_paged_append(const tqkv_paged_kv* kv, const uint16_t* k, const uint
  * softmax weights, summed over the query heads of its KV head, are added to
  * it (f32, in a fixed order).
  * Scores and sums are f32, and weights carry 16 bits over bf16 rows and 11 over
- * affine ones; there weights below 2^-32 of a head's largest may vanish. Rows and
- * groups may differ in magnitude as the type allows, and no channel loses bits to
+ * affine ones; there weights below 2^-32 of a head's largest may vanish, and a
+ * query's channels below 2^-27 of its largest lose bits. Values of rows and groups
+ * may differ in magnitude as the type allows, and no channel loses bits to
  * another's (affine values that differ by more than 2^8 cost a second pass); an
  * infinite or NaN value stays in its channel. Outputs below 2^-80 lose bits.
  * workspace: tqkv_paged_decode_workspace_size() bytes, 16-byte aligned, or

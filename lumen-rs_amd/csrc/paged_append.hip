@@ -125,7 +125,11 @@ __device__ __forceinline__ void clear_weights(const Pool& p, const Dest* dest, i
 constexpr int kTokens = 4;
 // Quantized prompts: a workgroup's rows of a head lie side by side in a page
 // (13,548 tokens of 8 heads, 4 bits: 27 us at 4 tokens a workgroup, 24 at 8,
-// 25 at 16, 28 at 32); few tokens keep the smaller workgroups, for latency.
+// 25 at 16, 28 at 32); few tokens keep the smaller workgroups, for latency. With
+// 4 and 8 tokens a workgroup, D = 128, 8 heads: 1,024 tokens 4.6 and 5.1 us, 2,048
+// 5.9 and 6.0, 4,096 11.2 and 10.0. The line lies lower for shorter rows (D = 64:
+// 2,048 tokens 5.3 and 4.5) and higher for longer ones (D = 256: 4,096 15.7 and
+// 15.9).
 constexpr int kMany = 8, kManyTokens = 2048;
 
 template <int D>

@@ -36,11 +36,11 @@
 // over its rows once more and takes values and weights as bf16 pairs.
 //
 // Bound by HBM: the live rows once. At G heads of 16 the matrix cores do
-// 16 / G times the work that is needed and are still far from busy (7 to 20%).
+// 16 / G times the work that is needed and are still far from busy (4 to 20%).
 // Measured, with the join: bf16, 131,071 rows x 8 KV heads at D = 128 (537 MB)
 // 86 us, 6.2 TB/s; 4 bits, 16 x 32,768 x 8 at D = 256 (1.21 GB) 244 us, 5.0
-// TB/s, where unpacking keeps the vector units 72% busy. Short calls are bound
-// by latencies: 777 rows take 7.4 us and the join's 2.9.
+// TB/s, where unpacking keeps the vector units 74% busy. Short calls are bound
+// by latencies: 777 rows take 7.2 us and the join's 2.8.
 #pragma once
 
 #include <type_traits>
@@ -503,7 +503,7 @@ struct AffineRows {
     }
   }
   // Queries as f16 times 2^(14 - E), E the head's largest exponent (so they
-  // lie below 2^15; parts below 2^-28 of the largest lose bits), in unpack's
+  // lie below 2^15; channels below 2^-27 of the largest lose bits), in unpack's
   // order; the sums of the groups in the same unit as three bf16 parts, which
   // hold all bits of an f32, one a quarter. Channels of (group, quarter):
   // group GS + quarter GS / 4, then in order.
@@ -694,7 +694,7 @@ struct AffineRows {
   // so much larger than another that what f16 loses of its weight would matter
   // to the other's. Otherwise (infinite bounds too) the sums are given up, and
   // the second pass makes them: calls with such rows in every wavefront's part
-  // take 1.6 to 2.3 times as long (16 x 16,384 rows of 4 bits at D = 128: 147 us
+  // take 1.5 to 2.3 times as long (16 x 16,384 rows of 4 bits at D = 128: 147 us
   // for 80). Pairs in the loop itself spilled, and cost every call (32 sequences
   // of 17 to 16,000 rows: 57 us for 39).
   static constexpr bool kPairs = true;
