@@ -168,3 +168,39 @@ def test_spread_values_over_the_whole_card(T, D):
     for i in rng.integers(0, 9001, 200):
         times(p, 0, [i], [int(rng.integers(0, D // 64))], int(rng.integers(-30, 40)))
     attend(T, p, f"card {D}")
+
+
+@pytest.mark.parametrize("D", DIMS)
+@pytest.mark.parametrize("window", [70, 333])
+def test_spread_values_in_windows_of_two_sets_of_heads(T, D, window):
+    """20 query heads a KV head; the large group inside the window, and before
+    it, where it does not count."""
+    p = pool(D, 8, 8, 32, lens=(700, 33, 0, 340), track=True)
+    times(p, 0, [690], [1], 25)
+    times(p, 0, [100], [0], 60)
+    times(p, 3, [339], [-1], 40)
+    q = kv_bf16((p.B, 20, D), 6)
+    out, tol, gain, gtol = PB.attend(p, q, 0.1, window)
+    d = p.device(T)
+    print("[spread] windows", D, window, flush=True)
+    PB.check(O.bf16_to_f32(d.attend(q, 0.1, window)), out, tol, "windows")
+    PB.check(d.weights.numpy(), gain, gtol + 2.0 ** -23 * gain, "windows weights")
+
+
+@pytest.mark.parametrize("D", DIMS)
+def test_spread_values_in_some_of_many_short_sequences(T, D):
+    """Several sequences a workgroup, some of its wavefronts in a second pass
+    while others go on; the same every time."""
+    rng = np.random.default_rng(D)
+    p = pool(D, 4, 4, 64, lens=tuple(int(n) for n in rng.integers(0, 90, 500)), Hkv=2)
+    for b in range(0, 500, 2):
+        if p.lens[b]:
+            times(p, b, [int(rng.integers(0, p.lens[b]))], [int(rng.integers(0, D // 64))], int(rng.integers(10, 50)))
+    q = kv_bf16((p.B, 4, D), 7)
+    out, tol, _, _ = PB.attend(p, q, D ** -0.5)
+    d = p.device(T)
+    print("[spread] short", D, flush=True)
+    first = d.attend(q, D ** -0.5)
+    PB.check(O.bf16_to_f32(first), out, tol, "short")
+    for _ in range(5):
+        assert np.array_equal(d.attend(q, D ** -0.5), first)
