@@ -436,6 +436,193 @@ int32_t tqkv_paged_evict(const tqkv_paged_kv* kv, int64_t budget, int64_t sinks,
 size_t tqkv_paged_evict_workspace_size(const tqkv_paged_kv* kv, int64_t budget);
 
 /*
+ * The tables of a paged cache, built and taken down on the device (no
+ * counterpart in the reference). free_pages[0, *free_count) are the pages
+ * that no sequence holds, a stack whose top is its end.
+ *
+ * batch at most 1024, page_rows in {16, 32, 64, 128, 256}, num_pages below
+ * 2^31, table_stride * page_rows at most 2^30. All arrays are device int32,
+ * 4-byte aligned. lens and free_count are read as the paged calls read lens:
+ * below 0 as 0, above what the table (the stack) can hold as that.
+ */
+typedef struct tqkv_page_tables {
+  int32_t batch;
+  int32_t page_rows;
+  int64_t num_pages;
+  int64_t table_stride;
+  int32_t* table;      /* [batch, table_stride] */
+  int32_t* lens;       /* [batch] */
+  int32_t* free_pages; /* [num_pages] */
+  int32_t* free_count; /* [1] */
+} tqkv_page_tables;
+
+/*
+ * Gives every sequence room for counts[b] more rows (device int32 [batch];
+ * below 0 as 0): pages from the top of the stack where its last page does not
+ * hold them, lens[b] + counts[b] as its new length, and for the new tokens,
+ * which lie one behind the other, starts (int32 [batch + 1]) and slots
+ * (int32 [tokens, 4], or NULL): a token's page and row in it, its position
+ * in the sequence and the sequence. tqkv_paged_append and the prefill
+ * attention take starts as it is, tqkv_paged_append_rope the slots.
+ * Sequences are served in order: one is refused (and keeps its length) where
+ * its table cannot name the rows, where it needs pages and those that it and
+ * all before it that the table could hold ask for are more than are free, or where their tokens are more
+ * than `tokens`. granted (int32 [batch], or NULL): counts[b], or -1 where
+ * refused. The pages given out are the top ones of the stack, in its order;
+ * slots behind the last token are {-1, 0, -1, -1}, and a page that the table
+ * names wrongly is -1 in them. tokens: the host's bound on the sum of counts,
+ * below 2^31. One launch, two for 1,024 tokens and more; no allocation.
+ */
+int32_t tqkv_paged_reserve(const tqkv_page_tables* tables, const int32_t* counts, int64_t tokens,
+                           int32_t* starts, int32_t* granted, int32_t* slots,
+                           tqkv_stream stream);
+/*
+ * Takes rows back: sequence b keeps its first keep[b] rows (device int32
+ * [batch]; as many as it holds or more: all, 0: none), the pages behind them
+ * go on top of the stack in the order of the sequences and their rows, and
+ * their table entries become -1. shared (device int32 [batch], or NULL): the
+ * first shared[b] pages belong to another holder (a common prompt) and stay
+ * in the table and off the stack. Entries that name no page are not put back, nor is what the stack has
+ * no room for. A reserve and then a release of what it gave leave the stack as
+ * it was. One launch.
+ */
+int32_t tqkv_paged_release(const tqkv_page_tables* tables, const int32_t* keep,
+                           const int32_t* shared, tqkv_stream stream);
+
+/*
+ * Rotary positions (no counterpart in the reference's cache, which takes
+ * rotated keys). Channel pair i of a head's first rotary_dim channels turns
+ * by position * theta_i, theta_i = base^(-2 i / rotary_dim):
+ * (x, y) -> magnitude * (x cos - y sin, x sin + y cos).
+ *
+ * Scaled for contexts longer than `original` positions by `factor`:
+ *   TQKV_ROPE_LINEAR  theta / factor
+ *   TQKV_ROPE_BASE    base * factor^(rotary_dim / (rotary_dim - 2)) as base
+ *   TQKV_ROPE_BANDS   pairs that turn at most `low` times in `original`
+ *                     positions take theta / factor, those that turn at least
+ *                     `high` times theta, and between them the mean of the two
+ *                     weighted linearly by the turns
+ *   TQKV_ROPE_RAMP    the same ends as whole channels, floor and ceiling of
+ *                     rotary_dim ln(original / (2 pi turns)) / (2 ln base)
+ *                     within [0, rotary_dim - 1], weighted linearly by i
+ *                     between them, and a magnitude of 0.1 ln(factor) + 1
+ */
+#define TQKV_ROPE_PLAIN 0
+#define TQKV_ROPE_LINEAR 1
+#define TQKV_ROPE_BASE 2
+#define TQKV_ROPE_BANDS 3
+#define TQKV_ROPE_RAMP 4
+typedef struct tqkv_rope_config {
+  int32_t rotary_dim; /* even, 2 to 1024 */
+  int32_t scaling;
+  double base;     /* above 1 */
+  double factor;   /* above 0; unused by TQKV_ROPE_PLAIN */
+  double original; /* positions, above 0 (BANDS and RAMP) */
+  double low;      /* 0 < low < high (BANDS and RAMP) */
+  double high;
+} tqkv_rope_config;
+/* Host arithmetic only: turns (host uint64 [rotary_dim / 2]) receives
+ * theta_i / 2 pi in units of 2^-64 turn, magnitude (host) the factor. With a
+ * 64-bit fraction of a turn, position * turns is the angle modulo a turn to
+ * 2^-33 of a turn for every 31-bit position. */
+int32_t tqkv_rope_turns(const tqkv_rope_config* config, uint64_t* turns, float* magnitude);
+
+typedef struct tqkv_rope {
+  int32_t rotary_dim;
+  int32_t interleaved;   /* 0: pairs (i, i + rotary_dim / 2); 1: (2 i, 2 i + 1) */
+  float magnitude;
+  int32_t reserved;      /* 0 */
+  const uint64_t* turns; /* device [rotary_dim / 2], 8-byte aligned */
+} tqkv_rope;
+
+/*
+ * Rotates the heads of tokens: head h of token i at x + i * x_token_stride +
+ * h * x_head_stride (bf16 elements) by position positions[i *
+ * position_stride] (device int32), to out alike; channels from rotary_dim on
+ * are copied. out may be x with the same strides, and otherwise does not
+ * overlap it. A token of negative position is left out: its row of out stays
+ * as it was. Products and sums in f32, rounded once to bf16. Q and K heads
+ * that lie side by side are one call. dim: a multiple of 8 up to 1024, at
+ * least rotary_dim; heads at most 1024; x and out 16-byte aligned, strides
+ * multiples of 8. One launch.
+ */
+int32_t tqkv_rope_apply(const tqkv_rope* rope, const int32_t* positions, int64_t position_stride,
+                        int64_t tokens, const uint16_t* x, int32_t heads, int32_t dim,
+                        int64_t x_token_stride, int64_t x_head_stride, uint16_t* out,
+                        int64_t out_token_stride, int64_t out_head_stride, tqkv_stream stream);
+/*
+ * A layer's way into the paged cache in one launch: queries rotated to q_out,
+ * keys rotated and written with the values into their slots (device int32
+ * [tokens, 4], 16-byte aligned, as tqkv_paged_reserve makes them), bit for
+ * bit what tqkv_rope_apply and tqkv_paged_append give. Head h of token i:
+ * q + i * q_stride + h * dim to q_out + i * q_out_stride + h * dim, k and v
+ * at i * token_stride + h * head_stride. H = 0: no queries (q and q_out
+ * NULL). positions (with its stride) gives positions other than the slots';
+ * NULL takes those. A token of negative position is left out; one whose slot is no row of
+ * the pool has its queries rotated only. With kv->weights, a written row's are cleared
+ * (slots' sequence and position). kv->table and kv->lens are not read. q_out
+ * may be q with the same stride; H at most 1024; alignment as in
+ * tqkv_paged_append.
+ */
+int32_t tqkv_paged_append_rope(const tqkv_paged_kv* kv, const tqkv_rope* rope, const uint16_t* q,
+                               int32_t H, int64_t q_stride, uint16_t* q_out, int64_t q_out_stride,
+                               const uint16_t* k, const uint16_t* v, int64_t token_stride,
+                               int64_t head_stride, const int32_t* slots, int64_t tokens,
+                               const int32_t* positions, int64_t position_stride,
+                               tqkv_stream stream);
+
+/*
+ * Attention of whole prompts, softmax(scale * q.K^T + mask) . V, over
+ * sequences of different lengths that lie one behind the other: sequence b is
+ * tokens [starts[b], starts[b + 1]) (device int32 [batch + 1], ascending),
+ * and its queries see its own keys only: all of them, or with causal != 0
+ * those at their own position and before, and with window > 0 (causal only)
+ * of these the last `window`. No counterpart in the reference, which attends
+ * one sequence a call; the mask is tqkv_prefill_attend_affine's.
+ * Head h of token i: q + i * q_stride + h * D; k and v at i * token_stride +
+ * h * head_stride (a fused projection is read in place); out bf16 [tokens, H,
+ * D]. Query head h reads KV head h / (H / H_kv). Rows of out before starts[0]
+ * and from starts[batch] on stay as they were.
+ * Scores and sums are f32; weights multiply V as bf16, normalised by the sum
+ * of the rounded weights. Values keep bf16's range, and an infinite or NaN
+ * key or value reaches only the queries that see it.
+ * D in {64, 128, 256, 512}; H / H_kv from 1 to 32; batch at most 1024; tokens
+ * below 2^31; q, k, v 16-byte aligned, strides multiples of 8; out 16-byte
+ * aligned. workspace: tqkv_packed_attend_workspace_size() bytes, 16-byte
+ * aligned, or NULL for the library's scratch; calls that share one must not
+ * overlap in time.
+ */
+int32_t tqkv_packed_attend(const uint16_t* q, int64_t q_stride, const uint16_t* k,
+                           const uint16_t* v, int64_t token_stride, int64_t head_stride,
+                           int32_t batch, int32_t H, int32_t H_kv, int32_t D,
+                           const int32_t* starts, int64_t tokens, float scale, int32_t causal,
+                           int64_t window, uint16_t* out, void* workspace,
+                           size_t workspace_bytes, tqkv_stream stream);
+/* Host arithmetic only; 0 where none is needed and for sizes that the call
+ * refuses. */
+size_t tqkv_packed_attend_workspace_size(int32_t batch, int32_t H, int32_t H_kv, int32_t D,
+                                         int64_t tokens);
+
+/*
+ * The same for the newest tokens of each sequence over its pages, a whole
+ * prompt or a chunk of one (or drafted tokens): the count = starts[b + 1] -
+ * starts[b] queries of sequence b sit at its last positions, lens[b] - count
+ * and on (lens counts them already, and their rows are in the pages), and see
+ * its rows up to their own position, with window > 0 the last `window` of
+ * these. Rows of invalid pages get no attention; a query that sees no row
+ * gets zeros. max_rows: the host's bound on lens, as tqkv_paged_decode_attend
+ * takes it. Affine rows enter as tqkv_affine_dequantize's bf16 values.
+ * kv->weights is not touched. q, out, H and the workspace as above; results
+ * depend on starts, lens, tokens and max_rows, not on the run.
+ */
+int32_t tqkv_paged_prefill_attend(const tqkv_paged_kv* kv, const uint16_t* q, int64_t q_stride,
+                                  int32_t H, const int32_t* starts, int64_t tokens, float scale,
+                                  int64_t window, int64_t max_rows, uint16_t* out,
+                                  void* workspace, size_t workspace_bytes, tqkv_stream stream);
+size_t tqkv_paged_prefill_workspace_size(const tqkv_paged_kv* kv, int32_t H, int64_t tokens,
+                                         int64_t max_rows);
+
+/*
  * Which decode kernel tqkv_decode_attend_affine runs for a layout: "mfma"
  * (scores on the matrix cores; group_size 32, 64 or 128, D in {64, 128, 256},
  * heads a launch in {1, 2, 4, 8} with heads * D / group_size <= 16), "tiles"

@@ -1,0 +1,300 @@
+// Paged cache: pages given to sequences and taken back, on the device.
+//
+// Reserve: with n rows held and a more asked, a sequence needs
+// ceil((n + a) / R) - ceil(n / R) pages. One scan over the batch (at most
+// 1,024 sequences) of what is asked decides who is served, a second one of what is
+// granted places tokens and pages; every token then finds its sequence by a
+// search in LDS. Bound by a launch's time for a decode step, and for prompts
+// by the 16 bytes a token that the slots take.
+// Release: the same scan over the pages that come back; one workgroup walks
+// them in order, since entries that name no page are left out of the stack.
+#include "paged.hpp"
+
+namespace tqkv {
+namespace paged {
+namespace {
+
+struct Tables {
+  int32_t* table;
+  int32_t* lens;
+  int32_t* free_pages;
+  int32_t* free_count;
+  int64_t tstride;
+  int num_pages, batch, shift, cap;
+};
+
+__device__ __forceinline__ int clamp_to(int x, int most) { return x < 0 ? 0 : x < most ? x : most; }
+__device__ __forceinline__ int pages_of(int64_t rows, int shift) {
+  return int((rows + (1 << shift) - 1) >> shift);
+}
+
+// Exclusive sums over the workgroup of each thread's x; total: over all.
+template <int Threads>
+__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* total) {
+  __shared__ int64_t sums[Threads / 64];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  int64_t y = x;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int64_t up = __shfl_up(y, d, 64);
+    if (lane >= d) y += up;
+  }
+  __syncthreads();
+  if (lane == 63) sums[wave] = y;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < Threads / 64; ++w) {
+    if (w < wave) before += sums[w];
+    all += sums[w];
+  }
+  *total = all;
+  return before + y - x;
+}
+
+// The last of s[0, n] (ascending) that is not above i: s[b] <= i < s[b + 1].
+__device__ __forceinline__ int find(const int32_t* s, int n, int i) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (i >= s[mid]) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+struct ReserveArgs {
+  Tables t;
+  const int32_t* counts;
+  int32_t* starts;
+  int32_t* granted;
+  int4* slots;
+  int tokens;
+};
+
+// Fill: tokens' slots and the new table entries; Finish: lengths, the stack's
+// height, starts and granted, which other workgroups' decisions read. One
+// workgroup does both; with many tokens a grid fills and a second launch of
+// one workgroup finishes.
+template <int Threads, bool Fill, bool Finish>
+__global__ __launch_bounds__(Threads) void reserve_kernel(const ReserveArgs a) {
+  constexpr int kPer = kMaxBatch / Threads;
+  __shared__ int32_t start[kMaxBatch + 1], base[kMaxBatch + 1], rows[kMaxBatch];
+  const Tables& t = a.t;
+  const int avail = clamp_to(*t.free_count, t.num_pages);
+  // Consecutive sequences a thread.
+  int n[kPer], want[kPer], need[kPer];
+  int64_t pages = 0, places = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int b = threadIdx.x * kPer + i;
+    n[i] = b < t.batch ? clamp_to(t.lens[b], t.cap) : 0;
+    want[i] = b < t.batch ? max(a.counts[b], 0) : 0;
+    const bool fits = int64_t(n[i]) + want[i] <= t.cap;
+    need[i] = fits ? pages_of(int64_t(n[i]) + want[i], t.shift) - pages_of(n[i], t.shift) : -1;
+    pages += fits ? need[i] : 0;
+    places += fits ? want[i] : 0;
+  }
+  int64_t all;
+  int64_t page_sum = block_scan<Threads>(pages, &all);
+  int64_t place_sum = block_scan<Threads>(places, &all);
+  int got[kPer], take[kPer], gots = 0, takes = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const bool fits = need[i] >= 0;
+    page_sum += fits ? need[i] : 0;
+    place_sum += fits ? want[i] : 0;
+    const bool ok = fits && (need[i] == 0 || page_sum <= avail) &&
+                    (want[i] == 0 || place_sum <= a.tokens);
+    got[i] = ok ? want[i] : -1;
+    take[i] = ok ? need[i] : 0;
+    gots += ok ? want[i] : 0;
+    takes += take[i];
+  }
+  int64_t tokens, taken;
+  int first = int(block_scan<Threads>(gots, &tokens));
+  int page = int(block_scan<Threads>(takes, &taken));
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int b = threadIdx.x * kPer + i;
+    start[b] = first;
+    base[b] = page;
+    rows[b] = n[i];
+    first += max(got[i], 0);
+    page += take[i];
+    if (Finish && b < t.batch) {
+      a.starts[b] = start[b];
+      if (a.granted) a.granted[b] = got[i];
+      t.lens[b] = n[i] + max(got[i], 0);
+    }
+  }
+  const int total = int(tokens), top = avail - int(taken);
+  if (threadIdx.x == 0) {
+    start[kMaxBatch] = total;
+    base[kMaxBatch] = int(taken);
+    if (Finish) {
+      a.starts[t.batch] = total;
+      *t.free_count = top;  // every thread has read the old one: block_scan's barriers
+    }
+  }
+  if constexpr (!Fill) return;
+  __syncthreads();
+  const int grid = int(gridDim.x) * Threads;
+  for (int64_t j = int64_t(blockIdx.x) * Threads + threadIdx.x; j < taken; j += grid) {
+    const int b = find(base, kMaxBatch, int(j));
+    t.table[b * t.tstride + pages_of(rows[b], t.shift) + j - base[b]] = t.free_pages[top + j];
+  }
+  if (!a.slots) return;
+  for (int64_t i = int64_t(blockIdx.x) * Threads + threadIdx.x; i < a.tokens; i += grid) {
+    int4 s = make_int4(-1, 0, -1, -1);
+    if (i < total) {
+      const int b = find(start, kMaxBatch, int(i));
+      const int row = rows[b] + int(i) - start[b], held = pages_of(rows[b], t.shift);
+      const int p = row >> t.shift;
+      // Pages taken are read from the stack: the table's entries may not be there yet.
+      const int at = p < held ? t.table[b * t.tstride + p] : t.free_pages[top + base[b] + p - held];
+      s = make_int4(at >= 0 && at < t.num_pages ? at : -1, row & ((1 << t.shift) - 1), row, b);
+    }
+    a.slots[i] = s;
+  }
+}
+
+constexpr int kWalk = 1024, kEach = 8;
+
+__global__ __launch_bounds__(kWalk) void release_kernel(const Tables t, const int32_t* keep,
+                                                         const int32_t* shared) {
+  __shared__ int32_t base[kMaxBatch + 1], from[kMaxBatch];
+  __shared__ int32_t valid[kEach * (kWalk / 64)];
+  const int b = threadIdx.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  int count = 0;
+  const int height = clamp_to(*t.free_count, t.num_pages);
+  if (b < t.batch) {
+    const int n = clamp_to(t.lens[b], t.cap), k = clamp_to(keep[b], n);
+    int lo = pages_of(k, t.shift);
+    if (shared && shared[b] > lo) lo = shared[b];
+    from[b] = lo;
+    count = max(0, pages_of(n, t.shift) - lo);
+    t.lens[b] = k;
+  }
+  int64_t all;
+  const int64_t at = block_scan<kWalk>(count, &all);
+  // Positions in the walk are 32-bit: num_pages bounds what can be pushed, not
+  // what wrong tables can name, so a walk past 2^31 entries is cut there.
+  base[b] = int(at < 0x7fffffff ? at : 0x7fffffff);
+  if (threadIdx.x == 0) base[kMaxBatch] = int(all < 0x7fffffff ? all : 0x7fffffff);
+  __syncthreads();
+  const int64_t total = base[kMaxBatch];
+  int64_t pushed = height;
+  for (int64_t j0 = 0; j0 < total; j0 += kWalk * kEach) {
+    int page[kEach];
+    int64_t place[kEach];
+    unsigned long long mask[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int64_t j = j0 + i * kWalk + threadIdx.x;
+      page[i] = -1;
+      place[i] = -1;
+      if (j < total) {
+        const int s = find(base, kMaxBatch, int(j));
+        place[i] = s * t.tstride + from[s] + (j - base[s]);
+        page[i] = t.table[place[i]];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      mask[i] = __ballot(page[i] >= 0 && page[i] < t.num_pages);
+      if (lane == 0) valid[i * (kWalk / 64) + wave] = __popcll(mask[i]);
+    }
+    __syncthreads();
+    int sum = 0, mine[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach * (kWalk / 64); ++k) {
+      if (k % (kWalk / 64) == wave) mine[k / (kWalk / 64)] = sum;
+      sum += valid[k];
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (place[i] >= 0) t.table[place[i]] = -1;
+      const int64_t to = pushed + mine[i] + __popcll(mask[i] & ((1ull << lane) - 1));
+      if (page[i] >= 0 && page[i] < t.num_pages && to < t.num_pages) t.free_pages[to] = page[i];
+    }
+    pushed += sum;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *t.free_count = int(pushed < t.num_pages ? pushed : t.num_pages);
+}
+
+int32_t check_tables(const tqkv_page_tables* p, Tables* out) {
+  if (!p) return fail(TQKV_EINVAL_ARG, "null pointer");
+  const int R = p->page_rows;
+  if (p->batch < 1 || p->num_pages < 1 || p->table_stride < 1)
+    return fail(TQKV_EINVAL_SHAPE, "batch=%d num_pages=%lld table_stride=%lld", p->batch,
+                (long long)p->num_pages, (long long)p->table_stride);
+  if (p->batch > kMaxBatch || !(R == 16 || R == 32 || R == 64 || R == 128 || R == 256))
+    return fail(TQKV_EUNSUPPORTED, "batch=%d (at most %d) page_rows=%d", p->batch, kMaxBatch, R);
+  if (p->num_pages > 0x7fffffffLL || p->table_stride > (int64_t(1) << 30) / R)
+    return fail(TQKV_EINVAL_SHAPE, "num_pages=%lld table_stride=%lld page_rows=%d",
+                (long long)p->num_pages, (long long)p->table_stride, R);
+  if (!p->table || !p->lens || !p->free_pages || !p->free_count)
+    return fail(TQKV_EINVAL_ARG, "null pointer");
+  if (!aligned(p->table, 4) || !aligned(p->lens, 4) || !aligned(p->free_pages, 4) ||
+      !aligned(p->free_count, 4))
+    return fail(TQKV_EINVAL_ARG, "table, lens, free_pages or free_count not 4-byte aligned");
+  int shift = 4;
+  while ((1 << shift) < R) ++shift;
+  *out = Tables{p->table,         p->lens,  p->free_pages, p->free_count,
+                p->table_stride, int(p->num_pages), p->batch, shift,
+                int(p->table_stride * R)};
+  return TQKV_OK;
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace tqkv
+
+extern "C" int32_t tqkv_paged_reserve(const tqkv_page_tables* tables, const int32_t* counts,
+                                      int64_t tokens, int32_t* starts, int32_t* granted,
+                                      int32_t* slots, tqkv_stream stream) {
+  using namespace tqkv;
+  using namespace tqkv::paged;
+  ReserveArgs a{};
+  if (int32_t rc = check_tables(tables, &a.t)) return rc;
+  if (tokens < 0 || tokens > 0x7fffffffLL)
+    return fail(TQKV_EINVAL_SHAPE, "tokens=%lld", (long long)tokens);
+  if (!counts || !starts) return fail(TQKV_EINVAL_ARG, "null pointer");
+  if (!aligned(counts, 4) || !aligned(starts, 4) || !aligned(granted, 4) || !aligned(slots, 16))
+    return fail(TQKV_EINVAL_ARG, "counts, starts or granted not 4-byte aligned, or slots not 16-byte");
+  a.counts = counts;
+  a.starts = starts;
+  a.granted = granted;
+  a.slots = reinterpret_cast<int4*>(slots);
+  a.tokens = int(tokens);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (tokens < 1024) {
+    hipLaunchKernelGGL((reserve_kernel<1024, true, true>), dim3(1), dim3(1024), 0, st, a);
+    TQKV_LAUNCHED();
+    return ok();
+  }
+  const int64_t blocks = (tokens + 255) / 256;
+  hipLaunchKernelGGL((reserve_kernel<256, true, false>), dim3(unsigned(blocks < 2048 ? blocks : 2048)),
+                     dim3(256), 0, st, a);
+  TQKV_LAUNCHED();
+  hipLaunchKernelGGL((reserve_kernel<1024, false, true>), dim3(1), dim3(1024), 0, st, a);
+  TQKV_LAUNCHED();
+  return ok();
+}
+
+extern "C" int32_t tqkv_paged_release(const tqkv_page_tables* tables, const int32_t* keep,
+                                      const int32_t* shared, tqkv_stream stream) {
+  using namespace tqkv;
+  using namespace tqkv::paged;
+  Tables t;
+  if (int32_t rc = check_tables(tables, &t)) return rc;
+  if (!keep) return fail(TQKV_EINVAL_ARG, "null pointer");
+  if (!aligned(keep, 4) || !aligned(shared, 4))
+    return fail(TQKV_EINVAL_ARG, "keep or shared not 4-byte aligned");
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(release_kernel, dim3(1), dim3(kWalk), 0, st, t, keep, shared);
+  TQKV_LAUNCHED();
+  return ok();
+}

@@ -16,6 +16,11 @@ pub const TQKV_EINVAL_ARG: i32 = 6;
 pub const TQKV_ECORRUPT: i32 = 7;
 pub const TQKV_ABI_VERSION: i32 = 200;
 pub const TQKV_NOALLOC_SCRATCH_BYTES: i32 = 33554432;
+pub const TQKV_ROPE_PLAIN: i32 = 0;
+pub const TQKV_ROPE_LINEAR: i32 = 1;
+pub const TQKV_ROPE_BASE: i32 = 2;
+pub const TQKV_ROPE_BANDS: i32 = 3;
+pub const TQKV_ROPE_RAMP: i32 = 4;
 pub const TQKV_CACHE_BF16: i32 = 0;
 pub const TQKV_CACHE_AFFINE: i32 = 1;
 pub const TQKV_CACHE_CODEBOOK: i32 = 2;
@@ -62,6 +67,41 @@ pub struct tqkv_paged_kv {
     pub table: *const i32,
     pub lens: *const i32,
     pub weights: *mut f32,
+}
+
+#[repr(C)]
+#[derive(Debug, Copy, Clone)]
+pub struct tqkv_page_tables {
+    pub batch: i32,
+    pub page_rows: i32,
+    pub num_pages: i64,
+    pub table_stride: i64,
+    pub table: *mut i32,
+    pub lens: *mut i32,
+    pub free_pages: *mut i32,
+    pub free_count: *mut i32,
+}
+
+#[repr(C)]
+#[derive(Debug, Copy, Clone)]
+pub struct tqkv_rope_config {
+    pub rotary_dim: i32,
+    pub scaling: i32,
+    pub base: f64,
+    pub factor: f64,
+    pub original: f64,
+    pub low: f64,
+    pub high: f64,
+}
+
+#[repr(C)]
+#[derive(Debug, Copy, Clone)]
+pub struct tqkv_rope {
+    pub rotary_dim: i32,
+    pub interleaved: i32,
+    pub magnitude: f32,
+    pub reserved: i32,
+    pub turns: *const u64,
 }
 
 #[repr(C)]
@@ -156,6 +196,15 @@ extern "C" {
     pub fn tqkv_paged_decode_workspace_size(kv: *const tqkv_paged_kv, H: i32, max_rows: i64) -> usize;
     pub fn tqkv_paged_evict(kv: *const tqkv_paged_kv, budget: i64, sinks: i64, recent: i64, dst_table: *const i32, dst_stride: i64, dst_lens: *mut i32, dst_weights: *mut f32, kept: *mut i32, workspace: *mut c_void, workspace_bytes: usize, stream: tqkv_stream) -> i32;
     pub fn tqkv_paged_evict_workspace_size(kv: *const tqkv_paged_kv, budget: i64) -> usize;
+    pub fn tqkv_paged_reserve(tables: *const tqkv_page_tables, counts: *const i32, tokens: i64, starts: *mut i32, granted: *mut i32, slots: *mut i32, stream: tqkv_stream) -> i32;
+    pub fn tqkv_paged_release(tables: *const tqkv_page_tables, keep: *const i32, shared: *const i32, stream: tqkv_stream) -> i32;
+    pub fn tqkv_rope_turns(config: *const tqkv_rope_config, turns: *mut u64, magnitude: *mut f32) -> i32;
+    pub fn tqkv_rope_apply(rope: *const tqkv_rope, positions: *const i32, position_stride: i64, tokens: i64, x: *const u16, heads: i32, dim: i32, x_token_stride: i64, x_head_stride: i64, out: *mut u16, out_token_stride: i64, out_head_stride: i64, stream: tqkv_stream) -> i32;
+    pub fn tqkv_paged_append_rope(kv: *const tqkv_paged_kv, rope: *const tqkv_rope, q: *const u16, H: i32, q_stride: i64, q_out: *mut u16, q_out_stride: i64, k: *const u16, v: *const u16, token_stride: i64, head_stride: i64, slots: *const i32, tokens: i64, positions: *const i32, position_stride: i64, stream: tqkv_stream) -> i32;
+    pub fn tqkv_packed_attend(q: *const u16, q_stride: i64, k: *const u16, v: *const u16, token_stride: i64, head_stride: i64, batch: i32, H: i32, H_kv: i32, D: i32, starts: *const i32, tokens: i64, scale: f32, causal: i32, window: i64, out: *mut u16, workspace: *mut c_void, workspace_bytes: usize, stream: tqkv_stream) -> i32;
+    pub fn tqkv_packed_attend_workspace_size(batch: i32, H: i32, H_kv: i32, D: i32, tokens: i64) -> usize;
+    pub fn tqkv_paged_prefill_attend(kv: *const tqkv_paged_kv, q: *const u16, q_stride: i64, H: i32, starts: *const i32, tokens: i64, scale: f32, window: i64, max_rows: i64, out: *mut u16, workspace: *mut c_void, workspace_bytes: usize, stream: tqkv_stream) -> i32;
+    pub fn tqkv_paged_prefill_workspace_size(kv: *const tqkv_paged_kv, H: i32, tokens: i64, max_rows: i64) -> usize;
     pub fn tqkv_decode_kernel_name(H: i32, H_kv: i32, D: i32, group_size: i32, bits_k: i32, bits_v: i32) -> *const c_char;
     pub fn tqkv_decode_kernel_for_rows(H: i32, H_kv: i32, D: i32, group_size: i32, bits_k: i32, bits_v: i32, max_rows: i64) -> *const c_char;
     pub fn tqkv_decode_attend_codebook(q: *const u16, B: i32, H: i32, H_kv: i32, D: i32, scale: f32, rotation: *const f32, centroids_k: *const f32, bits_k: i32, centroids_v: *const f32, bits_v: i32, k_codes: *const u8, k_sigma: *const f32, v_codes: *const u8, v_sigma: *const f32, cap: i64, n: i64, out: *mut u16, workspace: *mut c_void, workspace_bytes: usize, stream: tqkv_stream) -> i32;

@@ -76,6 +76,25 @@ class PagedKv(ctypes.Structure):
                 ("lens", P), ("weights", P)]
 
 
+class PageTables(ctypes.Structure):
+    _fields_ = [("batch", I32), ("page_rows", I32), ("num_pages", I64), ("table_stride", I64),
+                ("table", P), ("lens", P), ("free_pages", P), ("free_count", P)]
+
+
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BANDS, ROPE_RAMP = 0, 1, 2, 3, 4
+
+
+class RopeConfig(ctypes.Structure):
+    _fields_ = [("rotary_dim", I32), ("scaling", I32), ("base", ctypes.c_double),
+                ("factor", ctypes.c_double), ("original", ctypes.c_double),
+                ("low", ctypes.c_double), ("high", ctypes.c_double)]
+
+
+class Rope(ctypes.Structure):
+    _fields_ = [("rotary_dim", I32), ("interleaved", I32), ("magnitude", F32), ("reserved", I32),
+                ("turns", P)]
+
+
 class TqConfig(ctypes.Structure):
     _fields_ = [("head_dim", I32), ("bits", I32), ("qjl_m", I32), ("lloyd_max_iter", I32),
                 ("seed", ctypes.c_uint64)]
@@ -130,6 +149,19 @@ _SIGS = {
     "tqkv_paged_evict": (I32, [ctypes.POINTER(PagedKv), I64, I64, I64, P, I64, P, P, P, P, SZ,
                                P]),
     "tqkv_paged_evict_workspace_size": (SZ, [ctypes.POINTER(PagedKv), I64]),
+    "tqkv_paged_reserve": (I32, [ctypes.POINTER(PageTables), P, I64, P, P, P, P]),
+    "tqkv_paged_release": (I32, [ctypes.POINTER(PageTables), P, P, P]),
+    "tqkv_rope_turns": (I32, [ctypes.POINTER(RopeConfig), P, P]),
+    "tqkv_rope_apply": (I32, [ctypes.POINTER(Rope), P, I64, I64, P, I32, I32, I64, I64, P, I64,
+                              I64, P]),
+    "tqkv_paged_append_rope": (I32, [ctypes.POINTER(PagedKv), ctypes.POINTER(Rope), P, I32, I64,
+                                     P, I64, P, P, I64, I64, P, I64, P, I64, P]),
+    "tqkv_packed_attend": (I32, [P, I64, P, P, I64, I64, I32, I32, I32, I32, P, I64, F32, I32, I64,
+                                 P, P, SZ, P]),
+    "tqkv_packed_attend_workspace_size": (SZ, [I32, I32, I32, I32, I64]),
+    "tqkv_paged_prefill_attend": (I32, [ctypes.POINTER(PagedKv), P, I64, I32, P, I64, F32, I64,
+                                        I64, P, P, SZ, P]),
+    "tqkv_paged_prefill_workspace_size": (SZ, [ctypes.POINTER(PagedKv), I32, I64, I64]),
     "tqkv_synth_bf16": (I32, [P, I64, I32, ctypes.c_uint64, F32, F32, P]),
     "tqkv_lloyd_max": (I32, [ctypes.c_uint32, SZ, P, P]),
     "tqkv_rotation_matrix": (I32, [I32, ctypes.c_uint64, P]),
@@ -549,6 +581,74 @@ def paged_evict(kv, budget, sinks, recent, dst_table, dst_stride, dst_lens, dst_
 
 def paged_evict_workspace_size(kv, budget):
     return lib().tqkv_paged_evict_workspace_size(ctypes.byref(kv), budget)
+
+
+def page_tables(batch, page_rows, num_pages, table, table_stride, lens, free_pages, free_count):
+    """Device pointers of a paged cache's tables (tqkv_page_tables)."""
+    return PageTables(batch, page_rows, num_pages, table_stride, table, lens, free_pages,
+                      free_count)
+
+
+def paged_reserve(tables, counts, tokens, starts, granted=None, slots=None, stream=None):
+    check(lib().tqkv_paged_reserve(ctypes.byref(tables), counts, tokens, starts, granted, slots,
+                                   stream))
+
+
+def paged_release(tables, keep, shared=None, stream=None):
+    check(lib().tqkv_paged_release(ctypes.byref(tables), keep, shared, stream))
+
+
+def rope_turns(rotary_dim, base=10000.0, scaling=ROPE_PLAIN, factor=1.0, original=1.0, low=1.0,
+               high=4.0):
+    """(turns a position of each pair in units of 2^-64, magnitude): turns go
+    to the device as uint64 for `rope`."""
+    config = RopeConfig(rotary_dim, scaling, base, factor, original, low, high)
+    turns = (ctypes.c_uint64 * max(1, rotary_dim // 2))()
+    magnitude = ctypes.c_float()
+    check(lib().tqkv_rope_turns(ctypes.byref(config), turns, ctypes.byref(magnitude)))
+    return list(turns), magnitude.value
+
+
+def rope(rotary_dim, interleaved, magnitude, turns):
+    """turns: device pointer."""
+    return Rope(rotary_dim, int(interleaved), magnitude, 0, turns)
+
+
+def rope_apply(rope, positions, position_stride, tokens, x, heads, dim, x_token_stride,
+               x_head_stride, out, out_token_stride, out_head_stride, stream=None):
+    check(lib().tqkv_rope_apply(ctypes.byref(rope), positions, position_stride, tokens, x, heads,
+                                dim, x_token_stride, x_head_stride, out, out_token_stride,
+                                out_head_stride, stream))
+
+
+def paged_append_rope(kv, rope, q, H, q_stride, q_out, q_out_stride, k, v, token_stride,
+                      head_stride, slots, tokens, positions=None, position_stride=1, stream=None):
+    check(lib().tqkv_paged_append_rope(ctypes.byref(kv), ctypes.byref(rope), q, H, q_stride, q_out,
+                                       q_out_stride, k, v, token_stride, head_stride, slots,
+                                       tokens, positions, position_stride, stream))
+
+
+def packed_attend(q, q_stride, k, v, token_stride, head_stride, batch, H, H_kv, D, starts, tokens,
+                  scale, out, causal=True, window=-1, workspace=None, workspace_bytes=0,
+                  stream=None):
+    check(lib().tqkv_packed_attend(q, q_stride, k, v, token_stride, head_stride, batch, H, H_kv, D,
+                                   starts, tokens, scale, int(causal), window, out, workspace,
+                                   workspace_bytes, stream))
+
+
+def packed_attend_workspace_size(batch, H, H_kv, D, tokens):
+    return lib().tqkv_packed_attend_workspace_size(batch, H, H_kv, D, tokens)
+
+
+def paged_prefill_attend(kv, q, q_stride, H, starts, tokens, scale, max_rows, out, window=-1,
+                         workspace=None, workspace_bytes=0, stream=None):
+    check(lib().tqkv_paged_prefill_attend(ctypes.byref(kv), q, q_stride, H, starts, tokens, scale,
+                                          window, max_rows, out, workspace, workspace_bytes,
+                                          stream))
+
+
+def paged_prefill_workspace_size(kv, H, tokens, max_rows):
+    return lib().tqkv_paged_prefill_workspace_size(ctypes.byref(kv), H, tokens, max_rows)
 
 
 def tq_rotate_query(rotation, q, dim, rq, stream=None):
