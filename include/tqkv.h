@@ -611,7 +611,10 @@ size_t tqkv_packed_attend_workspace_size(int32_t batch, int32_t H, int32_t H_kv,
  * its rows up to their own position, with window > 0 the last `window` of
  * these. Rows of invalid pages get no attention; a query that sees no row
  * gets zeros. max_rows: the host's bound on lens, as tqkv_paged_decode_attend
- * takes it. Affine rows enter as tqkv_affine_dequantize's bf16 values.
+ * takes it. Affine keys enter as scale * code + bias in 11 bits or more, what is
+ * below 2^-28 of their head's largest with fewer, and a query's channels
+ * below 2^-28 of its largest alike; affine values as
+ * tqkv_affine_dequantize's bf16 ones.
  * kv->weights is not touched. q, out, H and the workspace as above; results
  * depend on starts, lens, tokens and max_rows, not on the run.
  */

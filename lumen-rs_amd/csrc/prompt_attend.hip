@@ -5,116 +5,208 @@ namespace tqkv {
 namespace prompt {
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
+// Affine rows of the sequences that have queries, dequantized once a KV head: K
+// as f16 (11 bits where bf16 keeps 8, the scores' largest error) times a power
+// of two that brings the head's largest value below 2^15, V as bf16. First
+// the largest |value| that a head's scales and biases allow.
+constexpr int kRangeParts = 32;
 
-// Channel c of a stored row as a bf16 value in f32; rows of `bits` codes are
-// dequantized to bf16, one rounding.
-template <Source S>
-__device__ __forceinline__ float value_at(const Args& a, bool key, int64_t row, int D, int c) {
-  if constexpr (S == kPacked) {
-    return bf16_to_f32((key ? a.k : a.v)[row + c]);
-  } else if constexpr (S == kPagedBf16) {
-    return bf16_to_f32(static_cast<const uint16_t*>(a.slot[key ? 0 : 1])[row * D + c]);
-  } else {
-    const int at = key ? 0 : 3, bits = key ? a.bits_k : a.bits_v;
-    const uint32_t w = static_cast<const uint32_t*>(a.slot[at])[row * (D * bits / 32) + c * bits / 32];
-    const uint32_t code = (w >> (c * bits % 32)) & ((1u << bits) - 1u);
-    const int64_t g = row * (D / a.gs) + c / a.gs;
-    const float s = bf16_to_f32(static_cast<const uint16_t*>(a.slot[at + 1])[g]);
-    const float b = bf16_to_f32(static_cast<const uint16_t*>(a.slot[at + 2])[g]);
-    return bf16_to_f32(f32_to_bf16(fmaf(s, float(code), b)));
-  }
+struct Rows {
+  int lo, n;  // rows [lo, n) are seen by some query
+};
+__device__ __forceinline__ Rows seen_rows(const Args& a, int b) {
+  const Sequence s = sequence<kPagedAffine>(a, b);
+  const int p = s.keys - s.count;
+  const int lo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+  return Rows{lo, s.count > 0 ? s.keys : 0};
 }
 
-// The row of key t: an element offset (packed) or a pool row; -1: none.
-template <Source S>
-__device__ __forceinline__ int64_t row_of(const Args& a, int b, int64_t first, int h, int t) {
-  if constexpr (S == kPacked) {
-    return (first + t) * a.ts + h * a.hs;
-  } else {
-    const int page = a.pool.table[b * a.pool.tstride + (t >> a.pool.shift)];
-    if (!paged::valid_page(a.pool, page)) return -1;
-    return paged::pool_row(a.pool, page, h, t & ((1 << a.pool.shift) - 1));
+__global__ __launch_bounds__(256) void range_kernel(const Args a, int D, float* part) {
+  __shared__ float tops[4];
+  const int h = blockIdx.y, b = blockIdx.z, groups = D / a.gs;
+  const Rows rows = seen_rows(a, b);
+  const int span = max(0, rows.n - rows.lo), each = (span + kRangeParts - 1) / kRangeParts;
+  const int from = rows.lo + int(blockIdx.x) * each, to = min(from + each, rows.n);
+  const uint16_t* scales = static_cast<const uint16_t*>(a.slot[1]);
+  const uint16_t* biases = static_cast<const uint16_t*>(a.slot[2]);
+  const float most = float((1 << a.bits_k) - 1);
+  float top = 0.0f;
+  for (int i = threadIdx.x; i < (to - from) * groups; i += 256) {
+    const int64_t row = row_of<kPagedAffine>(a, b, 0, h, from + i / groups);
+    if (row < 0) continue;
+    const int64_t g = row * groups + i % groups;
+    const float s = bf16_to_f32(scales[g]), z = bf16_to_f32(biases[g]);
+    top = fmaxf(top, fmaxf(fabsf(z), fabsf(fmaf(s, most, z))));
   }
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+  if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    part[(int64_t(b) * a.Hkv + h) * kRangeParts + blockIdx.x] =
+        fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 }
 
-// One query row by one wavefront: a lane a key for the scores, channels for
-// the values. Hidden keys are left out, not multiplied by zero.
-template <int D, Source S>
-__device__ void attend_row(const Args& a, int b, const Sequence& s, int64_t token, int head) {
-  const int lane = threadIdx.x % 64, h = head / a.G;
-  const int64_t p = int64_t(s.keys) - s.count + (token - s.first);
-  const Range see = visible(a, p, s.keys);
-  const uint16_t* q = a.q + token * a.qs + int64_t(head) * D;
-  constexpr int C = D / 64;
-  float o[C], m = -INFINITY, l = 0.0f;
-  bool any = false;
+// 32 codes of `bits` from w as f32.
+__device__ __forceinline__ void codes_of(const uint32_t* w, int bits, float (&f)[32]) {
+  if (bits == 8) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) o[c] = 0.0f;
-  for (int t0 = see.lo; t0 < see.hi; t0 += 64) {
-    const int t = t0 + lane;
-    const int64_t row = t < see.hi ? row_of<S>(a, b, s.first, h, t) : -1;
-    const bool on = t < see.hi && !(S != kPacked && row < 0);
-    float x = 0.0f;
-    if (on)
-      for (int c = 0; c < D; ++c) x = fmaf(bf16_to_f32(q[c]), value_at<S>(a, true, row, D, c), x);
-    x = on ? x * a.scale * kLog2e : -INFINITY;
-    const unsigned long long live = __ballot(on);
-    if (!live) continue;
-    any = true;
-    float top = x;
+    for (int i = 0; i < 32; ++i) f[i] = float((w[i / 4] >> (8 * (i % 4))) & 0xffu);
+  } else {
 #pragma unroll
-    for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-    const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
-    const float alpha = m == -INFINITY ? 0.0f : exp2f(m - base);
-    m = mn;
-    const float w = on ? exp2f(x - base) : 0.0f;
-    float sum = w;
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t e = w[k] & 0x0f0f0f0fu, o = (w[k] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
-    for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d, 64);
-    l = l * alpha + sum;
-#pragma unroll
-    for (int c = 0; c < C; ++c) o[c] *= alpha;
-    for (int i = 0; i < 64; ++i) {
-      if (!((live >> i) & 1)) continue;
-      const float wi = __shfl(w, i, 64);
-      const int64_t ri = __shfl(row, i, 64);
-#pragma unroll
-      for (int c = 0; c < C; ++c) o[c] = fmaf(wi, value_at<S>(a, false, ri, D, c * 64 + lane), o[c]);
+      for (int j = 0; j < 4; ++j) {
+        f[8 * k + 2 * j] = float((e >> (8 * j)) & 0xffu);
+        f[8 * k + 2 * j + 1] = float((o >> (8 * j)) & 0xffu);
+      }
     }
   }
-  uint16_t* out = a.out + (token * a.H + head) * D;
-  const float inv = any ? 1.0f / l : 0.0f;
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void slab_kernel(const Args a, const float* part, uint16_t* slab_k,
+                                                   uint16_t* slab_v, int32_t* exponent) {
+  constexpr int kRuns = D / 32;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const Rows rows = seen_rows(a, b);
+  const int t0 = int(blockIdx.x) * 64;
+  if (t0 + 64 <= rows.lo || t0 >= rows.n) return;
+  const int64_t unit = int64_t(b) * a.Hkv + h;
+  float top = 0.0f;
 #pragma unroll
-  for (int c = 0; c < C; ++c) out[c * 64 + lane] = f32_to_bf16(any ? o[c] * inv : 0.0f);
-}
-
-template <int D, Source S>
-__global__ __launch_bounds__(256) void row_kernel(const Args a) {
-  const int64_t unit = int64_t(blockIdx.x) * 4 + threadIdx.x / 64;
-  const int64_t token = unit / a.H;
-  if (token >= a.tokens || token < a.starts[0] || token >= a.starts[a.batch]) return;
-  int lo = 0, hi = a.batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (token >= a.starts[mid]) lo = mid;
-    else hi = mid;
+  for (int i = 0; i < kRangeParts; ++i) top = fmaxf(top, part[unit * kRangeParts + i]);
+  const int up = top > 0.0f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+  if (threadIdx.x == 0) exponent[unit] = -up;  // every block of the head writes the same
+  for (int i = threadIdx.x; i < 64 * kRuns; i += 256) {
+    const int t = t0 + i / kRuns, run = i % kRuns;
+    if (t >= rows.n) break;
+    const int64_t row = row_of<kPagedAffine>(a, b, 0, h, t);
+    uint32_t k[16] = {}, v[16] = {};
+    if (row >= 0) {
+      uint32_t w[8];
+      float f[32];
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        const int bits = side ? a.bits_v : a.bits_k, at = 3 * side;
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(a.slot[at]) + row * (D * bits / 32) + run * bits);
+        const uint4 x = src[0], y = bits == 8 ? src[1] : make_uint4(0, 0, 0, 0);
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
+        codes_of(w, bits, f);
+        const int64_t g = row * (D / a.gs) + 32 * run / a.gs;
+        const float s = bf16_to_f32(static_cast<const uint16_t*>(a.slot[at + 1])[g]);
+        const float z = bf16_to_f32(static_cast<const uint16_t*>(a.slot[at + 2])[g]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p = fmaf(s, f[2 * e], z), q = fmaf(s, f[2 * e + 1], z);
+          if (side) {
+            v[e] = pack_bf16(p, q);
+          } else {
+            typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+            const f2_t x2 = {ldexpf(p, up), ldexpf(q, up)};
+            k[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x2, h2_t));
+          }
+        }
+      }
+    }
+    uint4* kd = reinterpret_cast<uint4*>(slab_k + (unit * a.slab_rows + t) * D + 32 * run);
+    uint4* vd = reinterpret_cast<uint4*>(slab_v + (unit * a.slab_rows + t) * D + 32 * run);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      kd[e] = make_uint4(k[4 * e], k[4 * e + 1], k[4 * e + 2], k[4 * e + 3]);
+      vd[e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+    }
   }
-  attend_row<D, S>(a, lo, sequence<S>(a, lo), token, int(unit % a.H));
 }
 
-template <Source S>
-int32_t launch(const Args& a, int D, hipStream_t st) {
-  const int64_t blocks = (a.tokens * a.H + 3) / 4;
-  if (blocks > 0xffffffffLL / 256) return fail(TQKV_EUNSUPPORTED, "tokens=%lld", (long long)a.tokens);
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(256), 0, st, a);
-  };
+// What a call launches, and its workspace; false for what it refuses.
+struct Plan {
+  int ids, splits, split_keys;
+  int64_t slab_rows;                    // 0: no slab
+  size_t slab, exponents, parts, bytes; // bytes: of all
+};
+constexpr int64_t kWanted = 512;     // workgroups
+constexpr int64_t kLeastKeys = 512;  // of a split
+
+bool plan_of(int batch, int H, int Hkv, int D, int64_t tokens, int64_t keys, bool slab, Plan* out) {
+  const int64_t block = D <= 128 ? Shape<128>::kRows : D == 256 ? Shape<256>::kRows : Shape<512>::kRows;
+  const int G = H / Hkv;
+  const int64_t ids = tokens * G / block + batch;
+  Plan p{};
+  if (units_of(Hkv, ids) > 0xffffffffLL / 512) return false;  // a grid: below 2^32 threads
+  p.ids = int(ids);
+  const int64_t units = (tokens * G / block + (tokens < batch ? tokens : batch)) * Hkv;
+  int64_t n = units > 0 ? kWanted / units : 1;
+  if (n > keys / kLeastKeys) n = keys / kLeastKeys;
+  if (n < 1) n = 1;
+  const int64_t len = ((keys + n - 1) / n + 63) / 64 * 64;
+  p.splits = int((keys + len - 1) / len);
+  p.split_keys = int(len);
+  if (p.splits < 1) p.splits = 1;
+  const auto whole = [](size_t x) { return (x + 255) / 256 * 256; };
+  if (slab) {
+    p.slab_rows = keys;
+    p.slab = whole(size_t(batch) * Hkv * size_t(keys) * D * 2);
+    p.exponents = whole(size_t(batch) * Hkv * 4) + whole(size_t(batch) * Hkv * kRangeParts * 4);
+  }
+  if (p.splits > 1) p.parts = whole(size_t(tokens) * H * p.splits * (D + 2) * 4);
+  p.bytes = 2 * p.slab + p.exponents + p.parts;
+  *out = p;
+  return true;
+}
+
+int32_t attend(Args& a, int D, Source source, const Plan& p, void* workspace, size_t workspace_bytes,
+               hipStream_t st) {
+  if (p.bytes) {
+    if (!workspace) {
+      if (int32_t rc = scratch_for_current_device(p.bytes, &workspace)) return rc;
+    } else if (workspace_bytes < p.bytes || !paged::aligned(workspace, 16)) {
+      return fail(TQKV_EINVAL_ARG, "workspace of %zu bytes (16-byte aligned), need %zu",
+                  workspace_bytes, p.bytes);
+    }
+  }
+  a.ids = p.ids;
+  a.splits = p.splits;
+  a.split_keys = p.split_keys;
+  char* at = static_cast<char*>(workspace);
+  if (p.slab_rows) {
+    uint16_t* k = reinterpret_cast<uint16_t*>(at);
+    uint16_t* v = reinterpret_cast<uint16_t*>(at + p.slab);
+    at += 2 * p.slab;
+    int32_t* exponent = reinterpret_cast<int32_t*>(at);
+    float* part = reinterpret_cast<float*>(at + (size_t(a.batch) * a.Hkv * 4 + 255) / 256 * 256);
+    at += p.exponents;
+    a.slab_k = k;
+    a.slab_v = v;
+    a.exponent = exponent;
+    a.slab_rows = p.slab_rows;
+    hipLaunchKernelGGL(range_kernel, dim3(kRangeParts, a.Hkv, a.batch), dim3(256), 0, st, a, D, part);
+    TQKV_LAUNCHED();
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(unsigned((p.slab_rows + 63) / 64), a.Hkv, a.batch), dim3(256), 0,
+                         st, a, part, k, v, exponent);
+    };
+    switch (D) {
+      case 64: go(slab_kernel<64>); break;
+      case 128: go(slab_kernel<128>); break;
+      case 256: go(slab_kernel<256>); break;
+      default: go(slab_kernel<512>); break;
+    }
+    TQKV_LAUNCHED();
+  }
+  if (p.splits > 1) {
+    const size_t slots = size_t(a.tokens) * a.H * p.splits;
+    a.part_o = reinterpret_cast<float*>(at);
+    a.part_m = a.part_o + slots * D;
+    a.part_l = a.part_m + slots;
+  }
   switch (D) {
-    case 64: go(row_kernel<64, S>); break;
-    case 128: go(row_kernel<128, S>); break;
-    case 256: go(row_kernel<256, S>); break;
-    default: go(row_kernel<512, S>); break;
+    case 64: launch_prompt<64>(a, source, st); break;
+    case 128: launch_prompt<128>(a, source, st); break;
+    case 256: launch_prompt<256>(a, source, st); break;
+    default: launch_prompt<512>(a, source, st); break;
   }
   TQKV_LAUNCHED();
   return ok();
@@ -140,7 +232,13 @@ int32_t check_queries(const uint16_t* q, int64_t q_stride, int H, int H_kv, cons
 
 extern "C" size_t tqkv_packed_attend_workspace_size(int32_t batch, int32_t H, int32_t H_kv,
                                                     int32_t D, int64_t tokens) {
-  return 0;
+  using namespace tqkv::prompt;
+  Plan p;
+  if (batch < 1 || batch > tqkv::paged::kMaxBatch || !(D == 64 || D == 128 || D == 256 || D == 512) ||
+      H < 1 || H_kv < 1 || H % H_kv != 0 || H / H_kv > 32 || tokens < 1 || tokens > 0x7fffffffLL ||
+      !plan_of(batch, H, H_kv, D, tokens, tokens, false, &p))
+    return 0;
+  return p.bytes;
 }
 
 extern "C" int32_t tqkv_packed_attend(const uint16_t* q, int64_t q_stride, const uint16_t* k,
@@ -175,17 +273,28 @@ extern "C" int32_t tqkv_packed_attend(const uint16_t* q, int64_t q_stride, const
   a.G = H / H_kv;
   a.scale = scale;
   a.causal = causal != 0;
-  a.window = window > 0 ? window : 0;
+  a.window = window > 0 && window < 0x7fffffff ? int(window) : 0;
   a.k = k;
   a.v = v;
   a.ts = token_stride;
   a.hs = head_stride;
-  return launch<kPacked>(a, D, reinterpret_cast<hipStream_t>(stream));
+  Plan p;
+  if (!plan_of(batch, H, H_kv, D, tokens, tokens, false, &p))
+    return fail(TQKV_EUNSUPPORTED, "tokens=%lld", (long long)tokens);
+  return attend(a, D, kPacked, p, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" size_t tqkv_paged_prefill_workspace_size(const tqkv_paged_kv* kv, int32_t H,
                                                     int64_t tokens, int64_t max_rows) {
-  return 0;
+  using namespace tqkv::prompt;
+  tqkv::paged::Pool pool;
+  Plan p;
+  if (tqkv::paged::check(kv, &pool) != TQKV_OK || H < 1 || H % kv->kv_heads != 0 ||
+      H / kv->kv_heads > 32 || tokens < 1 || tokens > 0x7fffffffLL || max_rows < 1 ||
+      max_rows > pool.cap ||
+      !plan_of(kv->batch, H, kv->kv_heads, kv->dim, tokens, max_rows, kv->kind == TQKV_CACHE_AFFINE, &p))
+    return 0;
+  return p.bytes;
 }
 
 extern "C" int32_t tqkv_paged_prefill_attend(const tqkv_paged_kv* kv, const uint16_t* q,
@@ -212,13 +321,16 @@ extern "C" int32_t tqkv_paged_prefill_attend(const tqkv_paged_kv* kv, const uint
   a.G = H / kv->kv_heads;
   a.scale = scale;
   a.causal = 1;
-  a.window = window > 0 ? window : 0;
+  a.window = window > 0 && window < 0x7fffffff ? int(window) : 0;
   for (int i = 0; i < 6; ++i) a.slot[i] = kv->slot[i];
   a.gs = kv->group_size;
   a.bits_k = kv->bits_k;
   a.bits_v = kv->bits_v;
   a.max_rows = int(max_rows);
-  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  return kv->kind == TQKV_CACHE_BF16 ? launch<kPagedBf16>(a, kv->dim, st)
-                                     : launch<kPagedAffine>(a, kv->dim, st);
+  const bool affine = kv->kind == TQKV_CACHE_AFFINE;
+  Plan p;
+  if (!plan_of(kv->batch, H, kv->kv_heads, kv->dim, tokens, max_rows, affine, &p))
+    return fail(TQKV_EUNSUPPORTED, "tokens=%lld max_rows=%lld", (long long)tokens, (long long)max_rows);
+  return attend(a, kv->dim, affine ? kSlab : kPagedBf16, p, workspace, workspace_bytes,
+                reinterpret_cast<hipStream_t>(stream));
 }

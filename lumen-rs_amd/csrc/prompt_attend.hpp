@@ -1,6 +1,33 @@
-// Attention of packed sequences: what its kernels share. Keys and values are
-// rows of the same packed tokens, or of the paged cache.
+// Attention of packed sequences on the matrix cores: softmax(scale Q K^T +
+// mask) V for the queries of many sequences, keys and values out of the same
+// packed tokens, the pages of a bf16 pool, or a slab of dequantized rows.
+//
+// Work split: a block takes kRows rows of one (sequence, KV head); the G query
+// heads of a KV head share its keys, so rows are (position, head) pairs, head
+// fastest, and see nearly the same keys. Block ids count over the packed
+// tokens: sequence b's begin at starts[b] G / kRows + b, which leaves each at
+// least the ids that it needs (floor(x + y) - floor(x) + 1 >= ceil(y)), so a
+// block finds its sequence from starts alone and the host needs no lengths.
+// Later ids (later positions, more keys) run first, and the blocks of a KV
+// head on as few XCDs as that allows, since they read the same rows.
+//
+// Per tile of kKeys keys: K and V rows go straight from HBM into LDS, two
+// tiles ahead where LDS holds them, every 16-byte piece at a place of its row
+// that leaves the operand reads free of bank conflicts. A wavefront owns kRW
+// rows: S^T = K Q^T (Q in registers), online softmax per row, whose running
+// maximum may lag by kTau so that the accumulators are seldom rescaled, then
+// O^T += V^T P^T, the scores' registers being the operand's layout and V
+// transposed by the LDS read. Weights are rounded to bf16 (V keeps bf16's
+// range; f16 would keep three more bits of the weights and lose the range),
+// and the row sum counts them as rounded.
+//
+// Weights of hidden keys are exact zeros, but zero times an infinite value is
+// NaN: a row that ends with a NaN anywhere is done again, one key at a time,
+// by attend_row, which leaves hidden keys out.
 #pragma once
+
+#include <type_traits>
+#include <utility>
 
 #include "paged.hpp"
 
@@ -8,7 +35,7 @@ namespace tqkv {
 namespace prompt {
 
 // Where keys and values lie.
-enum Source { kPacked, kPagedBf16, kPagedAffine };
+enum Source { kPacked, kPagedBf16, kPagedAffine, kSlab };
 
 struct Args {
   const uint16_t* q;  // head h of token i at q + i * qs + h * D
@@ -19,7 +46,7 @@ struct Args {
   int batch, H, Hkv, G;
   float scale;
   int causal;
-  int64_t window;  // 0: none
+  int window;  // 0: none
   // kPacked: head h of token i at i * ts + h * hs.
   const uint16_t* k;
   const uint16_t* v;
@@ -28,7 +55,22 @@ struct Args {
   paged::Pool pool;
   const void* slot[6];
   int gs, bits_k, bits_v, max_rows;
+  // kSlab: rows [batch, Hkv, slab_rows, D], K as f16 times 2^-exponent[batch,
+  // Hkv], V as bf16.
+  const uint16_t* slab_k;
+  const uint16_t* slab_v;
+  const int32_t* exponent;
+  int64_t slab_rows;
+  // Block ids a KV head. Key splits: split s covers keys [s * split_keys,
+  // (s + 1) * split_keys); with part_o set a row's (o unnormalised, maximum in
+  // log2 units, sum) go to slot (token * H + head) * splits + s.
+  int ids, splits, split_keys;
+  float* part_o;
+  float* part_m;
+  float* part_l;
 };
+
+constexpr float kLog2e = 1.44269504088896340736f;
 
 // A sequence's queries [first, first + count) and the keys that it has.
 struct Sequence {
@@ -36,12 +78,14 @@ struct Sequence {
   int count, keys;
 };
 // starts is taken as ascending within [0, tokens]; what is not stays in bounds.
+__device__ __forceinline__ int64_t start_of(const Args& a, int b) {
+  const int64_t s = a.starts[b];
+  return s < 0 ? 0 : s < a.tokens ? s : a.tokens;
+}
 template <Source S>
 __device__ __forceinline__ Sequence sequence(const Args& a, int b) {
-  int64_t lo = a.starts[b], hi = a.starts[b + 1];
-  lo = lo < 0 ? 0 : lo < a.tokens ? lo : a.tokens;
-  hi = hi < lo ? lo : hi < a.tokens ? hi : a.tokens;
-  const int count = int(hi - lo);
+  const int64_t lo = start_of(a, b), hi = start_of(a, b + 1);
+  const int count = int(hi < lo ? 0 : hi - lo);
   if constexpr (S == kPacked) return Sequence{lo, count, count};
   return Sequence{lo, count, paged::held(a.pool, b, a.max_rows)};
 }
@@ -58,6 +102,628 @@ __device__ __forceinline__ Range visible(const Args& a, int64_t p, int n) {
   }
   if (hi < 0) hi = 0;
   return Range{int(lo < hi ? lo : hi), int(hi)};
+}
+
+// Channel c of a stored row in f32; values of affine rows are rounded to bf16,
+// keys are not (their f16 operands keep 11 bits).
+template <Source S>
+__device__ __forceinline__ float value_at(const Args& a, bool key, int64_t row, int D, int c) {
+  if constexpr (S == kPacked) {
+    return bf16_to_f32((key ? a.k : a.v)[row + c]);
+  } else if constexpr (S == kPagedBf16) {
+    return bf16_to_f32(static_cast<const uint16_t*>(a.slot[key ? 0 : 1])[row * D + c]);
+  } else {
+    const int at = key ? 0 : 3, bits = key ? a.bits_k : a.bits_v;
+    const uint32_t w = static_cast<const uint32_t*>(a.slot[at])[row * (D * bits / 32) + c * bits / 32];
+    const uint32_t code = (w >> (c * bits % 32)) & ((1u << bits) - 1u);
+    const int64_t g = row * (D / a.gs) + c / a.gs;
+    const float s = bf16_to_f32(static_cast<const uint16_t*>(a.slot[at + 1])[g]);
+    const float b = bf16_to_f32(static_cast<const uint16_t*>(a.slot[at + 2])[g]);
+    const float x = fmaf(s, float(code), b);
+    return key ? x : bf16_to_f32(f32_to_bf16(x));
+  }
+}
+
+// The row of key t: an element offset (packed) or a pool row; -1: none.
+template <Source S>
+__device__ __forceinline__ int64_t row_of(const Args& a, int b, int64_t first, int h, int t) {
+  if constexpr (S == kPacked) {
+    return (first + t) * a.ts + h * a.hs;
+  } else {
+    const int page = a.pool.table[b * a.pool.tstride + (t >> a.pool.shift)];
+    if (!paged::valid_page(a.pool, page)) return -1;
+    return paged::pool_row(a.pool, page, h, t & ((1 << a.pool.shift) - 1));
+  }
+}
+
+// One query row by one wavefront, in f32: a lane a key for the scores,
+// channels for the values. Hidden keys are left out, not multiplied by zero.
+template <int D, Source S>
+__device__ __forceinline__ void attend_row(const Args& a, int b, int64_t token, int head) {
+  const Sequence s = sequence<S>(a, b);
+  const int lane = threadIdx.x % 64, h = head / a.G;
+  const int64_t p = int64_t(s.keys) - s.count + (token - s.first);
+  const Range see = visible(a, p, s.keys);
+  const uint16_t* q = a.q + token * a.qs + int64_t(head) * D;
+  constexpr int C = D / 64;
+  float o[C], m = -INFINITY, l = 0.0f;
+  bool any = false;
+#pragma unroll
+  for (int c = 0; c < C; ++c) o[c] = 0.0f;
+  for (int t0 = see.lo; t0 < see.hi; t0 += 64) {
+    const int t = t0 + lane;
+    const int64_t row = t < see.hi ? row_of<S>(a, b, s.first, h, t) : -1;
+    const bool on = t < see.hi && !(S != kPacked && row < 0);
+    float x = 0.0f;
+    if (on)
+#pragma unroll 4
+      for (int c = 0; c < D; ++c) x = fmaf(bf16_to_f32(q[c]), value_at<S>(a, true, row, D, c), x);
+    x = on ? x * a.scale * kLog2e : -INFINITY;
+    const unsigned long long live = __ballot(on);
+    if (!live) continue;
+    any = true;
+    float top = x;
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
+    const float alpha = m == -INFINITY ? 0.0f : exp2f(m - base);
+    m = mn;
+    const float w = on ? exp2f(x - base) : 0.0f;
+    float sum = w;
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d, 64);
+    l = l * alpha + sum;
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] *= alpha;
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i) {
+      if (!((live >> i) & 1)) continue;
+      const float wi = __shfl(w, i, 64);
+      const int64_t ri = __shfl(row, i, 64);
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] = fmaf(wi, value_at<S>(a, false, ri, D, c * 64 + lane), o[c]);
+    }
+  }
+  uint16_t* out = a.out + (token * a.H + head) * D;
+  const float inv = any ? 1.0f / l : 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) out[c * 64 + lane] = f32_to_bf16(any ? o[c] * inv : 0.0f);
+}
+
+// ------------------------------------------------------------- matrix cores
+constexpr int kWave = 64;
+constexpr int kXcds = 8;
+constexpr float kTau = 8.0f;
+
+typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+
+// Launch shapes. Late: the second wavefront of each SIMD multiplies by V one
+// tile late, so that one's softmax meets the other's products.
+template <int D>
+struct Shape {
+  static constexpr int kWaves = 8;
+  static constexpr int kRW = D <= 128 ? 32 : 16;       // rows a wavefront
+  static constexpr int kKeys = D <= 128 ? 64 : 32;     // keys a tile
+  static constexpr bool kLate = D <= 256;
+  static constexpr int kAhead = D <= 256 ? 2 : 1;      // tiles in flight
+  static constexpr int kKBufs = kAhead + 1, kVBufs = kAhead + 1 + (kLate ? 1 : 0);
+  static constexpr int kRows = kWaves * kRW;
+  static constexpr int kThreads = kWaves * kWave;
+  static constexpr int kPieces = kKeys * D * 2 / 1024 / kWaves;  // 1 KB pieces of K (of V) a wavefront
+  static_assert(kPieces >= 1 && (kKBufs + kVBufs) * kKeys * D * 2 <= 160 * 1024, "LDS");
+};
+
+// The place of 16-byte piece c in row r of a tile: rows that fall on the same
+// LDS banks (256 / D rows cover them) are turned against each other by two
+// pieces, which 16 rows x 2 pieces (K) and 8 rows x 2 pieces (V) read at once
+// need.
+template <int D>
+__device__ __forceinline__ int turn_of(int r) {
+  constexpr int n = D >= 256 ? 1 : 256 / D;
+  return 2 * ((r / n) & (16 / n - 1));
+}
+
+// 16 bytes from each lane's src to LDS [lds + 16 lane, + 16). As assembly, so
+// that the compiler does not make later LDS reads wait for it; the kernel
+// waits (vmcnt) before the barrier that publishes a tile. M0 holds the LDS
+// address, and its write needs a wait state before the load reads it.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void to_lds(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return uint32_t(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
+}
+// At most N of the wavefront's loads outstanding.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
+__device__ __forceinline__ u2_t read_transposed(const uint16_t* p) {
+  return __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                      (__attribute__((address_space(3))) s4_t*)(p)));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+  const f2_t f = {x, y};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf2_t));
+}
+__device__ __forceinline__ bf2_t as_bf2(uint32_t x) { return __builtin_bit_cast(bf2_t, x); }
+// acc + both halves of a packed pair.
+__device__ __forceinline__ float add_two(uint32_t w, float acc) {
+  const bf2_t one = {__bf16(1.0f), __bf16(1.0f)};
+  return __builtin_amdgcn_fdot2_f32_bf16(as_bf2(w), one, acc, false);
+}
+// Lane l with lanes l ^ 16 and l ^ 32 (the lanes of one row).
+__device__ __forceinline__ float max_of(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ float row_max(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = max_of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return max_of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float row_sum(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Keeps a block that few tiles take behind its branch.
+__device__ __forceinline__ void rare() { asm volatile(""); }
+
+// What rows of pages that are none read instead.
+__device__ const uint4 kZeroRow[64] = {};
+
+// The id-th block of KV head h, of `ids`: later ids first, a KV head's blocks
+// on 8 / Hkv XCDs (workgroup i runs on XCD i % 8), several heads on one where
+// there are more.
+struct Unit {
+  int head, id;
+};
+__device__ __forceinline__ Unit unit_of(const Args& a, int i) {
+  int h, t;
+  if (a.Hkv % kXcds == 0) {
+    const int j = i / kXcds;
+    h = i % kXcds + kXcds * (j / a.ids);
+    t = j % a.ids;
+  } else if (kXcds % a.Hkv == 0) {
+    const int f = kXcds / a.Hkv;
+    h = i % kXcds / f;
+    t = i / kXcds * f + i % f;
+  } else {
+    h = i % a.Hkv;
+    t = i / a.Hkv;
+  }
+  return Unit{h, a.ids - 1 - t};
+}
+// Workgroups of that (host).
+inline int64_t units_of(int Hkv, int64_t ids) {
+  if (Hkv < kXcds && kXcds % Hkv == 0) {
+    const int f = kXcds / Hkv;
+    return (ids + f - 1) / f * kXcds;
+  }
+  return ids * Hkv;
+}
+
+template <int D, Source S>
+__global__ __launch_bounds__(Shape<D>::kThreads)
+__attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(const Args a) {
+  typedef Shape<D> W;
+  constexpr int kWaves = W::kWaves, RW = W::kRW, NR = RW / 16, KT = W::kKeys, NI = KT / 16;
+  constexpr int ND = D / 32, NT = D / 16, NU = KT / 32, NP = W::kPieces;
+  constexpr bool F16 = S == kSlab;
+  __shared__ __attribute__((aligned(16))) uint16_t tiles[W::kKBufs + W::kVBufs][KT * D];
+  const int tid = threadIdx.x, lane = tid % kWave, lr = lane % 16, lg = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+
+  // The block's sequence and rows.
+  const Unit unit = unit_of(a, int(blockIdx.x));
+  if (unit.id < 0) return;
+  const int kvh = unit.head;
+  int b = -1, begin = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kWave) {
+    const int i = b0 + lane;
+    const int64_t at = i < a.batch ? start_of(a, i) * a.G / W::kRows + i : 0;
+    const unsigned long long on = __ballot(i < a.batch && at <= unit.id);
+    if (!on) break;
+    const int last = 63 - __clzll(on);
+    b = b0 + last;
+    begin = __shfl(int(at), last, 64);  // below 2^29
+    if (last < kWave - 1) break;
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  begin = __builtin_amdgcn_readfirstlane(begin);
+  if (b < 0) return;
+  Sequence seq = sequence<S>(a, b);
+  // Alike in every lane; said so, the tile loop runs on scalars.
+  seq.first = __builtin_amdgcn_readfirstlane(int(seq.first));
+  seq.count = __builtin_amdgcn_readfirstlane(seq.count);
+  seq.keys = __builtin_amdgcn_readfirstlane(seq.keys);
+  const int64_t rows = int64_t(seq.count) * a.G;
+  const int64_t row0 = int64_t(unit.id - begin) * W::kRows;
+  if (row0 >= rows) return;
+  const int64_t row_end = row0 + W::kRows < rows ? row0 + W::kRows : rows;
+  const int n = seq.keys, p0 = n - seq.count;  // p0: the first query's position
+  const int pos_lo = p0 + int(row0 / a.G), pos_hi = p0 + int((row_end - 1) / a.G);
+  const int split = blockIdx.y;
+  // Keys that some row of the block sees, within the split.
+  int key_lo = split * a.split_keys, key_hi = n;
+  if (n - key_lo > a.split_keys) key_hi = key_lo + a.split_keys;
+  if (a.causal) {
+    if (pos_hi + 1 < key_hi) key_hi = pos_hi + 1;
+    if (a.window > 0 && pos_lo - a.window + 1 > key_lo) key_lo = pos_lo - a.window + 1;
+  }
+  if (a.part_o && key_lo >= key_hi) return;  // the join leaves such splits out
+
+  using op_t = std::conditional_t<F16, h8_t, bf8_t>;
+  op_t qf[NR][ND];
+  int pos[NR];       // of this lane's rows
+  float qscale[NR];  // scores to log2 units
+  const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+  auto row_at = [&](int j) __attribute__((always_inline)) { return row0 + wave * RW + 16 * j + lr; };
+#pragma unroll
+  for (int j = 0; j < NR; ++j) {
+    const int64_t r = row_at(j) < rows ? row_at(j) : rows - 1;
+    pos[j] = p0 + int(r / a.G);
+    const uint16_t* src = a.q + (seq.first + r / a.G) * a.qs + (int64_t(kvh) * a.G + r % a.G) * D;
+    qscale[j] = a.scale * sign * kLog2e;
+    u4_t x[ND];
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int s = 0; s < ND; ++s) {
+      x[s] = *reinterpret_cast<const u4_t*>(src + 32 * s + 8 * lg);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[s][e] ^= flip;
+      if constexpr (!F16) qf[j][s] = __builtin_bit_cast(bf8_t, x[s]);
+    }
+    if constexpr (F16) {
+      // The row as f16, its largest channel in [2^14, 2^15): channels below
+      // 2^-28 of it lose bits.
+      float top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < ND; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          top = fmaxf(top, fabsf(__uint_as_float(x[s][e] << 16)));
+          top = fmaxf(top, fabsf(__uint_as_float(x[s][e] & 0xffff0000u)));
+        }
+      top = row_max(top);
+      const int e2 = top > 0.0f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+      for (int s = 0; s < ND; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          qf[j][s][2 * e] = _Float16(ldexpf(__uint_as_float(x[s][e] << 16), e2));
+          qf[j][s][2 * e + 1] = _Float16(ldexpf(__uint_as_float(x[s][e] & 0xffff0000u), e2));
+        }
+      qscale[j] = ldexpf(qscale[j], a.exponent[b * a.Hkv + kvh] - e2);
+    }
+  }
+
+  // Per row: the running maximum (log2 units), its negative (0 while no key
+  // was seen), and the raw score above which it must move.
+  float m[NR], nm[NR], thr[NR], lsum[NR];
+  f4_t o[NT][NR];
+#pragma unroll
+  for (int j = 0; j < NR; ++j) {
+    m[j] = thr[j] = -INFINITY;
+    nm[j] = lsum[j] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  if (key_lo < key_hi) {
+    const int t_lo = key_lo / KT, t_hi = (key_hi - 1) / KT;
+    // This wavefront's pieces of a tile: piece i is rows [first row of it,
+    // + 512 / D), lane l of it fills place l % (D / 8) of its row, which holds
+    // the piece of the row that turn_of puts there.
+    constexpr int kPieceRows = 512 / D, kRowPieces = D / 8;
+    const int lrow = lane / kRowPieces;
+    auto page_of = [&](int t) __attribute__((always_inline)) {
+      // The tables are written by no one while the kernel runs.
+      typedef const __attribute__((address_space(4))) int32_t* constant;
+      return ((constant)(a.pool.table + b * a.pool.tstride))[t >> a.pool.shift];
+    };
+    // Rows past the last key read that one again: hidden, and finite where it
+    // is.
+    auto fetch = [&](int tile, int kb, int vb) __attribute__((always_inline)) {
+      const int tc = tile < t_hi ? tile : t_hi;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int piece = wave * NP + i;
+        const int r = piece * kPieceRows + lrow;  // row in the tile
+        const int t = min(tc * KT + r, n - 1);
+        const int c = ((lane % kRowPieces) ^ turn_of<D>(r)) * 8;
+        const uint16_t *ks, *vs;
+        if constexpr (S == kPacked) {
+          const int64_t at = (seq.first + t) * a.ts + kvh * a.hs + c;
+          ks = a.k + at;
+          vs = a.v + at;
+        } else if constexpr (S == kSlab) {
+          const int64_t at = ((int64_t(b) * a.Hkv + kvh) * a.slab_rows + t) * D + c;
+          ks = a.slab_k + at;
+          vs = a.slab_v + at;
+        } else {
+          // A piece's rows lie in one page (of 16 rows or more).
+          const int page = page_of(min(tc * KT + piece * kPieceRows, n - 1));
+          const bool ok = paged::valid_page(a.pool, page);
+          const int64_t at = paged::pool_row(a.pool, ok ? page : 0, kvh, t & ((1 << a.pool.shift) - 1)) * D + c;
+          const uint16_t* zero = reinterpret_cast<const uint16_t*>(kZeroRow) + c;
+          ks = ok ? static_cast<const uint16_t*>(a.slot[0]) + at : zero;
+          vs = ok ? static_cast<const uint16_t*>(a.slot[1]) + at : zero;
+        }
+        to_lds(ks, __builtin_amdgcn_readfirstlane(lds_address(tiles[kb])) + piece * 1024);
+        to_lds(vs, __builtin_amdgcn_readfirstlane(lds_address(tiles[W::kKBufs + vb])) + piece * 1024);
+      }
+    };
+    // Which of the tile's groups of 16 keys lie in pages.
+    auto held_groups = [&](int tile) __attribute__((always_inline)) {
+      uint32_t on = 0xffu;
+      if constexpr (S == kPagedBf16 || S == kSlab) {
+        on = 0;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+          if (paged::valid_page(a.pool, page_of(min(tile * KT + 16 * i, n - 1)))) on |= 1u << i;
+      }
+      return on;
+    };
+    // Operand reads: K piece 4 s + lg of row lr (+ 16 i rows), V piece 2 t +
+    // (lr / 2) % 2 of row 4 lg + lr / 4 (+ 16, 32 u rows).
+    const int kturn = turn_of<D>(lr), vturn = turn_of<D>(4 * lg + lr / 4);
+    const bool live = row0 + wave * RW < rows;
+
+    auto rescale = [&](int j, bool up, float mx) __attribute__((always_inline)) {
+      const float mn = up ? mx * qscale[j] : m[j];
+      const float alpha = up ? __builtin_amdgcn_exp2f(m[j] - mn) : 1.0f;
+      lsum[j] *= alpha;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) o[t][j] *= alpha;
+      m[j] = mn;
+      nm[j] = mn == -INFINITY ? 0.0f : -mn;
+      thr[j] = (mn + kTau) / qscale[j];
+    };
+    auto scores = [&](const uint16_t* K, f4_t (&sc)[NI][NR]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NR; ++j) sc[i][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < ND; ++s)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const op_t ka = *reinterpret_cast<const op_t*>(K + (16 * i + lr) * D + ((4 * s + lg) ^ kturn) * 8);
+#pragma unroll
+          for (int j = 0; j < NR; ++j) {
+            if constexpr (F16)
+              sc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[j][s], sc[i][j], 0, 0, 0);
+            else
+              sc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[j][s], sc[i][j], 0, 0, 0);
+          }
+        }
+    };
+    auto softmax = [&](int tile, f4_t (&sc)[NI][NR], bf8_t (&pp)[NU][NR]) __attribute__((always_inline)) {
+      const int kbase = tile * KT;
+      // Hidden keys, where the block sees the tile in part.
+      const uint32_t on = held_groups(tile);
+      const bool whole = kbase >= key_lo && kbase + KT <= key_hi && on == (S == kPacked ? 0xffu : (1u << NI) - 1u) &&
+                         (!a.causal || (kbase + KT - 1 <= pos_lo && (a.window <= 0 || pos_hi - a.window < kbase)));
+      if (!whole) {
+        rare();
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+          int hi = key_hi - kbase, lo = key_lo - kbase;  // visible: [lo, hi)
+          if (a.causal) {
+            hi = min(hi, pos[j] + 1 - kbase);
+            if (a.window > 0) lo = max(lo, pos[j] - a.window + 1 - kbase);
+          }
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int k = 16 * i + 4 * lg + r;
+              if (k < lo || k >= hi || !((on >> i) & 1)) sc[i][j][r] = -INFINITY;
+            }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NR; ++j) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[i][j][r]);
+        if (__any(mx > thr[j])) {
+          rare();
+          mx = row_max(mx);
+          rescale(j, mx > thr[j], mx);
+        }
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          u4_t w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f4_t s = sc[2 * u + e / 2][j];
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2)], qscale[j], nm[j]));
+            const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2) + 1], qscale[j], nm[j]));
+            w[e] = pack_bf16(x, y);
+            lsum[j] = add_two(w[e], lsum[j]);
+          }
+          pp[u][j] = __builtin_bit_cast(bf8_t, w);
+        }
+      }
+    };
+    auto values = [&](const bf8_t (&pp)[NU][NR], const uint16_t* V) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const uint16_t* src = V + (32 * u + 4 * lg + lr / 4) * D + ((2 * t + lr % 4 / 2) ^ vturn) * 8 + 4 * (lr % 2);
+          const u2_t x = read_transposed(src), y = read_transposed(src + 16 * D);
+          const bf8_t va = __builtin_bit_cast(bf8_t, u4_t{x.x, x.y, y.x, y.y});
+#pragma unroll
+          for (int j = 0; j < NR; ++j)
+            o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pp[u][j], o[t][j], 0, 0, 0);
+        }
+    };
+
+    auto run = [&](auto late) __attribute__((always_inline)) {
+      constexpr bool LATE = decltype(late)::value;
+      wait_loads<0>();  // the queries
+      fetch(t_lo, 0, 0);
+      if constexpr (W::kAhead == 2) fetch(t_lo + 1, 1, 1);
+      wait_loads<(W::kAhead - 1) * 2 * NP>();
+      __syncthreads();
+      bf8_t pp[NU][NR];
+      int kc = 0, vc = 0;
+      const auto plus = [](int c, int d, int bufs) { return c + d >= bufs ? c + d - bufs : c + d; };
+      for (int tile = t_lo; tile <= t_hi; ++tile) {
+        // Into buffers last read before the barrier that ended the tile before.
+        fetch(tile + W::kAhead, plus(kc, W::kAhead, W::kKBufs), plus(vc, W::kAhead, W::kVBufs));
+        if (live) {
+          if constexpr (W::kLate) __builtin_amdgcn_s_setprio(1);
+          if constexpr (LATE)
+            if (tile > t_lo) values(pp, tiles[W::kKBufs + plus(vc, W::kVBufs - 1, W::kVBufs)]);
+          f4_t sc[NI][NR];
+          scores(tiles[kc], sc);
+          if constexpr (W::kLate) __builtin_amdgcn_s_setprio(0);
+          softmax(tile, sc, pp);
+          if constexpr (!LATE) {
+            if constexpr (W::kLate) __builtin_amdgcn_s_setprio(1);
+            values(pp, tiles[W::kKBufs + vc]);
+            if constexpr (W::kLate) __builtin_amdgcn_s_setprio(0);
+          }
+        }
+        wait_loads<(W::kAhead - 1) * 2 * NP>();
+        __syncthreads();
+        kc = plus(kc, 1, W::kKBufs);
+        vc = plus(vc, 1, W::kVBufs);
+      }
+      if constexpr (LATE)
+        if (live) values(pp, tiles[W::kKBufs + plus(vc, W::kVBufs - 1, W::kVBufs)]);
+      wait_loads<0>();  // before the workgroup's LDS is given back
+    };
+    if (W::kLate && wave >= kWaves / 2) run(std::true_type{});
+    else run(std::false_type{});
+  }
+
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < NR; ++j) {
+    const float sum = row_sum(lsum[j]);
+    const int64_t r = row_at(j);
+    if (r >= rows) continue;
+    const int64_t row = (seq.first + r / a.G) * a.H + int64_t(kvh) * a.G + r % a.G;
+    if (a.part_o) {
+      const int64_t slot = row * a.splits + split;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        *reinterpret_cast<f4_t*>(a.part_o + slot * D + 16 * t + 4 * lg) = o[t][j];
+      if (lg == 0) {
+        a.part_m[slot] = m[j];
+        a.part_l[slot] = sum;
+      }
+      continue;
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    bad |= !(sum > 0.0f);  // no key, or none of a score above -infinity
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const f4_t v = o[t][j] * inv;
+      bad |= !(v[0] == v[0] && v[1] == v[1] && v[2] == v[2] && v[3] == v[3]);
+      *reinterpret_cast<u2_t*>(a.out + row * D + 16 * t + 4 * lg) = u2_t{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+    }
+  }
+  if (__any(bad)) {
+    rare();
+    constexpr Source R = S == kSlab ? kPagedAffine : S;
+#pragma unroll 1
+    for (int i = 0; i < RW; ++i) {
+      const int64_t r = row0 + wave * RW + i;
+      if (r >= rows) break;
+      attend_row<D, R>(a, b, seq.first + r / a.G, kvh * a.G + int(r % a.G));
+    }
+  }
+}
+
+// Joins the splits of one (token, head) row a wavefront: those that its own
+// keys meet, which its block has written.
+constexpr int kJoinThreads = 256;
+
+template <int D, Source S>
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(const Args a) {
+  const int lane = threadIdx.x % kWave;
+  const int64_t unit = int64_t(blockIdx.x) * (kJoinThreads / kWave) + threadIdx.x / kWave;
+  const int64_t token = unit / a.H;
+  const int head = int(unit % a.H);
+  if (token >= a.tokens || token < start_of(a, 0) || token >= start_of(a, a.batch)) return;
+  int b = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kWave) {
+    const unsigned long long on = __ballot(b0 + lane < a.batch && start_of(a, min(b0 + lane, a.batch - 1)) <= token);
+    if (!on) break;
+    b = b0 + 63 - __clzll(on);
+  }
+  const Sequence seq = sequence<S>(a, b);
+  if (token >= seq.first + seq.count) return;  // starts that do not ascend
+  const Range see = visible(a, int64_t(seq.keys) - seq.count + (token - seq.first), seq.keys);
+  const int64_t slot0 = (token * a.H + head) * a.splits;
+  constexpr int C = D / kWave;
+  float o[C], m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) o[c] = 0.0f;
+  if (see.lo < see.hi) {
+    const int s0 = see.lo / a.split_keys, s1 = (see.hi - 1) / a.split_keys;
+    for (int s = s0; s <= s1; ++s) m = fmaxf(m, a.part_m[slot0 + s]);
+    for (int s = s0; s <= s1; ++s) {
+      const float ms = a.part_m[slot0 + s], f = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - m);
+      l = fmaf(f, a.part_l[slot0 + s], l);
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] = fmaf(f, a.part_o[(slot0 + s) * D + c * kWave + lane], o[c]);
+    }
+  }
+  const float inv = 1.0f / l;
+  bool bad = !(l > 0.0f);
+  uint16_t* out = a.out + (token * a.H + head) * D;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const float v = o[c] * inv;
+    bad |= !(v == v);
+    out[c * kWave + lane] = f32_to_bf16(v);
+  }
+  constexpr Source R = S == kSlab ? kPagedAffine : S;
+  if (__any(bad)) attend_row<D, R>(a, b, token, head);
+}
+
+// Launches prompt_kernel<D, S> and, for split keys, the join. Defined a head
+// dim a file.
+template <int D>
+void launch_prompt(const Args& a, Source s, hipStream_t st);
+
+template <int D, Source S>
+void launch_source(const Args& a, hipStream_t st) {
+  hipLaunchKernelGGL((prompt_kernel<D, S>), dim3(unsigned(units_of(a.Hkv, a.ids)), unsigned(a.splits)),
+                     dim3(Shape<D>::kThreads), 0, st, a);
+  if (a.part_o)
+    hipLaunchKernelGGL((join_kernel<D, S>), dim3(unsigned((a.tokens * a.H + 3) / 4)), dim3(kJoinThreads), 0, st, a);
+}
+template <int D>
+void launch_prompt(const Args& a, Source s, hipStream_t st) {
+  if (s == kPacked) launch_source<D, kPacked>(a, st);
+  else if (s == kPagedBf16) launch_source<D, kPagedBf16>(a, st);
+  else launch_source<D, kSlab>(a, st);
 }
 
 }  // namespace prompt

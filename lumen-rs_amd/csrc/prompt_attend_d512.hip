@@ -1,0 +1,8 @@
+// Attention of packed sequences, head dim 512.
+#include "prompt_attend.hpp"
+
+namespace tqkv {
+namespace prompt {
+template void launch_prompt<512>(const Args&, Source, hipStream_t);
+}  // namespace prompt
+}  // namespace tqkv

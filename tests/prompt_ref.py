@@ -6,7 +6,7 @@ import math
 import numpy as np
 
 import oracle_lib as O
-from paged_ref import codes_of
+from paged_ref import codes_of, values_of
 
 
 # ------------------------------------------------------------------- tables
@@ -124,7 +124,7 @@ def rotated(x, positions, theta, magnitude, interleaved):
 
 # ---------------------------------------------------------------- attention
 def bf16_values(side, bits, gs):
-    """f64 of the bf16 values that stored rows are attended as: bf16 rows, or
+    """f64 of the bf16 values that stored V rows are attended as: bf16 rows, or
     scale * code + bias rounded to f32 (the fused multiply-add) and to bf16."""
     if bits == 16:
         return O.bf16_to_f32(side[0]).astype(np.float64)
@@ -133,9 +133,10 @@ def bf16_values(side, bits, gs):
     return O.bf16_to_f32(O.bf16_from_f32(x)).astype(np.float64)
 
 
-def attend(q, k, v, at, scale, causal=True, window=-1, ok=None):
+def attend(q, k, v, at, scale, causal=True, window=-1, ok=None, off=0.0):
     """One sequence and one KV head: q f64 [m, G, D] at positions `at`, k and v
-    f64 [n, D], ok: keys that can be seen at all. (out, tolerance) f64.
+    f64 [n, D], ok: keys that can be seen at all, off: how far a key's channel
+    may be from k, relative to it. (out, tolerance) f64.
 
     Tolerance: half a bf16 step of the output (2^-8 of it); the weights'
     rounding to bf16, 2^-8 each at most, which the sum of the rounded weights
@@ -161,7 +162,9 @@ def attend(q, k, v, at, scale, causal=True, window=-1, ok=None):
         w = np.exp(s - s.max(-1, keepdims=True))
         w /= w.sum(-1, keepdims=True)
         out[i] = w @ vs
-        sums = (D + 16) * 2.0 ** -24 * (np.abs(q[i]) @ np.abs(ks).T).max(-1) * abs(scale)
+        sums = ((D + 16) * 2.0 ** -24 + off) * (np.abs(q[i]) @ np.abs(ks).T).max(-1) * abs(scale)
+        if off:  # f16's subnormals: 2^-25 where the largest is 2^14 or more
+            sums = sums + 2.0 ** -39 * np.abs(k).max() * np.abs(q[i]).sum(-1) * abs(scale)
         d = 2 * (sums + 2.0 ** -22 * (np.abs(s).max(-1) + 4)) + see.sum() * 2.0 ** -24
         for g in range(G):
             spread = w[g] @ np.abs(vs - out[i, g])
@@ -199,9 +202,11 @@ def paged(p, q, starts, scale, window=-1, max_rows=None):
         ok = (page >= 0) & (page < p.pages)
         for h in range(p.Hkv):
             at = (np.where(ok, page, 0), h, r % p.R)
-            k = bf16_values([t[at] for t in p.sides[0]], p.bk, p.gs)
+            # Affine keys: scale * code + bias (an f32 fused multiply-add, 2^-24) as f16, 2^-11.
+            k = values_of([t[at] for t in p.sides[0]], p.bk, p.gs)
+            k[~ok] = 0.0
             v = bf16_values([t[at] for t in p.sides[1]], p.bv, p.gs)
-            o, t = attend(qf[a:b, h * G:(h + 1) * G], k, v, np.arange(n - (b - a), n), scale, True, window, ok)
+            o, t = attend(qf[a:b, h * G:(h + 1) * G], k, v, np.arange(n - (b - a), n), scale, True, window, ok, 0.0 if p.bk == 16 else 2.0 ** -11 + 2.0 ** -24)
             out[a:b, h * G:(h + 1) * G], tol[a:b, h * G:(h + 1) * G] = o, t
     return out, tol
 
