@@ -28,28 +28,46 @@ __device__ __forceinline__ int pages_of(int64_t rows, int shift) {
   return int((rows + (1 << shift) - 1) >> shift);
 }
 
-// Exclusive sums over the workgroup of each thread's x; total: over all.
+// Sums that stop at 2^32 - 1 (wrong tables and counts can ask for more).
+__device__ __forceinline__ uint32_t plus(uint32_t x, uint32_t y) { return __builtin_elementwise_add_sat(x, y); }
+
+// Inclusive sums over the wavefront: within rows of 16 lanes, then across.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x = plus(x, __builtin_amdgcn_update_dpp(0, int(x), 0x111, 0xf, 0xf, true));  // row_shr 1, 2, 4, 8
+  x = plus(x, __builtin_amdgcn_update_dpp(0, int(x), 0x112, 0xf, 0xf, true));
+  x = plus(x, __builtin_amdgcn_update_dpp(0, int(x), 0x114, 0xf, 0xf, true));
+  x = plus(x, __builtin_amdgcn_update_dpp(0, int(x), 0x118, 0xf, 0xf, true));
+  x = plus(x, __builtin_amdgcn_update_dpp(0, int(x), 0x142, 0xa, 0xf, false));  // row_bcast 15, 31
+  x = plus(x, __builtin_amdgcn_update_dpp(0, int(x), 0x143, 0xc, 0xf, false));
+  return x;
+}
+
+// Sums of x and y over the threads before this one, and over all.
+struct Sums {
+  uint32_t x, y, all_x, all_y;
+};
 template <int Threads>
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* total) {
-  __shared__ int64_t sums[Threads / 64];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  int64_t y = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t up = __shfl_up(y, d, 64);
-    if (lane >= d) y += up;
-  }
+__device__ __forceinline__ Sums block_scan(uint32_t x, uint32_t y) {
+  __shared__ uint2 sums[Threads / 64];
+  const int wave = threadIdx.x / 64;
+  const uint32_t u = wave_scan(x), v = wave_scan(y);
   __syncthreads();
-  if (lane == 63) sums[wave] = y;
+  if (threadIdx.x % 64 == 63) sums[wave] = make_uint2(u, v);
   __syncthreads();
-  int64_t before = 0, all = 0;
+  // The lanes before: shifted, since a sum that stopped cannot be taken back.
+  Sums s{uint32_t(__shfl_up(int(u), 1, 64)), uint32_t(__shfl_up(int(v), 1, 64)), 0, 0};
+  if (threadIdx.x % 64 == 0) s.x = s.y = 0;
+  uint32_t before_x = 0, before_y = 0;
 #pragma unroll
   for (int w = 0; w < Threads / 64; ++w) {
-    if (w < wave) before += sums[w];
-    all += sums[w];
+    const uint2 t = sums[w];
+    if (w == wave) before_x = s.all_x, before_y = s.all_y;
+    s.all_x = plus(s.all_x, t.x);
+    s.all_y = plus(s.all_y, t.y);
   }
-  *total = all;
-  return before + y - x;
+  s.x = plus(s.x, before_x);
+  s.y = plus(s.y, before_y);
+  return s;
 }
 
 // The last of s[0, n] (ascending) that is not above i: s[b] <= i < s[b + 1].
@@ -84,7 +102,7 @@ __global__ __launch_bounds__(Threads) void reserve_kernel(const ReserveArgs a) {
   const int avail = clamp_to(*t.free_count, t.num_pages);
   // Consecutive sequences a thread.
   int n[kPer], want[kPer], need[kPer];
-  int64_t pages = 0, places = 0;
+  uint32_t pages = 0, places = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int b = threadIdx.x * kPer + i;
@@ -92,28 +110,27 @@ __global__ __launch_bounds__(Threads) void reserve_kernel(const ReserveArgs a) {
     want[i] = b < t.batch ? max(a.counts[b], 0) : 0;
     const bool fits = int64_t(n[i]) + want[i] <= t.cap;
     need[i] = fits ? pages_of(int64_t(n[i]) + want[i], t.shift) - pages_of(n[i], t.shift) : -1;
-    pages += fits ? need[i] : 0;
-    places += fits ? want[i] : 0;
+    pages = plus(pages, fits ? need[i] : 0);
+    places = plus(places, fits ? want[i] : 0);
   }
-  int64_t all;
-  int64_t page_sum = block_scan<Threads>(pages, &all);
-  int64_t place_sum = block_scan<Threads>(places, &all);
-  int got[kPer], take[kPer], gots = 0, takes = 0;
+  Sums sum = block_scan<Threads>(pages, places);
+  int got[kPer], take[kPer];
+  uint32_t gots = 0, takes = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const bool fits = need[i] >= 0;
-    page_sum += fits ? need[i] : 0;
-    place_sum += fits ? want[i] : 0;
-    const bool ok = fits && (need[i] == 0 || page_sum <= avail) &&
-                    (want[i] == 0 || place_sum <= a.tokens);
+    sum.x = plus(sum.x, fits ? need[i] : 0);
+    sum.y = plus(sum.y, fits ? want[i] : 0);
+    const bool ok = fits && (need[i] == 0 || sum.x <= uint32_t(avail)) &&
+                    (want[i] == 0 || sum.y <= uint32_t(a.tokens));
     got[i] = ok ? want[i] : -1;
     take[i] = ok ? need[i] : 0;
     gots += ok ? want[i] : 0;
     takes += take[i];
   }
-  int64_t tokens, taken;
-  int first = int(block_scan<Threads>(gots, &tokens));
-  int page = int(block_scan<Threads>(takes, &taken));
+  sum = block_scan<Threads>(takes, gots);
+  int first = int(sum.y), page = int(sum.x);
+  const int taken = int(sum.all_x), total = int(sum.all_y), top = avail - taken;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int b = threadIdx.x * kPer + i;
@@ -128,10 +145,9 @@ __global__ __launch_bounds__(Threads) void reserve_kernel(const ReserveArgs a) {
       t.lens[b] = n[i] + max(got[i], 0);
     }
   }
-  const int total = int(tokens), top = avail - int(taken);
   if (threadIdx.x == 0) {
     start[kMaxBatch] = total;
-    base[kMaxBatch] = int(taken);
+    base[kMaxBatch] = taken;
     if (Finish) {
       a.starts[t.batch] = total;
       *t.free_count = top;  // every thread has read the old one: block_scan's barriers
@@ -164,7 +180,7 @@ constexpr int kWalk = 1024, kEach = 8;
 __global__ __launch_bounds__(kWalk) void release_kernel(const Tables t, const int32_t* keep,
                                                          const int32_t* shared) {
   __shared__ int32_t base[kMaxBatch + 1], from[kMaxBatch];
-  __shared__ int32_t valid[kEach * (kWalk / 64)];
+  __shared__ int32_t valid[kWalk / 64];
   const int b = threadIdx.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   int count = 0;
   const int height = clamp_to(*t.free_count, t.num_pages);
@@ -176,49 +192,50 @@ __global__ __launch_bounds__(kWalk) void release_kernel(const Tables t, const in
     count = max(0, pages_of(n, t.shift) - lo);
     t.lens[b] = k;
   }
-  int64_t all;
-  const int64_t at = block_scan<kWalk>(count, &all);
-  // Positions in the walk are 32-bit: num_pages bounds what can be pushed, not
-  // what wrong tables can name, so a walk past 2^31 entries is cut there.
-  base[b] = int(at < 0x7fffffff ? at : 0x7fffffff);
-  if (threadIdx.x == 0) base[kMaxBatch] = int(all < 0x7fffffff ? all : 0x7fffffff);
+  const Sums sum = block_scan<kWalk>(count, 0);
+  // A walk past 2^31 entries, which only wrong tables can ask for, is cut there.
+  base[b] = int(min(sum.x, 0x7fffffffu));
+  const int total = int(min(sum.all_x, 0x7fffffffu));
+  if (threadIdx.x == 0) base[kMaxBatch] = total;
   __syncthreads();
-  const int64_t total = base[kMaxBatch];
   int64_t pushed = height;
   for (int64_t j0 = 0; j0 < total; j0 += kWalk * kEach) {
-    int page[kEach];
+    // A wavefront's entries lie side by side.
+    int page[kEach], s = -1;
     int64_t place[kEach];
-    unsigned long long mask[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int64_t j = j0 + i * kWalk + threadIdx.x;
+      const int64_t j = j0 + (wave * kEach + i) * 64 + lane;
       page[i] = -1;
       place[i] = -1;
       if (j < total) {
-        const int s = find(base, kMaxBatch, int(j));
+        if (s < 0 || j >= base[s + 1]) s = find(base, kMaxBatch, int(j));
         place[i] = s * t.tstride + from[s] + (j - base[s]);
         page[i] = t.table[place[i]];
       }
     }
+    int mine = 0, at[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      mask[i] = __ballot(page[i] >= 0 && page[i] < t.num_pages);
-      if (lane == 0) valid[i * (kWalk / 64) + wave] = __popcll(mask[i]);
+      const unsigned long long mask = __ballot(page[i] >= 0 && page[i] < t.num_pages);
+      at[i] = mine + __popcll(mask & ((1ull << lane) - 1));
+      mine += __popcll(mask);
     }
+    if (lane == 0) valid[wave] = mine;
     __syncthreads();
-    int sum = 0, mine[kEach];
+    int before = 0, all = 0;
 #pragma unroll
-    for (int k = 0; k < kEach * (kWalk / 64); ++k) {
-      if (k % (kWalk / 64) == wave) mine[k / (kWalk / 64)] = sum;
-      sum += valid[k];
+    for (int w = 0; w < kWalk / 64; ++w) {
+      if (w == wave) before = all;
+      all += valid[w];
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       if (place[i] >= 0) t.table[place[i]] = -1;
-      const int64_t to = pushed + mine[i] + __popcll(mask[i] & ((1ull << lane) - 1));
+      const int64_t to = pushed + before + at[i];
       if (page[i] >= 0 && page[i] < t.num_pages && to < t.num_pages) t.free_pages[to] = page[i];
     }
-    pushed += sum;
+    pushed += all;
     __syncthreads();
   }
   if (threadIdx.x == 0) *t.free_count = int(pushed < t.num_pages ? pushed : t.num_pages);

@@ -127,8 +127,12 @@ struct Plan {
   int64_t slab_rows;                    // 0: no slab
   size_t slab, exponents, parts, bytes; // bytes: of all
 };
-constexpr int64_t kWanted = 512;     // workgroups
-constexpr int64_t kLeastKeys = 512;  // of a split
+// Workgroups that splits make up to where few rows' blocks are short, and keys
+// that a split holds at least. Two 2,048-token chunks over 30,011 rows, unsplit
+// at 512 and in 2 and 4 splits at 1,024 and 2,048: 1,950, 2,030, 2,115 us; 32
+// sequences' 6 tokens over up to 24,000 rows: 305, 175, 178.
+constexpr int64_t kWanted = 512, kWantedFew = 1024, kFewRows = 64;
+constexpr int64_t kLeastKeys = 512;
 
 bool plan_of(int batch, int H, int Hkv, int D, int64_t tokens, int64_t keys, bool slab, Plan* out) {
   const int64_t block = D <= 128 ? Shape<128>::kRows : D == 256 ? Shape<256>::kRows : Shape<512>::kRows;
@@ -137,9 +141,14 @@ bool plan_of(int batch, int H, int Hkv, int D, int64_t tokens, int64_t keys, boo
   Plan p{};
   if (units_of(Hkv, ids) > 0xffffffffLL / 512) return false;  // a grid: below 2^32 threads
   p.ids = int(ids);
-  const int64_t units = (tokens * G / block + (tokens < batch ? tokens : batch)) * Hkv;
-  int64_t n = units > 0 ? kWanted / units : 1;
-  if (n > keys / kLeastKeys) n = keys / kLeastKeys;
+  const int64_t sequences = tokens < batch ? tokens : batch;
+  const int64_t units = (tokens * G / block + sequences) * Hkv;
+  // Rows of a block that hold queries, on the average; a split writes and reads
+  // their partials.
+  const int64_t live = tokens * G / sequences < block ? tokens * G / sequences : block;
+  const int64_t least = 16 * live > kLeastKeys ? 16 * live : kLeastKeys;
+  int64_t n = ((live <= kFewRows ? kWantedFew : kWanted) + units - 1) / units;
+  if (n > keys / least) n = keys / least;
   if (n < 1) n = 1;
   const int64_t len = ((keys + n - 1) / n + 63) / 64 * 64;
   p.splits = int((keys + len - 1) / len);
