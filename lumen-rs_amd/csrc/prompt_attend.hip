@@ -1,5 +1,5 @@
 // Attention of packed sequences, over their own tokens or the paged cache.
-#include "prompt_attend.hpp"
+#include "prompt_few.hpp"
 
 namespace tqkv {
 namespace prompt {
@@ -123,31 +123,35 @@ __global__ __launch_bounds__(256) void slab_kernel(const Args a, const float* pa
 
 // What a call launches, and its workspace; false for what it refuses.
 struct Plan {
+  bool few;  // few_kernel
   int ids, splits, split_keys;
-  int64_t slab_rows;                    // 0: no slab
-  size_t slab, exponents, parts, bytes; // bytes: of all
+  int64_t slab_rows;                     // 0: no slab
+  size_t slab, exponents, parts, bytes;  // bytes: of all
 };
-// Workgroups that splits make up to where few rows' blocks are short, and keys
-// that a split holds at least. Two 2,048-token chunks over 30,011 rows, unsplit
-// at 512 and in 2 and 4 splits at 1,024 and 2,048: 1,950, 2,030, 2,115 us; 32
-// sequences' 6 tokens over up to 24,000 rows: 305, 175, 178.
-constexpr int64_t kWanted = 512, kWantedFew = 1024, kFewRows = 64;
-constexpr int64_t kLeastKeys = 512;
+// Workgroups that splits make up to, and keys that a split holds at least.
+constexpr int64_t kWanted = 512, kWantedFew = 2048;
+constexpr int64_t kLeastKeys = 512, kLeastFew = 256;
 
-bool plan_of(int batch, int H, int Hkv, int D, int64_t tokens, int64_t keys, bool slab, Plan* out) {
-  const int64_t block = D <= 128 ? Shape<128>::kRows : D == 256 ? Shape<256>::kRows : Shape<512>::kRows;
+bool plan_of(int batch, int H, int Hkv, int D, int64_t tokens, int64_t keys, Source source, Plan* out) {
   const int G = H / Hkv;
-  const int64_t ids = tokens * G / block + batch;
+  const int64_t sequences = tokens < batch ? tokens : batch, rows = tokens * G;
   Plan p{};
+  // Rows of a sequence on the average: the host knows no more.
+  const int64_t few_rows = D >= 256 ? Few<256>::kRows : Few<128>::kRows;
+  p.few = source != kPacked && rows <= sequences * few_rows;
+  const int64_t block = p.few ? few_rows
+                        : D <= 128 ? Shape<128>::kRows
+                        : D == 256 ? Shape<256>::kRows
+                                   : Shape<512>::kRows;
+  const int64_t ids = rows / block + batch;
   if (units_of(Hkv, ids) > 0xffffffffLL / 512) return false;  // a grid: below 2^32 threads
   p.ids = int(ids);
-  const int64_t sequences = tokens < batch ? tokens : batch;
-  const int64_t units = (tokens * G / block + sequences) * Hkv;
-  // Rows of a block that hold queries, on the average; a split writes and reads
-  // their partials.
-  const int64_t live = tokens * G / sequences < block ? tokens * G / sequences : block;
-  const int64_t least = 16 * live > kLeastKeys ? 16 * live : kLeastKeys;
-  int64_t n = ((live <= kFewRows ? kWantedFew : kWanted) + units - 1) / units;
+  const int64_t units = (rows / block + sequences) * Hkv;
+  // A split writes and reads its block's partials: 16 keys a row pay for them.
+  const int64_t live = rows / sequences < block ? rows / sequences : block;
+  int64_t least = p.few ? kLeastFew : kLeastKeys;
+  if (least < 16 * live) least = 16 * live;
+  int64_t n = ((p.few ? kWantedFew : kWanted) + units - 1) / units;
   if (n > keys / least) n = keys / least;
   if (n < 1) n = 1;
   const int64_t len = ((keys + n - 1) / n + 63) / 64 * 64;
@@ -155,7 +159,7 @@ bool plan_of(int batch, int H, int Hkv, int D, int64_t tokens, int64_t keys, boo
   p.split_keys = int(len);
   if (p.splits < 1) p.splits = 1;
   const auto whole = [](size_t x) { return (x + 255) / 256 * 256; };
-  if (slab) {
+  if (source == kPagedAffine && !p.few) {
     p.slab_rows = keys;
     p.slab = whole(size_t(batch) * Hkv * size_t(keys) * D * 2);
     p.exponents = whole(size_t(batch) * Hkv * 4) + whole(size_t(batch) * Hkv * kRangeParts * 4);
@@ -212,10 +216,10 @@ int32_t attend(Args& a, int D, Source source, const Plan& p, void* workspace, si
     a.part_l = a.part_m + slots;
   }
   switch (D) {
-    case 64: launch_prompt<64>(a, source, st); break;
-    case 128: launch_prompt<128>(a, source, st); break;
-    case 256: launch_prompt<256>(a, source, st); break;
-    default: launch_prompt<512>(a, source, st); break;
+    case 64: (p.few ? launch_few<64> : launch_prompt<64>)(a, source, st); break;
+    case 128: (p.few ? launch_few<128> : launch_prompt<128>)(a, source, st); break;
+    case 256: (p.few ? launch_few<256> : launch_prompt<256>)(a, source, st); break;
+    default: (p.few ? launch_few<512> : launch_prompt<512>)(a, source, st); break;
   }
   TQKV_LAUNCHED();
   return ok();
@@ -245,7 +249,7 @@ extern "C" size_t tqkv_packed_attend_workspace_size(int32_t batch, int32_t H, in
   Plan p;
   if (batch < 1 || batch > tqkv::paged::kMaxBatch || !(D == 64 || D == 128 || D == 256 || D == 512) ||
       H < 1 || H_kv < 1 || H % H_kv != 0 || H / H_kv > 32 || tokens < 1 || tokens > 0x7fffffffLL ||
-      !plan_of(batch, H, H_kv, D, tokens, tokens, false, &p))
+      !plan_of(batch, H, H_kv, D, tokens, tokens, kPacked, &p))
     return 0;
   return p.bytes;
 }
@@ -288,7 +292,7 @@ extern "C" int32_t tqkv_packed_attend(const uint16_t* q, int64_t q_stride, const
   a.ts = token_stride;
   a.hs = head_stride;
   Plan p;
-  if (!plan_of(batch, H, H_kv, D, tokens, tokens, false, &p))
+  if (!plan_of(batch, H, H_kv, D, tokens, tokens, kPacked, &p))
     return fail(TQKV_EUNSUPPORTED, "tokens=%lld", (long long)tokens);
   return attend(a, D, kPacked, p, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
@@ -301,7 +305,8 @@ extern "C" size_t tqkv_paged_prefill_workspace_size(const tqkv_paged_kv* kv, int
   if (tqkv::paged::check(kv, &pool) != TQKV_OK || H < 1 || H % kv->kv_heads != 0 ||
       H / kv->kv_heads > 32 || tokens < 1 || tokens > 0x7fffffffLL || max_rows < 1 ||
       max_rows > pool.cap ||
-      !plan_of(kv->batch, H, kv->kv_heads, kv->dim, tokens, max_rows, kv->kind == TQKV_CACHE_AFFINE, &p))
+      !plan_of(kv->batch, H, kv->kv_heads, kv->dim, tokens, max_rows,
+               kv->kind == TQKV_CACHE_AFFINE ? kPagedAffine : kPagedBf16, &p))
     return 0;
   return p.bytes;
 }
@@ -336,10 +341,10 @@ extern "C" int32_t tqkv_paged_prefill_attend(const tqkv_paged_kv* kv, const uint
   a.bits_k = kv->bits_k;
   a.bits_v = kv->bits_v;
   a.max_rows = int(max_rows);
-  const bool affine = kv->kind == TQKV_CACHE_AFFINE;
+  const Source source = kv->kind == TQKV_CACHE_AFFINE ? kPagedAffine : kPagedBf16;
   Plan p;
-  if (!plan_of(kv->batch, H, kv->kv_heads, kv->dim, tokens, max_rows, affine, &p))
+  if (!plan_of(kv->batch, H, kv->kv_heads, kv->dim, tokens, max_rows, source, &p))
     return fail(TQKV_EUNSUPPORTED, "tokens=%lld max_rows=%lld", (long long)tokens, (long long)max_rows);
-  return attend(a, kv->dim, affine ? kSlab : kPagedBf16, p, workspace, workspace_bytes,
+  return attend(a, kv->dim, p.slab_rows ? kSlab : source, p, workspace, workspace_bytes,
                 reinterpret_cast<hipStream_t>(stream));
 }

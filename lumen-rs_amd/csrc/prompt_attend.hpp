@@ -319,6 +319,40 @@ inline int64_t units_of(int Hkv, int64_t ids) {
   return ids * Hkv;
 }
 
+// The block with this id, of `each` rows: its sequence and first row. All lanes
+// call it and get the same; false for ids that no rows need.
+struct Block {
+  int b;
+  Sequence seq;
+  int64_t row0;
+};
+template <Source S>
+__device__ __forceinline__ bool find_block(const Args& a, int id, int each, Block* out) {
+  const int lane = threadIdx.x % kWave;
+  int b = -1, begin = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kWave) {
+    const int i = b0 + lane;
+    const int64_t at = i < a.batch ? start_of(a, i) * a.G / each + i : 0;
+    const unsigned long long on = __ballot(i < a.batch && at <= id);
+    if (!on) break;
+    const int last = 63 - __clzll(on);
+    b = b0 + last;
+    begin = __shfl(int(at), last, 64);  // ids are 32-bit
+    if (last < kWave - 1) break;
+  }
+  // Said to be alike in every lane, so that what follows runs on scalars.
+  b = __builtin_amdgcn_readfirstlane(b);
+  begin = __builtin_amdgcn_readfirstlane(begin);
+  if (b < 0) return false;
+  const Sequence s = sequence<S>(a, b);
+  out->b = b;
+  out->seq.first = __builtin_amdgcn_readfirstlane(int(s.first));
+  out->seq.count = __builtin_amdgcn_readfirstlane(s.count);
+  out->seq.keys = __builtin_amdgcn_readfirstlane(s.keys);
+  out->row0 = int64_t(id - begin) * each;
+  return out->row0 < int64_t(out->seq.count) * a.G;
+}
+
 template <int D, Source S>
 __global__ __launch_bounds__(Shape<D>::kThreads)
 __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(const Args a) {
@@ -334,28 +368,11 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
   const Unit unit = unit_of(a, int(blockIdx.x));
   if (unit.id < 0) return;
   const int kvh = unit.head;
-  int b = -1, begin = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kWave) {
-    const int i = b0 + lane;
-    const int64_t at = i < a.batch ? start_of(a, i) * a.G / W::kRows + i : 0;
-    const unsigned long long on = __ballot(i < a.batch && at <= unit.id);
-    if (!on) break;
-    const int last = 63 - __clzll(on);
-    b = b0 + last;
-    begin = __shfl(int(at), last, 64);  // below 2^29
-    if (last < kWave - 1) break;
-  }
-  b = __builtin_amdgcn_readfirstlane(b);
-  begin = __builtin_amdgcn_readfirstlane(begin);
-  if (b < 0) return;
-  Sequence seq = sequence<S>(a, b);
-  // Alike in every lane; said so, the tile loop runs on scalars.
-  seq.first = __builtin_amdgcn_readfirstlane(int(seq.first));
-  seq.count = __builtin_amdgcn_readfirstlane(seq.count);
-  seq.keys = __builtin_amdgcn_readfirstlane(seq.keys);
-  const int64_t rows = int64_t(seq.count) * a.G;
-  const int64_t row0 = int64_t(unit.id - begin) * W::kRows;
-  if (row0 >= rows) return;
+  Block blk;
+  if (!find_block<S>(a, unit.id, W::kRows, &blk)) return;
+  const int b = blk.b;
+  const Sequence seq = blk.seq;
+  const int64_t rows = int64_t(seq.count) * a.G, row0 = blk.row0;
   const int64_t row_end = row0 + W::kRows < rows ? row0 + W::kRows : rows;
   const int n = seq.keys, p0 = n - seq.count;  // p0: the first query's position
   const int pos_lo = p0 + int(row0 / a.G), pos_hi = p0 + int((row_end - 1) / a.G);
@@ -707,10 +724,12 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const Args a) {
   if (__any(bad)) attend_row<D, R>(a, b, token, head);
 }
 
-// Launches prompt_kernel<D, S> and, for split keys, the join. Defined a head
-// dim a file.
+// Launches prompt_kernel<D, S> (few_kernel of prompt_few.hpp) and, for split
+// keys, the join. Defined a head dim a file.
 template <int D>
 void launch_prompt(const Args& a, Source s, hipStream_t st);
+template <int D>
+void launch_few(const Args& a, Source s, hipStream_t st);
 
 template <int D, Source S>
 void launch_source(const Args& a, hipStream_t st) {

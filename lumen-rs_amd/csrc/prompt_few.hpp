@@ -1,0 +1,402 @@
+// Attention of packed sequences with few rows each over the paged cache
+// (drafted tokens, the ends of prompts): bound by reading keys and values.
+//
+// A block's rows are all of its wavefronts', which take every kWaves-th tile
+// of 32 keys for themselves: no barrier in the loop, each wavefront's tile in
+// LDS of its own (K's is on its way while the weights multiply V, and V's
+// while K meets Q). What the wavefronts gathered meets in LDS at the end.
+//
+// Affine rows are dequantized on the way into LDS, out of registers that the
+// next tile's codes have been loaded into meanwhile: V to bf16, K to a pair of
+// bf16 (16 bits: one bf16 would cost the scores what their sums keep), whose
+// second halves lie where V's tile will.
+#pragma once
+
+#include "prompt_attend.hpp"
+
+namespace tqkv {
+namespace prompt {
+
+template <int D>
+struct Few {
+  static constexpr int kWaves = D == 512 ? 2 : 4;
+  static constexpr int kRW = D >= 256 ? 16 : 32;
+  static constexpr int kRows = kRW;  // a block
+  static constexpr int kThreads = kWaves * kWave;
+  static constexpr int kKeys = 32;
+  static constexpr int kPieces = kKeys * D * 2 / 1024;
+  // Blocks that a CU's LDS holds, as wavefronts a SIMD.
+  static constexpr int kPerEu = D == 64 ? 3 : D == 128 ? 2 : 1;
+};
+
+// 16 codes of 4 or 8 bits out of w (2 or 4 words) as f32.
+template <int BITS>
+__device__ __forceinline__ void codes16(const uint32_t* w, float (&f)[16]) {
+  if constexpr (BITS == 8) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = float((w[i / 4] >> (8 * (i % 4))) & 0xffu);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t e = w[k] & 0x0f0f0f0fu, o = (w[k] >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[8 * k + 2 * j] = float((e >> (8 * j)) & 0xffu);
+        f[8 * k + 2 * j + 1] = float((o >> (8 * j)) & 0xffu);
+      }
+    }
+  }
+}
+
+template <int D, Source S, int BK, int BV>
+__global__ __launch_bounds__(Few<D>::kThreads) __attribute__((amdgpu_waves_per_eu(Few<D>::kPerEu)))
+void few_kernel(const Args a) {
+  typedef Few<D> W;
+  constexpr int kWaves = W::kWaves, RW = W::kRW, NR = RW / 16, KT = W::kKeys, NI = KT / 16;
+  constexpr int ND = D / 32, NT = D / 16, NP = W::kPieces;
+  constexpr bool AFFINE = S == kPagedAffine;
+  __shared__ __attribute__((aligned(16))) uint16_t tiles[kWaves][2][KT * D];
+  __shared__ float part_m[kWaves][RW], part_l[kWaves][RW];
+  static_assert(sizeof(tiles[0]) >= sizeof(float) * RW * D, "what a wavefront gathered fits its tiles");
+  const int tid = threadIdx.x, lane = tid % kWave, lr = lane % 16, lg = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+
+  const Unit unit = unit_of(a, int(blockIdx.x));
+  if (unit.id < 0) return;
+  const int kvh = unit.head;
+  Block blk;
+  if (!find_block<S>(a, unit.id, W::kRows, &blk)) return;
+  const int b = blk.b;
+  const Sequence seq = blk.seq;
+  const int64_t rows = int64_t(seq.count) * a.G, row0 = blk.row0;
+  const int64_t row_end = row0 + RW < rows ? row0 + RW : rows;
+  const int n = seq.keys, p0 = n - seq.count;
+  const int pos_lo = p0 + int(row0 / a.G), pos_hi = p0 + int((row_end - 1) / a.G);
+  const int split = blockIdx.y;
+  int key_lo = split * a.split_keys, key_hi = n;
+  if (n - key_lo > a.split_keys) key_hi = key_lo + a.split_keys;
+  if (pos_hi + 1 < key_hi) key_hi = pos_hi + 1;
+  if (a.window > 0 && pos_lo - a.window + 1 > key_lo) key_lo = pos_lo - a.window + 1;
+  if (a.part_o && key_lo >= key_hi) return;
+
+  const int t_lo = key_lo / KT, t_hi = (key_hi - 1) / KT;  // used where key_lo < key_hi
+  const bool working = key_lo < key_hi && t_lo + wave <= t_hi;
+
+  bf8_t qf[NR][ND];
+  int pos[NR];
+  const float sign = a.scale < 0.0f ? -1.0f : 1.0f, qscale = a.scale * sign * kLog2e;
+#pragma unroll
+  for (int j = 0; j < NR; ++j) {
+    const int64_t at = row0 + 16 * j + lr, r = at < rows ? at : rows - 1;
+    pos[j] = p0 + int(r / a.G);
+    const uint16_t* src = a.q + (seq.first + r / a.G) * a.qs + (int64_t(kvh) * a.G + r % a.G) * D;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int s = 0; s < ND; ++s) {
+      u4_t x = *reinterpret_cast<const u4_t*>(src + 32 * s + 8 * lg);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] ^= flip;
+      qf[j][s] = __builtin_bit_cast(bf8_t, x);
+    }
+  }
+  float m[NR], nm[NR], thr[NR], lsum[NR];
+  f4_t o[NT][NR];
+  const float iqs = 1.0f / qscale;
+#pragma unroll
+  for (int j = 0; j < NR; ++j) {
+    m[j] = thr[j] = -INFINITY;
+    nm[j] = lsum[j] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  uint16_t* K = tiles[wave][0];
+  uint16_t* V = tiles[wave][1];
+  auto page_of = [&](int t) __attribute__((always_inline)) {
+    typedef const __attribute__((address_space(4))) int32_t* constant;
+    return ((constant)(a.pool.table + b * a.pool.tstride))[t >> a.pool.shift];
+  };
+  const int kturn = turn_of<D>(lr), vturn = turn_of<D>(4 * lg + lr / 4);
+
+  auto scores = [&](const uint16_t* from, f4_t (&sc)[NI][NR]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < ND; ++s)
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const bf8_t ka = *reinterpret_cast<const bf8_t*>(from + (16 * i + lr) * D + ((4 * s + lg) ^ kturn) * 8);
+#pragma unroll
+        for (int j = 0; j < NR; ++j)
+          sc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[j][s], sc[i][j], 0, 0, 0);
+      }
+  };
+  auto softmax = [&](int tile, f4_t (&sc)[NI][NR], bf8_t (&pp)[NR]) __attribute__((always_inline)) {
+    const int kbase = tile * KT;
+    uint32_t on = 0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      if (paged::valid_page(a.pool, page_of(min(kbase + 16 * i, n - 1)))) on |= 1u << i;
+    const bool whole = kbase >= key_lo && kbase + KT <= key_hi && on == (1u << NI) - 1u &&
+                       kbase + KT - 1 <= pos_lo && (a.window <= 0 || pos_hi - a.window < kbase);
+    if (!whole) {
+      rare();
+#pragma unroll
+      for (int j = 0; j < NR; ++j) {
+        const int hi = min(key_hi, pos[j] + 1) - kbase;
+        const int lo = (a.window > 0 ? max(key_lo, pos[j] - a.window + 1) : key_lo) - kbase;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int k = 16 * i + 4 * lg + r;
+            if (k < lo || k >= hi || !((on >> i) & 1)) sc[i][j][r] = -INFINITY;
+          }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[i][j][r]);
+      if (__any(mx > thr[j])) {
+        rare();
+        mx = row_max(mx);
+        const bool up = mx > thr[j];
+        const float mn = up ? mx * qscale : m[j];
+        const float alpha = up ? __builtin_amdgcn_exp2f(m[j] - mn) : 1.0f;
+        lsum[j] *= alpha;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[t][j] *= alpha;
+        m[j] = mn;
+        nm[j] = mn == -INFINITY ? 0.0f : -mn;
+        thr[j] = (mn + kTau) * iqs;
+      }
+      u4_t w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f4_t s = sc[e / 2][j];
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2)], qscale, nm[j]));
+        const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2) + 1], qscale, nm[j]));
+        w[e] = pack_bf16(x, y);
+        lsum[j] = add_two(w[e], lsum[j]);
+      }
+      pp[j] = __builtin_bit_cast(bf8_t, w);
+    }
+  };
+  auto values = [&](const bf8_t (&pp)[NR]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint16_t* src = V + (4 * lg + lr / 4) * D + ((2 * t + lr % 4 / 2) ^ vturn) * 8 + 4 * (lr % 2);
+      const u2_t x = read_transposed(src), y = read_transposed(src + 16 * D);
+      const bf8_t va = __builtin_bit_cast(bf8_t, u4_t{x.x, x.y, y.x, y.y});
+#pragma unroll
+      for (int j = 0; j < NR; ++j)
+        o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pp[j], o[t][j], 0, 0, 0);
+    }
+  };
+  auto clear = [&](f4_t (&sc)[NI][NR]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NR; ++j) sc[i][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  };
+
+  if (working) {
+    const int t0 = t_lo + wave;
+    if constexpr (!AFFINE) {
+      constexpr int kPieceRows = 512 / D, kRowPieces = D / 8;
+      const int lrow = lane / kRowPieces;
+      // One side of a tile, 16 bytes a lane and piece (as prompt_kernel's).
+      auto fetch = [&](int tile, int side) __attribute__((always_inline)) {
+        const int tc = tile < t_hi ? tile : t_hi;
+        const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_address(tiles[wave][side]));
+        int page[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) page[i] = page_of(min(tc * KT + 16 * i, n - 1));
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int r = i * kPieceRows + lrow, t = min(tc * KT + r, n - 1);
+          const int c = ((lane % kRowPieces) ^ turn_of<D>(r)) * 8;
+          const int pg = page[i * kPieceRows / 16];
+          const bool ok = paged::valid_page(a.pool, pg);
+          const int64_t at = paged::pool_row(a.pool, ok ? pg : 0, kvh, t & ((1 << a.pool.shift) - 1)) * D + c;
+          const uint16_t* zero = reinterpret_cast<const uint16_t*>(kZeroRow) + c;
+          to_lds(ok ? static_cast<const uint16_t*>(a.slot[side]) + at : zero, lds + i * 1024);
+        }
+      };
+      wait_loads<0>();  // the queries
+      fetch(t0, 0);
+      fetch(t0, 1);
+      for (int tile = t0; tile <= t_hi; tile += kWaves) {
+        f4_t sc[NI][NR];
+        bf8_t pp[NR];
+        wait_loads<NP>();  // K
+        clear(sc);
+        scores(K, sc);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // K's reads are done (lgkmcnt 0)
+        fetch(tile + kWaves, 0);
+        softmax(tile, sc, pp);
+        wait_loads<NP>();  // V
+        values(pp);
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        fetch(tile + kWaves, 1);
+      }
+      wait_loads<0>();
+    } else {
+      // Lane l holds the codes of row l / 2, channels [l % 2 * D / 2, + D / 2).
+      constexpr int H = D / 2, KW = H * BK / 32, VW = H * BV / 32;
+      const int r = lane / 2, half = lane % 2, turn = turn_of<D>(r);
+      constexpr int NRUN = H / 32;
+      // One side of a tile: codes, and the scales and biases of their runs of 32.
+      auto load = [&](int tile, int side, auto& codes, float (&s)[NRUN], float (&z)[NRUN]) __attribute__((always_inline)) {
+        constexpr int words = sizeof(codes) / 4;
+        const int tc = tile < t_hi ? tile : t_hi;
+        const int t = min(tc * KT + r, n - 1);
+        const int page = r < 16 ? page_of(min(tc * KT, n - 1)) : page_of(min(tc * KT + 16, n - 1));
+        const bool ok = paged::valid_page(a.pool, page);
+        const int64_t row = paged::pool_row(a.pool, ok ? page : 0, kvh, t & ((1 << a.pool.shift) - 1));
+        const u4_t* src = reinterpret_cast<const u4_t*>(static_cast<const uint32_t*>(a.slot[3 * side]) + (2 * row + half) * words);
+#pragma unroll
+        for (int i = 0; i < words / 4; ++i) codes[i] = src[i];
+        const uint16_t* sc = static_cast<const uint16_t*>(a.slot[3 * side + 1]) + row * (D / a.gs);
+        const uint16_t* bi = static_cast<const uint16_t*>(a.slot[3 * side + 2]) + row * (D / a.gs);
+#pragma unroll
+        for (int i = 0; i < NRUN; ++i) {
+          const int g = (half * H + 32 * i) / a.gs;
+          s[i] = bf16_to_f32(sc[g]);
+          z[i] = bf16_to_f32(bi[g]);
+          if (!ok) s[i] = z[i] = 0.0f;  // hidden, and finite
+        }
+      };
+      u4_t kc[KW / 4], vc[VW / 4];
+      float ks[NRUN], kz[NRUN], vs[NRUN], vz[NRUN];
+      load(t0, 0, kc, ks, kz);
+      load(t0, 1, vc, vs, vz);
+      for (int tile = t0; tile <= t_hi; tile += kWaves) {
+        f4_t sc[NI][NR];
+        bf8_t pp[NR];
+#pragma unroll
+        for (int i = 0; i < H / 16; ++i) {
+          uint32_t w[BK / 2], hi[8], lo[8];
+          float f[16];
+#pragma unroll
+          for (int e = 0; e < BK / 2; ++e) w[e] = kc[(i * BK / 2 + e) / 4][(i * BK / 2 + e) % 4];
+          codes16<BK>(w, f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float x = fmaf(ks[i / 2], f[2 * e], kz[i / 2]), y = fmaf(ks[i / 2], f[2 * e + 1], kz[i / 2]);
+            hi[e] = pack_bf16(x, y);
+            lo[e] = pack_bf16(x - __uint_as_float(hi[e] << 16), y - __uint_as_float(hi[e] & 0xffff0000u));
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int at = r * D + ((half * (H / 8) + 2 * i + e) ^ turn) * 8;
+            *reinterpret_cast<u4_t*>(K + at) = u4_t{hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]};
+            *reinterpret_cast<u4_t*>(V + at) = u4_t{lo[4 * e], lo[4 * e + 1], lo[4 * e + 2], lo[4 * e + 3]};
+          }
+        }
+        load(tile + kWaves, 0, kc, ks, kz);
+        clear(sc);
+        scores(V, sc);
+        scores(K, sc);
+        softmax(tile, sc, pp);
+#pragma unroll
+        for (int i = 0; i < H / 16; ++i) {
+          uint32_t w[BV / 2], x[8];
+          float f[16];
+#pragma unroll
+          for (int e = 0; e < BV / 2; ++e) w[e] = vc[(i * BV / 2 + e) / 4][(i * BV / 2 + e) % 4];
+          codes16<BV>(w, f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] = pack_bf16(fmaf(vs[i / 2], f[2 * e], vz[i / 2]), fmaf(vs[i / 2], f[2 * e + 1], vz[i / 2]));
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<u4_t*>(V + r * D + ((half * (H / 8) + 2 * i + e) ^ turn) * 8) =
+                u4_t{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]};
+        }
+        load(tile + kWaves, 1, vc, vs, vz);
+        values(pp);
+      }
+    }
+  }
+
+  // The wavefronts' (m, l, o) meet.
+  float* mine = reinterpret_cast<float*>(tiles[wave][0]);  // [RW][D]
+#pragma unroll
+  for (int j = 0; j < NR; ++j) {
+    const float sum = row_sum(lsum[j]);
+    if (lg == 0) {
+      part_m[wave][16 * j + lr] = m[j];
+      part_l[wave][16 * j + lr] = sum;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      *reinterpret_cast<f4_t*>(mine + (16 * j + lr) * D + ((4 * t + lg) ^ (lr & 7)) * 4) = o[t][j];
+  }
+  __syncthreads();
+  bool bad = false;
+  // A thread takes four channels of a row.
+  for (int i = tid; i < RW * (D / 4); i += W::kThreads) {
+    const int rr = i / (D / 4), c4 = i % (D / 4);
+    const int64_t r = row0 + rr;
+    if (r >= rows) break;
+    float top = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, part_m[w][rr]);
+    f4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = part_m[w][rr] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part_m[w][rr] - top);
+      l = fmaf(f, part_l[w][rr], l);
+      const f4_t x = *reinterpret_cast<const f4_t*>(reinterpret_cast<const float*>(tiles[w][0]) + rr * D + (c4 ^ (rr & 7)) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, x[e], sum[e]);
+    }
+    const int64_t row = (seq.first + r / a.G) * a.H + int64_t(kvh) * a.G + r % a.G;
+    if (a.part_o) {
+      const int64_t slot = row * a.splits + split;
+      *reinterpret_cast<f4_t*>(a.part_o + slot * D + 4 * c4) = sum;
+      if (c4 == 0) {
+        a.part_m[slot] = top;
+        a.part_l[slot] = l;
+      }
+      continue;
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const f4_t v = sum * inv;
+    bad |= !(l > 0.0f) || !(v[0] == v[0] && v[1] == v[1] && v[2] == v[2] && v[3] == v[3]);
+    *reinterpret_cast<u2_t*>(a.out + row * D + 4 * c4) = u2_t{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+  }
+  if (a.part_o) return;
+  if (__syncthreads_or(bad)) {
+    rare();
+#pragma unroll 1
+    for (int i = wave; i < RW; i += kWaves) {
+      const int64_t r = row0 + i;
+      if (r >= rows) break;
+      attend_row<D, S>(a, b, seq.first + r / a.G, kvh * a.G + int(r % a.G));
+    }
+  }
+}
+
+template <int D>
+void launch_few(const Args& a, Source s, hipStream_t st) {
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(unsigned(units_of(a.Hkv, a.ids)), unsigned(a.splits)), dim3(Few<D>::kThreads), 0, st, a);
+  };
+  if (s == kPagedBf16) go(few_kernel<D, kPagedBf16, 16, 16>);
+  else if (a.bits_k == 4 && a.bits_v == 4) go(few_kernel<D, kPagedAffine, 4, 4>);
+  else if (a.bits_k == 4) go(few_kernel<D, kPagedAffine, 4, 8>);
+  else if (a.bits_v == 4) go(few_kernel<D, kPagedAffine, 8, 4>);
+  else go(few_kernel<D, kPagedAffine, 8, 8>);
+  auto join = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(unsigned((a.tokens * a.H + 3) / 4)), dim3(kJoinThreads), 0, st, a);
+  };
+  if (a.part_o && s == kPagedBf16) join(join_kernel<D, kPagedBf16>);
+  else if (a.part_o) join(join_kernel<D, kPagedAffine>);
+}
+
+}  // namespace prompt
+}  // namespace tqkv

@@ -1,0 +1,8 @@
+// Attention of packed sequences with few rows, head dim 256.
+#include "prompt_few.hpp"
+
+namespace tqkv {
+namespace prompt {
+template void launch_few<256>(const Args&, Source, hipStream_t);
+}  // namespace prompt
+}  // namespace tqkv
