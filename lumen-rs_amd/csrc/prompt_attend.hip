@@ -129,7 +129,7 @@ struct Plan {
   size_t slab, exponents, parts, bytes;  // bytes: of all
 };
 // Workgroups that splits make up to, and keys that a split holds at least.
-constexpr int64_t kWanted = 512, kWantedFew = 2048;
+constexpr int64_t kWanted = 384, kWantedFew = 2048;
 constexpr int64_t kLeastKeys = 512, kLeastFew = 256;
 
 bool plan_of(int batch, int H, int Hkv, int D, int64_t tokens, int64_t keys, Source source, Plan* out) {
@@ -151,7 +151,7 @@ bool plan_of(int batch, int H, int Hkv, int D, int64_t tokens, int64_t keys, Sou
   const int64_t live = rows / sequences < block ? rows / sequences : block;
   int64_t least = p.few ? kLeastFew : kLeastKeys;
   if (least < 16 * live) least = 16 * live;
-  int64_t n = ((p.few ? kWantedFew : kWanted) + units - 1) / units;
+  int64_t n = p.few ? (kWantedFew + units - 1) / units : kWanted / units;
   if (n > keys / least) n = keys / least;
   if (n < 1) n = 1;
   const int64_t len = ((keys + n - 1) / n + 63) / 64 * 64;
@@ -274,6 +274,8 @@ extern "C" int32_t tqkv_packed_attend(const uint16_t* q, int64_t q_stride, const
     return fail(TQKV_EINVAL_ARG,
                 "k and v are 16-byte aligned, strides multiples of 8 elements (token %lld, head %lld)",
                 (long long)token_stride, (long long)head_stride);
+  if (token_stride < 0 || token_stride >= (int64_t(1) << 27))  // a lane's offset is 32-bit
+    return fail(TQKV_EUNSUPPORTED, "token_stride=%lld (below 2^27)", (long long)token_stride);
   Args a{};
   a.q = q;
   a.qs = q_stride;

@@ -205,29 +205,33 @@ typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 
 // Launch shapes. Late: the second wavefront of each SIMD multiplies by V one
-// tile late, so that one's softmax meets the other's products.
+// tile late, so that one's softmax meets the other's products. At D = 512 LDS
+// holds one tile of K and one of V: K's next is on its way while the weights
+// multiply V, V's while K meets Q.
 template <int D>
 struct Shape {
   static constexpr int kWaves = 8;
-  static constexpr int kRW = D <= 128 ? 32 : 16;       // rows a wavefront
-  static constexpr int kKeys = D <= 128 ? 64 : 32;     // keys a tile
-  static constexpr bool kLate = D <= 256;
-  static constexpr int kAhead = D <= 256 ? 2 : 1;      // tiles in flight
+  static constexpr int kRW = D <= 128 ? 32 : 16;  // rows a wavefront
+  static constexpr int kKeys = 64;                // keys a tile
+  static constexpr bool kLate = D <= 128;
+  static constexpr int kAhead = D <= 128 ? 2 : D == 256 ? 1 : 0;  // tiles in flight
   static constexpr int kKBufs = kAhead + 1, kVBufs = kAhead + 1 + (kLate ? 1 : 0);
+  static constexpr int kGroupK = 4, kGroupV = 4;  // operand reads in flight
   static constexpr int kRows = kWaves * kRW;
   static constexpr int kThreads = kWaves * kWave;
   static constexpr int kPieces = kKeys * D * 2 / 1024 / kWaves;  // 1 KB pieces of K (of V) a wavefront
   static_assert(kPieces >= 1 && (kKBufs + kVBufs) * kKeys * D * 2 <= 160 * 1024, "LDS");
 };
 
-// The place of 16-byte piece c in row r of a tile: rows that fall on the same
-// LDS banks (256 / D rows cover them) are turned against each other by two
-// pieces, which 16 rows x 2 pieces (K) and 8 rows x 2 pieces (V) read at once
-// need.
+// The place of 16-byte piece c in row r of a tile is c ^ turn_of(r): rows that
+// fall on the same 256 bytes of LDS banks are turned against each other by two
+// pieces, so that 8 rows x 2 pieces, which K's and V's reads meet at once, lie on
+// banks of their own (a probe of these reads alone: 246 and 220 bytes a cycle
+// and CU, 126 where rows 2 i and 2 i + 1 are turned alike at D = 128).
 template <int D>
 __device__ __forceinline__ int turn_of(int r) {
-  constexpr int n = D >= 256 ? 1 : 256 / D;
-  return 2 * ((r / n) & (16 / n - 1));
+  constexpr int n = D >= 128 ? 1 : 128 / D;
+  return 2 * ((r / n) & (8 / n - 1));
 }
 
 // 16 bytes from each lane's src to LDS [lds + 16 lane, + 16). As assembly, so
@@ -240,6 +244,11 @@ __device__ __forceinline__ void to_lds(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds)
                : "memory", "m0");
 }
+// The same from a uniform base and a lane's offset below 2^32.
+__device__ __forceinline__ void to_lds_at(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+               : "memory", "m0");
+}
 #pragma clang diagnostic pop
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return uint32_t(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
@@ -250,9 +259,29 @@ __device__ __forceinline__ void wait_loads() {
   __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
-__device__ __forceinline__ u2_t read_transposed(const uint16_t* p) {
+// Reads at an LDS address.
+template <typename T>
+__device__ __forceinline__ T read_lds(uint32_t at) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) T*>(at);
+}
+__device__ __forceinline__ u2_t read_transposed(uint32_t at) {
   return __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                      (__attribute__((address_space(3))) s4_t*)(p)));
+                                      reinterpret_cast<__attribute__((address_space(3))) s4_t*>(at)));
+}
+// Operand addresses, bytes from a tile's beginning. Tiles begin at multiples of
+// 1 KB, so that the pieces' turns and the operands' numbers meet in one XOR:
+// K, lane (row r, group g): row r + 16 i, piece (4 s + g) turned: k_lane ^ 64 s,
+// plus the rows. V: row 4 g + r / 4 (+ 16, 32 u), piece (2 t + (r / 2) % 2)
+// turned: v_lane ^ 32 t.
+template <int D>
+__device__ __forceinline__ uint32_t k_lane(int lane) {
+  const int r = lane % 16, g = lane / 16;
+  return uint32_t(r * D * 2 + (g ^ turn_of<D>(r)) * 16);
+}
+template <int D>
+__device__ __forceinline__ uint32_t v_lane(int lane) {
+  const int r = 4 * (lane / 16) + lane % 16 / 4;
+  return uint32_t(r * D * 2 + ((lane % 4 / 2) ^ turn_of<D>(r)) * 16 + 8 * (lane % 2));
 }
 __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
   const f2_t f = {x, y};
@@ -282,8 +311,41 @@ __device__ __forceinline__ float row_sum(float v) {
   r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+// The lane's index, where D is large computed anew at each use: what depends
+// on it (addresses) is then recomputed a tile and not held in registers that
+// the accumulators need.
+template <int D>
+__device__ __forceinline__ int lane_now(int lane) {
+  if constexpr (D < 256) return lane;
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
+}
 // Keeps a block that few tiles take behind its branch.
 __device__ __forceinline__ void rare() { asm volatile(""); }
+
+// Products of `Count` operands out of LDS, `Group` at a time: a group's reads are
+// issued before the products of the group before it, which cover their
+// latency. (Left to itself the compiler reads each operand right before its
+// products and waits for it; a list of scheduling groups over a whole tile's
+// products is ignored.) read(i) gives operand i, use(i, x) multiplies it.
+template <int Count, int Group, typename Op, typename Read, typename Use>
+__device__ __forceinline__ void pipelined(Read read, Use use) {
+  static_assert(Count % Group == 0, "whole groups");
+  Op x[2][Group];
+#pragma unroll
+  for (int i = 0; i < Group; ++i) x[0][i] = read(i);
+#pragma unroll
+  for (int g = 0; g < Count / Group; ++g) {
+    if (g + 1 < Count / Group)
+#pragma unroll
+      for (int i = 0; i < Group; ++i) x[(g + 1) % 2][i] = read((g + 1) * Group + i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < Group; ++i) use(g * Group + i, x[g % 2][i]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
 
 // What rows of pages that are none read instead.
 __device__ const uint4 kZeroRow[64] = {};
@@ -360,7 +422,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
   constexpr int kWaves = W::kWaves, RW = W::kRW, NR = RW / 16, KT = W::kKeys, NI = KT / 16;
   constexpr int ND = D / 32, NT = D / 16, NU = KT / 32, NP = W::kPieces;
   constexpr bool F16 = S == kSlab;
-  __shared__ __attribute__((aligned(16))) uint16_t tiles[W::kKBufs + W::kVBufs][KT * D];
+  __shared__ __attribute__((aligned(1024))) uint16_t tiles[W::kKBufs + W::kVBufs][KT * D];
   const int tid = threadIdx.x, lane = tid % kWave, lr = lane % 16, lg = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
 
@@ -445,62 +507,77 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
 
   if (key_lo < key_hi) {
     const int t_lo = key_lo / KT, t_hi = (key_hi - 1) / KT;
-    // This wavefront's pieces of a tile: piece i is rows [first row of it,
-    // + 512 / D), lane l of it fills place l % (D / 8) of its row, which holds
-    // the piece of the row that turn_of puts there.
-    constexpr int kPieceRows = 512 / D, kRowPieces = D / 8;
-    const int lrow = lane / kRowPieces;
+    // A wavefront fetches kMine rows of each tile, which lie in one page (of
+    // 16 rows or more), in pieces of 1 KB: lane l of piece i fills place l %
+    // (D / 8) of row i 512 / D + l / (D / 8), which holds the piece of the row
+    // that turn_of puts there.
+    constexpr int kMine = KT / kWaves, kPieceRows = 512 / D, kRowPieces = D / 8;
+    static_assert(kMine == NP * kPieceRows && 16 % kMine == 0, "a wavefront's rows lie in one page");
+    const std::true_type kKey{};
+    const std::false_type kValue{};
     auto page_of = [&](int t) __attribute__((always_inline)) {
       // The tables are written by no one while the kernel runs.
       typedef const __attribute__((address_space(4))) int32_t* constant;
       return ((constant)(a.pool.table + b * a.pool.tstride))[t >> a.pool.shift];
     };
-    // Rows past the last key read that one again: hidden, and finite where it
-    // is.
-    auto fetch = [&](int tile, int kb, int vb) __attribute__((always_inline)) {
-      const int tc = tile < t_hi ? tile : t_hi;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int piece = wave * NP + i;
-        const int r = piece * kPieceRows + lrow;  // row in the tile
-        const int t = min(tc * KT + r, n - 1);
-        const int c = ((lane % kRowPieces) ^ turn_of<D>(r)) * 8;
-        const uint16_t *ks, *vs;
-        if constexpr (S == kPacked) {
-          const int64_t at = (seq.first + t) * a.ts + kvh * a.hs + c;
-          ks = a.k + at;
-          vs = a.v + at;
-        } else if constexpr (S == kSlab) {
-          const int64_t at = ((int64_t(b) * a.Hkv + kvh) * a.slab_rows + t) * D + c;
-          ks = a.slab_k + at;
-          vs = a.slab_v + at;
-        } else {
-          // A piece's rows lie in one page (of 16 rows or more).
-          const int page = page_of(min(tc * KT + piece * kPieceRows, n - 1));
-          const bool ok = paged::valid_page(a.pool, page);
-          const int64_t at = paged::pool_row(a.pool, ok ? page : 0, kvh, t & ((1 << a.pool.shift) - 1)) * D + c;
-          const uint16_t* zero = reinterpret_cast<const uint16_t*>(kZeroRow) + c;
-          ks = ok ? static_cast<const uint16_t*>(a.slot[0]) + at : zero;
-          vs = ok ? static_cast<const uint16_t*>(a.slot[1]) + at : zero;
-        }
-        to_lds(ks, __builtin_amdgcn_readfirstlane(lds_address(tiles[kb])) + piece * 1024);
-        to_lds(vs, __builtin_amdgcn_readfirstlane(lds_address(tiles[W::kKBufs + vb])) + piece * 1024);
+    // Where row t of the sequence lies, and the bytes between rows; NULL for a
+    // page that is none.
+    auto row_bytes = [&]() __attribute__((always_inline)) { return S == kPacked ? uint32_t(a.ts) * 2 : uint32_t(D * 2); };
+    auto row_from = [&](int t, auto key) __attribute__((always_inline)) -> const char* {
+      constexpr bool KEY = decltype(key)::value;
+      if constexpr (S == kPacked) {
+        return reinterpret_cast<const char*>((KEY ? a.k : a.v) + (seq.first + t) * a.ts + kvh * a.hs);
+      } else if constexpr (S == kSlab) {
+        return reinterpret_cast<const char*>((KEY ? a.slab_k : a.slab_v) + ((int64_t(b) * a.Hkv + kvh) * a.slab_rows + t) * D);
+      } else {
+        const int page = page_of(t);
+        if (!paged::valid_page(a.pool, page)) return nullptr;
+        return static_cast<const char*>(a.slot[KEY ? 0 : 1]) +
+               paged::pool_row(a.pool, page, kvh, t & ((1 << a.pool.shift) - 1)) * (D * 2);
       }
     };
+    auto fetch = [&](int tile, auto key, int buf) __attribute__((always_inline)) {
+      constexpr bool KEY = decltype(key)::value;
+      const int tc = tile < t_hi ? tile : t_hi, ln = lane_now<D>(lane);
+      const uint32_t lds = lds_address(tiles[KEY ? buf : W::kKBufs + buf]) + wave * NP * 1024;
+      const int first = tc * KT + wave * kMine;
+      const char* base = first + kMine <= n ? row_from(first, key) : nullptr;
+      if (base) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int r = i * kPieceRows + ln / kRowPieces;
+          const int c = (ln % kRowPieces) ^ turn_of<D>(wave * kMine + r);
+          to_lds_at(base, uint32_t(r) * row_bytes() + 16 * c, lds + i * 1024);
+        }
+      } else {
+        // Past the last key, which is read again (hidden, and finite where it
+        // is), and in no page.
+        rare();
+#pragma unroll 1
+        for (int i = 0; i < NP; ++i) {
+          const int r = i * kPieceRows + ln / kRowPieces, t = min(first + r, n - 1);
+          const int c = (ln % kRowPieces) ^ turn_of<D>(wave * kMine + r);
+          const char* row = row_from(t, key);
+          to_lds((row ? row : reinterpret_cast<const char*>(kZeroRow)) + 16 * c, lds + i * 1024);
+        }
+      }
+    };
+    // Pages that are none, in the range that the block reads: looked for once.
+    bool holes = false;
+    if constexpr (S == kPagedBf16 || S == kSlab) {
+      const int32_t* table = a.pool.table + b * a.pool.tstride;
+      for (int i = (key_lo >> a.pool.shift) + tid; i <= (key_hi - 1) >> a.pool.shift; i += W::kThreads)
+        holes |= !paged::valid_page(a.pool, table[i]);
+      holes = __syncthreads_or(holes);
+    }
     // Which of the tile's groups of 16 keys lie in pages.
     auto held_groups = [&](int tile) __attribute__((always_inline)) {
-      uint32_t on = 0xffu;
-      if constexpr (S == kPagedBf16 || S == kSlab) {
-        on = 0;
+      uint32_t on = 0;
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-          if (paged::valid_page(a.pool, page_of(min(tile * KT + 16 * i, n - 1)))) on |= 1u << i;
-      }
+      for (int i = 0; i < NI; ++i)
+        if (paged::valid_page(a.pool, page_of(min(tile * KT + 16 * i, n - 1)))) on |= 1u << i;
       return on;
     };
-    // Operand reads: K piece 4 s + lg of row lr (+ 16 i rows), V piece 2 t +
-    // (lr / 2) % 2 of row 4 lg + lr / 4 (+ 16, 32 u rows).
-    const int kturn = turn_of<D>(lr), vturn = turn_of<D>(4 * lg + lr / 4);
     const bool live = row0 + wave * RW < rows;
 
     auto rescale = [&](int j, bool up, float mx) __attribute__((always_inline)) {
@@ -511,32 +588,37 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
       for (int t = 0; t < NT; ++t) o[t][j] *= alpha;
       m[j] = mn;
       nm[j] = mn == -INFINITY ? 0.0f : -mn;
-      thr[j] = (mn + kTau) / qscale[j];
+      thr[j] = (mn + kTau) * __builtin_amdgcn_rcpf(qscale[j]);  // need not be exact
     };
-    auto scores = [&](const uint16_t* K, f4_t (&sc)[NI][NR]) __attribute__((always_inline)) {
+    auto scores = [&](uint32_t K, f4_t (&sc)[NI][NR]) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int j = 0; j < NR; ++j) sc[i][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      const uint32_t at = K + k_lane<D>(lane_now<D>(lane));
+      pipelined<ND * NI, W::kGroupK, op_t>(
+          [&](int x) __attribute__((always_inline)) { return read_lds<op_t>((at ^ (64 * (x / NI))) + 16 * (x % NI) * D * 2); },
+          [&](int x, op_t ka) __attribute__((always_inline)) {
+            const int s = x / NI, i = x % NI;
 #pragma unroll
-      for (int s = 0; s < ND; ++s)
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const op_t ka = *reinterpret_cast<const op_t*>(K + (16 * i + lr) * D + ((4 * s + lg) ^ kturn) * 8);
-#pragma unroll
-          for (int j = 0; j < NR; ++j) {
-            if constexpr (F16)
-              sc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[j][s], sc[i][j], 0, 0, 0);
-            else
-              sc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[j][s], sc[i][j], 0, 0, 0);
-          }
-        }
+            for (int j = 0; j < NR; ++j) {
+              if constexpr (F16)
+                sc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[j][s], sc[i][j], 0, 0, 0);
+              else
+                sc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[j][s], sc[i][j], 0, 0, 0);
+            }
+          });
     };
     auto softmax = [&](int tile, f4_t (&sc)[NI][NR], bf8_t (&pp)[NU][NR]) __attribute__((always_inline)) {
       const int kbase = tile * KT;
       // Hidden keys, where the block sees the tile in part.
-      const uint32_t on = held_groups(tile);
-      const bool whole = kbase >= key_lo && kbase + KT <= key_hi && on == (S == kPacked ? 0xffu : (1u << NI) - 1u) &&
+      uint32_t on = (1u << NI) - 1u;
+      if constexpr (S != kPacked)
+        if (holes) {
+          rare();
+          on = held_groups(tile);
+        }
+      const bool whole = kbase >= key_lo && kbase + KT <= key_hi && on == (1u << NI) - 1u &&
                          (!a.causal || (kbase + KT - 1 <= pos_lo && (a.window <= 0 || pos_hi - a.window < kbase)));
       if (!whole) {
         rare();
@@ -583,54 +665,70 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
         }
       }
     };
-    auto values = [&](const bf8_t (&pp)[NU][NR], const uint16_t* V) __attribute__((always_inline)) {
+    auto values = [&](const bf8_t (&pp)[NU][NR], uint32_t V) __attribute__((always_inline)) {
+      const uint32_t at = V + v_lane<D>(lane_now<D>(lane));
+      pipelined<NU * NT, W::kGroupV, bf8_t>(
+          [&](int x) __attribute__((always_inline)) {
+            const uint32_t src = (at ^ (32 * (x % NT))) + 32 * (x / NT) * D * 2;
+            const u2_t y = read_transposed(src), z = read_transposed(src + 16 * D * 2);
+            return __builtin_bit_cast(bf8_t, u4_t{y.x, y.y, z.x, z.y});
+          },
+          [&](int x, bf8_t va) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < NU; ++u)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const uint16_t* src = V + (32 * u + 4 * lg + lr / 4) * D + ((2 * t + lr % 4 / 2) ^ vturn) * 8 + 4 * (lr % 2);
-          const u2_t x = read_transposed(src), y = read_transposed(src + 16 * D);
-          const bf8_t va = __builtin_bit_cast(bf8_t, u4_t{x.x, x.y, y.x, y.y});
-#pragma unroll
-          for (int j = 0; j < NR; ++j)
-            o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pp[u][j], o[t][j], 0, 0, 0);
-        }
+            for (int j = 0; j < NR; ++j)
+              o[x % NT][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pp[x / NT][j], o[x % NT][j], 0, 0, 0);
+          });
     };
 
     auto run = [&](auto late) __attribute__((always_inline)) {
       constexpr bool LATE = decltype(late)::value;
       wait_loads<0>();  // the queries
-      fetch(t_lo, 0, 0);
-      if constexpr (W::kAhead == 2) fetch(t_lo + 1, 1, 1);
-      wait_loads<(W::kAhead - 1) * 2 * NP>();
+      fetch(t_lo, kKey, 0);
+      if constexpr (W::kAhead > 0) fetch(t_lo, kValue, 0);
+      if constexpr (W::kAhead == 2) {
+        fetch(t_lo + 1, kKey, 1);
+        fetch(t_lo + 1, kValue, 1);
+      }
+      wait_loads<(W::kAhead == 2 ? 2 : 0) * NP>();
       __syncthreads();
       bf8_t pp[NU][NR];
       int kc = 0, vc = 0;
       const auto plus = [](int c, int d, int bufs) { return c + d >= bufs ? c + d - bufs : c + d; };
       for (int tile = t_lo; tile <= t_hi; ++tile) {
         // Into buffers last read before the barrier that ended the tile before.
-        fetch(tile + W::kAhead, plus(kc, W::kAhead, W::kKBufs), plus(vc, W::kAhead, W::kVBufs));
+        if constexpr (W::kAhead > 0) {
+          fetch(tile + W::kAhead, kKey, plus(kc, W::kAhead, W::kKBufs));
+          fetch(tile + W::kAhead, kValue, plus(vc, W::kAhead, W::kVBufs));
+        } else {
+          fetch(tile, kValue, 0);
+        }
         if (live) {
           if constexpr (W::kLate) __builtin_amdgcn_s_setprio(1);
           if constexpr (LATE)
-            if (tile > t_lo) values(pp, tiles[W::kKBufs + plus(vc, W::kVBufs - 1, W::kVBufs)]);
+            if (tile > t_lo) values(pp, lds_address(tiles[W::kKBufs + plus(vc, W::kVBufs - 1, W::kVBufs)]));
           f4_t sc[NI][NR];
-          scores(tiles[kc], sc);
+          scores(lds_address(tiles[kc]), sc);
           if constexpr (W::kLate) __builtin_amdgcn_s_setprio(0);
           softmax(tile, sc, pp);
-          if constexpr (!LATE) {
-            if constexpr (W::kLate) __builtin_amdgcn_s_setprio(1);
-            values(pp, tiles[W::kKBufs + vc]);
-            if constexpr (W::kLate) __builtin_amdgcn_s_setprio(0);
-          }
         }
-        wait_loads<(W::kAhead - 1) * 2 * NP>();
+        if constexpr (W::kAhead == 0) {
+          // V is here, and every wavefront is done with K.
+          wait_loads<0>();
+          __syncthreads();
+          fetch(tile + 1, kKey, 0);
+        }
+        if (!LATE && live) {
+          if constexpr (W::kLate) __builtin_amdgcn_s_setprio(1);
+          values(pp, lds_address(tiles[W::kKBufs + vc]));
+          if constexpr (W::kLate) __builtin_amdgcn_s_setprio(0);
+        }
+        wait_loads<(W::kAhead == 2 ? 2 : 0) * NP>();
         __syncthreads();
         kc = plus(kc, 1, W::kKBufs);
         vc = plus(vc, 1, W::kVBufs);
       }
       if constexpr (LATE)
-        if (live) values(pp, tiles[W::kKBufs + plus(vc, W::kVBufs - 1, W::kVBufs)]);
+        if (live) values(pp, lds_address(tiles[W::kKBufs + plus(vc, W::kVBufs - 1, W::kVBufs)]));
       wait_loads<0>();  // before the workgroup's LDS is given back
     };
     if (W::kLate && wave >= kWaves / 2) run(std::true_type{});

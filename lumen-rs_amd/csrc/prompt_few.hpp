@@ -55,7 +55,7 @@ void few_kernel(const Args a) {
   constexpr int kWaves = W::kWaves, RW = W::kRW, NR = RW / 16, KT = W::kKeys, NI = KT / 16;
   constexpr int ND = D / 32, NT = D / 16, NP = W::kPieces;
   constexpr bool AFFINE = S == kPagedAffine;
-  __shared__ __attribute__((aligned(16))) uint16_t tiles[kWaves][2][KT * D];
+  __shared__ __attribute__((aligned(1024))) uint16_t tiles[kWaves][2][KT * D];
   __shared__ float part_m[kWaves][RW], part_l[kWaves][RW];
   static_assert(sizeof(tiles[0]) >= sizeof(float) * RW * D, "what a wavefront gathered fits its tiles");
   const int tid = threadIdx.x, lane = tid % kWave, lr = lane % 16, lg = lane / 16;
@@ -116,14 +116,14 @@ void few_kernel(const Args a) {
     typedef const __attribute__((address_space(4))) int32_t* constant;
     return ((constant)(a.pool.table + b * a.pool.tstride))[t >> a.pool.shift];
   };
-  const int kturn = turn_of<D>(lr), vturn = turn_of<D>(4 * lg + lr / 4);
 
   auto scores = [&](const uint16_t* from, f4_t (&sc)[NI][NR]) __attribute__((always_inline)) {
+    const uint32_t at = lds_address(from) + k_lane<D>(lane);
 #pragma unroll
     for (int s = 0; s < ND; ++s)
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const bf8_t ka = *reinterpret_cast<const bf8_t*>(from + (16 * i + lr) * D + ((4 * s + lg) ^ kturn) * 8);
+        const bf8_t ka = read_lds<bf8_t>((at ^ (64 * s)) + 16 * i * D * 2);
 #pragma unroll
         for (int j = 0; j < NR; ++j)
           sc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[j][s], sc[i][j], 0, 0, 0);
@@ -185,10 +185,10 @@ void few_kernel(const Args a) {
     }
   };
   auto values = [&](const bf8_t (&pp)[NR]) __attribute__((always_inline)) {
+    const uint32_t at = lds_address(V) + v_lane<D>(lane);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const uint16_t* src = V + (4 * lg + lr / 4) * D + ((2 * t + lr % 4 / 2) ^ vturn) * 8 + 4 * (lr % 2);
-      const u2_t x = read_transposed(src), y = read_transposed(src + 16 * D);
+      const u2_t x = read_transposed(at ^ (32 * t)), y = read_transposed((at ^ (32 * t)) + 16 * D * 2);
       const bf8_t va = __builtin_bit_cast(bf8_t, u4_t{x.x, x.y, y.x, y.y});
 #pragma unroll
       for (int j = 0; j < NR; ++j)

@@ -120,6 +120,7 @@ def test_packed_refusals():
                           (dict(batch=0), T.EINVAL_SHAPE), (dict(batch=1025), T.EUNSUPPORTED), (dict(D=96), T.EUNSUPPORTED),
                           (dict(D=0), T.EUNSUPPORTED), (dict(H=0), T.EINVAL_SHAPE), (dict(H=6), T.EINVAL_SHAPE), (dict(H_kv=0), T.EINVAL_SHAPE),
                           (dict(H=132), T.EUNSUPPORTED), (dict(tokens=-1), T.EINVAL_SHAPE), (dict(tokens=1 << 31), T.EINVAL_SHAPE),
+                          (dict(token_stride=-1024), T.EUNSUPPORTED), (dict(token_stride=1 << 27), T.EUNSUPPORTED),
                           (dict(window=4, causal=False), T.EINVAL_ARG)]:
         refused(status, T.packed_attend, **{**ok, **other})
     T.packed_attend(**{**ok, "tokens": 0, "q": None})
