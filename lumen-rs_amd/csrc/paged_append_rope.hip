@@ -13,7 +13,7 @@ namespace paged {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMostTokens = 8;
+using rope::kMostTokens;
 
 struct EnterArgs {
   Pool pool;
@@ -27,6 +27,7 @@ struct EnterArgs {
   const int32_t* positions;
   void* slot[6];
   int H, gs, per_block;
+  rope::Jobs q_jobs, k_jobs;
 };
 
 // A token's place in the workgroup: its rotary position, and its pool row of
@@ -49,10 +50,10 @@ __device__ __forceinline__ void find_places(const EnterArgs& a, int64_t t0, int 
     place[t] = Place{position, row ? pool_row(p, s.x, 0, s.y) : -1};
   }
   if (turn)
-    for (int i = threadIdx.x; i < n * a.rope.pairs; i += kThreads) {
-      const int t = i / a.rope.pairs;
+    for (int t = 0; t < n; ++t) {
       const int position = a.positions ? a.positions[(t0 + t) * a.pstride] : a.slots[t0 + t].z;
-      angles[i] = rope::angle_of(a.rope, position, i % a.rope.pairs);
+      for (int pair = threadIdx.x; pair < a.rope.pairs; pair += kThreads)
+        angles[t * a.rope.pairs + pair] = rope::angle_of(a.rope, position, pair);
     }
   __syncthreads();
 }
@@ -71,24 +72,24 @@ __device__ __forceinline__ void clear_weights(const EnterArgs& a, int64_t t0, in
 }
 
 __device__ __forceinline__ void enter_queries(const EnterArgs& a, int64_t t0, int n, int dim,
-                                              const Place* place, const rope::Angle* angles) {
+                                              Place* place, rope::Angle* angles) {
   rope::turn_rows<kThreads>(
-      a.rope, angles, n, a.H, dim, a.q != a.q_out,
+      a.rope, a.q_jobs, angles, n, dim,
       [&](int t, int h) { return a.q + (t0 + t) * a.qs + h * dim; },
       [&](int t, int h) -> uint16_t* {
         return place[t].position < 0 ? nullptr : a.q_out + (t0 + t) * a.qos + h * dim;
-      });
+      },
+      [&]() { find_places(a, t0, n, true, place, angles); });
 }
 
 template <int D>
 __global__ __launch_bounds__(kThreads) void enter_bf16_kernel(const EnterArgs a) {
   __shared__ Place place[kMostTokens];
-  __shared__ rope::Angle angles[kMostTokens * (D / 2)];
+  extern __shared__ rope::Angle angles[];  // [per_block][pairs]
   const Pool& p = a.pool;
   const int64_t t0 = int64_t(blockIdx.x) * a.per_block;
   const int n = a.tokens - t0 < a.per_block ? int(a.tokens - t0) : a.per_block;
   const int part = blockIdx.y;
-  find_places(a, t0, n, part != kValues, place, angles);
   if (part == kQueries) return enter_queries(a, t0, n, D, place, angles);
   const uint16_t* x = part == kKeys ? a.k : a.v;
   uint16_t* out = static_cast<uint16_t*>(a.slot[part]);
@@ -97,10 +98,12 @@ __global__ __launch_bounds__(kThreads) void enter_bf16_kernel(const EnterArgs a)
     return place[t].row < 0 ? nullptr : out + (place[t].row + (int64_t(h) << p.shift)) * D;
   };
   if (part == kKeys) {
-    rope::turn_rows<kThreads>(a.rope, angles, n, p.Hkv, D, true, from, to);
+    rope::turn_rows<kThreads>(a.rope, a.k_jobs, angles, n, D, from, to,
+                              [&]() { find_places(a, t0, n, true, place, angles); });
     clear_weights(a, t0, n, place);
     return;
   }
+  find_places(a, t0, n, false, place, angles);
   constexpr int LPR = D / 8;
   for (int i = threadIdx.x; i < n * p.Hkv * LPR; i += kThreads) {
     const int r = i / LPR, c = i % LPR * 8;
@@ -142,13 +145,13 @@ __device__ __forceinline__ void load_turned(const rope::Rope& r, const rope::Ang
 template <int D, int BK, int BV>
 __global__ __launch_bounds__(kThreads) void enter_affine_kernel(const EnterArgs a) {
   __shared__ Place place[kMostTokens];
-  __shared__ rope::Angle angles[kMostTokens * (D / 2)];
+  extern __shared__ rope::Angle angles[];  // [per_block][pairs]
   const Pool& p = a.pool;
   const int64_t t0 = int64_t(blockIdx.x) * a.per_block;
   const int n = a.tokens - t0 < a.per_block ? int(a.tokens - t0) : a.per_block;
   const int part = blockIdx.y;
-  find_places(a, t0, n, part != kValues, place, angles);
   if (part == kQueries) return enter_queries(a, t0, n, D, place, angles);
+  find_places(a, t0, n, part != kValues, place, angles);
   constexpr int LPR = D / aq::kLaneElems;
   const int bits = part == kKeys ? BK : BV;
   const uint16_t* x = part == kKeys ? a.k : a.v;
@@ -191,7 +194,8 @@ template <int D>
 void launch(const tqkv_paged_kv* kv, const EnterArgs& a, hipStream_t st) {
   const unsigned blocks = unsigned((a.tokens + a.per_block - 1) / a.per_block);
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(blocks, a.H > 0 ? 3 : 2), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(kernel, dim3(blocks, a.H > 0 ? 3 : 2), dim3(kThreads),
+                       a.per_block * a.rope.pairs * sizeof(rope::Angle), st, a);
   };
   if (kv->kind == TQKV_CACHE_BF16) go(enter_bf16_kernel<D>);
   else if (kv->bits_k == 4 && kv->bits_v == 4) go(enter_affine_kernel<D, 4, 4>);
@@ -246,7 +250,9 @@ extern "C" int32_t tqkv_paged_append_rope(const tqkv_paged_kv* kv, const tqkv_ro
   for (int i = 0; i < 6; ++i) a.slot[i] = kv->slot[i];
   a.H = H;
   a.gs = kv->group_size;
-  a.per_block = 1;
+  a.q_jobs = rope::jobs_of(a.rope, H, kv->dim, q != q_out);
+  a.k_jobs = rope::jobs_of(a.rope, kv->kv_heads, kv->dim, true);
+  a.per_block = rope::tokens_of(a.k_jobs, tokens);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (kv->dim) {
     case 64: launch<64>(kv, a, st); break;

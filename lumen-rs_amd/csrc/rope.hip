@@ -25,7 +25,6 @@ int32_t check(const tqkv_rope* rope, int32_t dim, Rope* out) {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMostTokens = 8;
 
 struct ApplyArgs {
   Rope rope;
@@ -33,27 +32,29 @@ struct ApplyArgs {
   int64_t pstride, tokens, xts, xhs, ots, ohs;
   const uint16_t* x;
   uint16_t* out;
-  int heads, dim, per_block;
-  bool copy;  // the channels behind the rotated ones too
+  int dim, per_block;
+  Jobs jobs;
 };
 
 __global__ __launch_bounds__(kThreads) void rope_kernel(const ApplyArgs a) {
-  __shared__ Angle angles[kMostTokens * kMostPairs];
+  extern __shared__ Angle angles[];  // [per_block][pairs]
   __shared__ int32_t positions[kMostTokens];
   const int64_t t0 = int64_t(blockIdx.x) * a.per_block;
   const int n = a.tokens - t0 < a.per_block ? int(a.tokens - t0) : a.per_block;
-  for (int i = threadIdx.x; i < n * a.rope.pairs; i += kThreads) {
-    const int t = i / a.rope.pairs, pair = i % a.rope.pairs;
-    const int position = a.positions[(t0 + t) * a.pstride];
-    angles[i] = angle_of(a.rope, position, pair);
-    if (pair == 0) positions[t] = position;
-  }
-  __syncthreads();
   turn_rows<kThreads>(
-      a.rope, angles, n, a.heads, a.dim, a.copy,
+      a.rope, a.jobs, angles, n, a.dim,
       [&](int t, int h) { return a.x + (t0 + t) * a.xts + h * a.xhs; },
       [&](int t, int h) -> uint16_t* {
         return positions[t] < 0 ? nullptr : a.out + (t0 + t) * a.ots + h * a.ohs;
+      },
+      [&]() {
+        for (int t = 0; t < n; ++t) {
+          const int position = a.positions[(t0 + t) * a.pstride];
+          if (threadIdx.x == 0) positions[t] = position;
+          for (int pair = threadIdx.x; pair < a.rope.pairs; pair += kThreads)
+            angles[t * a.rope.pairs + pair] = angle_of(a.rope, position, pair);
+        }
+        __syncthreads();
       });
 }
 
@@ -141,13 +142,12 @@ extern "C" int32_t tqkv_rope_apply(const tqkv_rope* rope, const int32_t* positio
   a.ohs = out_head_stride;
   a.x = x;
   a.out = out;
-  a.heads = heads;
   a.dim = dim;
-  a.copy = !same;
-  a.per_block = 1;
+  a.jobs = jobs_of(a.rope, heads, dim, !same);
+  a.per_block = tokens_of(a.jobs, tokens);
   const int64_t blocks = (tokens + a.per_block - 1) / a.per_block;
-  hipLaunchKernelGGL(rope_kernel, dim3(unsigned(blocks)), dim3(kThreads), 0,
-                     reinterpret_cast<hipStream_t>(stream), a);
+  hipLaunchKernelGGL(rope_kernel, dim3(unsigned(blocks)), dim3(kThreads),
+                     a.per_block * a.rope.pairs * sizeof(Angle), reinterpret_cast<hipStream_t>(stream), a);
   TQKV_LAUNCHED();
   return ok();
 }

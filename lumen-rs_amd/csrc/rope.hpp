@@ -74,48 +74,106 @@ __device__ __forceinline__ void turn_halves(uint4& x, uint4& y, const Angle* a) 
   y = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// The heads of a workgroup's tokens. A job is what one thread turns or copies
-// at once: eight channels (neighbours, and channels behind the rotated ones),
+// A quotient by a number fixed for a launch: x / d for x * d below 2^32.
+struct Divisor {
+  uint32_t d, m;
+};
+inline Divisor divisor(int d) { return Divisor{uint32_t(d), uint32_t(((uint64_t(1) << 32) + d - 1) / d)}; }
+__device__ __forceinline__ uint32_t quotient(uint32_t x, Divisor d) { return d.d == 1 ? x : __umulhi(x, d.m); }
+
+// The heads of a workgroup's tokens as jobs, what one thread turns or copies at
+// once: eight channels (neighbours, and channels behind the rotated ones),
 // twice eight (halves that are whole pieces of eight) or single pairs and
-// channels (other halves). from(t, h) and to(t, h): rows of token t and head
-// h; to gives NULL where nothing is written. angles: [tokens][pairs] in LDS.
-// A pair's two channels are read and written by one thread, so rows may turn
-// in place.
-template <int Threads, typename From, typename To>
-__device__ __forceinline__ void turn_rows(const Rope& r, const Angle* angles, int tokens, int heads,
-                                          int dim, bool copy, From from, To to) {
+// channels (other halves). A pair's two channels are read and written by one
+// thread, so rows may turn in place.
+struct Jobs {
+  Divisor a_head, a_token;  // jobs
+  int turning;              // of a head; the others copy
+  int singles;
+};
+inline Jobs jobs_of(const Rope& r, int heads, int dim, bool copy) {
   const int rd = 2 * r.pairs;
-  const bool singles = !r.interleaved && r.pairs % 8 != 0;
-  const int turning = singles ? r.pairs : r.interleaved ? (rd + 7) / 8 : r.pairs / 8;
-  const int behind = singles ? dim - rd : (dim - (r.interleaved ? turning * 8 : rd)) / 8;
-  const int jobs = turning + (copy ? behind : 0);
-  const int per_token = jobs * heads, all = per_token * tokens;
-  for (int i = threadIdx.x; i < all; i += Threads) {
-    const int t = i / per_token, h = i % per_token / jobs, j = i % jobs;
-    uint16_t* dst = to(t, h);
-    if (!dst) continue;
-    const uint16_t* src = from(t, h);
-    const Angle* a = angles + t * r.pairs;
-    if (singles) {
-      if (j < turning) {
+  Jobs j;
+  j.singles = !r.interleaved && r.pairs % 8 != 0;
+  j.turning = j.singles ? r.pairs : r.interleaved ? (rd + 7) / 8 : r.pairs / 8;
+  const int behind = j.singles ? dim - rd : (dim - (r.interleaved ? j.turning * 8 : rd)) / 8;
+  const int each = j.turning + (copy ? behind : 0);
+  j.a_head = divisor(each);
+  j.a_token = divisor(each * (heads > 0 ? heads : 1));
+  return j;
+}
+// Tokens a workgroup: enough jobs for every thread to have kDeep on their way.
+constexpr int kDeep = 4, kMostTokens = 8;
+inline int tokens_of(const Jobs& j, int64_t tokens) {
+  int n = 1;
+  while (n < kMostTokens && n * int(j.a_token.d) < 1024 && tokens >= 512 * n) n *= 2;
+  return n;
+}
+
+// from(t, h) and to(t, h): rows of token t and head h; to gives NULL where
+// nothing is written. ready() makes the angles, [tokens][pairs] in LDS, and
+// what `to` needs, barrier included: the first jobs' channels are on their way
+// meanwhile.
+template <int Threads, typename From, typename To, typename Ready>
+__device__ __forceinline__ void turn_rows(const Rope& r, const Jobs& jobs, const Angle* angles,
+                                          int tokens, int dim, From from, To to, Ready ready) {
+  const uint32_t all = jobs.a_token.d * tokens;
+  const int rd = 2 * r.pairs;
+  if (jobs.singles) {
+    ready();
+    for (uint32_t i = threadIdx.x; i < all; i += Threads) {
+      const int t = quotient(i, jobs.a_token), in = i - t * jobs.a_token.d;
+      const int h = quotient(in, jobs.a_head), j = in - h * jobs.a_head.d;
+      uint16_t* dst = to(t, h);
+      if (!dst) continue;
+      const uint16_t* src = from(t, h);
+      if (j < jobs.turning) {
+        const Angle a = angles[t * r.pairs + j];
         const float x = bf16_to_f32(src[j]), y = bf16_to_f32(src[j + r.pairs]);
-        dst[j] = f32_to_bf16(turned_x(x, y, a[j]));
-        dst[j + r.pairs] = f32_to_bf16(turned_y(x, y, a[j]));
+        dst[j] = f32_to_bf16(turned_x(x, y, a));
+        dst[j + r.pairs] = f32_to_bf16(turned_y(x, y, a));
       } else {
-        dst[rd + j - turning] = src[rd + j - turning];
+        dst[rd + j - jobs.turning] = src[rd + j - jobs.turning];
       }
-    } else if (j >= turning) {
-      const int c = dim - 8 * (jobs - j);
-      *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-    } else if (r.interleaved) {
-      const uint4 x = *reinterpret_cast<const uint4*>(src + 8 * j);
-      *reinterpret_cast<uint4*>(dst + 8 * j) = turn_neighbours(x, a, 4 * j, r.pairs);
-    } else {
-      uint4 x = *reinterpret_cast<const uint4*>(src + 8 * j);
-      uint4 y = *reinterpret_cast<const uint4*>(src + 8 * j + r.pairs);
-      turn_halves(x, y, a + 8 * j);
-      *reinterpret_cast<uint4*>(dst + 8 * j) = x;
-      *reinterpret_cast<uint4*>(dst + 8 * j + r.pairs) = y;
+    }
+    return;
+  }
+  bool first = true;
+  for (uint32_t i0 = 0; i0 < all || first; i0 += Threads * kDeep) {
+    uint4 x[kDeep], y[kDeep];
+    int t[kDeep], h[kDeep], j[kDeep];
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      const uint32_t i = i0 + k * Threads + threadIdx.x;
+      t[k] = -1;
+      if (i < all) {
+        t[k] = quotient(i, jobs.a_token);
+        const uint32_t in = i - t[k] * jobs.a_token.d;
+        h[k] = quotient(in, jobs.a_head);
+        j[k] = in - h[k] * jobs.a_head.d;
+        const bool copied = j[k] >= jobs.turning;
+        const uint16_t* src = from(t[k], h[k]);
+        x[k] = *reinterpret_cast<const uint4*>(src + (copied ? dim - 8 * (int(jobs.a_head.d) - j[k]) : 8 * j[k]));
+        if (!copied && !r.interleaved) y[k] = *reinterpret_cast<const uint4*>(src + 8 * j[k] + r.pairs);
+      }
+    }
+    if (first) ready();
+    first = false;
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      if (t[k] < 0) continue;
+      uint16_t* dst = to(t[k], h[k]);
+      if (!dst) continue;
+      const Angle* a = angles + t[k] * r.pairs;
+      if (j[k] >= jobs.turning) {
+        *reinterpret_cast<uint4*>(dst + dim - 8 * (int(jobs.a_head.d) - j[k])) = x[k];
+      } else if (r.interleaved) {
+        *reinterpret_cast<uint4*>(dst + 8 * j[k]) = turn_neighbours(x[k], a, 4 * j[k], r.pairs);
+      } else {
+        turn_halves(x[k], y[k], a + 8 * j[k]);
+        *reinterpret_cast<uint4*>(dst + 8 * j[k]) = x[k];
+        *reinterpret_cast<uint4*>(dst + 8 * j[k] + r.pairs) = y[k];
+      }
     }
   }
 }
