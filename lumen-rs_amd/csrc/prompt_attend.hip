@@ -130,14 +130,14 @@ struct Plan {
 };
 // Workgroups that splits make up to, and keys that a split holds at least.
 constexpr int64_t kWanted = 384, kWantedFew = 2048;
-constexpr int64_t kLeastKeys = 512, kLeastFew = 256;
+constexpr int64_t kLeastKeys = 512, kLeastFew = 512;
 
 bool plan_of(int batch, int H, int Hkv, int D, int64_t tokens, int64_t keys, Source source, Plan* out) {
   const int G = H / Hkv;
   const int64_t sequences = tokens < batch ? tokens : batch, rows = tokens * G;
   Plan p{};
   // Rows of a sequence on the average: the host knows no more.
-  const int64_t few_rows = D >= 256 ? Few<256>::kRows : Few<128>::kRows;
+  const int64_t few_rows = D >= 256 ? Few<256, false>::kRows : Few<128, false>::kRows;
   p.few = source != kPacked && rows <= sequences * few_rows;
   const int64_t block = p.few ? few_rows
                         : D <= 128 ? Shape<128>::kRows

@@ -259,10 +259,13 @@ __device__ __forceinline__ void wait_loads() {
   __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
-// Reads at an LDS address.
+// Reads and writes at an LDS address.
 template <typename T>
 __device__ __forceinline__ T read_lds(uint32_t at) {
   return *reinterpret_cast<const __attribute__((address_space(3))) T*>(at);
+}
+__device__ __forceinline__ void write_lds(uint32_t at, u4_t x) {
+  *reinterpret_cast<__attribute__((address_space(3))) u4_t*>(at) = x;
 }
 __device__ __forceinline__ u2_t read_transposed(uint32_t at) {
   return __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -415,6 +418,53 @@ __device__ __forceinline__ bool find_block(const Args& a, int id, int each, Bloc
   return out->row0 < int64_t(out->seq.count) * a.G;
 }
 
+__device__ __forceinline__ f4_t product(bf8_t x, bf8_t y, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+}
+__device__ __forceinline__ f4_t product(h8_t x, h8_t y, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+}
+
+// A query row as the products' operand (lane group g holds channels 32 s + 8 g
+// + [0, 8)), its sign that of the scale; returns what takes its scores to log2
+// units, which is not negative. As f16 the row is taken times a power of two
+// that brings its largest channel into [2^14, 2^15): channels below 2^-28 of
+// that lose bits.
+template <int D, typename Op>
+__device__ __forceinline__ float load_query(const Args& a, const uint16_t* src, int g, Op (&qf)[D / 32]) {
+  const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+  float scale = fabsf(a.scale) * kLog2e;
+  u4_t x[D / 32];
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+    x[s] = *reinterpret_cast<const u4_t*>(src + 32 * s + 8 * g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[s][e] ^= flip;
+    if constexpr (std::is_same_v<Op, bf8_t>) qf[s] = __builtin_bit_cast(bf8_t, x[s]);
+  }
+  if constexpr (std::is_same_v<Op, h8_t>) {
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        top = fmaxf(top, fabsf(__uint_as_float(x[s][e] << 16)));
+        top = fmaxf(top, fabsf(__uint_as_float(x[s][e] & 0xffff0000u)));
+      }
+    top = row_max(top);
+    const int up = top > 0.0f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        qf[s][2 * e] = _Float16(ldexpf(__uint_as_float(x[s][e] << 16), up));
+        qf[s][2 * e + 1] = _Float16(ldexpf(__uint_as_float(x[s][e] & 0xffff0000u), up));
+      }
+    scale = ldexpf(scale, -up);
+  }
+  return scale;
+}
+
 template <int D, Source S>
 __global__ __launch_bounds__(Shape<D>::kThreads)
 __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(const Args a) {
@@ -452,45 +502,14 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
   op_t qf[NR][ND];
   int pos[NR];       // of this lane's rows
   float qscale[NR];  // scores to log2 units
-  const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
   auto row_at = [&](int j) __attribute__((always_inline)) { return row0 + wave * RW + 16 * j + lr; };
 #pragma unroll
   for (int j = 0; j < NR; ++j) {
     const int64_t r = row_at(j) < rows ? row_at(j) : rows - 1;
     pos[j] = p0 + int(r / a.G);
     const uint16_t* src = a.q + (seq.first + r / a.G) * a.qs + (int64_t(kvh) * a.G + r % a.G) * D;
-    qscale[j] = a.scale * sign * kLog2e;
-    u4_t x[ND];
-    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
-    for (int s = 0; s < ND; ++s) {
-      x[s] = *reinterpret_cast<const u4_t*>(src + 32 * s + 8 * lg);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[s][e] ^= flip;
-      if constexpr (!F16) qf[j][s] = __builtin_bit_cast(bf8_t, x[s]);
-    }
-    if constexpr (F16) {
-      // The row as f16, its largest channel in [2^14, 2^15): channels below
-      // 2^-28 of it lose bits.
-      float top = 0.0f;
-#pragma unroll
-      for (int s = 0; s < ND; ++s)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          top = fmaxf(top, fabsf(__uint_as_float(x[s][e] << 16)));
-          top = fmaxf(top, fabsf(__uint_as_float(x[s][e] & 0xffff0000u)));
-        }
-      top = row_max(top);
-      const int e2 = top > 0.0f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-#pragma unroll
-      for (int s = 0; s < ND; ++s)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          qf[j][s][2 * e] = _Float16(ldexpf(__uint_as_float(x[s][e] << 16), e2));
-          qf[j][s][2 * e + 1] = _Float16(ldexpf(__uint_as_float(x[s][e] & 0xffff0000u), e2));
-        }
-      qscale[j] = ldexpf(qscale[j], a.exponent[b * a.Hkv + kvh] - e2);
-    }
+    qscale[j] = load_query<D>(a, src, lg, qf[j]);
+    if constexpr (F16) qscale[j] = ldexpf(qscale[j], a.exponent[b * a.Hkv + kvh]);
   }
 
   // Per row: the running maximum (log2 units), its negative (0 while no key
@@ -601,12 +620,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
           [&](int x, op_t ka) __attribute__((always_inline)) {
             const int s = x / NI, i = x % NI;
 #pragma unroll
-            for (int j = 0; j < NR; ++j) {
-              if constexpr (F16)
-                sc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[j][s], sc[i][j], 0, 0, 0);
-              else
-                sc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[j][s], sc[i][j], 0, 0, 0);
-            }
+            for (int j = 0; j < NR; ++j) sc[i][j] = product(ka, qf[j][s], sc[i][j]);
           });
     };
     auto softmax = [&](int tile, f4_t (&sc)[NI][NR], bf8_t (&pp)[NU][NR]) __attribute__((always_inline)) {
@@ -801,13 +815,28 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const Args a) {
   for (int c = 0; c < C; ++c) o[c] = 0.0f;
   if (see.lo < see.hi) {
     const int s0 = see.lo / a.split_keys, s1 = (see.hi - 1) / a.split_keys;
-    for (int s = s0; s <= s1; ++s) m = fmaxf(m, a.part_m[slot0 + s]);
-    for (int s = s0; s <= s1; ++s) {
-      const float ms = a.part_m[slot0 + s], f = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - m);
-      l = fmaf(f, a.part_l[slot0 + s], l);
+    for (int s = s0 + lane; s <= s1; s += kWave) m = fmaxf(m, a.part_m[slot0 + s]);
 #pragma unroll
-      for (int c = 0; c < C; ++c) o[c] = fmaf(f, a.part_o[(slot0 + s) * D + c * kWave + lane], o[c]);
+    for (int d = 32; d > 0; d /= 2) m = fmaxf(m, __shfl_xor(m, d, kWave));
+    // 64 splits at a time: a lane a split for the factors, then channels.
+    for (int s = s0; s <= s1; s += kWave) {
+      float f = 0.0f;
+      if (s + lane <= s1) {
+        const float ms = a.part_m[slot0 + s + lane];
+        f = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - m);
+        l = fmaf(f, a.part_l[slot0 + s + lane], l);
+      }
+      const float* part = a.part_o + (slot0 + s) * D + lane;
+      const int count = min(kWave, s1 + 1 - s);
+#pragma unroll 8
+      for (int i = 0; i < count; ++i) {
+        const float fi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i));
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c] = fmaf(fi, part[i * D + c * kWave], o[c]);
+      }
     }
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) l += __shfl_xor(l, d, kWave);
   }
   const float inv = 1.0f / l;
   bool bad = !(l > 0.0f);

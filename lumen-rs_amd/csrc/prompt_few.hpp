@@ -7,9 +7,10 @@
 // while K meets Q). What the wavefronts gathered meets in LDS at the end.
 //
 // Affine rows are dequantized on the way into LDS, out of registers that the
-// next tile's codes have been loaded into meanwhile: V to bf16, K to a pair of
-// bf16 (16 bits: one bf16 would cost the scores what their sums keep), whose
-// second halves lie where V's tile will.
+// next tile's codes have been loaded into meanwhile: V to bf16, K to f16 (one
+// bf16 would cost the scores what their sums keep), every row times a power of
+// two that brings the largest value its scales and biases allow below 2^15,
+// which its scores take back.
 #pragma once
 
 #include "prompt_attend.hpp"
@@ -17,17 +18,24 @@
 namespace tqkv {
 namespace prompt {
 
-template <int D>
+template <int D, bool AFFINE>
 struct Few {
-  static constexpr int kWaves = D == 512 ? 2 : 4;
+  // (bf16 tiles of 32 KB for K and for V at D = 512: two wavefronts.)
+  static constexpr int kWaves = D == 512 && !AFFINE ? 2 : 4;
   static constexpr int kRW = D >= 256 ? 16 : 32;
   static constexpr int kRows = kRW;  // a block
   static constexpr int kThreads = kWaves * kWave;
   static constexpr int kKeys = 32;
   static constexpr int kPieces = kKeys * D * 2 / 1024;
-  // Blocks that a CU's LDS holds, as wavefronts a SIMD.
-  static constexpr int kPerEu = D == 64 ? 3 : D == 128 ? 2 : 1;
+  static constexpr int kGroup = D == 128 ? 8 : 4;  // operand reads in flight
+  // Tiles in a wavefront's LDS: K's and V's, or one for both in turn.
+  static constexpr int kBufs = AFFINE && D >= 256 ? 1 : 2;
+  // Blocks that a CU's LDS (and registers) hold, as wavefronts a SIMD.
+  static constexpr int kPerEu = D == 64 ? 3 : D == 128 || (D == 256 && AFFINE) ? 2 : 1;
 };
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ h2_t as_h2(uint32_t x) { return __builtin_bit_cast(h2_t, x); }
 
 // 16 codes of 4 or 8 bits out of w (2 or 4 words) as f32.
 template <int BITS>
@@ -48,14 +56,42 @@ __device__ __forceinline__ void codes16(const uint32_t* w, float (&f)[16]) {
   }
 }
 
+// The same as scale * code + bias in f16, rounded once, two an instruction: the
+// bits 0x6400 | c are 1,024 + c exactly (a byte's upper code 1,024 + 16 c), one
+// multiply-add takes the rest off exactly, one more scales.
+template <int BITS>
+__device__ __forceinline__ void halves16(const uint32_t* w, h2_t s, h2_t z, uint32_t (&x)[8]) {
+  constexpr uint32_t k1024 = 0x64646464u;
+  if constexpr (BITS == 8) {
+    const h2_t one = {_Float16(1.0f), _Float16(1.0f)}, off = {_Float16(-1024.0f), _Float16(-1024.0f)};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t at = 2 * (i % 2);
+      const h2_t c = __builtin_elementwise_fma(
+          as_h2(__builtin_amdgcn_perm(w[i / 2], k1024, (4u + at) | ((5u + at) << 16))), one, off);
+      x[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, s, z));
+    }
+  } else {
+    const h2_t mul = {_Float16(1.0f), _Float16(0.0625f)}, off = {_Float16(-1024.0f), _Float16(-64.0f)};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t at = 4u + i % 4;
+      const uint32_t y = __builtin_amdgcn_perm(w[i / 4], k1024, at | (at << 16)) & 0x64f0640fu;
+      const h2_t c = __builtin_elementwise_fma(as_h2(y), mul, off);
+      x[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, s, z));
+    }
+  }
+}
+
 template <int D, Source S, int BK, int BV>
-__global__ __launch_bounds__(Few<D>::kThreads) __attribute__((amdgpu_waves_per_eu(Few<D>::kPerEu)))
-void few_kernel(const Args a) {
-  typedef Few<D> W;
+__global__ __launch_bounds__((Few<D, S == kPagedAffine>::kThreads))
+__attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few_kernel(const Args a) {
+  typedef Few<D, S == kPagedAffine> W;
   constexpr int kWaves = W::kWaves, RW = W::kRW, NR = RW / 16, KT = W::kKeys, NI = KT / 16;
   constexpr int ND = D / 32, NT = D / 16, NP = W::kPieces;
   constexpr bool AFFINE = S == kPagedAffine;
-  __shared__ __attribute__((aligned(1024))) uint16_t tiles[kWaves][2][KT * D];
+  __shared__ __attribute__((aligned(1024))) uint16_t tiles[kWaves][W::kBufs][KT * D];
+  __shared__ __attribute__((aligned(16))) int32_t shifts[AFFINE ? kWaves : 1][KT];
   __shared__ float part_m[kWaves][RW], part_l[kWaves][RW];
   static_assert(sizeof(tiles[0]) >= sizeof(float) * RW * D, "what a wavefront gathered fits its tiles");
   const int tid = threadIdx.x, lane = tid % kWave, lr = lane % 16, lg = lane / 16;
@@ -82,26 +118,18 @@ void few_kernel(const Args a) {
   const int t_lo = key_lo / KT, t_hi = (key_hi - 1) / KT;  // used where key_lo < key_hi
   const bool working = key_lo < key_hi && t_lo + wave <= t_hi;
 
-  bf8_t qf[NR][ND];
+  using op_t = std::conditional_t<AFFINE, h8_t, bf8_t>;
+  op_t qf[NR][ND];
   int pos[NR];
-  const float sign = a.scale < 0.0f ? -1.0f : 1.0f, qscale = a.scale * sign * kLog2e;
+  float qscale[NR];
 #pragma unroll
   for (int j = 0; j < NR; ++j) {
     const int64_t at = row0 + 16 * j + lr, r = at < rows ? at : rows - 1;
     pos[j] = p0 + int(r / a.G);
-    const uint16_t* src = a.q + (seq.first + r / a.G) * a.qs + (int64_t(kvh) * a.G + r % a.G) * D;
-    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
-    for (int s = 0; s < ND; ++s) {
-      u4_t x = *reinterpret_cast<const u4_t*>(src + 32 * s + 8 * lg);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] ^= flip;
-      qf[j][s] = __builtin_bit_cast(bf8_t, x);
-    }
+    qscale[j] = load_query<D>(a, a.q + (seq.first + r / a.G) * a.qs + (int64_t(kvh) * a.G + r % a.G) * D, lg, qf[j]);
   }
   float m[NR], nm[NR], thr[NR], lsum[NR];
   f4_t o[NT][NR];
-  const float iqs = 1.0f / qscale;
 #pragma unroll
   for (int j = 0; j < NR; ++j) {
     m[j] = thr[j] = -INFINITY;
@@ -111,23 +139,20 @@ void few_kernel(const Args a) {
   }
 
   uint16_t* K = tiles[wave][0];
-  uint16_t* V = tiles[wave][1];
+  uint16_t* V = tiles[wave][W::kBufs - 1];
   auto page_of = [&](int t) __attribute__((always_inline)) {
     typedef const __attribute__((address_space(4))) int32_t* constant;
     return ((constant)(a.pool.table + b * a.pool.tstride))[t >> a.pool.shift];
   };
 
   auto scores = [&](const uint16_t* from, f4_t (&sc)[NI][NR]) __attribute__((always_inline)) {
-    const uint32_t at = lds_address(from) + k_lane<D>(lane);
+    const uint32_t at = lds_address(from) + k_lane<D>(lane_now<AFFINE ? 512 : D>(lane));
+    pipelined<ND * NI, W::kGroup, op_t>(
+        [&](int x) __attribute__((always_inline)) { return read_lds<op_t>((at ^ (64 * (x / NI))) + 16 * (x % NI) * D * 2); },
+        [&](int x, op_t ka) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 0; s < ND; ++s)
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const bf8_t ka = read_lds<bf8_t>((at ^ (64 * s)) + 16 * i * D * 2);
-#pragma unroll
-        for (int j = 0; j < NR; ++j)
-          sc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, qf[j][s], sc[i][j], 0, 0, 0);
-      }
+          for (int j = 0; j < NR; ++j) sc[x % NI][j] = product(ka, qf[j][x / NI], sc[x % NI][j]);
+        });
   };
   auto softmax = [&](int tile, f4_t (&sc)[NI][NR], bf8_t (&pp)[NR]) __attribute__((always_inline)) {
     const int kbase = tile * KT;
@@ -163,21 +188,21 @@ void few_kernel(const Args a) {
         rare();
         mx = row_max(mx);
         const bool up = mx > thr[j];
-        const float mn = up ? mx * qscale : m[j];
+        const float mn = up ? mx * qscale[j] : m[j];
         const float alpha = up ? __builtin_amdgcn_exp2f(m[j] - mn) : 1.0f;
         lsum[j] *= alpha;
 #pragma unroll
         for (int t = 0; t < NT; ++t) o[t][j] *= alpha;
         m[j] = mn;
         nm[j] = mn == -INFINITY ? 0.0f : -mn;
-        thr[j] = (mn + kTau) * iqs;
+        thr[j] = (mn + kTau) * __builtin_amdgcn_rcpf(qscale[j]);
       }
       u4_t w;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const f4_t s = sc[e / 2][j];
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2)], qscale, nm[j]));
-        const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2) + 1], qscale, nm[j]));
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2)], qscale[j], nm[j]));
+        const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2) + 1], qscale[j], nm[j]));
         w[e] = pack_bf16(x, y);
         lsum[j] = add_two(w[e], lsum[j]);
       }
@@ -185,15 +210,17 @@ void few_kernel(const Args a) {
     }
   };
   auto values = [&](const bf8_t (&pp)[NR]) __attribute__((always_inline)) {
-    const uint32_t at = lds_address(V) + v_lane<D>(lane);
+    const uint32_t at = lds_address(V) + v_lane<D>(lane_now<AFFINE ? 512 : D>(lane));
+    pipelined<NT, W::kGroup, bf8_t>(
+        [&](int t) __attribute__((always_inline)) {
+          const u2_t x = read_transposed(at ^ (32 * t)), y = read_transposed((at ^ (32 * t)) + 16 * D * 2);
+          return __builtin_bit_cast(bf8_t, u4_t{x.x, x.y, y.x, y.y});
+        },
+        [&](int t, bf8_t va) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const u2_t x = read_transposed(at ^ (32 * t)), y = read_transposed((at ^ (32 * t)) + 16 * D * 2);
-      const bf8_t va = __builtin_bit_cast(bf8_t, u4_t{x.x, x.y, y.x, y.y});
-#pragma unroll
-      for (int j = 0; j < NR; ++j)
-        o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pp[j], o[t][j], 0, 0, 0);
-    }
+          for (int j = 0; j < NR; ++j)
+            o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pp[j], o[t][j], 0, 0, 0);
+        });
   };
   auto clear = [&](f4_t (&sc)[NI][NR]) __attribute__((always_inline)) {
 #pragma unroll
@@ -246,7 +273,13 @@ void few_kernel(const Args a) {
     } else {
       // Lane l holds the codes of row l / 2, channels [l % 2 * D / 2, + D / 2).
       constexpr int H = D / 2, KW = H * BK / 32, VW = H * BV / 32;
-      const int r = lane / 2, half = lane % 2, turn = turn_of<D>(r);
+      const int r = lane / 2, half = lane % 2;
+      // Where the lane writes piece 2 i + e of its half row: a tile's address
+      // plus this, XOR 16 (2 i + e). Made anew a tile (see lane_now).
+      auto place = [&](const uint16_t* tile) __attribute__((always_inline)) {
+        const int ln = lane_now<512>(lane), row = ln / 2;
+        return lds_address(tile) + uint32_t(row * D * 2 + ((ln % 2 * (H / 8)) ^ turn_of<D>(row)) * 16);
+      };
       constexpr int NRUN = H / 32;
       // One side of a tile: codes, and the scales and biases of their runs of 32.
       auto load = [&](int tile, int side, auto& codes, float (&s)[NRUN], float (&z)[NRUN]) __attribute__((always_inline)) {
@@ -276,31 +309,41 @@ void few_kernel(const Args a) {
       for (int tile = t0; tile <= t_hi; tile += kWaves) {
         f4_t sc[NI][NR];
         bf8_t pp[NR];
+        float top = 0.0f;  // of the lane's half row, then of the row
+#pragma unroll
+        for (int i = 0; i < NRUN; ++i)
+          top = fmaxf(top, fmaxf(fabsf(kz[i]), fabsf(fmaf(ks[i], float((1 << BK) - 1), kz[i]))));
+        top = fmaxf(top, __shfl_xor(top, 1, kWave));
+        const int up = top > 0.0f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+        if (half == 0) shifts[wave][r] = -up;
+        const uint32_t kat = place(K);
 #pragma unroll
         for (int i = 0; i < H / 16; ++i) {
-          uint32_t w[BK / 2], hi[8], lo[8];
-          float f[16];
+          uint32_t w[BK / 2], x[8];
 #pragma unroll
           for (int e = 0; e < BK / 2; ++e) w[e] = kc[(i * BK / 2 + e) / 4][(i * BK / 2 + e) % 4];
-          codes16<BK>(w, f);
+          const _Float16 s = _Float16(ldexpf(ks[i / 2], up)), z = _Float16(ldexpf(kz[i / 2], up));
+          halves16<BK>(w, h2_t{s, s}, h2_t{z, z}, x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = fmaf(ks[i / 2], f[2 * e], kz[i / 2]), y = fmaf(ks[i / 2], f[2 * e + 1], kz[i / 2]);
-            hi[e] = pack_bf16(x, y);
-            lo[e] = pack_bf16(x - __uint_as_float(hi[e] << 16), y - __uint_as_float(hi[e] & 0xffff0000u));
-          }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int at = r * D + ((half * (H / 8) + 2 * i + e) ^ turn) * 8;
-            *reinterpret_cast<u4_t*>(K + at) = u4_t{hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]};
-            *reinterpret_cast<u4_t*>(V + at) = u4_t{lo[4 * e], lo[4 * e + 1], lo[4 * e + 2], lo[4 * e + 3]};
-          }
+          for (int e = 0; e < 2; ++e)
+            write_lds(kat ^ (16 * (2 * i + e)),
+                u4_t{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]});
+          __builtin_amdgcn_sched_barrier(0);  // few values at a time: registers
         }
         load(tile + kWaves, 0, kc, ks, kz);
         clear(sc);
-        scores(V, sc);
         scores(K, sc);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          typedef int i4_t __attribute__((ext_vector_type(4)));
+          const i4_t down = *reinterpret_cast<const i4_t*>(&shifts[wave][16 * i + 4 * lg]);
+#pragma unroll
+          for (int j = 0; j < NR; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[i][j][e] = ldexpf(sc[i][j][e], down[e]);
+        }
         softmax(tile, sc, pp);
+        const uint32_t vat = place(V);
 #pragma unroll
         for (int i = 0; i < H / 16; ++i) {
           uint32_t w[BV / 2], x[8];
@@ -313,8 +356,9 @@ void few_kernel(const Args a) {
             x[e] = pack_bf16(fmaf(vs[i / 2], f[2 * e], vz[i / 2]), fmaf(vs[i / 2], f[2 * e + 1], vz[i / 2]));
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<u4_t*>(V + r * D + ((half * (H / 8) + 2 * i + e) ^ turn) * 8) =
-                u4_t{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]};
+            write_lds(vat ^ (16 * (2 * i + e)),
+                u4_t{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]});
+          __builtin_amdgcn_sched_barrier(0);
         }
         load(tile + kWaves, 1, vc, vs, vz);
         values(pp);
@@ -383,8 +427,9 @@ void few_kernel(const Args a) {
 
 template <int D>
 void launch_few(const Args& a, Source s, hipStream_t st) {
+  const unsigned threads = s == kPagedBf16 ? Few<D, false>::kThreads : Few<D, true>::kThreads;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(unsigned(units_of(a.Hkv, a.ids)), unsigned(a.splits)), dim3(Few<D>::kThreads), 0, st, a);
+    hipLaunchKernelGGL(kernel, dim3(unsigned(units_of(a.Hkv, a.ids)), unsigned(a.splits)), dim3(threads), 0, st, a);
   };
   if (s == kPagedBf16) go(few_kernel<D, kPagedBf16, 16, 16>);
   else if (a.bits_k == 4 && a.bits_v == 4) go(few_kernel<D, kPagedAffine, 4, 4>);
