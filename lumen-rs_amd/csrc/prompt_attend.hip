@@ -3,6 +3,15 @@
 
 namespace tqkv {
 namespace prompt {
+// Each in a file of its own.
+extern template void launch_prompt<64>(const Args&, Source, hipStream_t);
+extern template void launch_few<64>(const Args&, Source, hipStream_t);
+extern template void launch_prompt<128>(const Args&, Source, hipStream_t);
+extern template void launch_few<128>(const Args&, Source, hipStream_t);
+extern template void launch_prompt<256>(const Args&, Source, hipStream_t);
+extern template void launch_few<256>(const Args&, Source, hipStream_t);
+extern template void launch_prompt<512>(const Args&, Source, hipStream_t);
+extern template void launch_few<512>(const Args&, Source, hipStream_t);
 namespace {
 
 // Affine rows of the sequences that have queries, dequantized once a KV head: K

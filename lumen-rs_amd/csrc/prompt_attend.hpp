@@ -216,7 +216,7 @@ struct Shape {
   static constexpr bool kLate = D <= 128;
   static constexpr int kAhead = D <= 128 ? 2 : D == 256 ? 1 : 0;  // tiles in flight
   static constexpr int kKBufs = kAhead + 1, kVBufs = kAhead + 1 + (kLate ? 1 : 0);
-  static constexpr int kGroupK = 4, kGroupV = 4;  // operand reads in flight
+  static constexpr int kGroupK = 2, kGroupV = 2;  // operand reads in flight
   static constexpr int kRows = kWaves * kRW;
   static constexpr int kThreads = kWaves * kWave;
   static constexpr int kPieces = kKeys * D * 2 / 1024 / kWaves;  // 1 KB pieces of K (of V) a wavefront
@@ -488,6 +488,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
   const int64_t row_end = row0 + W::kRows < rows ? row0 + W::kRows : rows;
   const int n = seq.keys, p0 = n - seq.count;  // p0: the first query's position
   const int pos_lo = p0 + int(row0 / a.G), pos_hi = p0 + int((row_end - 1) / a.G);
+  const uint32_t in_position = uint32_t(row0 % a.G);  // the block's first row
   const int split = blockIdx.y;
   // Keys that some row of the block sees, within the split.
   int key_lo = split * a.split_keys, key_hi = n;
@@ -500,26 +501,23 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
 
   using op_t = std::conditional_t<F16, h8_t, bf8_t>;
   op_t qf[NR][ND];
-  int pos[NR];       // of this lane's rows
   float qscale[NR];  // scores to log2 units
   auto row_at = [&](int j) __attribute__((always_inline)) { return row0 + wave * RW + 16 * j + lr; };
 #pragma unroll
   for (int j = 0; j < NR; ++j) {
     const int64_t r = row_at(j) < rows ? row_at(j) : rows - 1;
-    pos[j] = p0 + int(r / a.G);
     const uint16_t* src = a.q + (seq.first + r / a.G) * a.qs + (int64_t(kvh) * a.G + r % a.G) * D;
     qscale[j] = load_query<D>(a, src, lg, qf[j]);
     if constexpr (F16) qscale[j] = ldexpf(qscale[j], a.exponent[b * a.Hkv + kvh]);
   }
 
-  // Per row: the running maximum (log2 units), its negative (0 while no key
-  // was seen), and the raw score above which it must move.
-  float m[NR], nm[NR], thr[NR], lsum[NR];
+  // Per row: the running maximum (log2 units) and the sum.
+  float m[NR], lsum[NR];
   f4_t o[NT][NR];
 #pragma unroll
   for (int j = 0; j < NR; ++j) {
-    m[j] = thr[j] = -INFINITY;
-    nm[j] = lsum[j] = 0.0f;
+    m[j] = -INFINITY;
+    lsum[j] = 0.0f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -606,8 +604,6 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
 #pragma unroll
       for (int t = 0; t < NT; ++t) o[t][j] *= alpha;
       m[j] = mn;
-      nm[j] = mn == -INFINITY ? 0.0f : -mn;
-      thr[j] = (mn + kTau) * __builtin_amdgcn_rcpf(qscale[j]);  // need not be exact
     };
     auto scores = [&](uint32_t K, f4_t (&sc)[NI][NR]) __attribute__((always_inline)) {
 #pragma unroll
@@ -636,18 +632,20 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
                          (!a.causal || (kbase + KT - 1 <= pos_lo && (a.window <= 0 || pos_hi - a.window < kbase)));
       if (!whole) {
         rare();
+        const int ln = lane_now<D>(lane), g4 = 4 * (ln / 16);
 #pragma unroll
         for (int j = 0; j < NR; ++j) {
+          const int pos = pos_lo + int((in_position + uint32_t(wave * RW + 16 * j + ln % 16)) / uint32_t(a.G));
           int hi = key_hi - kbase, lo = key_lo - kbase;  // visible: [lo, hi)
           if (a.causal) {
-            hi = min(hi, pos[j] + 1 - kbase);
-            if (a.window > 0) lo = max(lo, pos[j] - a.window + 1 - kbase);
+            hi = min(hi, pos + 1 - kbase);
+            if (a.window > 0) lo = max(lo, pos - a.window + 1 - kbase);
           }
 #pragma unroll
           for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int k = 16 * i + 4 * lg + r;
+              const int k = 16 * i + g4 + r;
               if (k < lo || k >= hi || !((on >> i) & 1)) sc[i][j][r] = -INFINITY;
             }
         }
@@ -659,19 +657,21 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
         for (int i = 0; i < NI; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[i][j][r]);
-        if (__any(mx > thr[j])) {
+        // (In log2 units, for which nothing more is kept: registers.)
+        if (__any(mx * qscale[j] > m[j] + kTau)) {
           rare();
           mx = row_max(mx);
-          rescale(j, mx > thr[j], mx);
+          rescale(j, mx * qscale[j] > m[j] + kTau, mx);
         }
+        const float nm = m[j] == -INFINITY ? 0.0f : -m[j];
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
           u4_t w;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const f4_t s = sc[2 * u + e / 2][j];
-            const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2)], qscale[j], nm[j]));
-            const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2) + 1], qscale[j], nm[j]));
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2)], qscale[j], nm));
+            const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2) + 1], qscale[j], nm));
             w[e] = pack_bf16(x, y);
             lsum[j] = add_two(w[e], lsum[j]);
           }
