@@ -28,6 +28,7 @@ struct EnterArgs {
   void* slot[6];
   int H, gs, per_block;
   rope::Jobs q_jobs, k_jobs;
+  rope::Divisor heads;  // KV heads
 };
 
 // A token's place in the workgroup: its rotary position, and its pool row of
@@ -104,13 +105,25 @@ __global__ __launch_bounds__(kThreads) void enter_bf16_kernel(const EnterArgs a)
     return;
   }
   find_places(a, t0, n, false, place, angles);
-  constexpr int LPR = D / 8;
-  for (int i = threadIdx.x; i < n * p.Hkv * LPR; i += kThreads) {
-    const int r = i / LPR, c = i % LPR * 8;
-    uint16_t* dst = to(r / p.Hkv, r % p.Hkv);
-    if (dst)
-      *reinterpret_cast<uint4*>(dst + c) =
-          *reinterpret_cast<const uint4*>(from(r / p.Hkv, r % p.Hkv) + c);
+  // Values: 16 bytes a thread, kDeep of them on their way.
+  constexpr int LPR = D / 8, kDeep = rope::kDeep;
+  const int all = n * p.Hkv * LPR;
+  for (int i0 = threadIdx.x; i0 < all; i0 += kThreads * kDeep) {
+    uint4 y[kDeep];
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      const int i = min(i0 + k * kThreads, all - 1), r = i / LPR;
+      const int t = rope::quotient(r, a.heads), h = r - t * p.Hkv;
+      y[k] = *reinterpret_cast<const uint4*>(from(t, h) + i % LPR * 8);
+    }
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      const int i = i0 + k * kThreads, r = i / LPR;
+      if (i >= all) break;
+      const int t = rope::quotient(r, a.heads), h = r - t * p.Hkv;
+      uint16_t* dst = to(t, h);
+      if (dst) *reinterpret_cast<uint4*>(dst + i % LPR * 8) = y[k];
+    }
   }
 }
 
@@ -252,6 +265,7 @@ extern "C" int32_t tqkv_paged_append_rope(const tqkv_paged_kv* kv, const tqkv_ro
   a.gs = kv->group_size;
   a.q_jobs = rope::jobs_of(a.rope, H, kv->dim, q != q_out);
   a.k_jobs = rope::jobs_of(a.rope, kv->kv_heads, kv->dim, true);
+  a.heads = rope::divisor(kv->kv_heads);
   a.per_block = rope::tokens_of(a.k_jobs, tokens);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (kv->dim) {

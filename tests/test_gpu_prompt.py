@@ -246,6 +246,87 @@ def test_paged_edges(T, kind, D):
         assert np.all(want[starts[1]:starts[1] + 6] == 0.0)
 
 
+@pytest.mark.parametrize("kind,bk,bv", [(BF16, 16, 16), (AFFINE, 4, 8), (AFFINE, 8, 4)])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_few_rows_edges(T, kind, bk, bv, D):
+    """The same with few queries a sequence, which another kernel takes; one of
+    the sequences has many all the same."""
+    say("few edges", kind, bk, bv, D)
+    p = Paged([100, 3, -2, 1 << 30, 70, 64, 9, 190], 1, D, 16, kind, bk, bv, 32, stride=12, spare=1, seed=4).fill(3)
+    p.table[0, 2], p.table[0, 5] = -1, p.pages
+    p.table[4] = 2 ** 31 - 1
+    counts = [2, 5, 1, 3, 1, 1, 0, 25]
+    starts = starts_of(counts, 1)
+    q = kv_bf16((int(starts[-1]) + 1, 2, D), D)
+    for most, window in ((None, -1), (50, -1), (None, 7)):
+        want, tol = R.paged(p, q, starts, D ** -0.5, window, max_rows=most)
+        close(run_paged(T, p, q, starts, D ** -0.5, window, max_rows=most), want, tol, starts, "few edges")
+        assert np.all(want[starts[1]:starts[1] + 2] == 0.0)
+
+
+@pytest.mark.parametrize("counts", [[2, 3], [150, 90]])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1.5])
+def test_affine_scales(T, D, counts, scale):
+    say("affine scales", D, counts, scale)
+    p = Paged([200, 90], 1, D, 16, AFFINE, 8, 8, 64, seed=5).fill(3)
+    q = kv_bf16((sum(counts), 2, D), D)
+    want, tol = R.paged(p, q, starts_of(counts), scale)
+    close(run_paged(T, p, q, starts_of(counts), scale), want, tol, starts_of(counts), "affine scales")
+
+
+@pytest.mark.parametrize("counts", [[2, 3], [150, 90]])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("kq,ks,vs", [(1e18, 1e-18, 1e36), (1e-18, 1e18, 1e-34), (1e-3, 1.0, 1e5)])
+def test_affine_ranges(T, D, counts, kq, ks, vs):
+    """Keys and values of any magnitude, the queries to match; a few keys much
+    smaller than the others."""
+    say("affine ranges", D, counts, kq, ks, vs)
+    p = Paged([200, 90], 1, D, 16, AFFINE, 4, 8, 32, seed=5)
+    rng = np.random.default_rng(D)
+    for b in range(2):
+        for row in range(int(p.lens[b])):
+            small = 2.0 ** -6 if row % 7 == 3 else 1.0
+            k, v = (O.bf16_from_f32((rng.standard_normal((1, D)) * m).astype(np.float32)) for m in (ks * small, vs))
+            p.write(b, row, k, v)
+    q = O.bf16_from_f32((rng.standard_normal((sum(counts), 2, D)) * kq).astype(np.float32))
+    scale = D ** -0.5 / float(np.float32(kq * ks))
+    want, tol = R.paged(p, q, starts_of(counts), scale)
+    close(run_paged(T, p, q, starts_of(counts), scale), want, tol, starts_of(counts), "affine ranges")
+
+
+@pytest.mark.parametrize("kind", [BF16, AFFINE])
+@pytest.mark.parametrize("counts", [[6], [90]])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("what", ["v", "k"])
+def test_pages_with_infinities_and_nan(T, kind, D, counts, what):
+    """A later row's value (or key) is not finite: earlier queries are as
+    without it, and channels (queries) that it reaches are not finite."""
+    say("not finite", kind, D, counts, what)
+    n = 200
+    p = Paged([n], 1, D, 16, kind, 8, 8, 32, seed=5).fill(4)
+    starts = starts_of(counts)
+    q = kv_bf16((counts[0], 2, D), 3)
+    want, tol = R.paged(p, q, starts, D ** -0.5)
+    at = (p.table[0, (n - 4) // 16], 0, (n - 4) % 16)  # seen by the last four queries
+    side = p.sides[1 if what == "v" else 0]
+    if kind == BF16:
+        side[0][at][3] = 0x7F80 if what == "v" else 0x7FC0
+        reached = [3]
+    else:
+        side[1][at][0] = 0x7FC0  # a group's scale
+        reached = list(range(32))
+    got = O.bf16_to_f32(run_paged(T, p, q, starts, D ** -0.5))
+    m = counts[0] - 4
+    R.check(got[:m], want[:m], tol[:m], "before")
+    if what == "v":
+        assert not np.any(np.isfinite(got[m:][..., reached]))
+        rest = np.setdiff1d(np.arange(D), reached)
+        R.check(got[m:][..., rest], want[m:][..., rest], tol[m:][..., rest], "beside")
+    else:
+        assert np.all(np.isnan(got[m:]))
+
+
 @pytest.mark.parametrize("kind,D,R_", [(BF16, 128, 16), (AFFINE, 128, 64), (BF16, 64, 128), (BF16, 256, 32), (AFFINE, 512, 16)])
 @pytest.mark.parametrize("counts", [[1, 1], [5, 2], [40, 7]])
 def test_paged_long(T, kind, D, R_, counts):
