@@ -583,9 +583,9 @@ int32_t tqkv_paged_append_rope(const tqkv_paged_kv* kv, const tqkv_rope* rope, c
  * h * head_stride (a fused projection is read in place); out bf16 [tokens, H,
  * D]. Query head h reads KV head h / (H / H_kv). Rows of out before starts[0]
  * and from starts[batch] on stay as they were.
- * Scores and sums are f32; weights multiply V as bf16, normalised by the sum
- * of the rounded weights. Values keep bf16's range, and an infinite or NaN
- * key or value reaches only the queries that see it.
+ * Scores and sums are f32; weights multiply V in V's type (bf16 here),
+ * normalised by the sum of the rounded weights. Values keep bf16's range, and an
+ * infinite or NaN key or value reaches only the queries that see it.
  * D in {64, 128, 256, 512}; H / H_kv from 1 to 32; batch at most 1024; tokens
  * below 2^31; q, k, v 16-byte aligned, strides multiples of 8, token_stride
  * from 0 to below 2^27; out 16-byte aligned. workspace: tqkv_packed_attend_workspace_size() bytes, 16-byte
@@ -611,10 +611,11 @@ size_t tqkv_packed_attend_workspace_size(int32_t batch, int32_t H, int32_t H_kv,
  * its rows up to their own position, with window > 0 the last `window` of
  * these. Rows of invalid pages get no attention; a query that sees no row
  * gets zeros. max_rows: the host's bound on lens, as tqkv_paged_decode_attend
- * takes it. Affine keys enter as scale * code + bias in 11 bits or more, what is
- * below 2^-28 of their head's largest with fewer, and a query's channels
- * below 2^-28 of its largest alike; affine values as
- * tqkv_affine_dequantize's bf16 ones.
+ * takes it. Affine rows enter as scale * code + bias in 11 bits, what is below
+ * 2^-28 of their head's largest with fewer, and a query's channels below 2^-28
+ * of its largest alike; values in 11 bits of their group's largest, or in bf16's
+ * 8 where these lie 2^28 apart in a head (few queries over such rows cost much
+ * more).
  * kv->weights is not touched. q, out, H and the workspace as above; results
  * depend on starts, lens, tokens and max_rows, not on the run.
  */

@@ -14,10 +14,12 @@ extern template void launch_prompt<512>(const Args&, Source, hipStream_t);
 extern template void launch_few<512>(const Args&, Source, hipStream_t);
 namespace {
 
-// Affine rows of the sequences that have queries, dequantized once a KV head: K
-// as f16 (11 bits where bf16 keeps 8, the scores' largest error) times a power
-// of two that brings the head's largest value below 2^15, V as bf16. First
-// the largest |value| that a head's scales and biases allow.
+// Affine rows of the sequences that have queries, dequantized once a KV head, as
+// f16 (11 bits where bf16 keeps 8) times powers of two that bring the head's
+// largest K and V below 2^15; V as bf16 where its groups' largest values lie too
+// far apart for f16, since a query may see the small ones alone. First what a
+// head's scales and biases allow: (largest |K|, largest |V|, smallest |V| of a
+// group's largest but zero).
 constexpr int kRangeParts = 32;
 
 struct Rows {
@@ -30,30 +32,43 @@ __device__ __forceinline__ Rows seen_rows(const Args& a, int b) {
   return Rows{lo, s.count > 0 ? s.keys : 0};
 }
 
-__global__ __launch_bounds__(256) void range_kernel(const Args a, int D, float* part) {
-  __shared__ float tops[4];
+__global__ __launch_bounds__(256) void range_kernel(const Args a, int D, float4* part) {
+  __shared__ float4 tops[4];
   const int h = blockIdx.y, b = blockIdx.z, groups = D / a.gs;
   const Rows rows = seen_rows(a, b);
   const int span = max(0, rows.n - rows.lo), each = (span + kRangeParts - 1) / kRangeParts;
   const int from = rows.lo + int(blockIdx.x) * each, to = min(from + each, rows.n);
-  const uint16_t* scales = static_cast<const uint16_t*>(a.slot[1]);
-  const uint16_t* biases = static_cast<const uint16_t*>(a.slot[2]);
-  const float most = float((1 << a.bits_k) - 1);
-  float top = 0.0f;
+  const float most_k = float((1 << a.bits_k) - 1), most_v = float((1 << a.bits_v) - 1);
+  const auto bound = [&](int side, int64_t g, float most) {
+    const float s = bf16_to_f32(static_cast<const uint16_t*>(a.slot[3 * side + 1])[g]);
+    const float z = bf16_to_f32(static_cast<const uint16_t*>(a.slot[3 * side + 2])[g]);
+    const float x = fabsf(z), y = fabsf(fmaf(s, most, z));
+    return x < INFINITY && y < INFINITY ? fmaxf(x, y) : INFINITY;  // NaN too
+  };
+  float k = 0.0f, v = 0.0f, low = INFINITY;
   for (int i = threadIdx.x; i < (to - from) * groups; i += 256) {
     const int64_t row = row_of<kPagedAffine>(a, b, 0, h, from + i / groups);
     if (row < 0) continue;
     const int64_t g = row * groups + i % groups;
-    const float s = bf16_to_f32(scales[g]), z = bf16_to_f32(biases[g]);
-    top = fmaxf(top, fmaxf(fabsf(z), fabsf(fmaf(s, most, z))));
+    k = fmaxf(k, bound(0, g, most_k));
+    const float x = bound(1, g, most_v);
+    v = fmaxf(v, x);
+    if (x > 0.0f) low = fminf(low, x);
   }
 #pragma unroll
-  for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-  if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
+  for (int d = 32; d > 0; d /= 2) {
+    k = fmaxf(k, __shfl_xor(k, d, 64));
+    v = fmaxf(v, __shfl_xor(v, d, 64));
+    low = fminf(low, __shfl_xor(low, d, 64));
+  }
+  if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = make_float4(k, v, low, 0.0f);
   __syncthreads();
-  if (threadIdx.x == 0)
-    part[(int64_t(b) * a.Hkv + h) * kRangeParts + blockIdx.x] =
-        fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  if (threadIdx.x == 0) {
+    float4 x = tops[0];
+    for (int i = 1; i < 4; ++i)
+      x = make_float4(fmaxf(x.x, tops[i].x), fmaxf(x.y, tops[i].y), fminf(x.z, tops[i].z), 0.0f);
+    part[(int64_t(b) * a.Hkv + h) * kRangeParts + blockIdx.x] = x;
+  }
 }
 
 // 32 codes of `bits` from w as f32.
@@ -75,7 +90,7 @@ __device__ __forceinline__ void codes_of(const uint32_t* w, int bits, float (&f)
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void slab_kernel(const Args a, const float* part, uint16_t* slab_k,
+__global__ __launch_bounds__(256) void slab_kernel(const Args a, const float4* part, uint16_t* slab_k,
                                                    uint16_t* slab_v, int32_t* exponent) {
   constexpr int kRuns = D / 32;
   const int h = blockIdx.y, b = blockIdx.z;
@@ -83,11 +98,24 @@ __global__ __launch_bounds__(256) void slab_kernel(const Args a, const float* pa
   const int t0 = int(blockIdx.x) * 64;
   if (t0 + 64 <= rows.lo || t0 >= rows.n) return;
   const int64_t unit = int64_t(b) * a.Hkv + h;
-  float top = 0.0f;
+  float k_top = 0.0f, v_top = 0.0f, v_low = INFINITY;
 #pragma unroll
-  for (int i = 0; i < kRangeParts; ++i) top = fmaxf(top, part[unit * kRangeParts + i]);
-  const int up = top > 0.0f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-  if (threadIdx.x == 0) exponent[unit] = -up;  // every block of the head writes the same
+  for (int i = 0; i < kRangeParts; ++i) {
+    const float4 x = part[unit * kRangeParts + i];
+    k_top = fmaxf(k_top, x.x);
+    v_top = fmaxf(v_top, x.y);
+    v_low = fminf(v_low, x.z);
+  }
+  const auto up_of = [](float top) {
+    return top > 0.0f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+  };
+  const int k_up = up_of(k_top), v_up = up_of(v_top);
+  // A group whose largest is 2^-14 keeps 11 bits of that: f16's least step is 2^-24.
+  const bool halves = v_top < INFINITY && (v_top == 0.0f || ldexpf(v_low, v_up) >= 0x1p-14f);
+  if (threadIdx.x == 0) {  // every block of the head writes the same
+    exponent[2 * unit] = -k_up;
+    exponent[2 * unit + 1] = halves ? -v_up : kBf16;
+  }
   for (int i = threadIdx.x; i < 64 * kRuns; i += 256) {
     const int t = t0 + i / kRuns, run = i % kRuns;
     if (t >= rows.n) break;
@@ -110,13 +138,9 @@ __global__ __launch_bounds__(256) void slab_kernel(const Args a, const float* pa
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float p = fmaf(s, f[2 * e], z), q = fmaf(s, f[2 * e + 1], z);
-          if (side) {
-            v[e] = pack_bf16(p, q);
-          } else {
-            typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
-            const f2_t x2 = {ldexpf(p, up), ldexpf(q, up)};
-            k[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x2, h2_t));
-          }
+          if (!side) k[e] = pack_f16(ldexpf(p, k_up), ldexpf(q, k_up));
+          else if (halves) v[e] = pack_f16(ldexpf(p, v_up), ldexpf(q, v_up));
+          else v[e] = pack_bf16(p, q);
         }
       }
     }
@@ -171,7 +195,7 @@ bool plan_of(int batch, int H, int Hkv, int D, int64_t tokens, int64_t keys, Sou
   if (source == kPagedAffine && !p.few) {
     p.slab_rows = keys;
     p.slab = whole(size_t(batch) * Hkv * size_t(keys) * D * 2);
-    p.exponents = whole(size_t(batch) * Hkv * 4) + whole(size_t(batch) * Hkv * kRangeParts * 4);
+    p.exponents = whole(size_t(batch) * Hkv * 8) + whole(size_t(batch) * Hkv * kRangeParts * 16);
   }
   if (p.splits > 1) p.parts = whole(size_t(tokens) * H * p.splits * (D + 2) * 4);
   p.bytes = 2 * p.slab + p.exponents + p.parts;
@@ -198,7 +222,7 @@ int32_t attend(Args& a, int D, Source source, const Plan& p, void* workspace, si
     uint16_t* v = reinterpret_cast<uint16_t*>(at + p.slab);
     at += 2 * p.slab;
     int32_t* exponent = reinterpret_cast<int32_t*>(at);
-    float* part = reinterpret_cast<float*>(at + (size_t(a.batch) * a.Hkv * 4 + 255) / 256 * 256);
+    float4* part = reinterpret_cast<float4*>(at + (size_t(a.batch) * a.Hkv * 8 + 255) / 256 * 256);
     at += p.exponents;
     a.slab_k = k;
     a.slab_v = v;

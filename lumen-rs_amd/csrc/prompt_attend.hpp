@@ -22,8 +22,9 @@
 // and the row sum counts them as rounded.
 //
 // Weights of hidden keys are exact zeros, but zero times an infinite value is
-// NaN: a row that ends with a NaN anywhere is done again, one key at a time,
-// by attend_row, which leaves hidden keys out.
+// NaN (and sums of values next to f32's largest pass it): a row that ends with
+// anything that is not finite is done again, one key at a time, by attend_row,
+// which leaves hidden keys out.
 #pragma once
 
 #include <type_traits>
@@ -55,8 +56,9 @@ struct Args {
   paged::Pool pool;
   const void* slot[6];
   int gs, bits_k, bits_v, max_rows;
-  // kSlab: rows [batch, Hkv, slab_rows, D], K as f16 times 2^-exponent[batch,
-  // Hkv], V as bf16.
+  // kSlab: rows [batch, Hkv, slab_rows, D], K as f16 times 2^-exponent[2 u] of
+  // unit u = (sequence, KV head), V alike by exponent[2 u + 1], or as bf16 where
+  // that is kBf16.
   const uint16_t* slab_k;
   const uint16_t* slab_v;
   const int32_t* exponent;
@@ -71,6 +73,7 @@ struct Args {
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kBf16 = 0x7fffffff;
 
 // A sequence's queries [first, first + count) and the keys that it has.
 struct Sequence {
@@ -104,8 +107,7 @@ __device__ __forceinline__ Range visible(const Args& a, int64_t p, int n) {
   return Range{int(lo < hi ? lo : hi), int(hi)};
 }
 
-// Channel c of a stored row in f32; values of affine rows are rounded to bf16,
-// keys are not (their f16 operands keep 11 bits).
+// Channel c of a stored row in f32.
 template <Source S>
 __device__ __forceinline__ float value_at(const Args& a, bool key, int64_t row, int D, int c) {
   if constexpr (S == kPacked) {
@@ -119,8 +121,7 @@ __device__ __forceinline__ float value_at(const Args& a, bool key, int64_t row, 
     const int64_t g = row * (D / a.gs) + c / a.gs;
     const float s = bf16_to_f32(static_cast<const uint16_t*>(a.slot[at + 1])[g]);
     const float b = bf16_to_f32(static_cast<const uint16_t*>(a.slot[at + 2])[g]);
-    const float x = fmaf(s, float(code), b);
-    return key ? x : bf16_to_f32(f32_to_bf16(x));
+    return fmaf(s, float(code), b);
   }
 }
 
@@ -146,6 +147,7 @@ __device__ __forceinline__ void attend_row(const Args& a, int b, int64_t token, 
   const Range see = visible(a, p, s.keys);
   const uint16_t* q = a.q + token * a.qs + int64_t(head) * D;
   constexpr int C = D / 64;
+  constexpr float kDown = 0x1p-16f;  // sums of values next to f32's largest stay finite
   float o[C], m = -INFINITY, l = 0.0f;
   bool any = false;
 #pragma unroll
@@ -181,19 +183,22 @@ __device__ __forceinline__ void attend_row(const Args& a, int b, int64_t token, 
       const float wi = __shfl(w, i, 64);
       const int64_t ri = __shfl(row, i, 64);
 #pragma unroll
-      for (int c = 0; c < C; ++c) o[c] = fmaf(wi, value_at<S>(a, false, ri, D, c * 64 + lane), o[c]);
+      for (int c = 0; c < C; ++c) o[c] = fmaf(wi, value_at<S>(a, false, ri, D, c * 64 + lane) * kDown, o[c]);
     }
   }
   uint16_t* out = a.out + (token * a.H + head) * D;
   const float inv = any ? 1.0f / l : 0.0f;
 #pragma unroll
-  for (int c = 0; c < C; ++c) out[c * 64 + lane] = f32_to_bf16(any ? o[c] * inv : 0.0f);
+  for (int c = 0; c < C; ++c) out[c * 64 + lane] = f32_to_bf16(any ? o[c] * inv / kDown : 0.0f);
 }
 
 // ------------------------------------------------------------- matrix cores
 constexpr int kWave = 64;
 constexpr int kXcds = 8;
 constexpr float kTau = 8.0f;
+// A scale of zero as the least positive number: a hidden key's score, -infinity,
+// times it stays that.
+constexpr float kLeastScale = 0x1p-149f;
 
 typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
@@ -296,6 +301,24 @@ __device__ __forceinline__ float add_two(uint32_t w, float acc) {
   const bf2_t one = {__bf16(1.0f), __bf16(1.0f)};
   return __builtin_amdgcn_fdot2_f32_bf16(as_bf2(w), one, acc, false);
 }
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ h2_t as_h2(uint32_t x) { return __builtin_bit_cast(h2_t, x); }
+__device__ __forceinline__ uint32_t pack_f16(float x, float y) {
+  const f2_t f = {x, y};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, h2_t));
+}
+// Two weights as the products take them, and acc plus both as rounded.
+template <bool H>
+__device__ __forceinline__ uint32_t pack_weights(float x, float y) {
+  return H ? pack_f16(x, y) : pack_bf16(x, y);
+}
+template <bool H>
+__device__ __forceinline__ float add_weights(uint32_t w, float acc) {
+  if constexpr (!H) return add_two(w, acc);
+  const h2_t one = {_Float16(1.0f), _Float16(1.0f)};
+  return __builtin_amdgcn_fdot2(as_h2(w), one, acc, false);
+}
+
 // Lane l with lanes l ^ 16 and l ^ 32 (the lanes of one row).
 __device__ __forceinline__ float max_of(float a, float b) {
   float r;
@@ -418,6 +441,9 @@ __device__ __forceinline__ bool find_block(const Args& a, int id, int each, Bloc
   return out->row0 < int64_t(out->seq.count) * a.G;
 }
 
+__device__ __forceinline__ bool finite(f4_t v) {
+  return fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY;
+}
 __device__ __forceinline__ f4_t product(bf8_t x, bf8_t y, f4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
 }
@@ -508,7 +534,8 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
     const int64_t r = row_at(j) < rows ? row_at(j) : rows - 1;
     const uint16_t* src = a.q + (seq.first + r / a.G) * a.qs + (int64_t(kvh) * a.G + r % a.G) * D;
     qscale[j] = load_query<D>(a, src, lg, qf[j]);
-    if constexpr (F16) qscale[j] = ldexpf(qscale[j], a.exponent[b * a.Hkv + kvh]);
+    if constexpr (F16) qscale[j] = ldexpf(qscale[j], a.exponent[2 * (b * a.Hkv + kvh)]);
+    qscale[j] = fmaxf(qscale[j], kLeastScale);
   }
 
   // Per row: the running maximum (log2 units) and the sum.
@@ -521,6 +548,10 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
+
+  // V as f16 (11 bits of the values and of the weights), where its range allows.
+  int v_down = kBf16;
+  if constexpr (F16) v_down = __builtin_amdgcn_readfirstlane(a.exponent[2 * (b * a.Hkv + kvh) + 1]);
 
   if (key_lo < key_hi) {
     const int t_lo = key_lo / KT, t_hi = (key_hi - 1) / KT;
@@ -619,7 +650,8 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
             for (int j = 0; j < NR; ++j) sc[i][j] = product(ka, qf[j][s], sc[i][j]);
           });
     };
-    auto softmax = [&](int tile, f4_t (&sc)[NI][NR], bf8_t (&pp)[NU][NR]) __attribute__((always_inline)) {
+    auto softmax = [&](int tile, f4_t (&sc)[NI][NR], u4_t (&pp)[NU][NR], auto halves) __attribute__((always_inline)) {
+      constexpr bool H = decltype(halves)::value;
       const int kbase = tile * KT;
       // Hidden keys, where the block sees the tile in part.
       uint32_t on = (1u << NI) - 1u;
@@ -672,29 +704,30 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
             const f4_t s = sc[2 * u + e / 2][j];
             const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2)], qscale[j], nm));
             const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2) + 1], qscale[j], nm));
-            w[e] = pack_bf16(x, y);
-            lsum[j] = add_two(w[e], lsum[j]);
+            w[e] = pack_weights<H>(x, y);
+            lsum[j] = add_weights<H>(w[e], lsum[j]);
           }
-          pp[u][j] = __builtin_bit_cast(bf8_t, w);
+          pp[u][j] = w;
         }
       }
     };
-    auto values = [&](const bf8_t (&pp)[NU][NR], uint32_t V) __attribute__((always_inline)) {
+    auto values = [&](const u4_t (&pp)[NU][NR], uint32_t V, auto halves) __attribute__((always_inline)) {
+      using v_t = std::conditional_t<decltype(halves)::value, h8_t, bf8_t>;
       const uint32_t at = V + v_lane<D>(lane_now<D>(lane));
-      pipelined<NU * NT, W::kGroupV, bf8_t>(
+      pipelined<NU * NT, W::kGroupV, v_t>(
           [&](int x) __attribute__((always_inline)) {
             const uint32_t src = (at ^ (32 * (x % NT))) + 32 * (x / NT) * D * 2;
             const u2_t y = read_transposed(src), z = read_transposed(src + 16 * D * 2);
-            return __builtin_bit_cast(bf8_t, u4_t{y.x, y.y, z.x, z.y});
+            return __builtin_bit_cast(v_t, u4_t{y.x, y.y, z.x, z.y});
           },
-          [&](int x, bf8_t va) __attribute__((always_inline)) {
+          [&](int x, v_t va) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < NR; ++j)
-              o[x % NT][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pp[x / NT][j], o[x % NT][j], 0, 0, 0);
+              o[x % NT][j] = product(va, __builtin_bit_cast(v_t, pp[x / NT][j]), o[x % NT][j]);
           });
     };
 
-    auto run = [&](auto late) __attribute__((always_inline)) {
+    auto run = [&](auto late, auto halves) __attribute__((always_inline)) {
       constexpr bool LATE = decltype(late)::value;
       wait_loads<0>();  // the queries
       fetch(t_lo, kKey, 0);
@@ -705,7 +738,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
       }
       wait_loads<(W::kAhead == 2 ? 2 : 0) * NP>();
       __syncthreads();
-      bf8_t pp[NU][NR];
+      u4_t pp[NU][NR];
       int kc = 0, vc = 0;
       const auto plus = [](int c, int d, int bufs) { return c + d >= bufs ? c + d - bufs : c + d; };
       for (int tile = t_lo; tile <= t_hi; ++tile) {
@@ -719,11 +752,11 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
         if (live) {
           if constexpr (W::kLate) __builtin_amdgcn_s_setprio(1);
           if constexpr (LATE)
-            if (tile > t_lo) values(pp, lds_address(tiles[W::kKBufs + plus(vc, W::kVBufs - 1, W::kVBufs)]));
+            if (tile > t_lo) values(pp, lds_address(tiles[W::kKBufs + plus(vc, W::kVBufs - 1, W::kVBufs)]), halves);
           f4_t sc[NI][NR];
           scores(lds_address(tiles[kc]), sc);
           if constexpr (W::kLate) __builtin_amdgcn_s_setprio(0);
-          softmax(tile, sc, pp);
+          softmax(tile, sc, pp, halves);
         }
         if constexpr (W::kAhead == 0) {
           // V is here, and every wavefront is done with K.
@@ -733,7 +766,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
         }
         if (!LATE && live) {
           if constexpr (W::kLate) __builtin_amdgcn_s_setprio(1);
-          values(pp, lds_address(tiles[W::kKBufs + vc]));
+          values(pp, lds_address(tiles[W::kKBufs + vc]), halves);
           if constexpr (W::kLate) __builtin_amdgcn_s_setprio(0);
         }
         wait_loads<(W::kAhead == 2 ? 2 : 0) * NP>();
@@ -742,11 +775,15 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
         vc = plus(vc, 1, W::kVBufs);
       }
       if constexpr (LATE)
-        if (live) values(pp, lds_address(tiles[W::kKBufs + plus(vc, W::kVBufs - 1, W::kVBufs)]));
+        if (live) values(pp, lds_address(tiles[W::kKBufs + plus(vc, W::kVBufs - 1, W::kVBufs)]), halves);
       wait_loads<0>();  // before the workgroup's LDS is given back
     };
-    if (W::kLate && wave >= kWaves / 2) run(std::true_type{});
-    else run(std::false_type{});
+    auto by_order = [&](auto halves) __attribute__((always_inline)) {
+      if (W::kLate && wave >= kWaves / 2) run(std::bool_constant<W::kLate>{}, halves);
+      else run(std::false_type{}, halves);
+    };
+    if (F16 && v_down != kBf16) by_order(std::bool_constant<F16>{});
+    else by_order(std::false_type{});
   }
 
   bool bad = false;
@@ -754,6 +791,11 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
   for (int j = 0; j < NR; ++j) {
     const float sum = row_sum(lsum[j]);
     const int64_t r = row_at(j);
+    if (F16 && v_down != kBf16)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][j][e] = ldexpf(o[t][j][e], v_down);
     if (r >= rows) continue;
     const int64_t row = (seq.first + r / a.G) * a.H + int64_t(kvh) * a.G + r % a.G;
     if (a.part_o) {
@@ -772,7 +814,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const f4_t v = o[t][j] * inv;
-      bad |= !(v[0] == v[0] && v[1] == v[1] && v[2] == v[2] && v[3] == v[3]);
+      bad |= !finite(v);
       *reinterpret_cast<u2_t*>(a.out + row * D + 16 * t + 4 * lg) = u2_t{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
     }
   }
@@ -844,7 +886,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const Args a) {
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const float v = o[c] * inv;
-    bad |= !(v == v);
+    bad |= !(fabsf(v) < INFINITY);
     out[c * kWave + lane] = f32_to_bf16(v);
   }
   constexpr Source R = S == kSlab ? kPagedAffine : S;

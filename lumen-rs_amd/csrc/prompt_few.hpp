@@ -7,10 +7,12 @@
 // while K meets Q). What the wavefronts gathered meets in LDS at the end.
 //
 // Affine rows are dequantized on the way into LDS, out of registers that the
-// next tile's codes have been loaded into meanwhile: V to bf16, K to f16 (one
-// bf16 would cost the scores what their sums keep), every row times a power of
-// two that brings the largest value its scales and biases allow below 2^15,
-// which its scores take back.
+// next tile's codes have been loaded into meanwhile, to f16 (bf16 would cost the
+// results three bits): every row of K times a power of two that brings the
+// largest value its scales and biases allow below 2^15, which its scores take
+// back; V times one power of two for the wavefront's rows. Where V's groups'
+// largest values lie 2^28 apart (a query may see the small ones alone), attend_row
+// does the rows.
 #pragma once
 
 #include "prompt_attend.hpp"
@@ -34,30 +36,8 @@ struct Few {
   static constexpr int kPerEu = D == 64 ? 3 : D == 128 || (D == 256 && AFFINE) ? 2 : 1;
 };
 
-typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ h2_t as_h2(uint32_t x) { return __builtin_bit_cast(h2_t, x); }
-
-// 16 codes of 4 or 8 bits out of w (2 or 4 words) as f32.
-template <int BITS>
-__device__ __forceinline__ void codes16(const uint32_t* w, float (&f)[16]) {
-  if constexpr (BITS == 8) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = float((w[i / 4] >> (8 * (i % 4))) & 0xffu);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t e = w[k] & 0x0f0f0f0fu, o = (w[k] >> 4) & 0x0f0f0f0fu;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        f[8 * k + 2 * j] = float((e >> (8 * j)) & 0xffu);
-        f[8 * k + 2 * j + 1] = float((o >> (8 * j)) & 0xffu);
-      }
-    }
-  }
-}
-
-// The same as scale * code + bias in f16, rounded once, two an instruction: the
-// bits 0x6400 | c are 1,024 + c exactly (a byte's upper code 1,024 + 16 c), one
+// 16 codes of 4 or 8 bits out of w (2 or 4 words) as scale * code + bias in f16,
+// rounded once, two an instruction: the bits 0x6400 | c are 1,024 + c exactly (a byte's upper code 1,024 + 16 c), one
 // multiply-add takes the rest off exactly, one more scales.
 template <int BITS>
 __device__ __forceinline__ void halves16(const uint32_t* w, h2_t s, h2_t z, uint32_t (&x)[8]) {
@@ -115,6 +95,7 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
   if (a.window > 0 && pos_lo - a.window + 1 > key_lo) key_lo = pos_lo - a.window + 1;
   if (a.part_o && key_lo >= key_hi) return;
 
+  int v_up = 0;  // V as f16 is taken times 2^v_up
   const int t_lo = key_lo / KT, t_hi = (key_hi - 1) / KT;  // used where key_lo < key_hi
   const bool working = key_lo < key_hi && t_lo + wave <= t_hi;
 
@@ -126,7 +107,8 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
   for (int j = 0; j < NR; ++j) {
     const int64_t at = row0 + 16 * j + lr, r = at < rows ? at : rows - 1;
     pos[j] = p0 + int(r / a.G);
-    qscale[j] = load_query<D>(a, a.q + (seq.first + r / a.G) * a.qs + (int64_t(kvh) * a.G + r % a.G) * D, lg, qf[j]);
+    qscale[j] = fmaxf(load_query<D>(a, a.q + (seq.first + r / a.G) * a.qs + (int64_t(kvh) * a.G + r % a.G) * D, lg, qf[j]),
+                      kLeastScale);
   }
   float m[NR], nm[NR], thr[NR], lsum[NR];
   f4_t o[NT][NR];
@@ -154,7 +136,8 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
           for (int j = 0; j < NR; ++j) sc[x % NI][j] = product(ka, qf[j][x / NI], sc[x % NI][j]);
         });
   };
-  auto softmax = [&](int tile, f4_t (&sc)[NI][NR], bf8_t (&pp)[NR]) __attribute__((always_inline)) {
+  auto softmax = [&](int tile, f4_t (&sc)[NI][NR], u4_t (&pp)[NR], auto h) __attribute__((always_inline)) {
+    constexpr bool H16 = decltype(h)::value;
     const int kbase = tile * KT;
     uint32_t on = 0;
 #pragma unroll
@@ -203,23 +186,23 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
         const f4_t s = sc[e / 2][j];
         const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2)], qscale[j], nm[j]));
         const float y = __builtin_amdgcn_exp2f(fmaf(s[2 * (e % 2) + 1], qscale[j], nm[j]));
-        w[e] = pack_bf16(x, y);
-        lsum[j] = add_two(w[e], lsum[j]);
+        w[e] = pack_weights<H16>(x, y);
+        lsum[j] = add_weights<H16>(w[e], lsum[j]);
       }
-      pp[j] = __builtin_bit_cast(bf8_t, w);
+      pp[j] = w;
     }
   };
-  auto values = [&](const bf8_t (&pp)[NR]) __attribute__((always_inline)) {
+  auto values = [&](const u4_t (&pp)[NR], auto halves) __attribute__((always_inline)) {
+    using v_t = std::conditional_t<decltype(halves)::value, h8_t, bf8_t>;
     const uint32_t at = lds_address(V) + v_lane<D>(lane_now<AFFINE ? 512 : D>(lane));
-    pipelined<NT, W::kGroup, bf8_t>(
+    pipelined<NT, W::kGroup, v_t>(
         [&](int t) __attribute__((always_inline)) {
           const u2_t x = read_transposed(at ^ (32 * t)), y = read_transposed((at ^ (32 * t)) + 16 * D * 2);
-          return __builtin_bit_cast(bf8_t, u4_t{x.x, x.y, y.x, y.y});
+          return __builtin_bit_cast(v_t, u4_t{x.x, x.y, y.x, y.y});
         },
-        [&](int t, bf8_t va) __attribute__((always_inline)) {
+        [&](int t, v_t va) __attribute__((always_inline)) {
 #pragma unroll
-          for (int j = 0; j < NR; ++j)
-            o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pp[j], o[t][j], 0, 0, 0);
+          for (int j = 0; j < NR; ++j) o[t][j] = product(va, __builtin_bit_cast(v_t, pp[j]), o[t][j]);
         });
   };
   auto clear = [&](f4_t (&sc)[NI][NR]) __attribute__((always_inline)) {
@@ -257,15 +240,15 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
       fetch(t0, 1);
       for (int tile = t0; tile <= t_hi; tile += kWaves) {
         f4_t sc[NI][NR];
-        bf8_t pp[NR];
+        u4_t pp[NR];
         wait_loads<NP>();  // K
         clear(sc);
         scores(K, sc);
         __builtin_amdgcn_s_waitcnt(0xC07F);  // K's reads are done (lgkmcnt 0)
         fetch(tile + kWaves, 0);
-        softmax(tile, sc, pp);
+        softmax(tile, sc, pp, std::false_type{});
         wait_loads<NP>();  // V
-        values(pp);
+        values(pp, std::false_type{});
         __builtin_amdgcn_s_waitcnt(0xC07F);
         fetch(tile + kWaves, 1);
       }
@@ -281,17 +264,15 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
         return lds_address(tile) + uint32_t(row * D * 2 + ((ln % 2 * (H / 8)) ^ turn_of<D>(row)) * 16);
       };
       constexpr int NRUN = H / 32;
-      // One side of a tile: codes, and the scales and biases of their runs of 32.
-      auto load = [&](int tile, int side, auto& codes, float (&s)[NRUN], float (&z)[NRUN]) __attribute__((always_inline)) {
-        constexpr int words = sizeof(codes) / 4;
+      // The lane's pool row of a tile; not ok: in no page (row 0 of page 0).
+      auto lane_row = [&](int tile, bool& ok) __attribute__((always_inline)) {
         const int tc = tile < t_hi ? tile : t_hi;
         const int t = min(tc * KT + r, n - 1);
         const int page = r < 16 ? page_of(min(tc * KT, n - 1)) : page_of(min(tc * KT + 16, n - 1));
-        const bool ok = paged::valid_page(a.pool, page);
-        const int64_t row = paged::pool_row(a.pool, ok ? page : 0, kvh, t & ((1 << a.pool.shift) - 1));
-        const u4_t* src = reinterpret_cast<const u4_t*>(static_cast<const uint32_t*>(a.slot[3 * side]) + (2 * row + half) * words);
-#pragma unroll
-        for (int i = 0; i < words / 4; ++i) codes[i] = src[i];
+        ok = paged::valid_page(a.pool, page);
+        return paged::pool_row(a.pool, ok ? page : 0, kvh, t & ((1 << a.pool.shift) - 1));
+      };
+      auto load_scales = [&](int64_t row, bool ok, int side, float (&s)[NRUN], float (&z)[NRUN]) __attribute__((always_inline)) {
         const uint16_t* sc = static_cast<const uint16_t*>(a.slot[3 * side + 1]) + row * (D / a.gs);
         const uint16_t* bi = static_cast<const uint16_t*>(a.slot[3 * side + 2]) + row * (D / a.gs);
 #pragma unroll
@@ -302,13 +283,53 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
           if (!ok) s[i] = z[i] = 0.0f;  // hidden, and finite
         }
       };
+      // One side of a tile: codes, and the scales and biases of their runs of 32.
+      auto load = [&](int tile, int side, auto& codes, float (&s)[NRUN], float (&z)[NRUN]) __attribute__((always_inline)) {
+        constexpr int words = sizeof(codes) / 4;
+        bool ok;
+        const int64_t row = lane_row(tile, ok);
+        const u4_t* src = reinterpret_cast<const u4_t*>(static_cast<const uint32_t*>(a.slot[3 * side]) + (2 * row + half) * words);
+#pragma unroll
+        for (int i = 0; i < words / 4; ++i) codes[i] = src[i];
+        load_scales(row, ok, side, s, z);
+      };
+      // V's range in the wavefront's tiles, by the largest values that the runs'
+      // scales and biases allow (a sixteenth of the rows' bytes, read again later).
+      float v_top = 0.0f, v_low = INFINITY;
+      bool fine = true;
+#pragma unroll 4
+      for (int tile = t0; tile <= t_hi; tile += kWaves) {
+        bool ok;
+        const int64_t row = lane_row(tile, ok);
+        float s[NRUN], z[NRUN];
+        load_scales(row, ok, 1, s, z);
+#pragma unroll
+        for (int i = 0; i < NRUN; ++i) {
+          const float x = fabsf(z[i]), y = fabsf(fmaf(s[i], float((1 << BV) - 1), z[i]));
+          fine &= x < INFINITY && y < INFINITY;
+          v_top = fmaxf(v_top, fmaxf(x, y));
+          if (fmaxf(x, y) > 0.0f) v_low = fminf(v_low, fmaxf(x, y));
+        }
+      }
+#pragma unroll
+      for (int d = 32; d > 0; d /= 2) {
+        v_top = fmaxf(v_top, __shfl_xor(v_top, d, kWave));
+        v_low = fminf(v_low, __shfl_xor(v_low, d, kWave));
+      }
+      if (v_top > 0.0f && v_top < INFINITY) v_up = __builtin_amdgcn_readfirstlane(15 - __builtin_amdgcn_frexp_expf(v_top));
+      // Too far apart for f16: what is no number has attend_row do the rows.
+      if (!__all(fine && (v_top == 0.0f || ldexpf(v_low, v_up) >= 0x1p-14f))) {
+        rare();
+#pragma unroll
+        for (int j = 0; j < NR; ++j) lsum[j] = NAN;
+      }
       u4_t kc[KW / 4], vc[VW / 4];
       float ks[NRUN], kz[NRUN], vs[NRUN], vz[NRUN];
       load(t0, 0, kc, ks, kz);
       load(t0, 1, vc, vs, vz);
       for (int tile = t0; tile <= t_hi; tile += kWaves) {
         f4_t sc[NI][NR];
-        bf8_t pp[NR];
+        u4_t pp[NR];
         float top = 0.0f;  // of the lane's half row, then of the row
 #pragma unroll
         for (int i = 0; i < NRUN; ++i)
@@ -342,26 +363,22 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[i][j][e] = ldexpf(sc[i][j][e], down[e]);
         }
-        softmax(tile, sc, pp);
+        softmax(tile, sc, pp, std::true_type{});
         const uint32_t vat = place(V);
 #pragma unroll
         for (int i = 0; i < H / 16; ++i) {
           uint32_t w[BV / 2], x[8];
-          float f[16];
 #pragma unroll
           for (int e = 0; e < BV / 2; ++e) w[e] = vc[(i * BV / 2 + e) / 4][(i * BV / 2 + e) % 4];
-          codes16<BV>(w, f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            x[e] = pack_bf16(fmaf(vs[i / 2], f[2 * e], vz[i / 2]), fmaf(vs[i / 2], f[2 * e + 1], vz[i / 2]));
+          const _Float16 s = _Float16(ldexpf(vs[i / 2], v_up)), z = _Float16(ldexpf(vz[i / 2], v_up));
+          halves16<BV>(w, h2_t{s, s}, h2_t{z, z}, x);
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            write_lds(vat ^ (16 * (2 * i + e)),
-                u4_t{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]});
+            write_lds(vat ^ (16 * (2 * i + e)), u4_t{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]});
           __builtin_amdgcn_sched_barrier(0);
         }
         load(tile + kWaves, 1, vc, vs, vz);
-        values(pp);
+        values(pp, std::true_type{});
       }
     }
   }
@@ -375,6 +392,11 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
       part_m[wave][16 * j + lr] = m[j];
       part_l[wave][16 * j + lr] = sum;
     }
+    if constexpr (AFFINE)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][j][e] = ldexpf(o[t][j][e], -v_up);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
       *reinterpret_cast<f4_t*>(mine + (16 * j + lr) * D + ((4 * t + lg) ^ (lr & 7)) * 4) = o[t][j];
@@ -410,7 +432,7 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     const f4_t v = sum * inv;
-    bad |= !(l > 0.0f) || !(v[0] == v[0] && v[1] == v[1] && v[2] == v[2] && v[3] == v[3]);
+    bad |= !(l > 0.0f) || !finite(v);
     *reinterpret_cast<u2_t*>(a.out + row * D + 4 * c4) = u2_t{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
   }
   if (a.part_o) return;

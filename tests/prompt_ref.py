@@ -123,24 +123,24 @@ def rotated(x, positions, theta, magnitude, interleaved):
 
 
 # ---------------------------------------------------------------- attention
-def bf16_values(side, bits, gs):
-    """f64 of the bf16 values that stored V rows are attended as: bf16 rows, or
-    scale * code + bias rounded to f32 (the fused multiply-add) and to bf16."""
-    if bits == 16:
-        return O.bf16_to_f32(side[0]).astype(np.float64)
-    s, b = (np.repeat(O.bf16_to_f32(t).astype(np.float64), gs, axis=-1) for t in side[1:])
-    x = (codes_of(side[0], bits) * s + b).astype(np.float32)
-    return O.bf16_to_f32(O.bf16_from_f32(x)).astype(np.float64)
+def halves(side, bits, gs):
+    """Whether V's groups allow largest values within 2^26 of each other (the
+    library takes f16 within 2^28)."""
+    s, z = (O.bf16_to_f32(t).astype(np.float64) for t in side[1:])
+    top = np.maximum(np.abs(z), np.abs(s * (2 ** bits - 1) + z))
+    return top.max(initial=0.0) <= 2.0 ** 26 * top[top > 0].min(initial=np.inf)
 
 
-def attend(q, k, v, at, scale, causal=True, window=-1, ok=None, off=0.0):
+def attend(q, k, v, at, scale, causal=True, window=-1, ok=None, off=0.0, off_v=0.0, off_w=2.0 ** -8):
     """One sequence and one KV head: q f64 [m, G, D] at positions `at`, k and v
-    f64 [n, D], ok: keys that can be seen at all, off: how far a key's channel
-    may be from k, relative to it. (out, tolerance) f64.
+    f64 [n, D], ok: keys that can be seen at all, off, off_v, off_w: how far a
+    key's or value's channel or a weight may be rounded, relative to it. (out,
+    tolerance) f64.
 
     Tolerance: half a bf16 step of the output (2^-8 of it); the weights'
-    rounding to bf16, 2^-8 each at most, which the sum of the rounded weights
-    takes out of what they share: sum w |v - out|; and the f32 arithmetic: a
+    rounding, which the sum of the rounded weights takes out of what they share:
+    off_w sum w |v - out| (and where it is f16's, 2^-25 each of the largest for
+    subnormal ones); the values', off_v sum w |v|; and the f32 arithmetic: a
     score's sum (2^-24 of the products' magnitudes an addition) and exp2's
     argument and result move a weight by their size, twice for the sum's; the
     running sums of weights and outputs 2^-24 an addition."""
@@ -168,7 +168,9 @@ def attend(q, k, v, at, scale, causal=True, window=-1, ok=None, off=0.0):
         d = 2 * (sums + 2.0 ** -22 * (np.abs(s).max(-1) + 4)) + see.sum() * 2.0 ** -24
         for g in range(G):
             spread = w[g] @ np.abs(vs - out[i, g])
-            tol[i, g] = 2.0 ** -8 * np.abs(out[i, g]) + 1.02 * 2.0 ** -8 * spread + 1.01 * d[g] * (w[g] @ np.abs(vs)) + 1e-30
+            tol[i, g] = 2.0 ** -8 * np.abs(out[i, g]) + 1.02 * off_w * spread + 1.01 * (d[g] + off_v) * (w[g] @ np.abs(vs)) + 1e-30
+            if off_w < 2.0 ** -8:  # f16's subnormals: of weights, and of values whose largest is 2^14 or more
+                tol[i, g] += 2.0 ** -25 * np.abs(vs - out[i, g]).sum(0) + 2.0 ** -39 * np.abs(v).max()
     return out, tol
 
 
@@ -205,8 +207,13 @@ def paged(p, q, starts, scale, window=-1, max_rows=None):
             # Affine keys: scale * code + bias (an f32 fused multiply-add, 2^-24) as f16, 2^-11.
             k = values_of([t[at] for t in p.sides[0]], p.bk, p.gs)
             k[~ok] = 0.0
-            v = bf16_values([t[at] for t in p.sides[1]], p.bv, p.gs)
-            o, t = attend(qf[a:b, h * G:(h + 1) * G], k, v, np.arange(n - (b - a), n), scale, True, window, ok, 0.0 if p.bk == 16 else 2.0 ** -11 + 2.0 ** -24)
+            v = values_of([t[at] for t in p.sides[1]], p.bv, p.gs)
+            v[~ok] = 0.0
+            # Affine values and the weights with them: f16 (2^-11), or bf16 (2^-8).
+            h16 = p.bv != 16 and halves([t[at][ok] for t in p.sides[1]], p.bv, p.gs)
+            o, t = attend(qf[a:b, h * G:(h + 1) * G], k, v, np.arange(n - (b - a), n), scale, True, window, ok,
+                          0.0 if p.bk == 16 else 2.0 ** -11 + 2.0 ** -24, 0.0 if p.bv == 16 else 2.0 ** -11 + 2.0 ** -24 if h16 else 2.0 ** -8,
+                          2.0 ** -11 if h16 else 2.0 ** -8)
             out[a:b, h * G:(h + 1) * G], tol[a:b, h * G:(h + 1) * G] = o, t
     return out, tol
 

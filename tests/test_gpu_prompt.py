@@ -295,6 +295,43 @@ def test_affine_ranges(T, D, counts, kq, ks, vs):
     close(run_paged(T, p, q, starts_of(counts), scale), want, tol, starts_of(counts), "affine ranges")
 
 
+@pytest.mark.parametrize("counts", [[3, 3], [150, 90]])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_affine_values_far_apart(T, D, counts):
+    """The last rows' values are 2^60 times larger than the others': queries
+    that see the small ones alone keep them."""
+    say("far apart", D, counts)
+    p = Paged([150, 90], 1, D, 16, AFFINE, 8, 8, 32, seed=5)
+    rng = np.random.default_rng(D)
+    small = [147 if counts[0] == 3 else 60, 87 if counts[0] == 3 else 40]
+    for b in range(2):
+        for row in range(int(p.lens[b])):
+            k, v = (O.bf16_from_f32((rng.standard_normal((1, D)) * m).astype(np.float32)) for m in (1.0, 1.0 if row <= small[b] else 2.0 ** 60))
+            p.write(b, row, k, v)
+    q = kv_bf16((sum(counts), 2, D), D)
+    starts = starts_of(counts)
+    want, tol = R.paged(p, q, starts, D ** -0.5)
+    assert 0 < np.abs(want[0]).max() < 8.0 and tol[0].max() < 1.0  # no share of the large ones
+    close(run_paged(T, p, q, starts, D ** -0.5), want, tol, starts, "far apart")
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("few", [False, True])
+def test_values_next_to_the_largest(T, D, few):
+    """Sums of values that pass f32 where their mean does not."""
+    say("largest", D, few)
+    p = Paged([70], 1, D, 16, BF16, seed=5).fill(2)
+    top = O.bf16_from_f32(np.array([3.3e38], np.float32))[0]
+    p.sides[1][0][..., 7] = np.where(p.sides[1][0][..., 7] == GUARD, GUARD, top)
+    counts = [3] if few else [70]
+    q = kv_bf16((counts[0], 2, D), D)
+    starts = starts_of(counts)
+    want, tol = R.paged(p, q, starts, D ** -0.5)
+    assert want[..., 7].min() > 3.2e38
+    # The result may round up to the type's infinity: half a step below it does not.
+    close(run_paged(T, p, q, starts, D ** -0.5), want, tol, starts, "largest")
+
+
 @pytest.mark.parametrize("kind", [BF16, AFFINE])
 @pytest.mark.parametrize("counts", [[6], [90]])
 @pytest.mark.parametrize("D", [64, 128, 256, 512])
