@@ -74,12 +74,17 @@ __device__ __forceinline__ void turn_halves(uint4& x, uint4& y, const Angle* a) 
   y = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// A quotient by a number fixed for a launch: x / d for x * d below 2^32.
+// A quotient by a number fixed for a launch. m is 2^32 / d rounded up, less
+// than one too much: the product's upper half is x / d or, from x * d = 2^32
+// on, at times one more.
 struct Divisor {
   uint32_t d, m;
 };
 inline Divisor divisor(int d) { return Divisor{uint32_t(d), uint32_t(((uint64_t(1) << 32) + d - 1) / d)}; }
-__device__ __forceinline__ uint32_t quotient(uint32_t x, Divisor d) { return d.d == 1 ? x : __umulhi(x, d.m); }
+__device__ __forceinline__ uint32_t quotient(uint32_t x, Divisor d) {
+  const uint32_t q = d.d == 1 ? x : __umulhi(x, d.m);
+  return q * d.d > x ? q - 1 : q;
+}
 
 // The heads of a workgroup's tokens as jobs, what one thread turns or copies at
 // once: eight channels (neighbours, and channels behind the rotated ones),

@@ -57,7 +57,7 @@ CASES = [
     # D, rd, heads, tokens
     (128, 128, 40, 5), (128, 128, 1, 1), (64, 64, 3, 33), (256, 64, 7, 9), (512, 512, 2, 3), (512, 384, 16, 2),
     (128, 44, 5, 6), (64, 2, 2, 4), (128, 126, 3, 3), (96, 80, 4, 7), (8, 6, 9, 11), (1024, 1024, 2, 2), (24, 24, 1, 100),
-    (16, 16, 1024, 2),
+    (16, 16, 1024, 2), (1024, 1022, 1024, 2), (1024, 1022, 700, 3),
 ]
 
 
@@ -162,6 +162,9 @@ APPENDS = [
     (AFFINE, 8, 8, 32, 64, 32, 1, 5, 30, [1, 31], [1, 30]),
     (AFFINE, 8, 4, 32, 256, 64, 5, 1, 64, [100, 64, 65], [36, 64, 1]),
     (AFFINE, 4, 8, 128, 512, 128, 2, 0, 96, [300, 7], [299, 0]),
+    # A token's work in more than 2^16 pieces, of one token a workgroup and of two.
+    (BF16, 16, 16, 64, 512, 16, 1, 1020, 510, [3], [3]),
+    (AFFINE, 4, 4, 64, 128, 16, 1, 1020, 126, [520], [520]),
 ]
 
 
