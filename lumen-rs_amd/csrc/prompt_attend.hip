@@ -17,9 +17,9 @@ namespace {
 // Affine rows of the sequences that have queries, dequantized once a KV head, as
 // f16 (11 bits where bf16 keeps 8) times powers of two that bring the head's
 // largest K and V below 2^15; V as bf16 where its groups' largest values lie too
-// far apart for f16, since a query may see the small ones alone. First what a
-// head's scales and biases allow: (largest |K|, largest |V|, smallest |V| of a
-// group's largest but zero).
+// far apart for f16, since a query may see the small ones alone (K's are met by
+// kCoarse). First what a head's scales and biases allow: (largest finite |K|,
+// largest |V|, smallest |V| of a group's largest but zero).
 constexpr int kRangeParts = 32;
 
 struct Rows {
@@ -50,7 +50,8 @@ __global__ __launch_bounds__(256) void range_kernel(const Args a, int D, float4*
     const int64_t row = row_of<kPagedAffine>(a, b, 0, h, from + i / groups);
     if (row < 0) continue;
     const int64_t g = row * groups + i % groups;
-    k = fmaxf(k, bound(0, g, most_k));
+    const float y = bound(0, g, most_k);
+    if (y < INFINITY) k = fmaxf(k, y);
     const float x = bound(1, g, most_v);
     v = fmaxf(v, x);
     if (x > 0.0f) low = fminf(low, x);

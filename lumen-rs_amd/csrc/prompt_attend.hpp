@@ -17,9 +17,9 @@
 // rows: S^T = K Q^T (Q in registers), online softmax per row, whose running
 // maximum may lag by kTau so that the accumulators are seldom rescaled, then
 // O^T += V^T P^T, the scores' registers being the operand's layout and V
-// transposed by the LDS read. Weights are rounded to bf16 (V keeps bf16's
-// range; f16 would keep three more bits of the weights and lose the range),
-// and the row sum counts them as rounded.
+// transposed by the LDS read. Weights are rounded to bf16 over bf16 rows (V
+// keeps its range; f16 would keep three more bits of the weights and lose it),
+// to f16 over affine rows as f16, and the row sum counts them as rounded.
 //
 // Weights of hidden keys are exact zeros, but zero times an infinite value is
 // NaN (and sums of values next to f32's largest pass it): a row that ends with
@@ -74,6 +74,12 @@ struct Args {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kBf16 = 0x7fffffff;
+// The slab's keys share a power of two a (sequence, KV head): a channel is off by
+// up to 2^-25, half of f16's least step, where the largest key is 2^14 or more, and
+// a score by D 2^15 2^-25 of those units. A row whose unit makes that more than
+// kCoarse (in log2 units; it may see none of the large keys) is done by attend_row:
+// |q| |k| scale of 2^28 or so, far from where a softmax tells keys apart.
+constexpr float kCoarse = 0x1p-10f;
 
 // A sequence's queries [first, first + count) and the keys that it has.
 struct Sequence {
@@ -544,7 +550,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
 #pragma unroll
   for (int j = 0; j < NR; ++j) {
     m[j] = -INFINITY;
-    lsum[j] = 0.0f;
+    lsum[j] = F16 && qscale[j] * (D * 0x1p-10f) > kCoarse ? NAN : 0.0f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -810,7 +816,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
       continue;
     }
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    bad |= !(sum > 0.0f);  // no key, or none of a score above -infinity
+    bad |= !(sum > 0.0f);  // no key, none of a score above -infinity, or kCoarse
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const f4_t v = o[t][j] * inv;

@@ -315,6 +315,37 @@ def test_affine_values_far_apart(T, D, counts):
     close(run_paged(T, p, q, starts, D ** -0.5), want, tol, starts, "far apart")
 
 
+@pytest.mark.parametrize("counts", [[3, 3], [150, 90]])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("large", [2.0 ** 60, np.inf])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 18])
+def test_affine_keys_far_apart(T, D, counts, large, size):
+    """The last row's key is far larger than the others', or infinite: queries
+    before it are as with an ordinary one there, bounds included."""
+    say("keys far apart", D, counts, large, size)
+    pools = []
+    for top in (1.0, large):
+        p = Paged([150, 90], 1, D, 16, AFFINE, 8, 8, 32, seed=5)
+        rng = np.random.default_rng(D)
+        for b in range(2):
+            n = int(p.lens[b])
+            for row in range(n):
+                k, v = (rng.standard_normal((1, D)).astype(np.float32) for _ in range(2))
+                last = row == n - 1
+                k *= 2.0 ** 60 if last and top != 1.0 else size
+                p.write(b, row, O.bf16_from_f32(k), O.bf16_from_f32(v))
+            if top == np.inf:
+                p.sides[0][1][p.table[b, (n - 1) // 16], 0, (n - 1) % 16] = 0x7F80  # its scales
+        pools.append(p)
+    q = O.bf16_from_f32(np.random.default_rng(D + 1).standard_normal((sum(counts), 2, D)).astype(np.float32) / np.float32(size))
+    starts = starts_of(counts)
+    want, tol = R.paged(pools[0], q, starts, D ** -0.5)
+    got = O.bf16_to_f32(run_paged(T, pools[1], q, starts, D ** -0.5)[:sum(counts)])
+    before = np.ones(sum(counts), bool)
+    before[starts[1:] - 1] = False
+    R.check(got[before], want[before], tol[before], "keys far apart")
+
+
 @pytest.mark.parametrize("D", [64, 128, 256, 512])
 @pytest.mark.parametrize("few", [False, True])
 def test_values_next_to_the_largest(T, D, few):
