@@ -443,7 +443,8 @@ size_t tqkv_paged_evict_workspace_size(const tqkv_paged_kv* kv, int64_t budget);
  * batch at most 1024, page_rows in {16, 32, 64, 128, 256}, num_pages below
  * 2^31, table_stride * page_rows at most 2^30. All arrays are device int32,
  * 4-byte aligned. lens and free_count are read as the paged calls read lens:
- * below 0 as 0, above what the table (the stack) can hold as that.
+ * below 0 as 0, above what the table (the stack) can hold as that. Calls on
+ * the same tables must not overlap in time.
  */
 typedef struct tqkv_page_tables {
   int32_t batch;
@@ -562,7 +563,8 @@ int32_t tqkv_rope_apply(const tqkv_rope* rope, const int32_t* positions, int64_t
  * the pool has its queries rotated only. With kv->weights, a written row's are cleared
  * (slots' sequence and position). kv->table and kv->lens are not read. q_out
  * may be q with the same stride; H at most 1024; alignment as in
- * tqkv_paged_append.
+ * tqkv_paged_append. Two tokens of a call with the same slot leave it with a mixture
+ * of both.
  */
 int32_t tqkv_paged_append_rope(const tqkv_paged_kv* kv, const tqkv_rope* rope, const uint16_t* q,
                                int32_t H, int64_t q_stride, uint16_t* q_out, int64_t q_out_stride,
@@ -611,11 +613,15 @@ size_t tqkv_packed_attend_workspace_size(int32_t batch, int32_t H, int32_t H_kv,
  * its rows up to their own position, with window > 0 the last `window` of
  * these. Rows of invalid pages get no attention; a query that sees no row
  * gets zeros. max_rows: the host's bound on lens, as tqkv_paged_decode_attend
- * takes it. Affine rows enter as scale * code + bias in 11 bits, what is below
- * 2^-28 of their head's largest with fewer, and a query's channels below 2^-28
- * of its largest alike; values in 11 bits of their group's largest, or in bf16's
- * 8 where these lie 2^28 apart in a head (few queries over such rows cost much
- * more).
+ * takes it. Affine rows enter as scale * code + bias in 11 bits (keys down to
+ * 2^-28 of their head's largest or their own, a query's channels of its largest,
+ * values of their group's); values in bf16's 8 where their groups' largest lie
+ * 2^28 apart in a head. Few queries over such values, and scores of which f16's
+ * steps could be 2^-10 or more (|q| |k| scale of 2^28), are computed in f32, at
+ * many times the cost.
+ * Affine rows of longer chunks are dequantized once into the workspace, 4 * batch *
+ * H_kv * max_rows * dim bytes of it: a batch of many sequences of which few have
+ * queries is best called with a table of those alone.
  * kv->weights is not touched. q, out, H and the workspace as above; results
  * depend on starts, lens, tokens and max_rows, not on the run.
  */

@@ -142,6 +142,27 @@ def test_paged_prefill_refusals():
     assert T.paged_prefill_workspace_size(view(), 7, 64, 512) == 0
 
 
+def test_workspaces_that_are_too_small():
+    """A byte too few or off by 8: refused before any launch."""
+    affine = view(kind=T.CACHE_AFFINE, batch=2)
+    need = T.paged_prefill_workspace_size(affine, 8, 300, 512)
+    assert need >= 4 * 2 * affine.kv_heads * 512 * affine.dim  # the dequantized rows
+    ok = dict(kv=affine, q=A, q_stride=1024, H=8, starts=A, tokens=300, scale=0.1, max_rows=512, out=2 * A, workspace=A, workspace_bytes=need)
+    for other in (dict(workspace_bytes=need - 1), dict(workspace_bytes=0), dict(workspace=A + 8)):
+        refused(T.EINVAL_ARG, T.paged_prefill_attend, **{**ok, **other})
+    # Splits alone: long rows of one sequence.
+    long = view(kind=T.CACHE_BF16, batch=1, num_pages=4096, table_stride=4096)
+    rows = 4096 * long.page_rows
+    need = T.paged_prefill_workspace_size(long, 8, 2, rows)
+    assert need > 0
+    refused(T.EINVAL_ARG, T.paged_prefill_attend, **{**ok, "kv": long, "tokens": 2, "max_rows": rows, "workspace_bytes": need - 1})
+    # (A split holds at least 16 keys a row of its block: 4,096 of 256 rows.)
+    assert T.packed_attend_workspace_size(1, 8, 4, 128, 4096) == 0
+    need = T.packed_attend_workspace_size(1, 1, 1, 128, 8192)
+    assert need > 0
+    refused(T.EINVAL_ARG, T.packed_attend, A, 128, A, A, 128, 128, 1, 1, 1, 128, A, 8192, 0.1, 2 * A, workspace=A, workspace_bytes=need - 1)
+
+
 def test_struct_layouts_match_the_header(tmp_path):
     structs = {"tqkv_page_tables": T.PageTables, "tqkv_rope_config": T.RopeConfig, "tqkv_rope": T.Rope}
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "tqkv.h"', "int main(void) {"]
