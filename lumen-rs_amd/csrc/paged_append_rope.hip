@@ -3,7 +3,9 @@
 // once: bound by HBM, for a decode step by a launch's time. One kernel, as
 // parts (keys, values, queries) on the grid's second axis, so that a step's
 // few tokens meet many CUs. A token's slot says all that its rows need, so
-// nothing is searched for in every layer.
+// nothing is searched for in every layer. 23,100 tokens of 10 prompts, 48 heads of 128: 140 us
+// for 569 MB (4.1 TB/s; 162 with one job a thread on its way); 64 tokens of a
+// decode step: 3.9 us on the device, 11.6 with the host's call.
 #include "affine_quantize.hpp"
 #include "paged.hpp"
 #include "rope.hpp"

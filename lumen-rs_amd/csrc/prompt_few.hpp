@@ -13,6 +13,11 @@
 // back; V times one power of two for the wavefront's rows. Where V's groups'
 // largest values lie 2^28 apart (a query may see the small ones alone), attend_row
 // does the rows.
+//
+// 32 sequences of up to 24,000 bf16 rows, D = 128, 6 tokens each: 117 us for 453 MB
+// (3.9 TB/s; a large copy 4.9). The same of 4-bit rows: 134 us, 13 of them the pass
+// over the values' scales; 16 sequences of 8,000 at D = 256 252 us: the conversion's
+// vector operations bound it.
 #pragma once
 
 #include "prompt_attend.hpp"

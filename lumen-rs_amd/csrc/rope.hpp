@@ -107,7 +107,9 @@ inline Jobs jobs_of(const Rope& r, int heads, int dim, bool copy) {
   j.a_token = divisor(each * (heads > 0 ? heads : 1));
   return j;
 }
-// Tokens a workgroup: enough jobs for every thread to have kDeep on their way.
+// Tokens a workgroup: enough jobs for every thread to have kDeep on their way, as
+// long as there is a workgroup or two for every CU. Prompts' appends: 145 us with up
+// to 8 tokens, 149 with 4, 162 with 2, 180 with 1.
 constexpr int kDeep = 4, kMostTokens = 8;
 inline int tokens_of(const Jobs& j, int64_t tokens) {
   int n = 1;
