@@ -1,6 +1,8 @@
 """Attention of packed sequences on the GPU, over their own tokens and over the
 paged cache, against 64 bits; and the paged cache's calls as a server makes
 them, one after the other."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -480,6 +482,73 @@ def test_captured_without_a_workspace_size_to_grow(T):
             T.hip().copy_in(out.ptr, np.full((70, 2, 128), GUARD, np.uint16))
             launch()
             assert np.array_equal(out.numpy(), want)
+
+
+@pytest.mark.parametrize("kind", [BF16, AFFINE])
+@pytest.mark.parametrize("counts", [[3, 2], [150, 90]])
+def test_pages_past_32_bits(T, kind, counts):
+    """The same pages behind the first 2^32 bytes (and 2^31 elements) of a pool:
+    what the append writes there and the attention reads are the near ones' bits."""
+    say("far pages", kind, counts)
+    D, R_, Hkv, H = 512, 256, 4, 4
+    p = Paged([300, 200], Hkv, D, R_, kind, 8, 8, 64, seed=5).fill(2)
+    near = p.device(T)
+    page = p.sides[0][0][0].nbytes
+    far = (1 << 32) // page + 3  # bf16: 2^31 elements too
+    sides, big = [], []
+    for side in p.sides:
+        for x in side:
+            big.append(T.DeviceArray(((far + p.pages) * x[0].nbytes,), np.uint8))
+            T.hip().copy_in(big[-1].ptr + far * x[0].nbytes, x)
+            sides.append(big[-1].ptr)
+    table = T.DeviceArray.of(np.where(p.table >= 0, p.table + far, -1).astype(np.int32))
+    view = near.view(num_pages=far + p.pages, slots=sides, table=table.ptr)
+    n, width = sum(counts), (H + 2 * Hkv) * D
+    x = kv_bf16((n, width), 7)
+    dx, ds = T.DeviceArray.of(x), T.DeviceArray.of(starts_of(counts))
+    turns, m = T.rope_turns(128)
+    dt = T.DeviceArray.of(np.array(turns, np.uint64))
+    k = dx.ptr + 2 * H * D
+    slots = np.array([[p.table[b, row // R_], row % R_, row, b] for b, c in enumerate(counts)
+                      for row in range(int(p.lens[b]) - c, int(p.lens[b]))], np.int32)
+    outs = []
+    for kv, first in ((near.view(), 0), (view, far)):
+        s = slots.copy()
+        s[:, 0] += first
+        dsl, q, out = T.DeviceArray.of(s), T.DeviceArray((n, H, D), np.uint16), T.DeviceArray((n, H, D), np.uint16)
+        T.paged_append_rope(kv, T.rope(128, 0, m, dt.ptr), dx.ptr, H, width, q.ptr, H * D, k, k + 2 * Hkv * D, width, D, dsl.ptr, n)
+        T.paged_prefill_attend(kv, q.ptr, H * D, H, ds.ptr, n, D ** -0.5, 512, out.ptr)
+        T.hip().sync()
+        outs.append(out.numpy())
+    assert np.array_equal(*outs)
+    for t, b, x in zip([t for side in near.sides for t in side], big, [x for side in p.sides for x in side]):
+        assert np.array_equal(t.numpy(), T.hip().download(b.ptr + far * x[0].nbytes, x.shape, x.dtype))
+
+
+def test_two_streams_at_once(T):
+    """Calls on two streams with workspaces of their own, queued together."""
+    D, H = 128, 8
+    pools = [Paged([1500, 700], 2, D, 16, AFFINE, 4, 8, 64, seed=s).fill(s) for s in (1, 2)]
+    counts = [600, 700]
+    q = kv_bf16((sum(counts), H, D), 3)
+    starts = starts_of(counts)
+    alone = [run_paged(T, p, q, starts, D ** -0.5) for p in pools]
+    dq, ds = T.DeviceArray.of(q), T.DeviceArray.of(starts)
+    on = [p.device(T) for p in pools]
+    most = pools[0].stride * 16
+    need = T.paged_prefill_workspace_size(on[0].view(), H, sum(counts), most)
+    ws = [poisoned(T, need) for _ in on]
+    outs = [T.DeviceArray((sum(counts), H, D), np.uint16) for _ in on]
+    T.hip().sync()
+    streams = [T.hip().stream() for _ in on]
+    for _ in range(3):
+        for d, w, out, s in zip(on, ws, outs, streams):
+            T.paged_prefill_attend(d.view(), dq.ptr, H * D, H, ds.ptr, sum(counts), D ** -0.5, most, out.ptr, -1, w.ptr, need, s)
+    T.hip().sync()
+    for s in streams:
+        T.hip().h.hipStreamDestroy(ctypes.c_void_p(s))
+    for out, want in zip(outs, alone):
+        assert np.array_equal(out.numpy(), want)
 
 
 # ------------------------------------------------------------ as a server does
