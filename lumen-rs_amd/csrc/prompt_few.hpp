@@ -68,6 +68,36 @@ __device__ __forceinline__ void halves16(const uint32_t* w, h2_t s, h2_t z, uint
   }
 }
 
+// The same of s and z times 2^up, in units in which the results are below 2^15.
+// Where f16 does not hold these (its least step is 2^-24, a scale may be a 255th
+// of a group's largest) they are taken times a power of two more, up to what
+// brings the group's largest there too, and the results, rounded to 11 bits,
+// divided by it. So a value is off by its own rounding and half a step, whatever
+// the others are (scales rounded to the steps cost 8-bit values 2^22 below the
+// largest their bits).
+template <int BITS, bool STEPS>
+__device__ __forceinline__ void halves16(const uint32_t* w, float s, float z, int up, uint32_t (&x)[8]) {
+  int lift = 0;
+  if constexpr (STEPS) {
+    const float most = fmaxf(fabsf(z), fabsf(fmaf(s, float((1 << BITS) - 1), z)));
+    lift = min(15 - __builtin_amdgcn_frexp_expf(ldexpf(most, up)), 14);
+  }
+  const _Float16 sh = _Float16(ldexpf(s, up + lift)), zh = _Float16(ldexpf(z, up + lift));
+  halves16<BITS>(w, h2_t{sh, sh}, h2_t{zh, zh}, x);
+  if constexpr (STEPS) {
+    const _Float16 down = _Float16(ldexpf(1.0f, -lift));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_bit_cast(uint32_t, as_h2(x[i]) * h2_t{down, down});
+  }
+}
+// The least of them but zero: f16 holds bf16's 8 bits from 2^-17 on.
+__device__ __forceinline__ float least_of(float least, float s, float z) {
+  if (s != 0.0f) least = fminf(least, fabsf(s));
+  if (z != 0.0f) least = fminf(least, fabsf(z));
+  return least;
+}
+constexpr float kHeld = 0x1p-17f;
+
 template <int D, Source S, int BK, int BV>
 __global__ __launch_bounds__((Few<D, S == kPagedAffine>::kThreads))
 __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few_kernel(const Args a) {
@@ -298,9 +328,39 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
         for (int i = 0; i < words / 4; ++i) codes[i] = src[i];
         load_scales(row, ok, side, s, z);
       };
+      // A side's codes into its tile. The rare form in a loop of its own: a branch
+      // in each step cost the others 9% of a call's time at D = 128.
+      auto convert = [&](const auto& codes, const float (&s)[NRUN], const float (&z)[NRUN], int up, bool steps,
+                         const uint16_t* tile, auto width) __attribute__((always_inline)) {
+        constexpr int BITS = decltype(width)::value;
+        const uint32_t to = place(tile);
+        auto run = [&](auto form) __attribute__((always_inline)) {
+#pragma unroll
+          for (int i = 0; i < H / 16; ++i) {
+            uint32_t w[BITS / 2], x[8];
+#pragma unroll
+            for (int e = 0; e < BITS / 2; ++e) {
+              w[e] = codes[(i * BITS / 2 + e) / 4][(i * BITS / 2 + e) % 4];
+              // Not to be taken apart before the branch, for both: registers.
+              if constexpr (decltype(form)::value) asm volatile("" : "+v"(w[e]));
+            }
+            halves16<BITS, decltype(form)::value>(w, s[i / 2], z[i / 2], up, x);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              write_lds(to ^ (16 * (2 * i + e)), u4_t{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]});
+            __builtin_amdgcn_sched_barrier(0);  // few values at a time: registers
+          }
+        };
+        if (steps) {
+          rare();
+          run(std::true_type{});
+        } else {
+          run(std::false_type{});
+        }
+      };
       // V's range in the wavefront's tiles, by the largest values that the runs'
       // scales and biases allow (a sixteenth of the rows' bytes, read again later).
-      float v_top = 0.0f, v_low = INFINITY;
+      float v_top = 0.0f, v_low = INFINITY, v_least = INFINITY;  // least: of the scales and biases but zero
       bool fine = true;
 #pragma unroll 4
       for (int tile = t0; tile <= t_hi; tile += kWaves) {
@@ -314,12 +374,14 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
           fine &= x < INFINITY && y < INFINITY;
           v_top = fmaxf(v_top, fmaxf(x, y));
           if (fmaxf(x, y) > 0.0f) v_low = fminf(v_low, fmaxf(x, y));
+          v_least = least_of(v_least, s[i], z[i]);
         }
       }
 #pragma unroll
       for (int d = 32; d > 0; d /= 2) {
         v_top = fmaxf(v_top, __shfl_xor(v_top, d, kWave));
         v_low = fminf(v_low, __shfl_xor(v_low, d, kWave));
+        v_least = fminf(v_least, __shfl_xor(v_least, d, kWave));
       }
       if (v_top > 0.0f && v_top < INFINITY) v_up = __builtin_amdgcn_readfirstlane(15 - __builtin_amdgcn_frexp_expf(v_top));
       // Too far apart for f16: what is no number has attend_row do the rows.
@@ -328,6 +390,7 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
 #pragma unroll
         for (int j = 0; j < NR; ++j) lsum[j] = NAN;
       }
+      const bool v_steps = __any(ldexpf(v_least, v_up) < kHeld);
       u4_t kc[KW / 4], vc[VW / 4];
       float ks[NRUN], kz[NRUN], vs[NRUN], vz[NRUN];
       load(t0, 0, kc, ks, kz);
@@ -342,20 +405,11 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
         top = fmaxf(top, __shfl_xor(top, 1, kWave));
         const int up = top > 0.0f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
         if (half == 0) shifts[wave][r] = -up;
-        const uint32_t kat = place(K);
+        float k_least = INFINITY;
 #pragma unroll
-        for (int i = 0; i < H / 16; ++i) {
-          uint32_t w[BK / 2], x[8];
-#pragma unroll
-          for (int e = 0; e < BK / 2; ++e) w[e] = kc[(i * BK / 2 + e) / 4][(i * BK / 2 + e) % 4];
-          const _Float16 s = _Float16(ldexpf(ks[i / 2], up)), z = _Float16(ldexpf(kz[i / 2], up));
-          halves16<BK>(w, h2_t{s, s}, h2_t{z, z}, x);
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            write_lds(kat ^ (16 * (2 * i + e)),
-                u4_t{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]});
-          __builtin_amdgcn_sched_barrier(0);  // few values at a time: registers
-        }
+        for (int i = 0; i < NRUN; ++i) k_least = least_of(k_least, ks[i], kz[i]);
+        const bool k_steps = __any(ldexpf(k_least, up) < kHeld);
+        convert(kc, ks, kz, up, k_steps, K, std::integral_constant<int, BK>{});
         load(tile + kWaves, 0, kc, ks, kz);
         clear(sc);
         scores(K, sc);
@@ -369,19 +423,7 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
             for (int e = 0; e < 4; ++e) sc[i][j][e] = ldexpf(sc[i][j][e], down[e]);
         }
         softmax(tile, sc, pp, std::true_type{});
-        const uint32_t vat = place(V);
-#pragma unroll
-        for (int i = 0; i < H / 16; ++i) {
-          uint32_t w[BV / 2], x[8];
-#pragma unroll
-          for (int e = 0; e < BV / 2; ++e) w[e] = vc[(i * BV / 2 + e) / 4][(i * BV / 2 + e) % 4];
-          const _Float16 s = _Float16(ldexpf(vs[i / 2], v_up)), z = _Float16(ldexpf(vz[i / 2], v_up));
-          halves16<BV>(w, h2_t{s, s}, h2_t{z, z}, x);
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            write_lds(vat ^ (16 * (2 * i + e)), u4_t{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]});
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        convert(vc, vs, vz, v_up, v_steps, V, std::integral_constant<int, BV>{});
         load(tile + kWaves, 1, vc, vs, vz);
         values(pp, std::true_type{});
       }
