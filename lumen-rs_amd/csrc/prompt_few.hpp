@@ -10,7 +10,7 @@
 // next tile's codes have been loaded into meanwhile, to f16 (bf16 would cost the
 // results three bits): every row of K times a power of two that brings the
 // largest value its scales and biases allow below 2^15, which its scores take
-// back; V times one power of two for the wavefront's rows. Where V's groups'
+// back (rows whose steps would be more than kCoarse in a score are attend_row's); V times one power of two for the wavefront's rows. Where V's groups'
 // largest values lie 2^28 apart (a query may see the small ones alone), attend_row
 // does the rows.
 //
@@ -144,6 +144,17 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
     pos[j] = p0 + int(r / a.G);
     qscale[j] = fmaxf(load_query<D>(a, a.q + (seq.first + r / a.G) * a.qs + (int64_t(kvh) * a.G + r % a.G) * D, lg, qf[j]),
                       kLeastScale);
+  }
+  // The largest exponent of a key row's units that leaves f16's steps kCoarse in
+  // the scores of every row here.
+  int most_units = 0;
+  if constexpr (AFFINE) {
+    float top = qscale[0];
+    if constexpr (NR == 2) top = fmaxf(top, qscale[1]);
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) top = fmaxf(top, __shfl_xor(top, d, kWave));
+    top = fmaxf(top, 0x1p-100f) * (D * 0x1p-10f);
+    most_units = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(kCoarse / top) - 1);
   }
   float m[NR], nm[NR], thr[NR], lsum[NR];
   f4_t o[NT][NR];
@@ -409,6 +420,17 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
 #pragma unroll
         for (int i = 0; i < NRUN; ++i) k_least = least_of(k_least, ks[i], kz[i]);
         const bool k_steps = __any(ldexpf(k_least, up) < kHeld);
+        const int t = tile * KT + r;
+        const bool coarse = top > 0.0f && -up > most_units && t >= key_lo && t < key_hi;
+        if (__any(coarse)) {
+          rare();
+          int units = coarse ? -up : most_units;
+#pragma unroll
+          for (int d = 32; d > 0; d /= 2) units = max(units, __shfl_xor(units, d, kWave));
+#pragma unroll
+          for (int j = 0; j < NR; ++j)
+            if (ldexpf(qscale[j], units) * (D * 0x1p-10f) > kCoarse) lsum[j] = NAN;
+        }
         convert(kc, ks, kz, up, k_steps, K, std::integral_constant<int, BK>{});
         load(tile + kWaves, 0, kc, ks, kz);
         clear(sc);

@@ -87,3 +87,44 @@ def test_values_of_small_groups_keep_their_bits(T, counts, D, gs, bits, shape):
                     tol -= 2.0 ** -39 * np.abs(v).max()
                 assert tol.min() > 0.0
                 R.check(got[a:e], want, tol, f"small values {far} {window}")
+
+
+@pytest.mark.parametrize("counts", [FEW, MANY])
+@pytest.mark.parametrize("D,gs", [(64, 32), (128, 64), (256, 128), (512, 32)])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("far", [16, 20, 24, 32, 60])
+def test_keys_of_small_groups_keep_their_bits(T, counts, D, gs, bits, far):
+    """Every seventh key's first group is 2^far times larger than all others, and
+    the queries' channels there are zero: the scores are those of the other
+    groups. Where f16's steps could move them by 2^-10 they are f32's, with
+    nothing lost to the large ones."""
+    say("small keys", counts, D, gs, bits, far)
+    p = Paged(LENS, 1, D, 16, AFFINE, bits, 8, gs, seed=5)
+    rng = np.random.default_rng(D + bits)
+    for b, n in enumerate(LENS):
+        for row in range(n):
+            k, v = rng.standard_normal((2, 1, D))
+            if row % 7 == 3:
+                k[:, :gs] *= 2.0 ** far
+            p.write(b, row, bf16(k), bf16(v))
+    x = rng.standard_normal((sum(counts), 2, D))
+    x[..., :gs] = 0.0
+    q = bf16(x)
+    starts = starts_of(counts)
+    scale = 2.0 * D ** -0.5  # scores of a few units
+    got = O.bf16_to_f32(run_paged(T, p, q, starts, scale))
+    want, tol = R.paged(p, q, starts, scale)
+    # f16's steps in a score: D channels below 2^15 times half of 2^-24, in units
+    # in which the largest channels of the query and of the key are below 2^15.
+    # Where that is 2^-10 or more, it is f32 that the tolerance counts.
+    step = D * 2.0 ** 15 * 2.0 ** -25 * scale * np.log2(np.e) / 2.0 ** 30
+    qf = np.abs(O.bf16_to_f32(q)).max(-1)
+    for i, n in enumerate(LENS):
+        a, e = int(starts[i]), int(starts[i + 1])
+        k, v = (stored(p, i, n, side)[0] for side in range(2))
+        if step * qf[a:e].min() * np.abs(k).max() < 2.0 ** -10:
+            continue
+        f = O.bf16_to_f32(q[a:e]).astype(np.float64)
+        want[a:e], tol[a:e] = R.attend(f, k, v, np.arange(n - (e - a), n), scale, off_v=2.0 ** -11 + 2.0 ** -24, off_w=2.0 ** -11)
+    assert far < 32 or tol.max() < 0.2
+    R.check(got, want, tol, f"small keys {far}")
