@@ -38,6 +38,7 @@ __global__ __launch_bounds__(256) void range_kernel(const Args a, int D, float4*
   const Rows rows = seen_rows(a, b);
   const int span = max(0, rows.n - rows.lo), each = (span + kRangeParts - 1) / kRangeParts;
   const int from = rows.lo + int(blockIdx.x) * each, to = min(from + each, rows.n);
+  const int words = a.gs * a.bits_v / 32;  // of a group
   const float most_k = float((1 << a.bits_k) - 1), most_v = float((1 << a.bits_v) - 1);
   const auto bound = [&](int side, int64_t g, float most) {
     const float s = bf16_to_f32(static_cast<const uint16_t*>(a.slot[3 * side + 1])[g]);
@@ -53,6 +54,14 @@ __global__ __launch_bounds__(256) void range_kernel(const Args a, int D, float4*
     const float y = bound(0, g, most_k);
     if (y < INFINITY) k = fmaxf(k, y);
     const float x = bound(1, g, most_v);
+    // A quantizer stores zeros as codes of zero times its least scale: those are
+    // no small values.
+    if (x > 0.0f && x < INFINITY && !(static_cast<const uint16_t*>(a.slot[5])[g] & 0x7fff)) {
+      const uint32_t* codes = static_cast<const uint32_t*>(a.slot[3]) + g * words;
+      uint32_t any = 0;
+      for (int e = 0; e < words; ++e) any |= codes[e];
+      if (!any) continue;
+    }
     v = fmaxf(v, x);
     if (x > 0.0f) low = fminf(low, x);
   }

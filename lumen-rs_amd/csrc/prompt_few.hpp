@@ -92,9 +92,7 @@ __device__ __forceinline__ void halves16(const uint32_t* w, float s, float z, in
 }
 // The least of them but zero: f16 holds bf16's 8 bits from 2^-17 on.
 __device__ __forceinline__ float least_of(float least, float s, float z) {
-  if (s != 0.0f) least = fminf(least, fabsf(s));
-  if (z != 0.0f) least = fminf(least, fabsf(z));
-  return least;
+  return fminf(least, fminf(s != 0.0f ? fabsf(s) : INFINITY, z != 0.0f ? fabsf(z) : INFINITY));
 }
 constexpr float kHeld = 0x1p-17f;
 
@@ -370,31 +368,59 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
         }
       };
       // V's range in the wavefront's tiles, by the largest values that the runs'
-      // scales and biases allow (a sixteenth of the rows' bytes, read again later).
-      float v_top = 0.0f, v_low = INFINITY, v_least = INFINITY;  // least: of the scales and biases but zero
+      // scales and biases allow (a sixteenth of the rows' bytes, read again later),
+      // and the least of these. A quantizer stores zeros as codes of zero times
+      // its least scale, with a bias of zero: what such runs (`plain`) allow is no
+      // value. Their codes are looked at only where they would decide something:
+      // in a second pass, for the first one's loads are all on their way at once.
+      float v_top = 0.0f, v_low = INFINITY, v_least = INFINITY, plain_top = 0.0f, plain_least = INFINITY;
       bool fine = true;
+      auto range = [&](auto codes) __attribute__((always_inline)) {
 #pragma unroll 4
-      for (int tile = t0; tile <= t_hi; tile += kWaves) {
-        bool ok;
-        const int64_t row = lane_row(tile, ok);
-        float s[NRUN], z[NRUN];
-        load_scales(row, ok, 1, s, z);
+        for (int tile = t0; tile <= t_hi; tile += kWaves) {
+          bool ok;
+          const int64_t row = lane_row(tile, ok);
+          float s[NRUN], z[NRUN];
+          load_scales(row, ok, 1, s, z);
 #pragma unroll
-        for (int i = 0; i < NRUN; ++i) {
-          const float x = fabsf(z[i]), y = fabsf(fmaf(s[i], float((1 << BV) - 1), z[i]));
-          fine &= x < INFINITY && y < INFINITY;
-          v_top = fmaxf(v_top, fmaxf(x, y));
-          if (fmaxf(x, y) > 0.0f) v_low = fminf(v_low, fmaxf(x, y));
-          v_least = least_of(v_least, s[i], z[i]);
+          for (int i = 0; i < NRUN; ++i) {
+            const float x = fabsf(z[i]), y = fabsf(fmaf(s[i], float((1 << BV) - 1), z[i])), most = fmaxf(x, y);
+            bool out = z[i] == 0.0f;
+            if constexpr (decltype(codes)::value) {
+              if (!out || !(y > 0.0f)) continue;
+              const uint32_t* src = static_cast<const uint32_t*>(a.slot[3]) + (2 * row + half) * VW + i * BV;
+              uint32_t any = 0;
+#pragma unroll
+              for (int e = 0; e < BV; ++e) any |= src[e];
+              out = !any;
+            } else {  // no branches: loads of several tiles at once
+              fine &= x < INFINITY && y < INFINITY;
+              plain_top = fmaxf(plain_top, out ? y : 0.0f);
+              plain_least = fminf(plain_least, out && y > 0.0f ? fabsf(s[i]) : INFINITY);
+            }
+            v_top = fmaxf(v_top, out ? 0.0f : most);
+            v_low = fminf(v_low, out ? INFINITY : most);
+            v_least = fminf(v_least, out ? INFINITY : least_of(INFINITY, s[i], z[i]));
+          }
         }
-      }
 #pragma unroll
-      for (int d = 32; d > 0; d /= 2) {
-        v_top = fmaxf(v_top, __shfl_xor(v_top, d, kWave));
-        v_low = fminf(v_low, __shfl_xor(v_low, d, kWave));
-        v_least = fminf(v_least, __shfl_xor(v_least, d, kWave));
+        for (int d = 32; d > 0; d /= 2) {
+          v_top = fmaxf(v_top, __shfl_xor(v_top, d, kWave));
+          v_low = fminf(v_low, __shfl_xor(v_low, d, kWave));
+          v_least = fminf(v_least, __shfl_xor(v_least, d, kWave));
+        }
+      };
+      auto up_of = [&]() __attribute__((always_inline)) {
+        return v_top > 0.0f && v_top < INFINITY ? __builtin_amdgcn_readfirstlane(15 - __builtin_amdgcn_frexp_expf(v_top)) : 0;
+      };
+      range(std::false_type{});
+      v_up = up_of();
+      // (Of scales that f16 holds there is nothing to know: 15 times one is 2^-14.)
+      if (__any(plain_top > v_top || ldexpf(plain_least, v_up) < kHeld)) {
+        rare();
+        range(std::true_type{});
+        v_up = up_of();
       }
-      if (v_top > 0.0f && v_top < INFINITY) v_up = __builtin_amdgcn_readfirstlane(15 - __builtin_amdgcn_frexp_expf(v_top));
       // Too far apart for f16: what is no number has attend_row do the rows.
       if (!__all(fine && (v_top == 0.0f || ldexpf(v_low, v_up) >= 0x1p-14f))) {
         rare();

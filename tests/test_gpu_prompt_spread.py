@@ -7,7 +7,7 @@ import pytest
 import oracle_lib as O
 import prompt_ref as R
 from inputs import kv_bf16
-from paged_ref import AFFINE, Paged, values_of
+from paged_ref import AFFINE, Paged, codes_of, values_of
 from test_gpu_prompt import T, run_paged, say, starts_of  # noqa: F401 (T: the fixture)
 
 pytestmark = pytest.mark.gpu
@@ -128,3 +128,34 @@ def test_keys_of_small_groups_keep_their_bits(T, counts, D, gs, bits, far):
         want[a:e], tol[a:e] = R.attend(f, k, v, np.arange(n - (e - a), n), scale, off_v=2.0 ** -11 + 2.0 ** -24, off_w=2.0 ** -11)
     assert far < 32 or tol.max() < 0.2
     R.check(got, want, tol, f"small keys {far}")
+
+
+@pytest.mark.parametrize("counts", [[3, 2], MANY])
+@pytest.mark.parametrize("D,gs", [(64, 32), (128, 64), (256, 128), (512, 32)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_groups_of_zeros_cost_the_others_nothing(T, counts, D, gs, bits):
+    """The quantizer stores a group of zeros as a scale of -1e-7 (its least) with
+    codes and bias of zero: beside values of 20,000 the results are those, bit
+    for bit, of a scale of zero, of which nothing could be lost."""
+    say("zeros", counts, D, gs, bits)
+    p = Paged(LENS, 1, D, 16, AFFINE, 4, bits, gs, seed=5)
+    rng = np.random.default_rng(D + bits)
+    for b, n in enumerate(LENS):
+        for row in range(n):
+            k, v = rng.standard_normal((2, 1, D))
+            v *= 20000.0
+            if row % 5 == 2:
+                v[:, :gs] = 0.0
+            if row % 11 == 4:
+                v[:] = 0.0
+            p.write(b, row, bf16(k), bf16(v))
+    q = kv_bf16((sum(counts), 2, D), D)
+    starts = starts_of(counts)
+    want, tol = R.paged(p, q, starts, D ** -0.5)
+    first = run_paged(T, p, q, starts, D ** -0.5)
+    R.check(O.bf16_to_f32(first), want, tol, "zeros")
+    _, scales, biases = p.sides[1]
+    none = (biases == 0) & (np.abs(O.bf16_to_f32(scales)) < 1e-6)
+    assert none.sum() >= 40 and not codes_of(p.sides[1][0], bits).reshape(*none.shape, gs)[none].any()
+    scales[none] = 0
+    assert np.array_equal(run_paged(T, p, q, starts, D ** -0.5), first)
