@@ -615,8 +615,9 @@ size_t tqkv_packed_attend_workspace_size(int32_t batch, int32_t H, int32_t H_kv,
  * gets zeros. max_rows: the host's bound on lens, as tqkv_paged_decode_attend
  * takes it. Affine rows enter as scale * code + bias in 11 bits (keys down to
  * 2^-28 of their head's largest or their own, a query's channels of its largest,
- * values of their group's); values in bf16's 8 where their groups' largest lie
- * 2^28 apart in a head. Few queries over such values, and scores of which f16's
+ * values of their group's), weights over them in 11 bits down to 2^-21 of a row's
+ * largest, below that to 2^-32 of it; values and weights in bf16's 8 where groups'
+ * largest lie 2^28 apart in a head. Few queries over such values, and scores of which f16's
  * steps could be 2^-10 or more (|q| |k| scale of 2^28), are computed in f32, at
  * many times the cost.
  * Affine rows of longer chunks are dequantized once into the workspace, 4 * batch *

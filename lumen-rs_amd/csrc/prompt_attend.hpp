@@ -209,6 +209,11 @@ __device__ __forceinline__ void attend_row(const Args& a, int b, int64_t token, 
 constexpr int kWave = 64;
 constexpr int kXcds = 8;
 constexpr float kTau = 8.0f;
+// f16 weights are taken times 2^kLift: the largest, 2^kTau over the lagging
+// maximum, is 2^15 there, and f16's least step, 2^-24, 2^-31 of a row's largest
+// weight (of many keys 17 nats below a first one, times 1, all of the weight was
+// lost). Sums and results are given without it.
+constexpr int kLift = 7;
 // A scale of zero as the least positive number: a hidden key's score, -infinity,
 // times it stays that.
 constexpr float kLeastScale = 0x1p-149f;
@@ -708,7 +713,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
           mx = row_max(mx);
           rescale(j, mx * qscale[j] > m[j] + kTau, mx);
         }
-        const float nm = m[j] == -INFINITY ? 0.0f : -m[j];
+        const float nm = m[j] == -INFINITY ? 0.0f : (H ? kLift : 0.0f) - m[j];
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
           u4_t w;
@@ -802,13 +807,15 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
   bool bad = false;
 #pragma unroll
   for (int j = 0; j < NR; ++j) {
-    const float sum = row_sum(lsum[j]);
+    float sum = row_sum(lsum[j]);
     const int64_t r = row_at(j);
-    if (F16 && v_down != kBf16)
+    if (F16 && v_down != kBf16) {
+      sum *= 1.0f / (1 << kLift);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[t][j][e] = ldexpf(o[t][j][e], v_down);
+        for (int e = 0; e < 4; ++e) o[t][j][e] = ldexpf(o[t][j][e], v_down - kLift);
+    }
     if (r >= rows) continue;
     const int64_t row = (seq.first + r / a.G) * a.H + int64_t(kvh) * a.G + r % a.G;
     if (a.part_o) {

@@ -221,7 +221,7 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
 #pragma unroll
         for (int t = 0; t < NT; ++t) o[t][j] *= alpha;
         m[j] = mn;
-        nm[j] = mn == -INFINITY ? 0.0f : -mn;
+        nm[j] = mn == -INFINITY ? 0.0f : (H16 ? kLift : 0.0f) - mn;
         thr[j] = (mn + kTau) * __builtin_amdgcn_rcpf(qscale[j]);
       }
       u4_t w;
@@ -485,13 +485,13 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
     const float sum = row_sum(lsum[j]);
     if (lg == 0) {
       part_m[wave][16 * j + lr] = m[j];
-      part_l[wave][16 * j + lr] = sum;
+      part_l[wave][16 * j + lr] = AFFINE ? sum * (1.0f / (1 << kLift)) : sum;
     }
     if constexpr (AFFINE)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[t][j][e] = ldexpf(o[t][j][e], -v_up);
+        for (int e = 0; e < 4; ++e) o[t][j][e] = ldexpf(o[t][j][e], -v_up - kLift);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
       *reinterpret_cast<f4_t*>(mine + (16 * j + lr) * D + ((4 * t + lg) ^ (lr & 7)) * 4) = o[t][j];
