@@ -27,9 +27,7 @@ struct Rows {
 };
 __device__ __forceinline__ Rows seen_rows(const Args& a, int b) {
   const Sequence s = sequence<kPagedAffine>(a, b);
-  const int p = s.keys - s.count;
-  const int lo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
-  return Rows{lo, s.count > 0 ? s.keys : 0};
+  return Rows{first_seen(a, s.keys - s.count), s.count > 0 ? s.keys : 0};
 }
 
 __global__ __launch_bounds__(256) void range_kernel(const Args a, int D, float4* part) {

@@ -120,6 +120,12 @@ __device__ __forceinline__ Range visible(const Args& a, int64_t p, int n) {
   return Range{int(lo < hi ? lo : hi), int(hi)};
 }
 
+// The first of them. p may lie far before the first key, and the window be the
+// largest that the type holds.
+__device__ __forceinline__ int first_seen(const Args& a, int p) {
+  return a.window > 0 && p >= a.window ? p - a.window + 1 : 0;
+}
+
 // Channel c of a stored row in f32.
 template <Source S>
 __device__ __forceinline__ float value_at(const Args& a, bool key, int64_t row, int D, int c) {
@@ -539,7 +545,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
   if (n - key_lo > a.split_keys) key_hi = key_lo + a.split_keys;
   if (a.causal) {
     if (pos_hi + 1 < key_hi) key_hi = pos_hi + 1;
-    if (a.window > 0 && pos_lo - a.window + 1 > key_lo) key_lo = pos_lo - a.window + 1;
+    if (first_seen(a, pos_lo) > key_lo) key_lo = first_seen(a, pos_lo);
   }
   if (a.part_o && key_lo >= key_hi) return;  // the join leaves such splits out
 
@@ -679,7 +685,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
           on = held_groups(tile);
         }
       const bool whole = kbase >= key_lo && kbase + KT <= key_hi && on == (1u << NI) - 1u &&
-                         (!a.causal || (kbase + KT - 1 <= pos_lo && (a.window <= 0 || pos_hi - a.window < kbase)));
+                         (!a.causal || (kbase + KT - 1 <= pos_lo && first_seen(a, pos_hi) <= kbase));
       if (!whole) {
         rare();
         const int ln = lane_now<D>(lane), g4 = 4 * (ln / 16);
@@ -689,7 +695,7 @@ __attribute__((amdgpu_waves_per_eu(Shape<D>::kWaves / 4))) void prompt_kernel(co
           int hi = key_hi - kbase, lo = key_lo - kbase;  // visible: [lo, hi)
           if (a.causal) {
             hi = min(hi, pos + 1 - kbase);
-            if (a.window > 0) lo = max(lo, pos - a.window + 1 - kbase);
+            lo = max(lo, first_seen(a, pos) - kbase);
           }
 #pragma unroll
           for (int i = 0; i < NI; ++i)

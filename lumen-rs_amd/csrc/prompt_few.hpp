@@ -125,7 +125,7 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
   int key_lo = split * a.split_keys, key_hi = n;
   if (n - key_lo > a.split_keys) key_hi = key_lo + a.split_keys;
   if (pos_hi + 1 < key_hi) key_hi = pos_hi + 1;
-  if (a.window > 0 && pos_lo - a.window + 1 > key_lo) key_lo = pos_lo - a.window + 1;
+  if (first_seen(a, pos_lo) > key_lo) key_lo = first_seen(a, pos_lo);
   if (a.part_o && key_lo >= key_hi) return;
 
   int v_up = 0;  // V as f16 is taken times 2^v_up
@@ -188,13 +188,13 @@ __attribute__((amdgpu_waves_per_eu(Few<D, S == kPagedAffine>::kPerEu))) void few
     for (int i = 0; i < NI; ++i)
       if (paged::valid_page(a.pool, page_of(min(kbase + 16 * i, n - 1)))) on |= 1u << i;
     const bool whole = kbase >= key_lo && kbase + KT <= key_hi && on == (1u << NI) - 1u &&
-                       kbase + KT - 1 <= pos_lo && (a.window <= 0 || pos_hi - a.window < kbase);
+                       kbase + KT - 1 <= pos_lo && first_seen(a, pos_hi) <= kbase;
     if (!whole) {
       rare();
 #pragma unroll
       for (int j = 0; j < NR; ++j) {
         const int hi = min(key_hi, pos[j] + 1) - kbase;
-        const int lo = (a.window > 0 ? max(key_lo, pos[j] - a.window + 1) : key_lo) - kbase;
+        const int lo = max(key_lo, first_seen(a, pos[j])) - kbase;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
