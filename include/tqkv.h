@@ -469,7 +469,11 @@ typedef struct tqkv_page_tables {
  * its table cannot name the rows, where it needs pages and those that it and
  * all before it that the table could hold ask for are more than are free, or where their tokens are more
  * than `tokens`. granted (int32 [batch], or NULL): counts[b], or -1 where
- * refused. The pages given out are the top ones of the stack, in its order;
+ * refused. A refused sequence's tokens have no place in starts and slots, those
+ * of the sequences behind it move up: lay the step's tokens out by the slots
+ * (token i is the one at position slots[i][2] of sequence slots[i][3]), or drop
+ * the step where granted has a -1. Tokens that lie by the counts asked for would
+ * enter other sequences. The pages given out are the top ones of the stack, in its order;
  * slots behind the last token are {-1, 0, -1, -1}, and a page that the table
  * names wrongly is -1 in them. tokens: the host's bound on the sum of counts,
  * below 2^31. One launch, two for 1,024 tokens and more; no allocation.
