@@ -605,7 +605,9 @@ int32_t tqkv_packed_attend(const uint16_t* q, int64_t q_stride, const uint16_t* 
                            int64_t window, uint16_t* out, void* workspace,
                            size_t workspace_bytes, tqkv_stream stream);
 /* Host arithmetic only; 0 where none is needed and for sizes that the call
- * refuses. */
+ * refuses. Fewer tokens can need more than many, whose blocks fill the GPU
+ * without dividing keys: a workspace for calls of other sizes too takes the
+ * largest of theirs, or 4 (D + 2) * 98,304 + 256 bytes, which no call passes. */
 size_t tqkv_packed_attend_workspace_size(int32_t batch, int32_t H, int32_t H_kv, int32_t D,
                                          int64_t tokens);
 
@@ -634,6 +636,9 @@ int32_t tqkv_paged_prefill_attend(const tqkv_paged_kv* kv, const uint16_t* q, in
                                   int32_t H, const int32_t* starts, int64_t tokens, float scale,
                                   int64_t window, int64_t max_rows, uint16_t* out,
                                   void* workspace, size_t workspace_bytes, tqkv_stream stream);
+/* As tqkv_packed_attend_workspace_size; no call of up to max_rows rows passes
+ * 4 (dim + 2) * (98,304 + 32 * batch * kv_heads) + 1,024 bytes, over affine
+ * pages and 4 * batch * kv_heads * max_rows * dim + 520 * batch * kv_heads. */
 size_t tqkv_paged_prefill_workspace_size(const tqkv_paged_kv* kv, int32_t H, int64_t tokens,
                                          int64_t max_rows);
 

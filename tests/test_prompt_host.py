@@ -177,3 +177,28 @@ def test_struct_layouts_match_the_header(tmp_path):
         assert got[(cname, "size")] == ctypes.sizeof(py), cname
         for f, _ in py._fields_:
             assert got[(cname, f)] == getattr(py, f).offset, (cname, f)
+
+
+def test_workspace_bounds():
+    """What the header promises for all calls: partial results of a prompt's call
+    are kept for fewer than 384 workgroups of 256 rows, of few rows' for 2,048 of
+    32 and as many more as there are blocks."""
+    rng = np.random.default_rng(1)
+    tokens = np.unique(np.r_[1:300, np.geomspace(1, 2 ** 31 - 1, 400).astype(np.int64)])
+    fell = False
+    for D in (64, 128, 256, 512):
+        for batch, H_kv, G in [(1, 1, 1), (1, 1, 32), (2, 8, 4), (7, 3, 5), (64, 8, 4), (1024, 16, 1), (1024, 1, 32)]:
+            sizes = [T.packed_attend_workspace_size(batch, H_kv * G, H_kv, D, int(t)) for t in tokens]
+            assert max(sizes) <= 4 * (D + 2) * 98304 + 256, (D, batch, H_kv, G)
+            fell |= any(a > b for a, b in zip(sizes, sizes[1:]))
+            for kind in (T.CACHE_BF16, T.CACHE_AFFINE):
+                kv = view(kind=kind, batch=batch, kv_heads=H_kv, dim=D, num_pages=1 << 20, table_stride=1 << 14, bits_k=4, bits_v=8, group_size=32)
+                cap = (1 << 14) * kv.page_rows
+                for rows in (1, 900, int(rng.integers(1, cap)), cap):
+                    sizes = [T.paged_prefill_workspace_size(kv, H_kv * G, int(t), rows) for t in tokens[::3]]
+                    most = 4 * (D + 2) * (98304 + 32 * batch * H_kv) + 1024
+                    if kind == T.CACHE_AFFINE:
+                        most += 4 * batch * H_kv * rows * D + 520 * batch * H_kv
+                    assert max(sizes) <= most, (D, batch, H_kv, G, kind, rows)
+                    fell |= any(a > b for a, b in zip(sizes, sizes[1:]))
+    assert fell  # why there is a bound to state
