@@ -594,7 +594,7 @@ int32_t tqkv_paged_append_rope(const tqkv_paged_kv* kv, const tqkv_rope* rope, c
  * infinite or NaN key or value reaches only the queries that see it.
  * D in {64, 128, 256, 512}; H / H_kv from 1 to 32; batch at most 1024; tokens
  * below 2^31; q, k, v 16-byte aligned, strides multiples of 8, token_stride
- * from 0 to below 2^27; out 16-byte aligned. workspace: tqkv_packed_attend_workspace_size() bytes, 16-byte
+ * from 0 to below 2^27; out 16-byte aligned, no memory of q, k or v. workspace: tqkv_packed_attend_workspace_size() bytes, 16-byte
  * aligned, or NULL for the library's scratch; calls that share one must not
  * overlap in time.
  */

@@ -284,6 +284,8 @@ int32_t check_queries(const uint16_t* q, int64_t q_stride, int H, int H_kv, cons
       q_stride % 8 != 0)
     return fail(TQKV_EINVAL_ARG, "q and out are 16-byte aligned, q_stride (%lld) a multiple of 8",
                 (long long)q_stride);
+  // Rows that end with what is not finite are done again from their queries.
+  if (q == out) return fail(TQKV_EINVAL_ARG, "out is q");
   return TQKV_OK;
 }
 

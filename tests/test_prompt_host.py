@@ -202,3 +202,8 @@ def test_workspace_bounds():
                     assert max(sizes) <= most, (D, batch, H_kv, G, kind, rows)
                     fell |= any(a > b for a, b in zip(sizes, sizes[1:]))
     assert fell  # why there is a bound to state
+
+
+def test_out_is_not_q():
+    refused(T.EINVAL_ARG, T.packed_attend, A, 1024, A, A, 1024, 128, 2, 8, 4, 128, A, 64, 0.1, A, workspace=A, workspace_bytes=1 << 40)
+    refused(T.EINVAL_ARG, T.paged_prefill_attend, view(), A, 1024, 8, A, 64, 0.1, 512, A, workspace=A, workspace_bytes=1 << 40)
