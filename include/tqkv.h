@@ -510,7 +510,8 @@ int32_t tqkv_paged_release(const tqkv_page_tables* tables, const int32_t* keep,
  *   TQKV_ROPE_RAMP    the same ends as whole channels, floor and ceiling of
  *                     rotary_dim ln(original / (2 pi turns)) / (2 ln base)
  *                     within [0, rotary_dim - 1], weighted linearly by i
- *                     between them, and a magnitude of 0.1 ln(factor) + 1
+ *                     between them, and a magnitude of 0.1 ln(factor) + 1 (of any
+ *                     factor: below 1 where that is)
  */
 #define TQKV_ROPE_PLAIN 0
 #define TQKV_ROPE_LINEAR 1

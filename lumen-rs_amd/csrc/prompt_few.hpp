@@ -10,14 +10,16 @@
 // next tile's codes have been loaded into meanwhile, to f16 (bf16 would cost the
 // results three bits): every row of K times a power of two that brings the
 // largest value its scales and biases allow below 2^15, which its scores take
-// back (rows whose steps would be more than kCoarse in a score are attend_row's); V times one power of two for the wavefront's rows. Where V's groups'
-// largest values lie 2^28 apart (a query may see the small ones alone), attend_row
-// does the rows.
+// back (rows whose steps would be more than kCoarse in a score are attend_row's); V
+// times one power of two for the wavefront's rows. Where V's groups' largest values
+// lie 2^28 apart (a query may see the small ones alone), attend_row does the rows.
 //
 // 32 sequences of up to 24,000 bf16 rows, D = 128, 6 tokens each: 117 us for 453 MB
-// (3.9 TB/s; a large copy 4.9). The same of 4-bit rows: 134 us, 13 of them the pass
-// over the values' scales; 16 sequences of 8,000 at D = 256 252 us: the conversion's
-// vector operations bound it.
+// (3.9 TB/s; a large copy 4.9). The same of 4-bit rows: 135 to 138 us for 134 MB, of
+// 8-bit rows 144 for 180; 16 sequences of 8,000, D = 256, 3 tokens each, 168 us for 296
+// MB and 208 for 559. No unit bounds the affine forms (vector 42% of the CUs' cycles at 4
+// bits, matrix 7%, LDS conflicts 7 to 9%): a tile is one chain of conversion, LDS and
+// products, K's and then V's, with one or two wavefronts a SIMD to cover it.
 #pragma once
 
 #include "prompt_attend.hpp"
