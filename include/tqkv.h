@@ -624,9 +624,9 @@ size_t tqkv_packed_attend_workspace_size(int32_t batch, int32_t H, int32_t H_kv,
  * 2^-28 of their head's largest or their own, a query's channels of its largest,
  * values of their group's), weights over them in 11 bits down to 2^-21 of a row's
  * largest, below that to 2^-32 of it; values and weights in bf16's 8 where groups'
- * largest lie 2^28 apart in a head. Few queries over such values, and scores of which f16's
- * steps could be 2^-10 or more (|q| |k| scale of 2^28), are computed in f32, at
- * many times the cost.
+ * largest lie 2^28 apart in a head. Few queries over such values, and scores of
+ * which f16's steps could be 2^-10 or more (|q| |k| scale of 2^28), are computed
+ * in f32, at many times the cost.
  * Affine rows of longer chunks are dequantized once into the workspace, 4 * batch *
  * H_kv * max_rows * dim bytes of it: a batch of many sequences of which few have
  * queries is best called with a table of those alone.

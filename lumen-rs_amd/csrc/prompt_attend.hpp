@@ -25,9 +25,10 @@
 // up to 8,192 tokens, D = 128: 937 GF in 897 us where calls alternate with other work
 // (1.04 PF/s; a matrix product of 8,192 cubed 1.24) and 940 to 1,060 one call after the
 // other, when the clock falls (0.88 to 1.0 PF/s); the matrix pipes busy 47% of the CUs'
-// cycles, vector operations (exp2 and the rounding of the weights) 49%. D = 256 with 16 rows a wavefront and D = 512 with
-// one tile of K and V in LDS read LDS for every product: 400 and 665 TF/s over
-// windows and prompts whose blocks do not divide evenly among the CUs.
+// cycles, vector operations (exp2 and the rounding of the weights) 49%. D = 256 with
+// 16 rows a wavefront and D = 512 with one tile of K and V in LDS read LDS for every
+// product: 400 and 665 TF/s over windows and prompts whose blocks do not divide evenly
+// among the CUs.
 //
 // Weights of hidden keys are exact zeros, but zero times an infinite value is
 // NaN (and sums of values next to f32's largest pass it): a row that ends with
